@@ -59,6 +59,7 @@ HIP_API = {
     "f3s_naive_attention_fwd": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, c_i32, c_f32,
                                         c_vp]),
     "f3s_plan_create": (c_i32, [c_vp, c_vp, c_i32, c_i32, c_i32, c_vp, P_vp]),
+    "f3s_plan_create_scheduled": (c_i32, [c_vp, c_i32, c_i32, c_vp, P_vp]),
     "f3s_plan_destroy": (c_i32, [c_vp]),
     "f3s_plan_compile": (c_i32, [c_vp, c_vp, c_vp, c_i32, c_vp]),
     "f3s_plan_info": (c_i32, [c_vp, P_i64, P_i64, P_i64, P_i32]),
@@ -68,6 +69,14 @@ HIP_API = {
     "f3s_attention_fwd_packed": (c_i32, [c_vp, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_f32,
                                          c_vp]),
     "f3s_linear_f16": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_i64, c_i32, c_i32, c_vp]),
+    "f3s_reverse_csr": (c_i32, [c_vp, c_vp, c_i32, c_i64, c_vp, c_vp, c_vp]),
+    "f3s_diff_attention_workspace": (c_i32, [c_vp, c_vp, P_i64]),
+    "f3s_diff_attention_fwd": (c_i32, [c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp,
+                                       c_i64, c_vp, c_i32, c_i32, c_i32, c_f32, c_vp, c_i64,
+                                       c_vp]),
+    "f3s_diff_attention_bwd": (c_i32, [c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp,
+                                       c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64,
+                                       c_vp, c_i32, c_i32, c_i32, c_f32, c_vp, c_i64, c_vp]),
     "f3s_probe_gather": (c_i32, [c_vp, c_vp, c_i64, c_i32, c_vp, c_i64, c_i32, c_vp, c_vp]),
 }
 

@@ -48,15 +48,22 @@ def attention_fwd_timed(Q: DeviceArray, K: DeviceArray, V: DeviceArray, O: Devic
 
 
 class Plan:
-    """f3s_plan: segments of heavy windows merged inside the launch."""
+    """f3s_plan: segments of heavy windows merged inside the launch.
+    scheduled=True: f3s_plan_create_scheduled, in the library's own sequence."""
 
     def __init__(self, bsf: DeviceBSF, window_order: DeviceArray | None = None, H: int = 1,
-                 seg_tiles: int = 0, stream: Stream | None = None):
+                 seg_tiles: int = 0, stream: Stream | None = None, scheduled: bool = False):
         h = C.c_void_p()
-        check(_lib.hip().f3s_plan_create(bsf.window_offsets.ptr,
-                                         window_order.ptr if window_order is not None else None,
-                                         bsf.W, H, seg_tiles, stream.handle if stream else None,
-                                         C.byref(h)), "f3s_plan_create")
+        handle = stream.handle if stream else None
+        if scheduled:
+            if window_order is not None or seg_tiles:
+                raise ValueError("a scheduled plan takes no window order or segment size")
+            check(_lib.hip().f3s_plan_create_scheduled(bsf.window_offsets.ptr, bsf.W, H, handle,
+                                                       C.byref(h)), "f3s_plan_create_scheduled")
+        else:
+            check(_lib.hip().f3s_plan_create(
+                bsf.window_offsets.ptr, window_order.ptr if window_order is not None else None,
+                bsf.W, H, seg_tiles, handle, C.byref(h)), "f3s_plan_create")
         self.handle = h.value
         self.bsf = bsf
         self.H = H

@@ -1302,7 +1302,7 @@ namespace f3s {
 // tile-dense.)
 static f3s_status build_plan_sets(f3s_plan* p, const int32_t* d_window_offsets,
                                   const int32_t* d_window_order, int32_t seg_tiles,
-                                  hipStream_t st)
+                                  bool by_schedule, hipStream_t st)
 {
     const int32_t W = p->W, H = p->H;
     const bool automatic = seg_tiles == 0;
@@ -1311,7 +1311,7 @@ static f3s_status build_plan_sets(f3s_plan* p, const int32_t* d_window_offsets,
     const int32_t nsets = automatic ? 2 : 1;
     const int arrays = 3 * nsets;
     const bool scheduled = W > kHeavyMaxWindows && team_m == 1 && team_d == 1 &&
-                           (int64_t)W * H >= kSchedOrderedMin;
+                           (by_schedule || (int64_t)W * H >= kSchedOrderedMin);
     StreamBuffer sbuf(st);
     const int32_t* seq = d_window_order;   // the sequence of positions
     int32_t P = W;
@@ -1671,9 +1671,9 @@ f3s_status f3s_attention_fwd_noalloc(const uint16_t* Q, const uint16_t* K, const
                               d_window_order, W, n, d, H, scale, stream, sp);
 }
 
-f3s_status f3s_plan_create(const int32_t* d_window_offsets, const int32_t* d_window_order,
-                           int32_t W, int32_t H, int32_t seg_tiles, void* stream,
-                           f3s_plan** plan_out)
+static f3s_status create_plan(const int32_t* d_window_offsets, const int32_t* d_window_order,
+                              int32_t W, int32_t H, int32_t seg_tiles, bool by_schedule,
+                              void* stream, f3s_plan** plan_out)
 {
     F3S_REQUIRE(plan_out != nullptr, "f3s_plan_create: NULL out pointer");
     *plan_out = nullptr;
@@ -1696,13 +1696,26 @@ f3s_status f3s_plan_create(const int32_t* d_window_offsets, const int32_t* d_win
     // tile-dense chunk costs two whole tiles, ~15x a masked chunk per tile
     // on sparse graphs); graphs whose windows leave most SIMDs idle run teams
     // instead (team_for), as the unplanned launch does.
-    const f3s_status s = build_plan_sets(p, d_window_offsets, d_window_order, seg_tiles, st);
+    const f3s_status s = build_plan_sets(p, d_window_offsets, d_window_order, seg_tiles, by_schedule, st);
     if (s != F3S_OK) {
         delete p;
         return s;
     }
     *plan_out = p;
     return F3S_OK;
+}
+
+f3s_status f3s_plan_create(const int32_t* d_window_offsets, const int32_t* d_window_order,
+                           int32_t W, int32_t H, int32_t seg_tiles, void* stream,
+                           f3s_plan** plan_out)
+{
+    return create_plan(d_window_offsets, d_window_order, W, H, seg_tiles, false, stream, plan_out);
+}
+
+f3s_status f3s_plan_create_scheduled(const int32_t* d_window_offsets, int32_t W, int32_t H,
+                                     void* stream, f3s_plan** plan_out)
+{
+    return create_plan(d_window_offsets, nullptr, W, H, 0, true, stream, plan_out);
 }
 
 f3s_status f3s_plan_compile(f3s_plan* plan, const int32_t* d_block_col,

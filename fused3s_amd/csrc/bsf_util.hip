@@ -95,6 +95,58 @@ bsf_stats_kernel(const int32_t* __restrict__ block_col, const uint16_t* __restri
     }
 }
 
+// The reversed edges of a CSR: entries per column, their scan (the new row
+// pointer), then every entry to the next free place of its column.  The order
+// within a row is that of the atomics and differs from run to run; the converter
+// does not mind it, and its lists come out the same.  256 entries per workgroup:
+// the rows they span are found once, each entry's among those.
+__global__ void __launch_bounds__(256)
+clear_counts(int32_t* __restrict__ a, int64_t count)
+{
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < count) a[i] = 0;
+}
+
+__global__ void __launch_bounds__(256)
+column_counts(const int32_t* __restrict__ col_idx, int64_t nnz, int32_t n,
+              int32_t* __restrict__ counts)
+{
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (e >= nnz) return;
+    const int32_t c = col_idx[e];
+    if ((uint32_t)c < (uint32_t)n) atomicAdd(&counts[c], 1);
+}
+
+// The last of rows [lo, hi] that starts at or before entry e.
+__device__ __forceinline__ int32_t row_of(const int32_t* __restrict__ row_ptr, int32_t lo,
+                                          int32_t hi, int64_t e)
+{
+    while (lo < hi) {
+        const int32_t mid = lo + (hi - lo + 1) / 2;
+        if (row_ptr[mid] <= e) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(256)
+reverse_fill(const int32_t* __restrict__ row_ptr, const int32_t* __restrict__ col_idx, int64_t nnz,
+             int32_t n, const int32_t* __restrict__ out_ptr, int32_t* __restrict__ used,
+             int32_t* __restrict__ out_idx)
+{
+    __shared__ int32_t span[2];
+    const int64_t e0 = (int64_t)blockIdx.x * 256, e = e0 + threadIdx.x;
+    if (threadIdx.x < 2)
+        span[threadIdx.x] = row_of(row_ptr, 0, n - 1, threadIdx.x ? min(e0 + 255, nnz - 1) : e0);
+    __syncthreads();
+    if (e >= nnz) return;
+    const int32_t c = col_idx[e];
+    if ((uint32_t)c >= (uint32_t)n) return;
+    const int32_t row = row_of(row_ptr, span[0], max(span[0], span[1]), e);
+    const int64_t at = (int64_t)out_ptr[c] + atomicAdd(&used[c], 1);
+    if (at < nnz) out_idx[at] = row;
+}
+
 __global__ void warm_bsf_util_kernel() {}
 
 hipError_t warm_bsf_util(hipStream_t s)
@@ -175,6 +227,39 @@ f3s_status f3s_bsf_stats(const int32_t* d_block_col, const uint16_t* d_tile_mask
     F3S_HIP(hipStreamSynchronize(st));
     *occ_sum = (int64_t)h[0];
     *mask_bits = (int64_t)h[1];
+    return F3S_OK;
+}
+
+f3s_status f3s_reverse_csr(const int32_t* d_row_ptr, const int32_t* d_col_idx, int32_t n,
+                           int64_t nnz, int32_t* d_out_row_ptr, int32_t* d_out_col_idx,
+                           void* stream)
+{
+    F3S_REQUIRE(n >= 0 && nnz >= 0 && nnz <= INT32_MAX, "f3s_reverse_csr: bad size");
+    F3S_REQUIRE(n > 0 || nnz == 0, "f3s_reverse_csr: edges without nodes");
+    F3S_REQUIRE(d_row_ptr && d_out_row_ptr && (nnz == 0 || (d_col_idx && d_out_col_idx)),
+                "f3s_reverse_csr: NULL pointer");
+    F3S_TRY(require_device());
+    clear_error();
+    hipStream_t st = as_stream(stream);
+    const size_t words = (size_t)n + (n & 1);
+    StreamBuffer buf(st);
+    F3S_TRY(buf.reserve(2 * sizeof(int32_t) * words + sizeof(int64_t) * (size_t)(offsets_sum_elems(n) + 1)));
+    int32_t* counts = static_cast<int32_t*>(buf.ptr);
+    int32_t* used = counts + words;
+    int64_t* sums = reinterpret_cast<int64_t*>(used + words);
+    if (words)
+        hipLaunchKernelGGL(clear_counts, dim3((unsigned)ceil_div(2 * words, 256)), dim3(256), 0, st,
+                           counts, (int64_t)(2 * words));
+    const dim3 grid((unsigned)ceil_div(nnz, 256));
+    if (nnz)
+        hipLaunchKernelGGL(column_counts, grid, dim3(256), 0, st, d_col_idx, nnz, n, counts);
+    F3S_HIP(hipGetLastError());
+    F3S_TRY(counts_to_offsets(counts, d_out_row_ptr, n, sums + 1, sums, st));
+    if (nnz) {
+        hipLaunchKernelGGL(reverse_fill, grid, dim3(256), 0, st, d_row_ptr, d_col_idx, nnz, n,
+                           d_out_row_ptr, used, d_out_col_idx);
+        F3S_HIP(hipGetLastError());
+    }
     return F3S_OK;
 }
 

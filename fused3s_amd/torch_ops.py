@@ -117,6 +117,10 @@ class TorchGraph:
         self.plan = Plan(self.bsf, self.order, H=heads, stream=s)
         if masked:
             self.plan.compile(s)
+        self.device = torch.cuda.current_device()
+        self._scheduled: Plan | None = None  # diff_attention's plan, where it is not self.plan
+        self._reversed: Plan | None = None   # the reversed edges' (prepare_backward)
+        self._workspace = {}
 
     def attention(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                   scale: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -172,6 +176,200 @@ class TorchGraph:
                 self.n, HEAD_DIM, self.heads, float(scale),
                 torch.cuda.current_stream().cuda_stream), "f3s_attention_fwd_packed")
         return out
+
+    def prepare_backward(self) -> "TorchGraph":
+        """Builds what the gradient of diff_attention reads, a compiled plan of
+        the reversed edges; the first call that needs it does so otherwise.
+        Waits for the GPU, so before a capture."""
+        if self._reversed is None:
+            if not self.masked:
+                raise ValueError("a gradient needs the masked (edge-exact) semantics")
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("call prepare_backward() before the capture")
+            with torch.cuda.device(self.device):
+                s = current_stream()
+                csr, rev = self.csr, DeviceCSR.__new__(DeviceCSR)
+                rev.n, rev.nnz = csr.n, csr.nnz
+                rev.row_ptr = DeviceArray(csr.n + 1, np.int32)
+                rev.col_idx = DeviceArray(csr.nnz, np.int32)
+                check(_lib.hip().f3s_reverse_csr(csr.row_ptr.ptr, csr.col_idx.ptr, csr.n, csr.nnz,
+                                                 rev.row_ptr.ptr, rev.col_idx.ptr, s.handle),
+                      "f3s_reverse_csr")
+                bsf = convert_device(rev, masks=True, stream=s)
+                self._diff_plan()
+                self._reversed = self._compiled(bsf, s)
+        return self
+
+    def _compiled(self, bsf: DeviceBSF, s: Stream) -> Plan:
+        """A compiled plan in the library's sequence; small graphs' teams are the
+        same in every sequence."""
+        plan = Plan(bsf, H=self.heads, stream=s, scheduled=True)
+        plan.compile(s)
+        plan.bsf = None   # the compiled lists are all that is read
+        return plan
+
+    def _diff_plan(self) -> Plan:
+        """The plan of diff_attention: self.plan, where that follows the
+        library's sequence or the windows run on teams; else one that does, made
+        by the first call.  (Waits for the GPU then, so before a capture.)"""
+        if self._scheduled is None:
+            W = self.bsf.W
+            if W * self.heads <= 1024 or W * self.heads >= 2**18:
+                self._scheduled = self.plan
+            else:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("call the operator once, or prepare_backward(), before "
+                                       "the capture")
+                self._scheduled = self._compiled(self.bsf, current_stream())
+        return self._scheduled
+
+    def _diff_workspace(self, backward: bool) -> torch.Tensor:
+        size = self._workspace.get(backward)
+        if size is None:
+            need = C.c_int64()
+            check(_lib.hip().f3s_diff_attention_workspace(
+                self._diff_plan().handle, self._reversed.handle if backward else None,
+                C.byref(need)),
+                "f3s_diff_attention_workspace")
+            size = self._workspace[backward] = need.value
+        return torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
+
+    def _check_diff(self, lam, scale, **tensors) -> None:
+        if not self.masked:
+            raise ValueError("differential attention is edge-exact: it needs masked=True")
+        if torch.cuda.current_device() != self.device:
+            raise ValueError(f"the graph is on device {self.device}, which is not the current one")
+        n, H = self.n, self.heads
+        if (lam.dtype != torch.float32 or not lam.is_cuda or lam.device.index != self.device
+                or lam.shape != (H,)):
+            raise ValueError(f"lam must be a float32 tensor of {H} weights on the graph's device")
+        dtype = None
+        for name, t in tensors.items():
+            if (t.dtype not in _DTYPES or not t.is_cuda or t.device.index != self.device
+                    or (dtype or t.dtype) != t.dtype):
+                raise ValueError(f"{name} must be a float16 or bfloat16 tensor on the graph's "
+                                 "device, all of one type")
+            dtype = t.dtype
+
+    def diff_attention(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor,
+                       scale: float = 1.0) -> torch.Tensor:
+        """Differential attention over each node's neighbours: per head two maps
+        of 64 dims, the halves of q and k, and values of 128,
+        (softmax(scale * q1.k1) - lam[h] * softmax(scale * q2.k2)) v.
+        q, k, v: float16 or bfloat16 CUDA tensors [n, H, 128], each row's heads
+        contiguous, rows at any distance of a multiple of 8 values (a slice of a
+        projection's output is taken as it is; other layouts are copied);
+        lam: float32 [H].  Returns [n, H, 128] in q's type: sums in float32,
+        rounded once; nodes without edges get 0.  Differentiable in q, k, v and
+        lam (once).  A graph serves any number of calls at once."""
+        shape = (self.n, self.heads, 2 * HEAD_DIM)
+        self._check_diff(lam, scale, q=q, k=k, v=v)
+        for name, t in (("q", q), ("k", k), ("v", v)):
+            if t.shape != shape and t.shape != (self.n, self.heads * 2 * HEAD_DIM):
+                raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                        or lam.requires_grad):
+            self.prepare_backward()
+            return _DiffAttention.apply(self, float(scale), lam, q, k, v)
+        return _diff_forward(self, float(scale), lam, *(_rows(t, self) for t in (q, k, v)))
+
+    def diff_attention_packed(self, qkv: torch.Tensor, lam: torch.Tensor,
+                              scale: float = 1.0) -> torch.Tensor:
+        """diff_attention() on the [n, 3 * H * 128] output of one projection (q,
+        k and v side by side in each row), whose gradient is then one tensor
+        too, written in place of its thirds."""
+        self._check_diff(lam, scale, qkv=qkv)
+        if qkv.shape != (self.n, 3 * self.heads * 2 * HEAD_DIM):
+            raise ValueError(f"qkv must have shape {(self.n, 3 * self.heads * 2 * HEAD_DIM)}, "
+                             f"got {tuple(qkv.shape)}")
+        if torch.is_grad_enabled() and (qkv.requires_grad or lam.requires_grad):
+            self.prepare_backward()
+            return _DiffAttention.apply(self, float(scale), lam, qkv)
+        return _diff_forward(self, float(scale), lam, *_thirds(qkv, self))
+
+
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1}   # F3S_F16, F3S_BF16
+
+
+def _rows(t: torch.Tensor, graph: TorchGraph) -> torch.Tensor:
+    """[n, width] with each row contiguous, 16-byte aligned: t itself where its
+    layout is that already."""
+    n, width = graph.n, graph.heads * 2 * HEAD_DIM
+    if t.dim() == 3 and (t.stride(2) != 1 or t.stride(1) != 2 * HEAD_DIM and graph.heads > 1):
+        t = t.contiguous()
+    if t.dim() == 3:
+        t = t.as_strided((n, width), (t.stride(0), 1))
+    if t.stride(1) != 1 or t.stride(0) % 8 or t.stride(0) < width or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _thirds(qkv: torch.Tensor, graph: TorchGraph):
+    width = graph.heads * 2 * HEAD_DIM
+    if qkv.stride(-1) != 1 or qkv.stride(0) % 8 or qkv.data_ptr() % 16 or (
+            graph.n > 1 and qkv.stride(0) < 3 * width):
+        qkv = qkv.clone(memory_format=torch.contiguous_format)
+    return tuple(qkv[:, i * width:(i + 1) * width] for i in range(3))
+
+
+def _stride(t: torch.Tensor) -> int:
+    return max(t.stride(0), t.shape[1])
+
+
+def _diff_forward(graph: TorchGraph, scale: float, lam, q, k, v, lse=None) -> torch.Tensor:
+    n, H = graph.n, graph.heads
+    out = torch.empty((n, H, 2 * HEAD_DIM), dtype=q.dtype, device=q.device)
+    if n:
+        ws = graph._diff_workspace(False)
+        lam = lam.contiguous()
+        check(_lib.hip().f3s_diff_attention_fwd(
+            graph._diff_plan().handle, q.data_ptr(), _stride(q), k.data_ptr(), _stride(k), v.data_ptr(),
+            _stride(v), lam.data_ptr(), out.data_ptr(), H * 2 * HEAD_DIM,
+            lse.data_ptr() if lse is not None else None, _DTYPES[q.dtype], n, H, scale,
+            ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
+            torch.cuda.current_stream().cuda_stream), "f3s_diff_attention_fwd")
+    return out
+
+
+class _DiffAttention(torch.autograd.Function):
+    """diff_attention and its gradient; one packed tensor or three."""
+
+    @staticmethod
+    def forward(ctx, graph, scale, lam, *tensors):
+        packed = len(tensors) == 1
+        rows = _thirds(tensors[0], graph) if packed else [_rows(t, graph) for t in tensors]
+        lse = torch.empty((graph.n, graph.heads, 2), dtype=torch.float32, device=lam.device)
+        lam = lam.contiguous()
+        out = _diff_forward(graph, scale, lam, *rows, lse=lse)
+        ctx.graph, ctx.scale, ctx.shapes = graph, scale, [t.shape for t in tensors]
+        ctx.save_for_backward(lam, lse, *tensors)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        graph, n, H = ctx.graph, ctx.graph.n, ctx.graph.heads
+        width = H * 2 * HEAD_DIM
+        lam, lse, *tensors = ctx.saved_tensors
+        packed = len(tensors) == 1
+        q, k, v = _thirds(tensors[0], graph) if packed else (_rows(t, graph) for t in tensors)
+        grads = [torch.empty(shape, dtype=q.dtype, device=q.device) for shape in ctx.shapes]
+        if packed:
+            dq, dk, dv = (grads[0][:, i * width:(i + 1) * width] for i in range(3))
+        else:
+            dq, dk, dv = (t.view(n, width) for t in grads)
+        dlam = torch.empty_like(lam)
+        do = _rows(grad, graph)
+        with torch.cuda.device(graph.device):
+            ws = graph._diff_workspace(True)
+            check(_lib.hip().f3s_diff_attention_bwd(
+                graph._diff_plan().handle, graph._reversed.handle, q.data_ptr(), _stride(q),
+                k.data_ptr(), _stride(k), v.data_ptr(), _stride(v), lam.data_ptr(), lse.data_ptr(),
+                do.data_ptr(), _stride(do), dq.data_ptr(), _stride(dq), dk.data_ptr(), _stride(dk),
+                dv.data_ptr(), _stride(dv), dlam.data_ptr(), _DTYPES[q.dtype], n, H, ctx.scale,
+                ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
+                torch.cuda.current_stream().cuda_stream), "f3s_diff_attention_bwd")
+        return None, None, dlam, *grads
 
 
 _LINEAR_FORWARD, _LINEAR = torch.nn.Linear.forward, torch.nn.functional.linear

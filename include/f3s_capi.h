@@ -46,6 +46,10 @@ typedef int32_t f3s_status;
 
 #define F3S_ABI_VERSION 1
 
+/* 16-bit types of the calls that take both. */
+#define F3S_F16 0           /* IEEE binary16 */
+#define F3S_BF16 1          /* bfloat16 */
+
 /* Semantics of f3s_attention_fwd*: tile_mask == NULL selects TILE_DENSE
  * (every column < n of every active tile is attended: the reference kernel
  * and test ground truth, tests/test_fused_3s_v2.cu:17-59); a mask selects
@@ -243,6 +247,13 @@ typedef struct f3s_plan f3s_plan;
 f3s_status f3s_plan_create(const int32_t* d_window_offsets, const int32_t* d_window_order,
                            int32_t W, int32_t H, int32_t seg_tiles, void* stream,
                            f3s_plan** plan_out);
+/* f3s_plan_create (automatic segments) whose items follow the library's
+ * schedule from 513 windows on, where no teams run, not only from 2^18
+ * window-heads: each class's windows in eight contiguous shares, one for each
+ * XCD.  For passes of longer rows, which gain more from a community-ordered
+ * graph's L2 reuse (f3s_diff_attention_fwd). */
+f3s_status f3s_plan_create_scheduled(const int32_t* d_window_offsets, int32_t W, int32_t H,
+                                     void* stream, f3s_plan** plan_out);
 f3s_status f3s_plan_destroy(f3s_plan* plan);
 /* Lists, once per graph, the columns each planned item attends under the
  * masked semantics (32 row offsets + 32 row masks per 32-column chunk), so
@@ -288,6 +299,51 @@ f3s_status f3s_attention_fwd_packed(const f3s_plan* plan, const uint16_t* QKV, v
  * `stream`. */
 f3s_status f3s_linear_f16(const uint16_t* X, const uint16_t* W, const uint16_t* bias, uint16_t* Y,
                           int64_t n, int32_t K, int32_t M, void* stream);
+
+/* The reversed edges of a CSR (no reference counterpart): entry (i, j) becomes
+ * (j, i).  d_out_row_ptr holds n + 1 entries, d_out_col_idx nnz.  The order of
+ * the entries of a row is not defined (the converter's output does not depend on
+ * it).  Columns outside [0, n) are left out, and the converter then refuses the
+ * result.  Asynchronous on `stream`; scratch from the library's cache. */
+f3s_status f3s_reverse_csr(const int32_t* d_row_ptr, const int32_t* d_col_idx, int32_t n,
+                           int64_t nnz, int32_t* d_out_row_ptr, int32_t* d_out_col_idx,
+                           void* stream);
+
+/* Differential attention over the edges of a compiled plan (no reference
+ * counterpart): per head two maps of 64 dims, q = [q1 q2], k = [k1 k2], and
+ * values of 128,
+ *   O[i] = sum_j (softmax_j(scale q1.k1) - lam[h] softmax_j(scale q2.k2)) V[j]
+ * over the edges (i, j) (masked semantics); rows without edges get 0.  H is the
+ * plan's; a head of a row is 128 contiguous values of `dtype` (F3S_F16 or
+ * F3S_BF16), heads adjacent, rows `*_stride` values apart (a multiple of 8, at
+ * least H * 128), pointers 16-byte aligned: the thirds of a packed
+ * [n][3][H][128] tensor are taken as they lie.  lam float32 [H].  lse, where
+ * not NULL, receives [n][H][2] float32 for the gradient.  Sums and softmax
+ * statistics are float32, O is rounded once.  An infinite or NaN value reaches
+ * the rows with an edge to its node only (an infinite value of V makes their
+ * sums NaN).  Deterministic.
+ * workspace: f3s_diff_attention_workspace bytes (reversed NULL), 16-byte
+ * aligned, this call's alone until it is done; nothing else is allocated or
+ * kept, so calls may overlap and be captured.  Asynchronous on `stream`. */
+f3s_status f3s_diff_attention_workspace(const f3s_plan* plan, const f3s_plan* reversed,
+                                        int64_t* bytes);
+f3s_status f3s_diff_attention_fwd(const f3s_plan* plan, const uint16_t* Q, int64_t q_stride,
+                                  const uint16_t* K, int64_t k_stride, const uint16_t* V,
+                                  int64_t v_stride, const float* lam, uint16_t* O, int64_t o_stride,
+                                  float* lse, int32_t dtype, int32_t n, int32_t H, float scale,
+                                  void* workspace, int64_t workspace_bytes, void* stream);
+/* Its gradient: dQ, dK, dV in `dtype`, dlam float32 [H], from dO and the
+ * forward call's lse.  `reversed` is a plan of the reversed edges
+ * (f3s_reverse_csr, converted) of the same n and H, compiled.  No atomics:
+ * deterministic.  F3S_EUNSUPPORTED from n * H = 2^28 on. */
+f3s_status f3s_diff_attention_bwd(const f3s_plan* plan, const f3s_plan* reversed,
+                                  const uint16_t* Q, int64_t q_stride, const uint16_t* K,
+                                  int64_t k_stride, const uint16_t* V, int64_t v_stride,
+                                  const float* lam, const float* lse, const uint16_t* dO,
+                                  int64_t do_stride, uint16_t* dQ, int64_t dq_stride, uint16_t* dK,
+                                  int64_t dk_stride, uint16_t* dV, int64_t dv_stride, float* dlam,
+                                  int32_t dtype, int32_t n, int32_t H, float scale, void* workspace,
+                                  int64_t workspace_bytes, void* stream);
 
 /* Measurement only (no reference counterpart): the device's random-gather
  * ceiling for the fused pass's access pattern.  For each of `count` columns
