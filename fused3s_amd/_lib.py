@@ -69,6 +69,11 @@ HIP_API = {
     "f3s_attention_fwd_packed": (c_i32, [c_vp, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_f32,
                                          c_vp]),
     "f3s_linear_f16": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_i64, c_i32, c_i32, c_vp]),
+    "f3s_linear_workspace": (c_i32, [c_i64, c_i64, c_i64, c_i32, c_i32, P_i64]),
+    "f3s_linear_fwd": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64,
+                               c_i32, c_i32, c_vp, c_i64, c_vp]),
+    "f3s_linear_bwd": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64,
+                               c_i64, c_i64, c_i32, c_i32, c_vp, c_i64, c_vp]),
     "f3s_reverse_csr": (c_i32, [c_vp, c_vp, c_i32, c_i64, c_vp, c_vp, c_vp]),
     "f3s_diff_attention_workspace": (c_i32, [c_vp, c_vp, P_i64]),
     "f3s_diff_attention_fwd": (c_i32, [c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp,

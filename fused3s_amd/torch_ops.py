@@ -372,6 +372,113 @@ class _DiffAttention(torch.autograd.Function):
         return None, None, dlam, *grads
 
 
+# F3S_ACT_NONE ..
+_ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+
+def _linear_workspace(n, K, M, act, backward, device):
+    need = C.c_int64()
+    check(_lib.hip().f3s_linear_workspace(n, K, M, act, backward, C.byref(need)),
+          "f3s_linear_workspace")
+    return torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+
+
+def _matrix(t: torch.Tensor) -> torch.Tensor:
+    """A matrix whose rows are contiguous and do not overlap."""
+    return t if t.stride(1) == 1 and (t.stride(0) >= t.shape[1] or t.shape[0] == 1) \
+        else t.contiguous()
+
+
+def _linear_forward(x, w, b, r, act):
+    (n, K), M = x.shape, w.shape[0]
+    y = torch.empty((n, M), dtype=x.dtype, device=x.device)
+    if n:
+        ws = _linear_workspace(n, K, M, act, 0, x.device) if n > 64 else None
+        check(_lib.hip().f3s_linear_fwd(
+            x.data_ptr(), _stride(x), w.data_ptr(), b.data_ptr() if b is not None else None,
+            r.data_ptr() if r is not None else None, _stride(r) if r is not None else 0,
+            y.data_ptr(), n, K, M, act, _DTYPES[x.dtype],
+            ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
+            torch.cuda.current_stream().cuda_stream), "f3s_linear_fwd")
+    return y
+
+
+class _Linear(torch.autograd.Function):
+    """linear()'s matrices and their gradients."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, r, act):
+        ctx.act = act
+        ctx.save_for_backward(x, w, b if act else None)
+        return _linear_forward(x, w, b, r, act)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, w, b = ctx.saved_tensors
+        (n, K), M, act = x.shape, w.shape[0], ctx.act
+        needs = ctx.needs_input_grad
+        empty = lambda wanted, *shape: (torch.empty(shape, dtype=x.dtype, device=x.device)
+                                        if wanted else None)
+        dx, dw, db = empty(needs[0], n, K), empty(needs[1], M, K), empty(needs[2], M)
+        if any(needs[:3]):
+            dy = _matrix(grad)
+            with torch.cuda.device(x.device):
+                ws = _linear_workspace(n, K, M, act, 1, x.device)
+                check(_lib.hip().f3s_linear_bwd(
+                    x.data_ptr(), _stride(x), w.data_ptr(),
+                    b.data_ptr() if b is not None else None, dy.data_ptr(), _stride(dy),
+                    *(t.data_ptr() if t is not None else None for t in (dx, dw, db)), n, K, M, act,
+                    _DTYPES[x.dtype], ws.data_ptr() if ws is not None else None,
+                    ws.numel() if ws is not None else 0, torch.cuda.current_stream().cuda_stream),
+                    "f3s_linear_bwd")
+        return dx, dw, db, grad if needs[3] else None, None
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
+           activation: str | None = None, residual: torch.Tensor | None = None) -> torch.Tensor:
+    """activation(x @ weight.T + bias) + residual in one kernel: x [..., K],
+    weight [M, K], bias [M], residual [..., M], all float16 or all bfloat16 on one
+    GPU; activation None, "relu", "gelu", "gelu_tanh" or "silu".  Sums and
+    epilogue are in float32, the result is rounded once.  Differentiable (once);
+    for the backward pass the product is computed again rather than kept."""
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"activation must be one of {list(_ACTIVATIONS)}, got {activation!r}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x [..., K] and weight [M, K] do not fit: {tuple(x.shape)}, "
+                         f"{tuple(weight.shape)}")
+    M, K = weight.shape
+    if M == 0 or K == 0:
+        raise ValueError("weight must not be empty")
+    shape = (*x.shape[:-1], M)
+    if bias is not None and bias.shape != (M,):
+        raise ValueError(f"bias must have shape {(M,)}, got {tuple(bias.shape)}")
+    if residual is not None and residual.shape != shape:
+        raise ValueError(f"residual must have shape {shape}, got {tuple(residual.shape)}")
+    for name, t in (("x", x), ("weight", weight), ("bias", bias), ("residual", residual)):
+        if t is not None and (t.dtype not in _DTYPES or t.dtype != x.dtype or not t.is_cuda
+                              or t.device != x.device):
+            raise ValueError(f"{name} must be a float16 or bfloat16 tensor on a GPU, of x's type "
+                             "and device")
+    if x.device.index != torch.cuda.current_device():
+        with torch.cuda.device(x.device):
+            return linear(x, weight, bias, activation, residual)
+    act = _ACTIVATIONS[activation]
+    x2 = _matrix(x if x.dim() == 2 else x.reshape(-1, K))
+    w = weight if weight.is_contiguous() else weight.contiguous()
+    b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
+    r = residual
+    if r is not None:
+        r = _matrix(r if r.dim() == 2 else r.reshape(-1, M))
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
+                                    or bias is not None and bias.requires_grad
+                                    or residual is not None and residual.requires_grad):
+        y = _Linear.apply(x2, w, b, r, act)
+    else:
+        y = _linear_forward(x2, w, b, r, act)
+    return y if x.dim() == 2 else y.view(shape)
+
+
 _LINEAR_FORWARD, _LINEAR = torch.nn.Linear.forward, torch.nn.functional.linear
 
 

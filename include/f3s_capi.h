@@ -300,6 +300,34 @@ f3s_status f3s_attention_fwd_packed(const f3s_plan* plan, const uint16_t* QKV, v
 f3s_status f3s_linear_f16(const uint16_t* X, const uint16_t* W, const uint16_t* bias, uint16_t* Y,
                           int64_t n, int32_t K, int32_t M, void* stream);
 
+/* A projection with its epilogue (no reference counterpart), of any size:
+ *   Y[n][M] = act(X[n][K] W[M][K]^T + bias[M]) + R[n][M]
+ * in `dtype` (F3S_F16 or F3S_BF16), sums and epilogue in float32, rounded once.
+ * bias and R may be NULL.  Rows of X and R are x_stride and r_stride values
+ * apart; W and Y are contiguous.  No alignment is needed; rows of a multiple of
+ * 16 bytes at 16-byte addresses are the fast ones.  K, M < 2^22, n < 2^36.
+ * workspace: f3s_linear_workspace bytes, 16-byte aligned, this call's alone
+ * until it is done; nothing is allocated, calls may overlap and be captured.
+ * Deterministic.  Asynchronous on `stream`. */
+#define F3S_ACT_NONE 0
+#define F3S_ACT_RELU 1
+#define F3S_ACT_GELU 2        /* z Phi(z) */
+#define F3S_ACT_GELU_TANH 3   /* its tanh approximation */
+#define F3S_ACT_SILU 4
+f3s_status f3s_linear_workspace(int64_t n, int64_t K, int64_t M, int32_t act, int32_t backward_pass,
+                                int64_t* bytes);
+f3s_status f3s_linear_fwd(const uint16_t* X, int64_t x_stride, const uint16_t* W,
+                          const uint16_t* bias, const uint16_t* R, int64_t r_stride, uint16_t* Y,
+                          int64_t n, int64_t K, int64_t M, int32_t act, int32_t dtype,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+/* Its gradient: dX[n][K], dW[M][K], db[M] (contiguous; NULL: not wanted) from
+ * dY, whose rows are dy_stride values apart (dR is dY).  With an activation z is
+ * computed again from X, W and bias: the forward call keeps nothing. */
+f3s_status f3s_linear_bwd(const uint16_t* X, int64_t x_stride, const uint16_t* W,
+                          const uint16_t* bias, const uint16_t* dY, int64_t dy_stride, uint16_t* dX,
+                          uint16_t* dW, uint16_t* db, int64_t n, int64_t K, int64_t M, int32_t act,
+                          int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* The reversed edges of a CSR (no reference counterpart): entry (i, j) becomes
  * (j, i).  d_out_row_ptr holds n + 1 entries, d_out_col_idx nnz.  The order of
  * the entries of a row is not defined (the converter's output does not depend on
