@@ -6,14 +6,19 @@ graph's edges, and an output projection.  Here torch supplies the device
 memory and the stream; the attention is the HIP library's planned pass
 (f3s_attention_fwd_planned), called on torch's current stream with the
 tensors' device pointers, and the layer's projections are its f3s_linear_f16
-(torch.nn.Linear's own product where that kernel is not the better one).  There is no CPU fallback and no autograd: the
-fused pass is forward-only, so calling it on tensors that require grad
-raises.
+(torch.nn.Linear's own product where that kernel is not the better one).  There is no CPU fallback, and
+that pass is forward-only: calling it on tensors that require grad raises.
+Differential attention (two softmax maps per head and their difference) and
+linear(), a projection with bias, activation and residual, have gradients.
 
     graph = TorchGraph(row_ptr, col_idx, heads=4)      # convert + plan + compile once
     o = graph.attention(q, k, v)                       # q/k/v [n, H, 64] fp16 -> fp32
     layer = GraphTransformerLayer(in_dim, heads=4).cuda().half()
     y = layer(x, graph)                                # x [n, in_dim] fp16
+
+    o = graph.diff_attention(q, k, v, lam)             # q/k/v [n, H, 128] fp16 or bf16, autograd
+    y = linear(x, weight, bias, "gelu", residual)      # autograd
+    layer = DiffGraphTransformerLayer(in_dim, heads=4, ffn_dim=512).cuda().bfloat16()
 
 The drop-in launch is also a registered torch operator, on the block-sparse
 form held in torch tensors (no plan, no state between calls):
@@ -583,6 +588,81 @@ class GraphTransformerLayer(torch.nn.Module):
             q, k, v = (qkv[:, i].contiguous() for i in range(3))
             o = graph.attention(q, k, v, scale=self.scale)
         return _project(self.proj, o.view(n, self.heads * HEAD_DIM).to(dtype), watched)
+
+
+_TORCH_ACTIVATIONS = {
+    None: lambda z: z, "relu": torch.nn.functional.relu, "gelu": torch.nn.functional.gelu,
+    "gelu_tanh": lambda z: torch.nn.functional.gelu(z, approximate="tanh"),
+    "silu": torch.nn.functional.silu}
+
+
+def _dense(m: torch.nn.Module, x: torch.Tensor, watched: bool, activation: str | None = None,
+           residual: torch.Tensor | None = None) -> torch.Tensor:
+    """activation(m(x)) + residual: linear() where m is a plain Linear of a type
+    it takes and nothing watches the call, else torch's own operations."""
+    if (not watched and _is_plain_linear(m) and type(x) is torch.Tensor and x.is_cuda
+            and x.dtype in _DTYPES and m.weight.dtype == x.dtype and m.weight.device == x.device
+            and (residual is None or residual.dtype == x.dtype)):
+        return linear(x, m.weight, m.bias, activation, residual)
+    y = _TORCH_ACTIVATIONS[activation](m(x))
+    return y if residual is None else y + residual
+
+
+class DiffGraphTransformerLayer(torch.nn.Module):
+    """Differential attention over a graph's edges with its projections, and
+    optionally a feed-forward part; trainable.
+
+        o_h = rms_norm(diff_attention(x W_qkv)_h) * (1 - lambda_init)
+        y = concat(o) W_o + x                      (residual=True)
+        y = activation(y W_up) W_down + y          (ffn_dim given)
+
+    A head's weight is exp(lambda_q1 . lambda_k1) - exp(lambda_q2 . lambda_k2) +
+    lambda_init, from four learned vectors.  Two maps of 64 dims and values of
+    128 per head, so `heads` heads project to heads * 128 features; the graph has
+    to be made for `heads` heads.  Computes in the module's type (float16 or
+    bfloat16; a float32 module's attention runs in float16)."""
+
+    def __init__(self, in_dim: int, heads: int = 1, out_dim: int | None = None, bias: bool = True,
+                 lambda_init: float = 0.8, residual: bool = True, ffn_dim: int | None = None,
+                 activation: str = "gelu", eps: float = 1e-5):
+        super().__init__()
+        out_dim = out_dim or in_dim
+        if residual and out_dim != in_dim:
+            raise ValueError("a residual needs out_dim == in_dim")
+        if activation not in _ACTIVATIONS:
+            raise ValueError(f"activation must be one of {list(_ACTIVATIONS)}")
+        self.heads, self.lambda_init, self.residual = heads, float(lambda_init), residual
+        self.activation, self.eps, self.scale = activation, eps, HEAD_DIM ** -0.5
+        self.qkv = torch.nn.Linear(in_dim, 3 * heads * 2 * HEAD_DIM, bias=bias)
+        self.proj = torch.nn.Linear(heads * 2 * HEAD_DIM, out_dim, bias=bias)
+        self.norm = torch.nn.Parameter(torch.ones(2 * HEAD_DIM))
+        for name in ("lambda_q1", "lambda_k1", "lambda_q2", "lambda_k2"):
+            setattr(self, name, torch.nn.Parameter(0.1 * torch.randn(heads, HEAD_DIM)))
+        self.up = torch.nn.Linear(out_dim, ffn_dim, bias=bias) if ffn_dim else None
+        self.down = torch.nn.Linear(ffn_dim, out_dim, bias=bias) if ffn_dim else None
+
+    def head_weights(self) -> torch.Tensor:
+        """lam, float32 [heads]."""
+        q1, k1, q2, k2 = (t.float() for t in (self.lambda_q1, self.lambda_k1, self.lambda_q2,
+                                              self.lambda_k2))
+        return torch.exp((q1 * k1).sum(-1)) - torch.exp((q2 * k2).sum(-1)) + self.lambda_init
+
+    def forward(self, x: torch.Tensor, graph: TorchGraph) -> torch.Tensor:
+        if graph.heads != self.heads:
+            raise ValueError("graph was planned for a different head count")
+        watched = _watched()
+        qkv = _dense(self.qkv, x, watched)
+        if qkv.dtype not in _DTYPES:
+            qkv = qkv.to(torch.float16)
+        o = graph.diff_attention_packed(qkv, self.head_weights(), self.scale)
+        dtype = self.proj.weight.dtype
+        o = torch.nn.functional.rms_norm(o.to(dtype), (2 * HEAD_DIM,),
+                                         self.norm * (1.0 - self.lambda_init), self.eps)
+        y = _dense(self.proj, o.view(x.shape[0], self.heads * 2 * HEAD_DIM), watched, None,
+                   x if self.residual else None)
+        if self.up is not None:
+            y = _dense(self.down, _dense(self.up, y, watched, self.activation), watched, None, y)
+        return y
 
 
 # ------------------------------------------------------------------ operator
