@@ -31,7 +31,12 @@
 // window that have no edge to it (0 x inf).  So a window whose sums are not
 // finite at the end is done twice more: once to mark the sums that have such a
 // value on an edge of theirs, which become NaN, and once without those values.
+// Large graphs leave that to a second launch, which finds nothing as a rule: in
+// the pass itself its registers would be taken from the loads in flight.
 #include <algorithm>
+#include <cfloat>
+#include <cmath>
+#include <cstddef>
 
 #include "attn_plan.hpp"
 #include "half_types.hpp"
@@ -47,6 +52,14 @@ constexpr int kHeadBytes = kHeadD * 2;
 // transposing reads take, then lie in distinct banks without padding.
 constexpr int kRowHalves = kHeadD;
 __device__ __forceinline__ int swizzle(int row) { return ((row & 7) << 1) | ((row >> 3) & 1); }
+
+// The lane again, for the compiler a new value: what is derived from it is then made
+// where it is used and not held in registers through the chunk loop.
+__device__ __forceinline__ int anew(int lane)
+{
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
 
 enum DiffPass : int { kDiffForward = 0, kDiffRows = 1, kDiffColumns = 2 };
 
@@ -75,8 +88,14 @@ struct DiffParams {
     int64_t num_items, num_split;
     int32_t W, n, H;
     int32_t xcd_contiguous;
-    int32_t refs_are_nodes; // column lists of node indices, else of node * H * 128
-    uint32_t heads_magic;   // ceil(2^31 / H): (x * magic) >> 31 = x / H for x < 2^25
+    // the lists' references: node indices, or node * H * 128 (below kNoRow);
+    // node = ((ref >> shift) * magic) >> 31, magic 2^31 or ceil(2^31 / H), which is
+    // exact below 2^25
+    uint32_t ref_shift, ref_magic, no_ref;
+    uint32_t* queue;        // next unit of each XCD's share, kQueueStride apart; NULL: a unit
+                            // per wave
+    uint32_t* odd;          // [items][H]: sums that are not finite (kDiffMain writes,
+                            // kDiffRepair reads)
     float scale, scale_log2;
 };
 
@@ -129,6 +148,11 @@ __device__ __forceinline__ void absorb(DiffState& s, const float* src, int lane)
 {
     const f4 xy = *reinterpret_cast<const f4*>(&src[(16 * kWave + lane) * 4]);
     const f4 z = *reinterpret_cast<const f4*>(&src[(17 * kWave + lane) * 4]);
+    f4 a[16];   // (all on their way before the first is waited for)
+#pragma unroll
+    for (int t = 0; t < 16; ++t)
+        a[t] = *reinterpret_cast<const f4*>(&src[(t * kWave + lane) * 4]);
+    __builtin_amdgcn_sched_barrier(0);
     float theirs[2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -146,8 +170,7 @@ __device__ __forceinline__ void absorb(DiffState& s, const float* src, int lane)
 #pragma unroll
     for (int t = 0; t < 16; ++t) {
         const int c = t / Scaled<PASS>::count;
-        const f4 a = *reinterpret_cast<const f4*>(&src[(t * kWave + lane) * 4]);
-        s.acc[t] += c < 2 ? a * theirs[c] : a;
+        s.acc[t] += c < 2 ? a[t] * theirs[c] : a[t];
     }
 }
 
@@ -157,6 +180,7 @@ struct DiffRecord {
     uint32_t at1[kChunk], at2[kChunk], rm[kChunk], st[kChunk];
 };
 constexpr int kBlockRecs = 2;   // records read, converted and handed out together
+static_assert(kBlockRecs * 2 * kChunk == 2 * kWave, "two words per lane");
 struct __align__(256) DiffLds {
     _Float16 x1[kChunk * kRowHalves];
     _Float16 x2[kChunk * kRowHalves];
@@ -245,19 +269,32 @@ __device__ __forceinline__ typename Half<T>::v8 transposed(const Places& p, uint
                               s8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
 }
 
-// acc[i][t] += sum over the chunk's slots of w[i] (the lane's slots of row r)
-// times the 16 dims of tile t0 + t, four tiles.
-template <typename T, int N>
-__device__ __forceinline__ void mix(const Places& p, uint32_t stage, int t0,
-                                    const typename Half<T>::v8 (&w)[N], f4* const (&acc)[N])
-{
+// acc[t] += sum over the chunk's slots of w (the lane's slots of row r) times the
+// 16 dims of tile t0 + t, N tiles x.  (Products of one sum are N apart: they need
+// not wait for each other.)
+template <typename T, int N = 4>
+struct Tiles {
+    typename Half<T>::v8 x[N];
+    __device__ __forceinline__ Tiles(const Places& p, uint32_t stage, int t0)
+    {
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const typename Half<T>::v8 x = transposed<T>(p, stage, t0 + t);
-#pragma unroll
-        for (int i = 0; i < N; ++i) acc[i][t] = Half<T>::mfma(x, w[i], acc[i][t]);
+        for (int t = 0; t < N; ++t) x[t] = transposed<T>(p, stage, t0 + t);
     }
-}
+    __device__ __forceinline__ void mix(const typename Half<T>::v8& hi,
+                                        const typename Half<T>::v8& lo, f4* acc) const
+    {
+#pragma unroll
+        for (int t = 0; t < N; ++t) acc[t] = Half<T>::mfma(x[t], hi, acc[t]);
+#pragma unroll
+        for (int t = 0; t < N; ++t) acc[t] = Half<T>::mfma(x[t], lo, acc[t]);
+    }
+    __device__ __forceinline__ void mix(const float (&w)[8], f4* acc) const
+    {
+        typename Half<T>::v8 hi, lo;
+        split8<T>(w, hi, lo);
+        mix(hi, lo, acc);
+    }
+};
 
 // 16 rows of a stage times the window's rows, dims 32 (f0 + f) .., NF of them.
 template <typename T, int NF>
@@ -271,10 +308,11 @@ __device__ __forceinline__ f4 products(const Places& p, uint32_t stage, int f0,
     return s;
 }
 
-// A staged chunk's values: MARK: 1 where infinite or NaN, else 0; CLEAN: 0 there.
+// A staged chunk's values, to stage `to`: MARK: 1 where infinite or NaN, else 0;
+// CLEAN: 0 there.
 enum Sweep : int { kSweepPlain = 0, kSweepMark = 1, kSweepClean = 2 };
 template <typename T>
-__device__ __forceinline__ void replace_odd(const Places& p, uint32_t stage, int sweep)
+__device__ __forceinline__ void replace_odd(const Places& p, uint32_t stage, uint32_t to, int sweep)
 {
     typedef typename Half<T>::v8 v8;
     wave_lds_order();   // its readers so far are done
@@ -288,48 +326,69 @@ __device__ __forceinline__ void replace_odd(const Places& p, uint32_t stage, int
             const bool odd = !(f - f == 0.f);
             x[k] = sweep == kSweepMark ? (T)(odd ? 1.f : 0.f) : odd ? (T)0.f : x[k];
         }
-        lds_write(at, x);
+        lds_write(at - stage + to, x);
     }
     wave_lds_order();
 }
 
+// Which of the lane's eight slots row r attends: all bits or none.
+typedef uint32_t Attends[8];
+__device__ __forceinline__ float where(uint32_t on, float x, float other)
+{
+    return __uint_as_float((__float_as_uint(x) & on) | (__float_as_uint(other) & ~on));
+}
+__device__ __forceinline__ float where(uint32_t on, float x)
+{
+    return __uint_as_float(__float_as_uint(x) & on);
+}
+
+// From a record's masks at `masks`, anew wherever they are used: two LDS reads,
+// where eight registers would be held.
+__device__ __forceinline__ void attends(uint32_t masks, int lane, Attends& on)
+{
+    const int l = anew(lane), r = l & 15, rbit = (r & 1) ? 16 + (r >> 1) : (r >> 1);
+    const uint32_t at = masks + 16 * (l >> 4);   // slots 4 g .. and 16 + 4 g ..
+    const u4 a = lds_read<u4>(at), b = lds_read<u4>(at + 64);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        on[j] = (uint32_t)__builtin_amdgcn_sbfe((int)(j < 4 ? a[j & 3] : b[j & 3]), rbit, 1);
+}
+
 template <int N>
-__device__ __forceinline__ void edge_weights(float (&w)[N][8], uint32_t valid)
+__device__ __forceinline__ void edge_weights(float (&w)[N][8], const Attends& on)
 {
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[i][j] = (valid >> j) & 1u ? 1.f : 0.f;
+        for (int j = 0; j < 8; ++j) w[i][j] = where(on[j], 1.f);
 }
 
-// Running maximum of one map (log2): moved when a chunk's exceeds it by more
-// than kLazy.  p[j] = 2^(x - m), 0 where not attended; l is the lane's share.
-__device__ __forceinline__ void map_update(DiffState& st, int c, const f4 s0, const f4 s1,
-                                           uint32_t valid, float scale_log2, float (&p)[8])
+// One map's softmax step (log2): x = s c, c > 0; the running maximum is moved when
+// a chunk's exceeds it by more than kLazy.  p[j] = 2^(x - m), 0 where not attended;
+// y is the lane's share of l.
+__device__ __forceinline__ void map_update(DiffState& st, int m, const f4 s0, const f4 s1,
+                                           const Attends& on, float c, float (&p)[8])
 {
-    float x[8];
+    float s[8];
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-        x[v] = ((valid >> v) & 1u) ? s0[v] * scale_log2 : -INFINITY;
-        x[4 + v] = ((valid >> (4 + v)) & 1u) ? s1[v] * scale_log2 : -INFINITY;
-    }
-    float cm = x[0];
+    for (int j = 0; j < 8; ++j) s[j] = where(on[j], j < 4 ? s0[j & 3] : s1[j & 3], -INFINITY);
+    float top = s[0];
 #pragma unroll
-    for (int j = 1; j < 8; ++j) cm = __builtin_fmaxf(cm, x[j]);
-    cm = row_max4(cm);
-    if (__ballot(cm > st.x[c] + kLazy)) {
-        if (cm > st.x[c] + kLazy) {
-            const float corr = fast_exp2(st.x[c] - cm);
-            st.y[c] *= corr;
-            rescale<kDiffForward>(st, c, corr);
-            st.x[c] = cm;
+    for (int j = 1; j < 8; ++j) top = __builtin_fmaxf(top, s[j]);
+    top = row_max4(top) * c;
+    if (__ballot(top > st.x[m] + kLazy)) {
+        if (top > st.x[m] + kLazy) {
+            const float corr = fast_exp2(st.x[m] - top);
+            st.y[m] *= corr;
+            rescale<kDiffForward>(st, m, corr);
+            st.x[m] = top;
         }
     }
-    const float mu = st.x[c] == -INFINITY ? 0.f : st.x[c];
+    const float mu = st.x[m] == -INFINITY ? 0.f : st.x[m];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        p[j] = fast_exp2(x[j] - mu);
-        st.y[c] += p[j];
+        p[j] = fast_exp2(__builtin_fmaf(s[j], c, -mu));
+        st.y[m] += p[j];
     }
 }
 
@@ -394,12 +453,12 @@ __device__ __forceinline__ float over_groups(float x)
 // A window's results from its sums.  `stage`: 2 x 16 rows.
 template <typename T, int PASS>
 __device__ __forceinline__ void diff_finish(const DiffParams& p, DiffState& st, _Float16* stage,
-                                            int32_t w, int h, int lane)
+                                            int32_t w, int h, float lam, int lane)
 {
+    lane = anew(lane);
     const int g = lane >> 4, r = lane & 15;
     const int32_t row = w * 16 + r;
     const uint32_t head_off = (uint32_t)h * kHeadBytes;
-    const float lam = p.lam[h];
     if constexpr (PASS == kDiffForward) {
         const float l1 = over_groups(st.y[0]), l2 = over_groups(st.y[1]);
         const bool some = l1 != 0.f;   // (a row of NaN is some)
@@ -445,312 +504,487 @@ __device__ __forceinline__ void diff_finish(const DiffParams& p, DiffState& st, 
     }
 }
 
-template <typename T, int PASS, bool WIDE, int WPG, bool TEAM>
-__global__ void __launch_bounds__(kWave * WPG) __attribute__((amdgpu_waves_per_eu(2)))
+constexpr int kDiffWaves = 4;   // per workgroup
+static_assert(kDiffWaves == kTeamSmall, "a team fills its workgroup");
+
+constexpr int kQueueStride = 64;   // words: a counter per cache line and more
+
+// kDiffMain: a window (or segment) per wave, windows one after another; kDiffTeam:
+// four waves share a window (small graphs); kDiffRepair: the windows that kDiffMain
+// marked in p.odd.
+enum DiffMode : int { kDiffMain = 0, kDiffTeam = 1, kDiffRepair = 2 };
+
+// A wave's work: one item and head.  there: such an item is; w < 0: without a
+// window; end: past the last one.
+struct Unit {
+    uint32_t item;
+    int32_t w, slot, h, cb, ce;
+    float lam;
+    bool there, end;
+};
+
+__device__ __forceinline__ float uniform(float x)
+{
+    return __uint_as_float(__builtin_amdgcn_readfirstlane((int)__float_as_uint(x)));
+}
+
+template <typename V>
+__device__ __forceinline__ V scalar_load(const V* at)
+{
+    typedef const __attribute__((address_space(4))) V* Constant;
+    return *(Constant)(uintptr_t)at;
+}
+
+// Large graphs' waves take unit after unit from a queue, their chunks one stream:
+// the records, own rows and first chunk of a unit are loaded while the one before
+// it is still being computed.  (A window has some 7 to 20 chunks; a wave of its
+// own for each met three memory latencies before its first.  500,000 nodes, 6.5 M
+// edges, microseconds, a wave per window -> queue: forward 452 -> 398, rows 774 ->
+// 427, columns 626 -> 514; 100,000 nodes of communities, 4.1 M edges, two heads,
+// bfloat16: 382 -> 323, 432 -> 399, 471 -> 439.  Part of it is that nothing is
+// spilled any more: a reload in the chunk loop waits for every gather in flight.)
+template <typename T, int PASS, bool WIDE, int MODE>
+__global__ void __launch_bounds__(kWave * kDiffWaves) __attribute__((amdgpu_waves_per_eu(2)))
 diff_kernel(const DiffParams p)
 {
     typedef typename Half<T>::v8 v8;
-    static_assert(!TEAM || WPG == kTeamSmall, "a team fills its workgroup");
-    __shared__ DiffLds lds_all[WPG];
-    const int wave = threadIdx.x / kWave;
+    __shared__ DiffLds lds_all[kDiffWaves];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int lane = threadIdx.x % kWave;
     const int g = lane >> 4, r = lane & 15;
     DiffLds& L = lds_all[wave];
-    const int H = p.H;
-
-    // wave -> (item, head).  A scheduled plan's items are eight interleaved shares,
-    // share x for XCD x, and the dispatcher deals workgroups to the XCDs in turn:
-    // workgroup b takes items of share b % 8, the heads of an item adjacent.
-    int64_t item_idx;
-    int h;
-    if constexpr (TEAM) {
-        const uint32_t gb = (uint32_t)logical_block(p.xcd_contiguous);
-        item_idx = (int64_t)(gb / (uint32_t)H) * WPG + wave;
-        h = (int)(gb % (uint32_t)H);
-    } else {
-        const uint32_t b = (uint32_t)logical_block(p.xcd_contiguous);
-        const uint32_t at = b / kXcds * WPG + wave;
-        item_idx = (int64_t)(at / (uint32_t)H) * kXcds + b % kXcds;
-        if (p.xcd_contiguous) item_idx = (int64_t)((b * WPG + wave) / (uint32_t)H);
-        h = (int)((p.xcd_contiguous ? b * WPG + wave : at) % (uint32_t)H);
-    }
-    if (item_idx >= p.num_items) return;   // (a team's four are there or not together)
-    const Item it = p.items[item_idx];
-    const int32_t w = it.w;
-    if (w < 0 || w >= p.W) return;
+    const uint32_t H = (uint32_t)p.H;
     const int32_t n = p.n;
-    const uint32_t head_off = (uint32_t)h * kHeadBytes;
-    const float lam = p.lam[h];
 
     const __amdgpu_buffer_rsrc_t r1 = make_rsrc(p.x1.ptr, p.x1.bytes);
     const __amdgpu_buffer_rsrc_t r2 = make_rsrc(p.x2.ptr, p.x2.bytes);
     const __amdgpu_buffer_rsrc_t rst = make_rsrc(p.stats, p.stats_bytes);
 
-    // ---- the window's own rows, in operand order: dims 32 f + 8 g .. of row r ----
-    const int32_t row = w * 16 + r;
-    auto own_load = [&](const DiffRows& x, v8 (&f)[4]) __attribute__((always_inline)) {
+    // Unit `at` of share x.  A scheduled plan's items are eight interleaved shares,
+    // share x for XCD x, and the dispatcher deals workgroups to the XCDs in turn:
+    // workgroup b takes items of share b % 8, the heads of an item one after another.
+    // A natural-order plan's shares are contiguous instead.
+    const uint32_t xcd = blockIdx.x % kXcds;
+    const uint32_t share = (uint32_t)((p.num_items + kXcds - 1) / kXcds);
+    // By scalar loads (the lists are constant; a wave's vector registers are all in
+    // use).  They are waited for with the next LDS access, so units are asked for
+    // where a wave waits for memory anyway.
+    auto unit = [&](uint32_t item, uint32_t h, bool there) __attribute__((always_inline)) -> Unit {
+        there = there && item < (uint32_t)p.num_items;
+        const uint32_t i = there ? item : 0;
+        const u4 it = scalar_load(reinterpret_cast<const u4*>(p.items + i));
+        Unit u;
+        u.item = i;
+        u.there = there;
+        u.w = there && (int32_t)it[0] < p.W ? (int32_t)it[0] : -1;
+        u.slot = (int32_t)it[3];
+        u.h = (int32_t)h;
+        u.cb = scalar_load(p.chunk_base + i);
+        u.ce = u.w < 0 ? u.cb : scalar_load(p.chunk_base + i + 1);
+        u.lam = scalar_load(p.lam + h);
+        u.end = false;
+        return u;
+    };
+    auto of_share = [&](uint32_t at) __attribute__((always_inline)) -> Unit {
+        const uint32_t i = at / H;
+        Unit u = unit(p.xcd_contiguous ? xcd * share + i : i * kXcds + xcd, at % H, i < share);
+        u.end = i >= share;
+        return u;
+    };
+    // The queue's next unit, asked for one unit ahead (one lane's atomic; every
+    // wave ends once its unit is past the share, which the counter only moves to).
+    auto ticket = [&]() __attribute__((always_inline)) -> uint32_t {
+        uint32_t t = 0;
+        if (p.queue && lane == 0) t = atomicAdd(p.queue + xcd * kQueueStride, 1u);
+        return t;
+    };
+    auto redeem = [&](uint32_t t) __attribute__((always_inline)) -> Unit {
+        return of_share(p.queue ? (uint32_t)__builtin_amdgcn_readfirstlane((int)t) : share * H);
+    };
+
+    // ---- the window's own rows, in operand order: dims 32 f + 8 g .. of row r
+    // (rows past the last are not stored) ----
+    auto own_load = [&](const DiffRows& x, const Unit& u, v8 (&f)[4]) __attribute__((always_inline)) {
+        const int l = anew(lane);
+        const int32_t row = min(max(u.w, 0) * 16 + (l & 15), n - 1);
+        const char* src = x.ptr + row * x.stride + (uint32_t)u.h * kHeadBytes + 16 * (l >> 4);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            f[i] = v8{};
-            if (row < n)
-                f[i] = *reinterpret_cast<const v8*>(x.ptr + row * x.stride + head_off + 64 * i + 16 * g);
-        }
+        for (int i = 0; i < 4; ++i) f[i] = *reinterpret_cast<const v8*>(src + 64 * i);
+    };
+    auto lse_load = [&](const Unit& u) __attribute__((always_inline)) -> float2 {
+        const int32_t row = min(max(u.w, 0) * 16 + (anew(lane) & 15), n - 1);
+        return *reinterpret_cast<const float2*>(p.lse + ((int64_t)row * H + u.h) * 2);
     };
     v8 o1[4], o2[4];
-    own_load(p.own1, o1);
-    if constexpr (PASS != kDiffForward) own_load(p.own2, o2);
-    if constexpr (PASS == kDiffRows) {
-        // The matrix cores' sums are rounded towards one side, by some 2^-30 of g:
-        // nothing, but for dlam, where it adds up over all rows (500,000 of them:
-        // 1.4e-5 of it).  Odd rows take -do, and their sums of p g are negated at
-        // the end, so that it cancels.
-        if (r & 1) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o2[i] = -o2[i];
-        }
-    }
-    float lse1 = 0.f, lse2 = 0.f;
-    if constexpr (PASS == kDiffRows) {
-        if (row < n) {
-            const float2 l = *reinterpret_cast<const float2*>(p.lse + ((int64_t)row * H + h) * 2);
-            lse1 = l.x;
-            lse2 = l.y;
-            // (the columns' pass finds them beside D)
-            if (g == 0 && (!TEAM || wave == 0))
-                *reinterpret_cast<float2*>(p.stats + ((int64_t)row * H + h) * 4) = l;
-        }
-    }
+    float2 lse = make_float2(0.f, 0.f);
 
-    const int64_t cb = p.chunk_base[item_idx], ce = p.chunk_base[item_idx + 1];
-    const uint32_t extra = head_off + 16 * r;   // rows are read 16 lanes each, four at a time
     Places at = places(L.x1, lane);
-    const int rbit = (r & 1) ? 16 + (r >> 1) : (r >> 1);
-    const u4* __restrict__ recs = reinterpret_cast<const u4*>(p.columns);
-    // Two records of 32 references and 32 masks: lane l < 32 holds words 4 l .. 4 l + 3
-    // (the lists end in four spare records, so a block is read whole).
-    auto fetch = [&](int64_t c) __attribute__((always_inline)) -> u4 {
-        return c < ce && lane < 16 * kBlockRecs ? recs[c * 16 + lane] : u4{0u, 0u, 0u, 0u};
+    const uint32_t records = (uint32_t)__builtin_amdgcn_readfirstlane(
+        (int)(uint32_t)(uintptr_t)(LdsPtr)&L.rec[0]);
+    const u2* __restrict__ recs = reinterpret_cast<const u2*>(p.columns);
+    // Two records of 32 references and 32 masks, two words per lane (the lists end in
+    // four spare records, so a block is read whole).  They go to slots `to` and
+    // `to` + 1 of four, `to` 0 or 2.
+    auto fetch = [&](int32_t c) __attribute__((always_inline)) -> u2 {
+        return recs[(int64_t)c * 32 + anew(lane)];
     };
-    auto hand_out = [&](int64_t c, u4 blk) __attribute__((always_inline)) {
-        if (lane < 16 * kBlockRecs) {
-            DiffRecord& rec = L.rec[(c - cb + (lane >> 4)) % (2 * kBlockRecs)];
-            const int at = 4 * (lane & 7);
-            if (lane & 8) {
-                *reinterpret_cast<u4*>(&rec.rm[at]) = blk;
-            } else {
-                u4 a, b, s;
+    auto hand_out = [&](int32_t to, uint32_t h, u2 blk) __attribute__((always_inline)) {
+        const int l = anew(lane);
+        DiffRecord& rec = L.rec[to + (l >> 5)];
+        const int pos = 2 * (l & 15);
+        if (l & 16) {
+            *reinterpret_cast<u2*>(&rec.rm[pos]) = blk;
+        } else {
+            u2 a, b, s;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t ref = blk[i];
-                    const bool none = p.refs_are_nodes ? ref == kNoIdx : ref >= kNoRow;
-                    const uint32_t node =
-                        p.refs_are_nodes ? ref
-                                         : (uint32_t)(((uint64_t)(ref >> 7) * p.heads_magic) >> 31);
-                    if constexpr (WIDE) {
-                        a[i] = none ? kNoIdx : node;
-                    } else {
-                        a[i] = none ? kNoRow : node * (uint32_t)p.x1.stride;
-                        b[i] = none ? kNoRow : node * (uint32_t)p.x2.stride;
-                    }
-                    s[i] = none ? kNoRow : (node * H + h) * 16u;
+            for (int i = 0; i < 2; ++i) {
+                const bool none = blk[i] >= p.no_ref;
+                const uint32_t node =
+                    (uint32_t)(((uint64_t)(blk[i] >> p.ref_shift) * p.ref_magic) >> 31);
+                if constexpr (WIDE) {
+                    a[i] = none ? kNoIdx : node;
+                } else {
+                    a[i] = none ? kNoRow : node * (uint32_t)p.x1.stride;
+                    b[i] = none ? kNoRow : node * (uint32_t)p.x2.stride;
                 }
-                *reinterpret_cast<u4*>(&rec.at1[at]) = a;
-                if constexpr (!WIDE) *reinterpret_cast<u4*>(&rec.at2[at]) = b;
-                if constexpr (PASS == kDiffColumns) *reinterpret_cast<u4*>(&rec.st[at]) = s;
+                s[i] = none ? kNoRow : (node * H + h) * 16u;
             }
+            *reinterpret_cast<u2*>(&rec.at1[pos]) = a;
+            if constexpr (!WIDE) *reinterpret_cast<u2*>(&rec.at2[pos]) = b;
+            if constexpr (PASS == kDiffColumns) *reinterpret_cast<u2*>(&rec.st[pos]) = s;
+        }
+    };
+
+    v8 a[8], b[8];
+    f2 stat = {0.f, 0.f};   // (columns) half of slot lane / 2's
+    // the rows of the record in slot `rec`: 16 lanes each, four at a time
+    auto load1 = [&](int32_t slot, uint32_t h) __attribute__((always_inline)) {
+        // (the forward pass has the registers)
+        const int l = PASS == kDiffForward ? lane : anew(lane), g = l >> 4, r = l & 15;
+        const uint32_t extra = h * kHeadBytes + 16 * r;
+        const DiffRecord& rec = L.rec[slot];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a[i] = diff_load<T, WIDE>(r1, p.x1, rec.at1[4 * i + g], extra);
+    };
+    auto load2 = [&](int32_t slot, uint32_t h) __attribute__((always_inline)) {
+        // (the forward pass has the registers)
+        const int l = PASS == kDiffForward ? lane : anew(lane), g = l >> 4, r = l & 15;
+        const uint32_t extra = h * kHeadBytes + 16 * r;
+        const DiffRecord& rec = L.rec[slot];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            b[i] = diff_load<T, WIDE>(r2, p.x2, WIDE ? rec.at1[4 * i + g] : rec.at2[4 * i + g], extra);
+        if constexpr (PASS == kDiffColumns) {
+            const int l = anew(lane);
+            stat = __builtin_bit_cast(
+                f2, __builtin_amdgcn_raw_buffer_load_b64(rst, rec.st[l >> 1] + 8 * (l & 1), 0, 0));
         }
     };
 
     DiffState st;
-    uint64_t odd_sums = 0;   // bit 4 t + v: acc[t][v] has an odd value on an edge
-    int sweep = kSweepPlain;
-    for (;;) {
-        clear(st);
-        if (PASS != kDiffForward && !Half<T>::kRange) st.x[0] = st.x[1] = 0.f;
-
-        v8 a[8], b[8];
-        f4 stat = {0.f, 0.f, 0.f, 0.f};
-        u4 blk = fetch(cb);
-        wave_lds_order();
-        hand_out(cb, blk);
-        wave_lds_order();
-        blk = fetch(cb + kBlockRecs);
-        auto load1 = [&](int64_t c) __attribute__((always_inline)) {
-            const DiffRecord& rec = L.rec[(c - cb) % (2 * kBlockRecs)];
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                a[i] = diff_load<T, WIDE>(r1, p.x1, rec.at1[4 * i + g], extra);
-        };
-        auto load2 = [&](int64_t c) __attribute__((always_inline)) {
-            const DiffRecord& rec = L.rec[(c - cb) % (2 * kBlockRecs)];
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                b[i] = diff_load<T, WIDE>(r2, p.x2, WIDE ? rec.at1[4 * i + g] : rec.at2[4 * i + g],
-                                          extra);
-            if constexpr (PASS == kDiffColumns) {
-                const uint32_t at = lane < kChunk ? rec.st[lane] : kNoRow;
-                stat = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(rst, at, 0, 0));
-            }
-        };
-        if (cb < ce) {
-            load1(cb);
-            load2(cb);
+    Unit u, next;
+    uint32_t tick = 0;
+    uint64_t flagged = 0;     // (repair) units [base, base + 64) that are left
+    uint32_t base = 0;
+    if constexpr (MODE == kDiffMain) {
+        if (p.queue) {
+            tick = ticket();
+            const uint32_t second = ticket();
+            u = redeem(tick);
+            tick = second;
+        } else {
+            u = of_share(blockIdx.x / kXcds * kDiffWaves + wave);
         }
-        for (int64_t c = cb; c < ce; ++c) {
-            if ((c - cb) % kBlockRecs == 0) {
-                // the next block's records, so that the next chunk's are there
-                hand_out(c + kBlockRecs, blk);
-                blk = fetch(c + 2 * kBlockRecs);
+    } else if constexpr (MODE == kDiffTeam) {
+        const uint32_t gb = (uint32_t)logical_block(p.xcd_contiguous);
+        u = unit(gb / H * kDiffWaves + wave, gb % H, true);
+    } else {
+        base = (blockIdx.x * kDiffWaves + wave) * kWave;
+        u = unit(0, 0, false);
+    }
+    next = u;
+    next.ce = next.cb;
+    bool warm = false;        // u's own rows, first chunk and first records are on their way
+    u2 blk = {0u, 0u};
+    int32_t slot = 0;         // of the current chunk's record
+    for (;;) {
+        if constexpr (MODE == kDiffMain) {
+            if (u.end) break;
+            next = redeem(tick);
+            if (!next.end) tick = ticket();
+        } else if constexpr (MODE == kDiffRepair) {
+            const uint32_t units = (uint32_t)p.num_items * H;
+            while (!flagged) {
+                if (base >= units) return;
+                flagged = __ballot(base + lane < units && p.odd[min(base + lane, units - 1)] != 0u);
+                if (!flagged) base += gridDim.x * kDiffWaves * kWave;
             }
-            const DiffRecord& rec = L.rec[(c - cb) % (2 * kBlockRecs)];
-            const uint4 ra = *reinterpret_cast<const uint4*>(&rec.rm[4 * g]);
-            const uint4 rb = *reinterpret_cast<const uint4*>(&rec.rm[16 + 4 * g]);
-            const uint32_t valid =
-                ((ra.x >> rbit) & 1u) | (((ra.y >> rbit) & 1u) << 1) |
-                (((ra.z >> rbit) & 1u) << 2) | (((ra.w >> rbit) & 1u) << 3) |
-                (((rb.x >> rbit) & 1u) << 4) | (((rb.y >> rbit) & 1u) << 5) |
-                (((rb.z >> rbit) & 1u) << 6) | (((rb.w >> rbit) & 1u) << 7);
-            held(at);
-            write_rows(at, 0, a);
-            wave_lds_order();
-            if (c + 1 < ce) load1(c + 1);
-            // S^T of both maps: slots 4g.. and 16 + 4g.. of row r
-            f4 s[2][2];
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-                    s[m][t] = products<T, 2>(at, kHalfStage * t, 2 * m, o1);
-            write_rows(at, kStageBytes, b);
-            if constexpr (PASS == kDiffColumns) {
-                if (lane < kChunk) *reinterpret_cast<f4*>(&L.stats[4 * lane]) = stat;
+            const uint32_t at = base + __builtin_ctzll(flagged);
+            flagged &= flagged - 1;
+            if (!flagged) base += gridDim.x * kDiffWaves * kWave;
+            u = unit(at / H, at % H, true);
+        }
+        [[maybe_unused]] uint64_t odd_sums = 0;   // bit 4 t + v: acc[t][v] has an odd value on an edge
+        int sweep = MODE == kDiffRepair ? kSweepMark : kSweepPlain;
+        while (u.w >= 0) {
+            clear(st);
+            if (PASS != kDiffForward && !Half<T>::kRange) st.x[0] = st.x[1] = 0.f;
+            if (!warm) {
+                own_load(p.own1, u, o1);
+                if constexpr (PASS != kDiffForward) own_load(p.own2, u, o2);
+                if constexpr (PASS == kDiffRows) lse = lse_load(u);
+                slot = 0;
+                if (u.cb < u.ce) {
+                    blk = fetch(u.cb);
+                    wave_lds_order();
+                    hand_out(0, u.h, blk);
+                    wave_lds_order();
+                    load1(0, u.h);
+                    load2(0, u.h);
+                }
             }
-            wave_lds_order();
-            if (c + 1 < ce) load2(c + 1);
+            // the block of records after u's first, or the next unit's first
+            const bool go_on = MODE == kDiffMain && next.cb < next.ce;
+            auto fetch_after = [&](int32_t c) __attribute__((always_inline)) -> u2 {
+                return c + kBlockRecs < u.ce ? fetch(c + kBlockRecs) : fetch(go_on ? next.cb : u.cb);
+            };
+            if (u.cb < u.ce) blk = fetch_after(u.cb);
+            // |p_1 - lam p_2| <= 1 + |lam|: binary16's range needs lam out of it
+            float fit = 1.f, fit_lam = u.lam;   // (uniform)
+            if constexpr (PASS == kDiffColumns && Half<T>::kRange) {
+                fit = uniform(1.f / __builtin_fmaxf(1.f, __builtin_fabsf(u.lam)));
+                fit_lam = uniform(fit * u.lam);
+            }
+            if constexpr (PASS == kDiffRows) {
+                const int l = anew(lane);
+                const int32_t row = u.w * 16 + l;
+                // (the columns' pass finds them beside D)
+                if (l < 16 && row < n && (MODE != kDiffTeam || wave == 0))
+                    *reinterpret_cast<float2*>(p.stats + ((int64_t)row * H + u.h) * 4) = lse;
+                // The matrix cores' sums are rounded towards one side, by some 2^-30 of
+                // g: nothing, but for dlam, where it adds up over all rows (500,000 of
+                // them: 1.4e-5 of it).  Odd rows take -do, and their sums of p g are
+                // negated at the end, so that it cancels.
+                const uint32_t flip = (r & 1) ? 0x80008000u : 0u;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    o2[i] = __builtin_bit_cast(v8, __builtin_bit_cast(u4, o2[i]) ^ flip);
+            }
             if constexpr (PASS == kDiffForward) {
-                float pw[2][8];
+                // (the running maxima are of s c with c > 0)
+                const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
-                for (int m = 0; m < 2; ++m)
-                    map_update(st, m, s[m][0], s[m][1], valid, p.scale_log2, pw[m]);
-                if (sweep != kSweepPlain) {
-                    if (sweep == kSweepMark) edge_weights(pw, valid);
-                    replace_odd<T>(at, kStageBytes, sweep);
+                for (int i = 0; i < 4; ++i)
+                    o1[i] = __builtin_bit_cast(v8, __builtin_bit_cast(u4, o1[i]) ^ flip);
+            }
+            for (int32_t c = u.cb; c < u.ce; ++c) {
+                const bool last = c + 1 == u.ce;
+                if (((c - u.cb) % kBlockRecs) == 0) {
+                    // the block ahead, so that the next chunk's record is there
+                    const bool own_block = c + kBlockRecs < u.ce;
+                    hand_out((slot & 2) ^ 2, own_block ? u.h : next.h, blk);
+                    if (own_block) blk = fetch_after(c + kBlockRecs);
                 }
-                v8 wh[4];
-                split8<T>(pw[0], wh[0], wh[1]);
-                split8<T>(pw[1], wh[2], wh[3]);
+                const uint32_t masks = records + slot * (uint32_t)sizeof(DiffRecord) +
+                                       (uint32_t)offsetof(DiffRecord, rm);
+                // where the stream goes on: the unit's next chunk, or the next unit's first
+                const int32_t ahead = last ? (slot & 2) ^ 2 : (slot + 1) & 3;
+                const uint32_t ahead_h = last ? (uint32_t)next.h : (uint32_t)u.h;
+                const bool more = !last || go_on;
+                held(at);
+                write_rows(at, 0, a);
+                wave_lds_order();
+                if (more) load1(ahead, ahead_h);
+                // S^T of both maps: slots 4g.. and 16 + 4g.. of row r
+                f4 s[2][2];
+                if constexpr (PASS != kDiffRows) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    f4* const to[4] = {&st.acc[4 * u], &st.acc[4 * u], &st.acc[8 + 4 * u],
-                                       &st.acc[8 + 4 * u]};
-                    mix<T>(at, kStageBytes, 4 * u, wh, to);
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int t = 0; t < 2; ++t)
+                            s[m][t] = products<T, 2>(at, kHalfStage * t, 2 * m, o1);
                 }
-            } else {
-                // g = do . v for the same pairs
-                f4 gs[2];
+                write_rows(at, kStageBytes, b);
+                if constexpr (PASS == kDiffColumns) {
+                    *reinterpret_cast<f2*>(&L.stats[2 * anew(lane)]) = stat;
+                }
+                wave_lds_order();
+                // (columns in binary16, with range_update's registers: only once the
+                // weights are made)
+                constexpr bool kLate = PASS == kDiffColumns && Half<T>::kRange;
+                if (!kLate && more) load2(ahead, ahead_h);
+                if (PASS == kDiffForward && last && go_on) own_load(p.own1, next, o1);
+                if constexpr (PASS == kDiffForward) {
+                    Attends on;
+                    attends(masks, lane, on);
+                    float pw[2][8];
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
-                    gs[t] = products<T, 4>(at, kStageBytes + kHalfStage * t, 0, o2);
-                if constexpr (PASS == kDiffRows) {
-                    if (sweep != kSweepPlain) replace_odd<T>(at, 0, sweep);
+                    for (int m = 0; m < 2; ++m)
+                        map_update(st, m, s[m][0], s[m][1], on, p.scale_log2, pw[m]);
+                    if (MODE != kDiffMain && sweep != kSweepPlain) {
+                        if (sweep == kSweepMark) edge_weights(pw, on);
+                        replace_odd<T>(at, kStageBytes, kStageBytes, sweep);
+                    }
 #pragma unroll
-                    for (int m = 0; m < 2; ++m) {
-                        float pw[1][8], pg[1][8];
+                    for (int v = 0; v < 2; ++v) {
+                        const Tiles<T> x(at, kStageBytes, 4 * v);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const bool on = (valid >> j) & 1u;
-                            const float x = fast_exp2(__builtin_fmaf(s[m][j >> 2][j & 3],
-                                                                     p.scale_log2,
-                                                                     m ? -lse2 : -lse1));
-                            pw[0][j] = on ? x : 0.f;
-                            pg[0][j] = on ? x * gs[j >> 2][j & 3] : 0.f;
-                            st.y[m] += pg[0][j];
-                            st.z[m] += pw[0][j];
-                        }
-                        if (sweep == kSweepMark) {
-                            edge_weights(pg, valid);
-                            edge_weights(pw, valid);
-                        }
-                        range_update<T>(st, m, pg[0]);
-                        v8 wh[4];
-                        split8<T>(pg[0], wh[0], wh[1]);
-                        split8<T>(pw[0], wh[2], wh[3]);
-                        f4* const to[4] = {&st.acc[4 * m], &st.acc[4 * m], &st.acc[8 + 4 * m],
-                                           &st.acc[8 + 4 * m]};
-                        mix<T>(at, 0, 4 * m, wh, to);
+                        for (int m = 0; m < 2; ++m) x.mix(pw[m], &st.acc[8 * m + 4 * v]);
                     }
                 } else {
-                    // |p_1 - lam p_2| <= 1 + |lam|: binary16's range needs lam out of it
-                    const float fit =
-                        Half<T>::kRange ? 1.f / __builtin_fmaxf(1.f, __builtin_fabsf(lam)) : 1.f;
-                    float ds[2][8], wv[1][8];
+                    // g = do . v for the same pairs
+                    f4 gs[2];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const bool on = (valid >> j) & 1u;
-                        const float gj = gs[j >> 2][j & 3];
-                        const f4 sj = *reinterpret_cast<const f4*>(&L.stats[4 * slot_of(g, j)]);
-                        const float p1 =
-                            fast_exp2(__builtin_fmaf(s[0][j >> 2][j & 3], p.scale_log2, -sj[0]));
-                        const float p2 =
-                            fast_exp2(__builtin_fmaf(s[1][j >> 2][j & 3], p.scale_log2, -sj[1]));
-                        ds[0][j] = on ? p1 * (gj - sj[2]) : 0.f;
-                        ds[1][j] = on ? p2 * (gj - sj[3]) : 0.f;
-                        wv[0][j] = on ? p1 * fit - p2 * (lam * fit) : 0.f;
-                    }
-                    if (sweep != kSweepPlain) {
-                        if (sweep == kSweepMark) {
-                            edge_weights(ds, valid);
-                            edge_weights(wv, valid);
+                    for (int t = 0; t < 2; ++t)
+                        gs[t] = products<T, 4>(at, kStageBytes + kHalfStage * t, 0, o2);
+                    if (PASS == kDiffRows && last && go_on) own_load(p.own2, next, o2);
+                    if constexpr (PASS == kDiffRows) {
+                        // (a map's logits where its weights are made: registers)
+                        const bool replaced = MODE != kDiffMain && sweep != kSweepPlain;
+                        if (replaced) replace_odd<T>(at, 0, kStageBytes, sweep);
+                        const uint32_t mixed = replaced ? kStageBytes : 0;
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) {
+                            f4 sm[2];
+#pragma unroll
+                            for (int t = 0; t < 2; ++t)
+                                sm[t] = products<T, 2>(at, kHalfStage * t, 2 * m, o1);
+                            if (m == 1 && last && go_on) own_load(p.own1, next, o1);
+                            Attends on;
+                            attends(masks, lane, on);
+                            float pw[1][8], pg[1][8];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                const float e = fast_exp2(__builtin_fmaf(
+                                    sm[j >> 2][j & 3], p.scale_log2, m ? -lse.y : -lse.x));
+                                pw[0][j] = where(on[j], e);
+                                st.z[m] += pw[0][j];
+                            }
+                            if (MODE != kDiffMain && sweep == kSweepMark) edge_weights(pw, on);
+                            const Tiles<T> x(at, mixed, 4 * m);
+                            x.mix(pw[0], &st.acc[8 + 4 * m]);
+                            __builtin_amdgcn_sched_barrier(0);
+                            attends(masks, lane, on);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                pg[0][j] = where(on[j], pw[0][j] * gs[j >> 2][j & 3]);
+                                st.y[m] += pg[0][j];
+                            }
+                            if (MODE != kDiffMain && sweep == kSweepMark) edge_weights(pg, on);
+                            range_update<T>(st, m, pg[0]);
+                            x.mix(pg[0], &st.acc[4 * m]);
+                            __builtin_amdgcn_sched_barrier(0);
                         }
-                        replace_odd<T>(at, 0, sweep);
-                        replace_odd<T>(at, kStageBytes, sweep);
-                    }
-                    v8 wh[2];
+                        if (last && go_on) lse = lse_load(next);
+                    } else {
+                        Attends on;
+                        if (MODE != kDiffMain && sweep != kSweepPlain) {
+                            replace_odd<T>(at, 0, 0, sweep);
+                            replace_odd<T>(at, kStageBytes, kStageBytes, sweep);
+                        }
+                        float pw[2][8];
 #pragma unroll
-                    for (int m = 0; m < 2; ++m) {
-                        range_update<T>(st, m, ds[m]);
-                        split8<T>(ds[m], wh[0], wh[1]);
-                        f4* const to[2] = {&st.acc[4 * m], &st.acc[4 * m]};
-                        mix<T>(at, 0, 4 * m, wh, to);
-                    }
-                    split8<T>(wv[0], wh[0], wh[1]);
+                        for (int m = 0; m < 2; ++m) {
+                            __builtin_amdgcn_sched_barrier(0);
+                            attends(masks, lane, on);
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        f4* const to[2] = {&st.acc[8 + 4 * u], &st.acc[8 + 4 * u]};
-                        mix<T>(at, kStageBytes, 4 * u, wh, to);
+                            for (int j = 0; j < 8; ++j)
+                                pw[m][j] = where(on[j], fast_exp2(__builtin_fmaf(
+                                                            s[m][j >> 2][j & 3], p.scale_log2,
+                                                            -L.stats[4 * slot_of(g, j) + m])));
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (kLate && more) load2(ahead, ahead_h);
+                        {
+                            float wv[1][8];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) wv[0][j] = pw[0][j] * fit - pw[1][j] * fit_lam;
+                            if (MODE != kDiffMain && sweep == kSweepMark) edge_weights(wv, on);
+#pragma unroll
+                            for (int v = 0; v < 2; ++v) {
+                                Tiles<T>(at, kStageBytes, 4 * v).mix(wv[0], &st.acc[8 + 4 * v]);
+                                __builtin_amdgcn_sched_barrier(0);
+                            }
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) {
+                            attends(masks, lane, on);
+                            float ds[1][8];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                ds[0][j] = where(on[j], pw[m][j] * (gs[j >> 2][j & 3] -
+                                                                    L.stats[4 * slot_of(g, j) + 2 + m]));
+                            if (MODE != kDiffMain && sweep == kSweepMark) edge_weights(ds, on);
+                            __builtin_amdgcn_sched_barrier(0);
+                            range_update<T>(st, m, ds[0]);
+                            v8 hi, lo;
+                            split8<T>(ds[0], hi, lo);
+                            // (two tiles at a time: registers)
+#pragma unroll
+                            for (int v = 0; v < 2; ++v) {
+                                __builtin_amdgcn_sched_barrier(0);
+                                Tiles<T, 2>(at, 0, 4 * m + 2 * v).mix(hi, lo, &st.acc[4 * m + 2 * v]);
+                            }
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
                     }
                 }
+                wave_lds_order();
+                slot = ahead;
             }
-            wave_lds_order();
+            warm = u.cb < u.ce && go_on;
+            if (PASS == kDiffColumns && warm) {   // (inside the loop they cost it registers)
+                own_load(p.own1, next, o1);
+                own_load(p.own2, next, o2);
+            }
+            if (sweep == kSweepPlain) {
+                // (x - x is 0 for finite x, NaN otherwise)
+                float odd = 0.f;
+#pragma unroll
+                for (int t = 0; t < 16; ++t)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) odd += st.acc[t][v] - st.acc[t][v];
+                const bool any = __ballot(odd != 0.f) != 0;
+                if constexpr (MODE == kDiffMain) {
+                    if (lane == 0) p.odd[u.item * H + u.h] = any;
+                    break;
+                }
+                if (!any) break;
+                sweep = kSweepMark;
+            } else if (sweep == kSweepMark) {
+#pragma unroll
+                for (int t = 0; t < 16; ++t)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v)
+                        odd_sums |= (uint64_t)(st.acc[t][v] != 0.f) << (4 * t + v);
+                sweep = kSweepClean;
+            } else {
+#pragma unroll
+                for (int t = 0; t < 16; ++t)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v)
+                        if ((odd_sums >> (4 * t + v)) & 1u) st.acc[t][v] = NAN;
+                break;
+            }
         }
-        if (sweep == kSweepPlain) {
-            // (x - x is 0 for finite x, NaN otherwise)
-            float odd = 0.f;
-#pragma unroll
-            for (int t = 0; t < 16; ++t)
-#pragma unroll
-                for (int v = 0; v < 4; ++v) odd += st.acc[t][v] - st.acc[t][v];
-            if (!__ballot(odd != 0.f)) break;
-            sweep = kSweepMark;
-        } else if (sweep == kSweepMark) {
-#pragma unroll
-            for (int t = 0; t < 16; ++t)
-#pragma unroll
-                for (int v = 0; v < 4; ++v)
-                    odd_sums |= (uint64_t)(st.acc[t][v] != 0.f) << (4 * t + v);
-            sweep = kSweepClean;
-        } else {
-#pragma unroll
-            for (int t = 0; t < 16; ++t)
-#pragma unroll
-                for (int v = 0; v < 4; ++v)
-                    if ((odd_sums >> (4 * t + v)) & 1u) st.acc[t][v] = NAN;
-            break;
+        if (u.w < 0) {
+            warm = false;
+            if (MODE == kDiffMain && u.there && lane == 0) p.odd[u.item * H + u.h] = 0u;
         }
+        if constexpr (MODE == kDiffTeam) break;
+        if (u.w >= 0) {
+            if (u.slot >= 0)   // a segment: its sums wait for diff_merge_kernel
+                publish(st, p.partials + ((int64_t)u.slot * H + u.h) * kDiffPartial, lane);
+            else
+                diff_finish<T, PASS>(p, st, L.x1, u.w, u.h, u.lam, lane);
+        }
+        if constexpr (MODE == kDiffMain) u = next;
     }
-
-    if constexpr (TEAM) {
+    if constexpr (MODE == kDiffTeam) {
         // waves 2, 3 into 0, 1, then 1 into 0: two states fit the team's memory
+        // (a team's four are there or not together; teams have no segments)
+        if (u.w < 0) return;
         float* area = reinterpret_cast<float*>(&lds_all[wave & 1]);
         __syncthreads();
         if (wave >= 2) publish(st, area, lane);
@@ -761,12 +995,13 @@ diff_kernel(const DiffParams p)
         __syncthreads();
         if (wave != 0) return;
         absorb<PASS>(st, reinterpret_cast<const float*>(&lds_all[1]), lane);
+        diff_finish<T, PASS>(p, st, L.x1, u.w, u.h, u.lam, lane);
     }
-    if (it.slot >= 0) {   // a segment: its sums wait for diff_merge_kernel
-        publish(st, p.partials + ((int64_t)it.slot * H + h) * kDiffPartial, lane);
-        return;
-    }
-    diff_finish<T, PASS>(p, st, L.x1, w, h, lane);
+}
+
+__global__ void __launch_bounds__(256) clear_queues(uint32_t* __restrict__ queues, int32_t words)
+{
+    for (int32_t i = threadIdx.x; i < words; i += 256) queues[i] = 0u;
 }
 
 // The segments of a split window, in their order.
@@ -782,7 +1017,7 @@ diff_merge_kernel(const DiffParams p)
     clear(st);
     for (int32_t k = 0; k < si.nseg; ++k)
         absorb<PASS>(st, p.partials + ((int64_t)(si.first_slot + k) * p.H + h) * kDiffPartial, lane);
-    diff_finish<T, PASS>(p, st, stage, si.w, h, lane);
+    diff_finish<T, PASS>(p, st, stage, si.w, h, p.lam[h], lane);
 }
 
 // dlam[h] = -sum of its windows' shares, in one fixed order.
@@ -790,9 +1025,15 @@ __global__ void __launch_bounds__(1024)
 diff_dlam_kernel(const float* __restrict__ parts, int32_t W, float* __restrict__ dlam)
 {
     __shared__ double lds[1024 / kWave];
-    double s = 0.0;
     const float* src = parts + (int64_t)blockIdx.x * W;
-    for (int32_t i = threadIdx.x; i < W; i += 1024) s += src[i];
+    double s = 0.0;
+    for (int32_t i = threadIdx.x; i < W; i += 32 * 1024) {
+        float x[32];   // (in one batch: the loads' latency is all there is)
+#pragma unroll
+        for (int k = 0; k < 32; ++k) x[k] = i + k * 1024 < W ? src[i + k * 1024] : 0.f;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) s += x[k];
+    }
     s = wave_sum(s);
     if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = s;
     __syncthreads();
@@ -811,17 +1052,38 @@ hipError_t warm_diff(hipStream_t s)
     return hipGetLastError();
 }
 
-template <typename T, int PASS, bool WIDE>
-static void launch_diff(const DiffParams& p, int32_t team, hipStream_t st)
+constexpr int64_t kDiffResident = 512;   // workgroups: two per CU, by their LDS
+constexpr int32_t kRepairGroups = 256;
+
+// Four-unit workgroups of each XCD's share of a plan's items.
+static int64_t share_groups(const f3s_plan* plan)
 {
-    const int64_t waves = p.num_items * p.H;
-    if (team > 1)
-        hipLaunchKernelGGL((diff_kernel<T, PASS, WIDE, kTeamSmall, true>),
-                           dim3((unsigned)(waves / kTeamSmall)), dim3(kTeamSmall * kWave), 0, st, p);
-    else
-        hipLaunchKernelGGL((diff_kernel<T, PASS, WIDE, 4, false>),
-                           dim3((unsigned)(kXcds * ceil_div(ceil_div(p.num_items, kXcds) * p.H, 4))),
-                           dim3(4 * kWave), 0, st, p);
+    return ceil_div(ceil_div(plan->masked.num_items, kXcds) * plan->H, kDiffWaves);
+}
+// With a queue: two units for each wave and more.  (Below that it would be a launch
+// more for nothing ahead to load.)
+static bool has_queue(const f3s_plan* plan)
+{
+    return plan->masked.team == 1 && kXcds * share_groups(plan) >= 2 * kDiffResident;
+}
+
+template <typename T, int PASS, bool WIDE>
+static void launch_diff(const DiffParams& p, const f3s_plan* plan, hipStream_t st)
+{
+    if (plan->masked.team > 1) {
+        hipLaunchKernelGGL((diff_kernel<T, PASS, WIDE, kDiffTeam>),
+                           dim3((unsigned)(p.num_items / kTeamSmall * p.H)),
+                           dim3(kTeamSmall * kWave), 0, st, p);
+        return;
+    }
+    const int64_t groups = has_queue(plan) ? kDiffResident : kXcds * share_groups(plan);
+    hipLaunchKernelGGL((diff_kernel<T, PASS, WIDE, kDiffMain>), dim3((unsigned)groups),
+                       dim3(kDiffWaves * kWave), 0, st, p);
+    const int64_t units = p.num_items * p.H;
+    hipLaunchKernelGGL((diff_kernel<T, PASS, WIDE, kDiffRepair>),
+                       dim3((unsigned)std::min<int64_t>(kRepairGroups,
+                                                        ceil_div(units, kDiffWaves * kWave))),
+                       dim3(kDiffWaves * kWave), 0, st, p);
     if (p.num_split > 0)
         hipLaunchKernelGGL((diff_merge_kernel<T, PASS>), dim3((unsigned)(p.num_split * p.H)),
                            dim3(kWave), 0, st, p);
@@ -841,10 +1103,14 @@ static f3s_status launch_pass(DiffParams p, const f3s_plan* plan, int32_t dtype,
     p.W = plan->W;
     p.H = plan->H;
     p.xcd_contiguous = plan->xcd_contiguous;
-    p.refs_are_nodes = wide_features(p.n, p.H);
-    p.heads_magic = (uint32_t)ceil_div((int64_t)1 << 31, p.H);
+    const bool nodes = wide_features(p.n, p.H);
+    p.ref_shift = nodes ? 0 : 7;
+    p.ref_magic = nodes ? 1u << 31 : (uint32_t)ceil_div((int64_t)1 << 31, p.H);
+    p.no_ref = nodes ? kNoIdx : kNoRow;
     p.scale = scale;
     p.scale_log2 = scale * 1.4426950408889634f;
+    // (forward: q is negated for a negative scale; 0 x -inf is no logit)
+    if (PASS == kDiffForward) p.scale_log2 = std::max(std::fabs(p.scale_log2), FLT_MIN);
     if (p.num_items <= 0) return F3S_OK;
     F3S_REQUIRE(p.num_items * p.H < ((int64_t)1 << 31) && (set.team == 1 || set.team == kTeamSmall),
                 "differential attention: too many work items");
@@ -865,11 +1131,11 @@ static f3s_status launch_pass(DiffParams p, const f3s_plan* plan, int32_t dtype,
         p.stats_bytes = (uint32_t)bytes;
     }
     if (dtype == F3S_F16) {
-        if (wide) launch_diff<_Float16, PASS, true>(p, set.team, st);
-        else launch_diff<_Float16, PASS, false>(p, set.team, st);
+        if (wide) launch_diff<_Float16, PASS, true>(p, plan, st);
+        else launch_diff<_Float16, PASS, false>(p, plan, st);
     } else {
-        if (wide) launch_diff<__bf16, PASS, true>(p, set.team, st);
-        else launch_diff<__bf16, PASS, false>(p, set.team, st);
+        if (wide) launch_diff<__bf16, PASS, true>(p, plan, st);
+        else launch_diff<__bf16, PASS, false>(p, plan, st);
     }
     F3S_HIP(hipGetLastError());
     return F3S_OK;
@@ -881,6 +1147,36 @@ static size_t partial_bytes(const f3s_plan* plan)
 {
     return round_up(sizeof(float) * kDiffPartial * (size_t)plan->H *
                     (size_t)plan->masked.num_slots);
+}
+
+// Workspace of a pass: its queues (a call's passes' side by side at the start), the
+// marks of its units, its segments' sums.
+constexpr size_t kQueueBytes = sizeof(uint32_t) * kXcds * kQueueStride;
+struct PassSpace {
+    size_t odd, partials, bytes;
+};
+static PassSpace pass_space(const f3s_plan* plan)
+{
+    PassSpace s;
+    s.odd = 2 * kQueueBytes;
+    s.partials = s.odd;
+    if (plan->masked.team == 1)
+        s.partials += round_up(sizeof(uint32_t) * (size_t)plan->masked.num_items * plan->H);
+    s.bytes = s.partials + partial_bytes(plan);
+    return s;
+}
+static void set_space(DiffParams& p, const f3s_plan* plan, char* ws, int pass)
+{
+    const PassSpace s = pass_space(plan);
+    p.queue = has_queue(plan) ? reinterpret_cast<uint32_t*>(ws + pass * kQueueBytes) : nullptr;
+    p.odd = reinterpret_cast<uint32_t*>(ws + s.odd);
+    p.partials = reinterpret_cast<float*>(ws + s.partials);
+}
+static void launch_clear(const DiffParams& p, int passes, hipStream_t st)
+{
+    if (p.queue)
+        hipLaunchKernelGGL(clear_queues, dim3(1), dim3(256), 0, st, p.queue,
+                           passes * kXcds * kQueueStride);
 }
 
 static f3s_status check_plan(const f3s_plan* plan, int32_t n, int32_t H, const char* who)
@@ -914,10 +1210,10 @@ f3s_status f3s_diff_attention_workspace(const f3s_plan* plan, const f3s_plan* re
                                         int64_t* bytes)
 {
     F3S_REQUIRE(plan && bytes, "f3s_diff_attention_workspace: NULL pointer");
-    size_t need = partial_bytes(plan);
+    size_t need = pass_space(plan).bytes;
     if (reversed) {
         const size_t cells = (size_t)std::max(plan->compiled_n, 0) * plan->H;
-        need = std::max(need, partial_bytes(reversed)) + round_up(cells * 16) +
+        need = std::max(need, pass_space(reversed).bytes) + round_up(cells * 16) +
                round_up(sizeof(float) * (size_t)plan->W * plan->H);
     }
     *bytes = (int64_t)need;
@@ -938,8 +1234,8 @@ f3s_status f3s_diff_attention_fwd(const f3s_plan* plan, const uint16_t* Q, int64
                     rows_ok(O, o_stride, H) && lam && ((uintptr_t)lse & 7) == 0,
                 "f3s_diff_attention_fwd: NULL or misaligned pointer, or a row stride that is no "
                 "multiple of 8 or below H * 128");
-    F3S_REQUIRE(workspace_bytes >= (int64_t)partial_bytes(plan) &&
-                    (workspace || partial_bytes(plan) == 0) && ((uintptr_t)workspace & 15) == 0,
+    F3S_REQUIRE(workspace_bytes >= (int64_t)pass_space(plan).bytes && workspace &&
+                    ((uintptr_t)workspace & 15) == 0,
                 "f3s_diff_attention_fwd: workspace too small");
     F3S_TRY(require_device());
     clear_error();
@@ -950,8 +1246,9 @@ f3s_status f3s_diff_attention_fwd(const f3s_plan* plan, const uint16_t* Q, int64
     p.out1 = rows_of(O, o_stride);
     p.lam = lam;
     p.lse = lse;
-    p.partials = static_cast<float*>(workspace);
     p.n = n;
+    set_space(p, plan, static_cast<char*>(workspace), 0);
+    launch_clear(p, 1, as_stream(stream));
     return launch_pass<kDiffForward>(p, plan, dtype, scale, as_stream(stream));
 }
 
@@ -977,8 +1274,7 @@ f3s_status f3s_diff_attention_bwd(const f3s_plan* plan, const f3s_plan* reversed
                 "multiple of 8 or below H * 128");
     int64_t need = 0;
     F3S_TRY(f3s_diff_attention_workspace(plan, reversed, &need));
-    F3S_REQUIRE(workspace_bytes >= need && (workspace || need == 0) &&
-                    ((uintptr_t)workspace & 15) == 0,
+    F3S_REQUIRE(workspace_bytes >= need && workspace && ((uintptr_t)workspace & 15) == 0,
                 "f3s_diff_attention_bwd: workspace too small");
     F3S_TRY(require_device());
     clear_error();
@@ -990,8 +1286,7 @@ f3s_status f3s_diff_attention_bwd(const f3s_plan* plan, const f3s_plan* reversed
         char* ws = static_cast<char*>(workspace);
         p.stats = reinterpret_cast<float*>(ws);
         p.dlam_parts = reinterpret_cast<float*>(ws + round_up((size_t)n * H * 16));
-        p.partials = reinterpret_cast<float*>(ws + round_up((size_t)n * H * 16) +
-                                              round_up(sizeof(float) * (size_t)plan->W * H));
+        char* spaces = ws + round_up((size_t)n * H * 16) + round_up(sizeof(float) * (size_t)plan->W * H);
         p.lse = const_cast<float*>(lse);
         DiffParams rows = p;
         rows.x1 = rows_of(K, k_stride);
@@ -999,8 +1294,12 @@ f3s_status f3s_diff_attention_bwd(const f3s_plan* plan, const f3s_plan* reversed
         rows.own1 = rows_of(Q, q_stride);
         rows.own2 = rows_of(dO, do_stride);
         rows.out1 = rows_of(dQ, dq_stride);
-        F3S_TRY(launch_pass<kDiffRows>(rows, plan, dtype, scale, st));
+        set_space(rows, plan, spaces, 0);
         DiffParams cols = p;
+        set_space(cols, reversed, spaces, 1);
+        if (rows.queue) launch_clear(rows, 2, st);
+        else launch_clear(cols, 1, st);
+        F3S_TRY(launch_pass<kDiffRows>(rows, plan, dtype, scale, st));
         cols.x1 = rows_of(Q, q_stride);
         cols.x2 = rows_of(dO, do_stride);
         cols.own1 = rows_of(K, k_stride);

@@ -11,6 +11,7 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b4 __attribute__((ext_vector_type(4)));
 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 typedef float f2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 
 // kRange: weights have to be scaled into the type's range (binary16 ends at
 // 65,504 and thins out below 2^-14; bfloat16 has float32's exponents).
