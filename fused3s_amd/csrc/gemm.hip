@@ -11,10 +11,10 @@
 //   dx       P = dz [n][M],     Q = W, transposed
 //   dW       P, Q = dz, x, both transposed, n cut into splits whose float32
 //            sums are added in order; db with it
-// A workgroup of four waves owns a TILE x TILE block of C, 64 contraction steps
-// at a time: both operands' tiles go from memory straight into LDS (16 bytes a
-// lane, no registers), one ahead of the products, in an order in which neither
-// plain nor transposing LDS reads meet bank conflicts.  Q is the MFMA's A operand,
+// A workgroup of four waves owns a block of C and goes through the contraction in
+// steps: both operands' tiles go from memory straight into LDS (16 bytes a lane, no
+// registers), ahead of the products, in an order in which neither plain nor
+// transposing LDS reads meet bank conflicts.  Q is the MFMA's A operand,
 // so a lane holds four consecutive outputs of a row; the epilogue passes them
 // through LDS, 16 rows at a time, so that whole lines are read (residual, dy) and
 // written.
@@ -30,6 +30,7 @@ enum Epilogue : int {
     kEpiSlope = 1,     // dy act'(z + bias), and the sums of its columns
     kEpiPlain = 2,     // z
     kEpiPart = 3,      // z in float32, one slice per split
+    kEpiPartSums = 4,  // and the sums of P's rows (dW: db)
 };
 
 struct GemmParams {
@@ -47,82 +48,107 @@ struct GemmParams {
     int32_t row_tiles, out_tiles, splits;
 };
 
-// erf by Abramowitz and Stegun 7.1.26 (absolute error 1.5e-7), here of z / sqrt 2
-// as the normal distribution's Phi(z), with e = exp(-z^2 / 2).
-__device__ __forceinline__ float normal_cdf(float z, float& e)
-{
-    const float a = __builtin_fabsf(z);
-    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f * 0.70710678f, a, 1.f));
-    e = fast_exp2(-0.72134752f * z * z);   // log2(e) / 2
-    float s = __builtin_fmaf(1.061405429f, t, -1.453152027f);
-    s = __builtin_fmaf(s, t, 1.421413741f);
-    s = __builtin_fmaf(s, t, -0.284496736f);
-    s = __builtin_fmaf(s, t, 0.254829592f);
-    const float tail = 0.5f * s * t * e;   // Phi(-|z|)
-    return z < 0.f ? tail : 1.f - tail;
-}
 __device__ __forceinline__ float logistic(float z)
 {
     return __builtin_amdgcn_rcpf(1.f + fast_exp2(-1.44269504f * z));
 }
+// Phi(z), the normal distribution's: the logistic function of z P(z^2), P fitted
+// (weighted minimax, degree 6, to z (Phi - its value) for |z| <= 8) to
+// log(Phi / (1 - Phi)) / z, positive everywhere: z Phi to 6e-7, Phi to 2e-7, and
+// both tails' ends.  One exponential and one reciprocal, eight other operations;
+// by erf's usual rational form there were 15.  (Where K is small the activation
+// bounds the kernel: 500,000 x 128 -> 512 is 256 M of them.)
+__device__ __forceinline__ float normal_cdf(float z)
+{
+    constexpr float c[7] = {-2.30220720e+00f,
+                            -1.04838581e-01f,
+                            9.55929293e-05f,
+                            1.59389413e-04f,
+                            -1.14524302e-05f,
+                            3.85045013e-07f,
+                            -5.20990915e-09f};   // by -log2(e)
+    const float t = z * z;
+    float s = c[6];
+#pragma unroll
+    for (int k = 5; k >= 0; --k) s = __builtin_fmaf(s, t, c[k]);
+    return __builtin_amdgcn_rcpf(1.f + fast_exp2(z * s));
+}
 constexpr float kTanhA = 0.79788456f, kTanhB = 0.044715f;   // sqrt(2 / pi)
 
-__device__ __forceinline__ float act_value(int act, float z)
+__device__ __forceinline__ float gelu_tanh_cdf(float z)   // (1 + tanh u) / 2 = logistic(2 u)
 {
-    float e;
+    return logistic(2.f * kTanhA * z * __builtin_fmaf(kTanhB * z, z, 1.f));
+}
+
+template <int N, typename F>
+__device__ __forceinline__ void each(float (&z)[N], F f)
+{
+#pragma unroll
+    for (int k = 0; k < N; ++k) z[k] = f(z[k]);
+}
+// z -> act(z), and z -> act'(z); act is uniform.
+template <int N>
+__device__ __forceinline__ void act_values(int act, float (&z)[N])
+{
     switch (act) {
-    case kActRelu: return z < 0.f ? 0.f : z;   // (NaN stays)
-    case kActGelu: return z * normal_cdf(z, e);
-    case kActGeluTanh: return z * logistic(2.f * kTanhA * z * __builtin_fmaf(kTanhB * z, z, 1.f));
-    case kActSilu: return z * logistic(z);
-    default: return z;
+    case kActRelu: each(z, [](float x) { return x < 0.f ? 0.f : x; }); break;   // (NaN stays)
+    case kActGelu: each(z, [](float x) { return x * normal_cdf(x); }); break;
+    case kActGeluTanh: each(z, [](float x) { return x * gelu_tanh_cdf(x); }); break;
+    case kActSilu: each(z, [](float x) { return x * logistic(x); }); break;
+    default: break;
     }
 }
-__device__ __forceinline__ float act_slope(int act, float z)
+template <int N>
+__device__ __forceinline__ void act_slopes(int act, float (&z)[N])
 {
-    float e;
     switch (act) {
-    case kActRelu: return z > 0.f ? 1.f : z == z ? 0.f : z;
-    case kActGelu: {
-        const float c = normal_cdf(z, e);
-        return __builtin_fmaf(0.39894228f * z, e, c);   // 1 / sqrt(2 pi)
-    }
-    case kActGeluTanh: {   // (1 + tanh u) / 2 is the logistic function of 2 u
-        const float s = logistic(2.f * kTanhA * z * __builtin_fmaf(kTanhB * z, z, 1.f));
-        return s + z * s * (1.f - s) * 2.f * kTanhA * __builtin_fmaf(3.f * kTanhB * z, z, 1.f);
-    }
-    case kActSilu: {
-        const float s = logistic(z);
-        return s * (1.f + z * (1.f - s));
-    }
-    default: return 1.f;
+    case kActRelu: each(z, [](float x) { return x > 0.f ? 1.f : x == x ? 0.f : x; }); break;
+    case kActGelu:   // Phi + x phi
+        each(z, [](float x) {
+            return __builtin_fmaf(0.39894228f * x, fast_exp2(-0.72134752f * x * x), normal_cdf(x));
+        });
+        break;
+    case kActGeluTanh:
+        each(z, [](float x) {
+            const float s = gelu_tanh_cdf(x);
+            return s + x * s * (1.f - s) * 2.f * kTanhA * __builtin_fmaf(3.f * kTanhB * x, x, 1.f);
+        });
+        break;
+    case kActSilu:
+        each(z, [](float x) {
+            const float s = logistic(x);
+            return s * (1.f + x * (1.f - s));
+        });
+        break;
+    default: each(z, [](float) { return 1.f; }); break;
     }
 }
 
+constexpr int kStep = 64;   // contraction steps per tile
+
 // Where piece p (16 bytes) of a stored row lies in LDS, by exclusive or.  Row by
-// row: 128-byte rows, whose piece of one number 16 rows' lanes read together.
+// row, 128 bytes each: the pieces of one number that 16 rows' lanes read together
+// lie in distinct banks.
 __device__ __forceinline__ int place_rows(int row) { return (row >> 1) & 7; }
 // Contraction by contraction: the transposing reads take rows 8 g + i, i < 4,
 // and pairs of pieces, two groups g at once.
 template <int TILE>
 __device__ __forceinline__ int place_steps(int row)
 {
-    if constexpr (TILE == 128)
+    if constexpr (TILE >= 128)
         return ((row & 3) << 1) | (((row >> 3) & 1) << 3) | ((row >> 2) & 1);
     else
         return (row & 2) | (((row >> 3) & 1) << 2);
 }
 
-constexpr int kStep = 64;   // contraction steps per tile
-
 // Loads one operand's tile, rows (or outputs) from `first` and steps from `step`,
 // into LDS at `lds`.  FAST: rows 16-byte aligned, whole pieces inside or outside.
-template <typename T, bool TRANS, int TILE, bool FAST>
+template <typename T, bool TRANS, int TILE, int WAVES, bool FAST>
 __device__ __forceinline__ void load_tile(const char* base, int64_t ld, int64_t first, int64_t count,
                                           int64_t step, int64_t end, char* lds, int wave, int lane)
 {
     constexpr int kPieces = (TRANS ? TILE : kStep) / 8;     // per stored row
-    constexpr int kLoads = TILE * kStep * 2 / 1024 / 4;     // 1,024 bytes per wave and load
+    constexpr int kLoads = TILE * kStep * 2 / 1024 / WAVES;  // 1,024 bytes per wave and load
     // stored rows and columns from here on
     const int64_t r0 = TRANS ? step : first, c0 = TRANS ? first : step;
     const int64_t rows = (TRANS ? end : count) - r0, cols = (TRANS ? count : end) - c0;
@@ -130,7 +156,7 @@ __device__ __forceinline__ void load_tile(const char* base, int64_t ld, int64_t 
     const int row_in = lane / kPieces, pos = lane % kPieces;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-        const int chunk = i * 4 + wave;
+        const int chunk = i * WAVES + wave;
         const int row = chunk * (64 / kPieces) + row_in;
         const int piece = pos ^ (TRANS ? place_steps<TILE>(row) : place_rows(row));
         char* to = lds + chunk * 1024;
@@ -180,12 +206,13 @@ __device__ __forceinline__ typename Half<T>::v8 fragment(const char* lds, int t,
     }
 }
 
-// Workgroup -> tile.  Each XCD takes a contiguous range of them (the dispatcher
-// deals workgroups to the XCDs in turn), in groups of 8 row tiles by all output
+// Number -> tile.  Each XCD takes a contiguous range of them (the dispatcher deals
+// workgroups to the XCDs in turn, and a workgroup's numbers are a multiple of eight
+// apart), in groups of 8 row tiles by all output
 // tiles: the row tiles' operand stays in its L2 while the others pass by.
-__device__ __forceinline__ void tile_of(const GemmParams& p, int32_t& row, int32_t& out)
+__device__ __forceinline__ void tile_of(const GemmParams& p, int64_t b, int32_t& row, int32_t& out)
 {
-    const int64_t G = (int64_t)p.row_tiles * p.out_tiles, b = blockIdx.x;
+    const int64_t G = (int64_t)p.row_tiles * p.out_tiles;
     const int64_t x = b % kXcds, q = G / kXcds, rem = G % kXcds;
     const int64_t id = x * q + min(x, rem) + b / kXcds;
     constexpr int kGroup = 8;
@@ -225,12 +252,15 @@ __device__ __forceinline__ void finish8(const GemmParams& p, int64_t row, int64_
         }
         float r[8] = {};
         if (p.R) load(reinterpret_cast<const T*>(p.R) + row * p.ldr + out, r);
+        if constexpr (EPI == kEpiForward) {
+            act_values(p.act, z);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            if constexpr (EPI == kEpiForward) {
-                z[k] = act_value(p.act, z[k]) + r[k];
-            } else {
-                z[k] = r[k] * act_slope(p.act, z[k]);
+            for (int k = 0; k < 8; ++k) z[k] += r[k];
+        } else {
+            act_slopes(p.act, z);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                z[k] *= r[k];
                 sum[k] += z[k];
             }
         }
@@ -247,127 +277,171 @@ __device__ __forceinline__ void finish8(const GemmParams& p, int64_t row, int64_
     }
 }
 
-template <typename T, bool PT, bool QT, int TILE, int EPI, bool FAST>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
+// Tiles of C, contraction steps of 64, the next one's tiles on their way meanwhile.
+// 64 and 128: a quarter for each of four waves, two workgroups per CU and more;
+// 256: eight waves of 128 rows by 64 outputs.  (What bounds the small ones is the
+// way from L2 to LDS, 64 bytes per clock and CU: 128 x 128 x 64 products take its
+// time as long as the matrix cores'; 256 x 256 x 64 half of it.  32,768 x 1,024 ->
+// 4,096, TFLOP/s: 64 560, 128 737, 256 839; three steps of 32 with the next one's
+// operands read ahead into registers, 256 x 256 743, 256 x 128 698.)
+template <int SIZE>
+struct Shape {
+    static constexpr int wave_rows = 2, wave_outs = SIZE == 256 ? 4 : 2, waves = wave_rows * wave_outs;
+    static constexpr int rows = SIZE / wave_rows, outs = SIZE / wave_outs;   // of a wave
+    static constexpr int tile_bytes = SIZE * kStep * 2;
+};
+
+template <typename T, bool PT, bool QT, int SIZE, int EPI, bool FAST>
+__global__ void __launch_bounds__(Shape<SIZE>::waves * kWave) __attribute__((amdgpu_waves_per_eu(2)))
 gemm_kernel(const GemmParams p)
 {
     typedef typename Half<T>::v8 v8;
-    constexpr int kTileBytes = TILE * kStep * 2;
-    constexpr int kW = TILE / 2;         // a wave's block of C is kW x kW
-    constexpr int kN = kW / 16;
-    constexpr int kOutRow = kW + 4;      // floats of a staged row
-    __shared__ __align__(256) char lds[2][2][kTileBytes];   // [buffer][P, Q]
-    static_assert(sizeof(lds) >= 4 * 16 * kOutRow * sizeof(float), "the waves' epilogue stages");
+    typedef Shape<SIZE> S;
+    constexpr int kNo = S::outs / 16, kNr = S::rows / 16;
+    constexpr int kOutRow = S::outs + 4;      // floats of a staged row
+    __shared__ __align__(256) char lds[2][2][S::tile_bytes];   // [buffer][P, Q]
+    static_assert(sizeof(lds[0]) >= S::waves * 16 * kOutRow * sizeof(float), "the waves' epilogue stages");
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int lane = threadIdx.x % kWave;
     const int g = lane >> 4, r = lane & 15;
-    const int wr = wave >> 1, wo = wave & 1;
-    int32_t rt, ot;
-    tile_of(p, rt, ot);
-    const int64_t row0 = (int64_t)rt * TILE, out0 = (int64_t)ot * TILE;
+    const int wr = wave / S::wave_outs, wo = wave % S::wave_outs;
     const int64_t begin = (int64_t)blockIdx.y * p.split, end = min(p.depth, begin + p.split);
-
-    f4 acc[kN][kN];   // [outputs][rows]
-    f4 col[kN];       // sums of P's rows (dW's splits: db)
-#pragma unroll
-    for (int i = 0; i < kN; ++i) {
-        col[i] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < kN; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
-    }
-    const bool with_sums = EPI == kEpiPart && p.sums && ot == 0 && wo == 0;
+    const int64_t total = (int64_t)p.row_tiles * p.out_tiles;
+    constexpr bool kSums = EPI == kEpiPartSums, kPart = EPI == kEpiPart || kSums;
     v8 ones;
+    if constexpr (kSums) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) ones[k] = (T)1.f;
-
-    auto load = [&](int64_t c, int buf) __attribute__((always_inline)) {
-        load_tile<T, PT, TILE, FAST>(p.P, p.ldp, row0, p.rows, c, end, lds[buf][0], wave, lane);
-        load_tile<T, QT, TILE, FAST>(p.Q, p.ldq, out0, p.outs, c, end, lds[buf][1], wave, lane);
-    };
-    if (begin < end) load(begin, 0);
-    int buf = 0;
-    for (int64_t c = begin; c < end; c += kStep, buf ^= 1) {
-        // this tile has landed (loads into LDS are waited for by hand: the barrier
-        // does not), and the last one's readers are done
-        __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
-        __syncthreads();
-        if (c + kStep < end) load(c + kStep, buf ^ 1);
-        const char* pt = lds[buf][0];
-        const char* qt = lds[buf][1];
-#pragma unroll
-        for (int f = 0; f < kStep / 32; ++f) {
-            v8 a[kN], b[kN];
-#pragma unroll
-            for (int i = 0; i < kN; ++i) {
-                a[i] = fragment<T, QT, TILE>(qt, kN * wo + i, f, lane);
-                b[i] = fragment<T, PT, TILE>(pt, kN * wr + i, f, lane);
-            }
-#pragma unroll
-            for (int i = 0; i < kN; ++i)
-#pragma unroll
-                for (int j = 0; j < kN; ++j) acc[i][j] = Half<T>::mfma(a[i], b[j], acc[i][j]);
-            if (with_sums) {
-#pragma unroll
-                for (int j = 0; j < kN; ++j) col[j] = Half<T>::mfma(ones, b[j], col[j]);
-            }
-        }
+        for (int k = 0; k < 8; ++k) ones[k] = (T)1.f;
     }
-    __syncthreads();
 
-    float* stage = reinterpret_cast<float*>(&lds[0][0][0]) + wave * 16 * kOutRow;
-    float sum[8] = {};
-    constexpr int kLanes = kW / 8;           // lanes per row of the block, 8 outputs each
-    constexpr int kRowsAtOnce = kWave / kLanes;
-    const int64_t out = out0 + kW * wo + 8 * (lane % kLanes);
-    float* part = EPI == kEpiPart ? reinterpret_cast<float*>(p.C) +
-                                        (int64_t)blockIdx.y * p.rows * p.outs : nullptr;
+    int32_t rt, ot;
+    auto load = [&](int64_t c, int buf) __attribute__((always_inline)) {
+        load_tile<T, PT, SIZE, S::waves, FAST>(p.P, p.ldp, (int64_t)rt * SIZE, p.rows, c, end,
+                                               lds[buf][0], wave, lane);
+        load_tile<T, QT, SIZE, S::waves, FAST>(p.Q, p.ldq, (int64_t)ot * SIZE, p.outs, c, end,
+                                               lds[buf][1], wave, lane);
+    };
+    int buf = 0;
+    int64_t tile = blockIdx.x;
+    tile_of(p, tile, rt, ot);
+    if (begin < end) load(begin, 0);
+    // A workgroup's tiles one after another: the next one's first step is on its
+    // way during the epilogue.
+    for (; tile < total; tile += gridDim.x) {
+        const int64_t row0 = (int64_t)rt * SIZE, out0 = (int64_t)ot * SIZE;
+        const bool with_sums = kSums && ot == 0 && wo == 0;
+        const int32_t this_rt = rt;
+        f4 acc[kNo][kNr], col[kSums ? kNr : 1];
 #pragma unroll
-    for (int j = 0; j < kN; ++j) {
-        wave_lds_order();
+        for (int j = 0; j < kNr; ++j) {
+            if constexpr (kSums) col[j] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < kN; ++i)
-            *reinterpret_cast<f4*>(&stage[r * kOutRow + 16 * i + 4 * g]) = acc[i][j];
-        wave_lds_order();
+            for (int i = 0; i < kNo; ++i) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+        }
+        for (int64_t c = begin; c < end; c += kStep, buf ^= 1) {
+            // this tile has landed (loads into LDS are waited for by hand: the barrier
+            // does not), and the last one's readers are done
+            __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
+            __syncthreads();
+            if (c + kStep < end) load(c + kStep, buf ^ 1);
+            const char* pt = lds[buf][0];
+            const char* qt = lds[buf][1];
+            v8 a[kStep / 32][kNo], b[kStep / 32][kNr];
+            auto read = [&](int f) __attribute__((always_inline)) {
 #pragma unroll
-        for (int v = 0; v < 16 / kRowsAtOnce; ++v) {
-            const int rr = v * kRowsAtOnce + lane / kLanes;
-            const float* src = &stage[rr * kOutRow + 8 * (lane % kLanes)];
-            const f4 lo = *reinterpret_cast<const f4*>(src), hi = *reinterpret_cast<const f4*>(src + 4);
-            const int64_t row = row0 + kW * wr + 16 * j + rr;
-            if constexpr (EPI == kEpiPart) {
-                if (row < p.rows && out < p.outs) {
-                    float* dst = part + row * p.outs + out;
-                    if constexpr (FAST) {
-                        *reinterpret_cast<f4*>(dst) = lo;
-                        *reinterpret_cast<f4*>(dst + 4) = hi;
-                    } else {
+                for (int i = 0; i < kNo; ++i) a[f][i] = fragment<T, QT, SIZE>(qt, kNo * wo + i, f, lane);
 #pragma unroll
-                        for (int k = 0; k < 8; ++k)
-                            if (out + k < p.outs) dst[k] = k < 4 ? lo[k & 3] : hi[k & 3];
+                for (int j = 0; j < kNr; ++j) b[f][j] = fragment<T, PT, SIZE>(pt, kNr * wr + j, f, lane);
+            };
+            // both halves' operands at once (128: 4 % faster) where there are registers
+            constexpr bool kBoth = SIZE != 256 && FAST;
+            read(0);
+            if constexpr (kBoth) {
+                __builtin_amdgcn_sched_barrier(0);
+                read(1);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int f = 0; f < kStep / 32; ++f) {
+                if (!kBoth && f) read(f);
+                if constexpr (SIZE == 256) __builtin_amdgcn_s_setprio(1);   // (4 % faster so)
+#pragma unroll
+                for (int j = 0; j < kNr; ++j)
+#pragma unroll
+                    for (int i = 0; i < kNo; ++i)
+                        acc[i][j] = Half<T>::mfma(a[f][i], b[f][j], acc[i][j]);
+                if constexpr (kSums) {
+                    if (with_sums) {
+#pragma unroll
+                        for (int j = 0; j < kNr; ++j) col[j] = Half<T>::mfma(ones, b[f][j], col[j]);
                     }
                 }
-            } else {
-                finish8<T, EPI, FAST>(p, row, out, lo, hi, sum);
+                if constexpr (SIZE == 256) __builtin_amdgcn_s_setprio(0);
             }
         }
-    }
-    if constexpr (EPI == kEpiSlope) {
-        if (p.sums) {
+        // the next tile's first step goes to `buf`, the epilogue's stages to the other
+        __syncthreads();
+        if (tile + gridDim.x < total) {
+            tile_of(p, tile + gridDim.x, rt, ot);
+            if (begin < end) load(begin, buf);
+        }
+
+        float* stage = reinterpret_cast<float*>(&lds[buf ^ 1][0][0]) + wave * 16 * kOutRow;
+        float sum[8] = {};
+        constexpr int kLanes = S::outs / 8;      // lanes per row of the block, 8 outputs each
+        constexpr int kRowsAtOnce = kWave / kLanes;
+        const int64_t out = out0 + S::outs * wo + 8 * (lane % kLanes);
+        float* part = kPart ? reinterpret_cast<float*>(p.C) + (int64_t)blockIdx.y * p.rows * p.outs
+                            : nullptr;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
+        for (int j = 0; j < kNr; ++j) {
+            wave_lds_order();
 #pragma unroll
-                for (int off = kLanes; off < kWave; off <<= 1) sum[k] += __shfl_xor(sum[k], off, kWave);
-                if (lane < kLanes && out + k < p.outs)
-                    p.sums[((int64_t)rt * 2 + wr) * p.outs + out + k] = sum[k];
+            for (int i = 0; i < kNo; ++i)
+                *reinterpret_cast<f4*>(&stage[r * kOutRow + 16 * i + 4 * g]) = acc[i][j];
+            wave_lds_order();
+#pragma unroll
+            for (int v = 0; v < 16 / kRowsAtOnce; ++v) {
+                const int rr = v * kRowsAtOnce + lane / kLanes;
+                const float* src = &stage[rr * kOutRow + 8 * (lane % kLanes)];
+                const f4 lo = *reinterpret_cast<const f4*>(src), hi = *reinterpret_cast<const f4*>(src + 4);
+                const int64_t row = row0 + S::rows * wr + 16 * j + rr;
+                if constexpr (kPart) {
+                    if (row < p.rows && out < p.outs) {
+                        float* dst = part + row * p.outs + out;
+                        if constexpr (FAST) {
+                            *reinterpret_cast<f4*>(dst) = lo;
+                            *reinterpret_cast<f4*>(dst + 4) = hi;
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 8; ++k)
+                                if (out + k < p.outs) dst[k] = k < 4 ? lo[k & 3] : hi[k & 3];
+                        }
+                    }
+                } else {
+                    finish8<T, EPI, FAST>(p, row, out, lo, hi, sum);
+                }
             }
         }
-    }
-    if constexpr (EPI == kEpiPart) {
-        if (with_sums && g == 0) {   // (every row of the ones' product is the sums)
+        if constexpr (EPI == kEpiSlope) {
+            if (p.sums) {
 #pragma unroll
-            for (int j = 0; j < kN; ++j) {
-                const int64_t row = row0 + kW * wr + 16 * j + r;
-                if (row < p.rows) p.sums[(int64_t)blockIdx.y * p.rows + row] = col[j][0];
+                for (int k = 0; k < 8; ++k) {
+#pragma unroll
+                    for (int off = kLanes; off < kWave; off <<= 1)
+                        sum[k] += __shfl_xor(sum[k], off, kWave);
+                    if (lane < kLanes && out + k < p.outs)
+                        p.sums[((int64_t)this_rt * 2 + wr) * p.outs + out + k] = sum[k];
+                }
+            }
+        }
+        if constexpr (kSums) {
+            if (with_sums && g == 0) {   // (every row of the ones' product is the sums)
+#pragma unroll
+                for (int j = 0; j < kNr; ++j) {
+                    const int64_t row = row0 + S::rows * wr + 16 * j + r;
+                    if (row < p.rows) p.sums[(int64_t)blockIdx.y * p.rows + row] = col[j][0];
+                }
             }
         }
     }
@@ -422,16 +496,141 @@ few_rows_kernel(const GemmParams p)
         for (int w = 1; w < kWaves; ++w) z += parts[w][t][lane];
         const int64_t row = 16 * t + r;
         if (row >= p.rows) continue;
+        float y[4] = {z[0], z[1], z[2], z[3]};
+        const int64_t out = out0 + 4 * g;
+        const int many = (int)min((int64_t)4, p.outs - out);
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+            if (p.bias && v < many) y[v] += (float)reinterpret_cast<const T*>(p.bias)[out + v];
+        act_values(p.act, y);
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-            const int64_t out = out0 + 4 * g + v;
-            if (out >= p.outs) break;
-            float y = z[v];
-            if (p.bias) y += (float)reinterpret_cast<const T*>(p.bias)[out];
-            y = act_value(p.act, y);
-            if (p.R) y += (float)reinterpret_cast<const T*>(p.R)[row * p.ldr + out];
-            reinterpret_cast<T*>(p.C)[row * p.outs + out] = (T)y;
+            if (v >= many) break;
+            if (p.R) y[v] += (float)reinterpret_cast<const T*>(p.R)[row * p.ldr + out + v];
+            reinterpret_cast<T*>(p.C)[row * p.outs + out + v] = (T)y[v];
         }
+    }
+}
+
+// Many rows of few inputs (K <= 256): W (or as many of its columns as 96 KB hold)
+// is laid out once per workgroup in LDS, in the order the MFMA operands are read,
+// and 16 waves stream blocks of 16 rows past it, their operands loaded straight
+// into registers, one block ahead.  W's rows are dealt to the tiles so that a lane
+// holds eight consecutive outputs of one row (two 16 x 16 tiles side by side); two
+// such pieces go through a small stage so that whole 128-byte lines are stored.
+// Bound by the rows in and out, and by the activation where it has one.
+constexpr int kRowWaves = 16, kRowPieces = 6144;
+template <typename T, int KF, bool RES>
+__global__ void __launch_bounds__(kRowWaves * kWave) __attribute__((amdgpu_waves_per_eu(4)))
+rows_kernel(const GemmParams p)
+{
+    typedef typename Half<T>::v8 v8;
+    __shared__ __align__(16) v8 wl[kRowPieces];
+    __shared__ __align__(16) T bl[kRowPieces / (4 * KF)];
+    __shared__ __align__(16) T stage[kRowWaves][16 * kStageRow];
+    const int tid = threadIdx.x, lane = tid % kWave;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int g = lane >> 4, r = lane & 15;
+    const int32_t K = (int32_t)p.depth, M = (int32_t)p.outs;
+    const int32_t cols = (int32_t)p.split;   // outputs per workgroup (blockIdx.y)
+    const int32_t m0 = blockIdx.y * cols, mc = min(cols, M - m0);   // multiples of 32
+    const T* W = reinterpret_cast<const T*>(p.Q);
+    const T* X = reinterpret_cast<const T*>(p.P);
+    const T* R = reinterpret_cast<const T*>(p.R);
+    const T* bias = reinterpret_cast<const T*>(p.bias);
+    T* Y = reinterpret_cast<T*>(p.C);
+    const v8 zero = {};
+
+    // piece (((pair * 2 + t) * KF + f) * 64 + l) is what lane l supplies for fragment
+    // f of tile t of that pair of tiles
+    for (int i = tid; i < mc * KF * 4; i += kRowWaves * kWave) {
+        const int l = i & 63, f = (i >> 6) % KF, tile = (i >> 6) / KF;
+        const int row = l & 15;
+        const int col = (tile >> 1) * 32 + 8 * (row >> 2) + 4 * (tile & 1) + (row & 3);
+        const int k = 32 * f + 8 * (l >> 4);
+        wl[i] = k < K ? *reinterpret_cast<const v8*>(W + (int64_t)(m0 + col) * p.ldq + k) : zero;
+    }
+    for (int i = tid; i < mc; i += kRowWaves * kWave) bl[i] = bias ? bias[m0 + i] : (T)0.f;
+    __syncthreads();
+
+    const int64_t blocks = (p.rows + 15) >> 4, step = (int64_t)gridDim.x * kRowWaves;
+    int64_t b = (int64_t)blockIdx.x * kRowWaves + wave;
+    if (b >= blocks) return;
+    auto load = [&](int64_t blk, v8 (&x)[KF]) __attribute__((always_inline)) {
+        const int64_t row = min(blk * 16 + r, p.rows - 1);   // (past the end: not stored)
+        const T* src = X + row * p.ldp + 8 * g;
+#pragma unroll
+        for (int f = 0; f < KF; ++f)
+            x[f] = 32 * f + 8 * g < K ? *reinterpret_cast<const v8*>(src + 32 * f) : zero;
+    };
+    v8 x[KF], nx[KF], res[2];
+    // outputs c + 8 g .. + 7 of row r of the block
+    auto product = [&](int32_t c, v8 rest) __attribute__((always_inline)) -> v8 {
+        typedef float f8 __attribute__((ext_vector_type(8)));
+        const v8* w = wl + (c >> 5) * (2 * KF * 64) + lane;
+        const f8 bf = __builtin_convertvector(*reinterpret_cast<const v8*>(&bl[c + 8 * g]), f8);
+        f4 a0 = {bf[0], bf[1], bf[2], bf[3]}, a1 = {bf[4], bf[5], bf[6], bf[7]};
+#pragma unroll
+        for (int f = 0; f < KF; ++f) {
+            a0 = Half<T>::mfma(w[f * 64], x[f], a0);
+            a1 = Half<T>::mfma(w[(KF + f) * 64], x[f], a1);
+        }
+        float y[8] = {a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
+        act_values(p.act, y);
+        if constexpr (RES) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] += (float)rest[k];
+        }
+        return __builtin_convertvector((f8{y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]}), v8);
+    };
+    auto residual = [&](int64_t blk, int32_t c) __attribute__((always_inline)) -> v8 {
+        const int64_t row = min(blk * 16 + r, p.rows - 1);
+        return *reinterpret_cast<const v8*>(R + row * p.ldr + m0 + c + 8 * g);
+    };
+    T* out = stage[wave];
+    load(b, x);
+    if constexpr (RES) {
+        res[0] = residual(b, 0);
+        if (mc >= 64) res[1] = residual(b, 32);
+    }
+    for (; b < blocks; b += step) {
+        const bool more = b + step < blocks;
+        if (more) load(b + step, nx);
+        int32_t c = 0;
+        for (; c + 64 <= mc; c += 64) {
+            const v8 now0 = res[0], now1 = res[1];
+            if constexpr (RES) {   // the next 64 columns', or the next block's first
+                const int32_t cn = c + 64 < mc ? c + 64 : 0;
+                if (cn || more) {
+                    const int64_t bn = cn ? b : b + step;
+                    res[0] = residual(bn, cn);
+                    if (cn + 64 <= mc) res[1] = residual(bn, cn + 32);
+                }
+            }
+            *reinterpret_cast<v8*>(&out[r * kStageRow + 8 * g]) = product(c, now0);
+            *reinterpret_cast<v8*>(&out[r * kStageRow + 32 + 8 * g]) = product(c + 32, now1);
+            wave_lds_order();
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                const int rr = 8 * v + (lane >> 3);
+                const v8 y = *reinterpret_cast<const v8*>(&out[rr * kStageRow + 8 * (lane & 7)]);
+                const int64_t row = b * 16 + rr;
+                if (row < p.rows) *reinterpret_cast<v8*>(Y + row * M + m0 + c + 8 * (lane & 7)) = y;
+            }
+            wave_lds_order();
+        }
+        if (c < mc) {   // 32 columns are left
+            const v8 now0 = res[0];
+            if (RES && more) {
+                res[0] = residual(b + step, 0);
+                if (mc >= 64) res[1] = residual(b + step, 32);
+            }
+            const v8 y = product(c, now0);
+            if (b * 16 + r < p.rows)
+                *reinterpret_cast<v8*>(Y + (b * 16 + r) * M + m0 + c + 8 * g) = y;
+        }
+#pragma unroll
+        for (int f = 0; f < KF; ++f) x[f] = nx[f];
     }
 }
 
@@ -462,12 +661,12 @@ join_forward(const GemmParams p, const float* __restrict__ parts)
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, count = p.rows * p.outs;
     if (i >= count) return;
     const int64_t row = i / p.outs, out = i - row * p.outs;
-    float y = 0.f;
-    for (int32_t k = 0; k < p.splits; ++k) y += parts[k * count + i];
-    if (p.bias) y += (float)reinterpret_cast<const T*>(p.bias)[out];
-    y = act_value(p.act, y);
-    if (p.R) y += (float)reinterpret_cast<const T*>(p.R)[row * p.ldr + out];
-    reinterpret_cast<T*>(p.C)[i] = (T)y;
+    float y[1] = {0.f};
+    for (int32_t k = 0; k < p.splits; ++k) y[0] += parts[k * count + i];
+    if (p.bias) y[0] += (float)reinterpret_cast<const T*>(p.bias)[out];
+    act_values(p.act, y);
+    if (p.R) y[0] += (float)reinterpret_cast<const T*>(p.R)[row * p.ldr + out];
+    reinterpret_cast<T*>(p.C)[i] = (T)y[0];
 }
 
 // Sums of the columns of in[rows][cols]: blockIdx.y's share of the rows, 64 columns
@@ -510,65 +709,117 @@ hipError_t warm_gemm(hipStream_t s)
 
 // ------------------------------------------------------------------ launches
 
-constexpr int64_t kFewRows = 64;
-constexpr int32_t kManyTiles = 512;   // two workgroups per CU
+constexpr int64_t kFewRows = 64, kManyRows = 48 * 1024;
 constexpr int64_t kSumShares = 64;
 
-// 128 x 128 tiles where they are enough for the chip's 256 CUs, else 64 x 64.
-static bool small_tiles(int64_t rows, int64_t outs)
+// Where the tiles of 256 serve: elsewhere they would need more registers than
+// there are.
+constexpr bool has_256(bool whole_pieces, int epi) { return whole_pieces && epi != kEpiPartSums; }
+
+// Size of the tiles and splits of the contraction, by what each choice would take:
+// full waves of workgroups at the rate that a large product reaches (900, 760 and
+// 580 TFLOP/s), 128 steps more for a tile's beginning and end, and for splits a
+// launch and their sums' bytes at 8 TB/s (they stay in the Infinity Cache).  (Microseconds with 64, 128, 256, chosen;
+// forward: 8,192 x 1,024 -> 1,024 32, 25, 40, 25; 200,003 x 512 -> 128 53, 55, 84,
+// 53; 2,048 x 2,048 -> 2,048 28, 28, 49, 28; 1,024 x 1,024 -> 1,024 12, 16, 25, 12.)
+struct Tiling {
+    int32_t tile, splits;
+};
+static Tiling tiling(int64_t rows, int64_t outs, int64_t depth, int64_t least, bool weights,
+                     bool sums = false)
 {
-    return ceil_div(rows, 128) * ceil_div(outs, 128) < 256;
-}
-static int64_t tiles(int64_t rows, int64_t outs, bool small)
-{
-    const int64_t t = small ? 64 : 128;
-    return ceil_div(rows, t) * ceil_div(outs, t);
-}
-// Splits of a contraction of `depth` steps: as many as give every CU two
-// workgroups, of `least` steps or more.
-static int32_t splits_for(int64_t rows, int64_t outs, int64_t depth, int64_t least)
-{
-    const int64_t t = tiles(rows, outs, small_tiles(rows, outs));
-    const int64_t want = std::min(ceil_div(kManyTiles, std::max<int64_t>(t, 1)), depth / least);
-    return (int32_t)std::max<int64_t>(1, std::min<int64_t>(want, 256));
+    struct Kind {
+        int32_t tile;
+        int64_t slots;   // workgroups at once
+        double alone;    // time of one of them alone on its CU, of that beside others
+        double rate;     // multiplications per microsecond, full chip
+    };
+    const Kind kinds[] = {{256, 256, 1.0, 450e6}, {128, 512, 0.76, 380e6},
+                          {64, 1280, 0.45, weights ? 230e6 : 290e6}};
+    Tiling best{64, 1};
+    double best_time = 1e300;
+    for (const Kind& k : kinds) {
+        if (weights && k.tile == 256 && sums) continue;
+        const int64_t n = ceil_div(rows, k.tile) * ceil_div(outs, k.tile);
+        for (int64_t s = 1; s <= 256 && (s == 1 || depth / s >= least); s += s < 4 ? 1 : s / 4) {
+            // (a wave that is not full is shorter as far as workgroups share CUs)
+            const double part = (double)(n * s % k.slots) / k.slots;
+            const double waves = (double)(n * s / k.slots) + (part > 0 ? std::max(part, k.alone) : 0);
+            double time = waves * k.slots * k.tile * k.tile * ((double)depth / s + 128) / k.rate;
+            if (weights || s > 1) time += 3.0 + (double)rows * outs * (8 * s + 2) / 8e6;
+            if (time < best_time) {
+                best_time = time;
+                best = Tiling{k.tile, (int32_t)s};
+            }
+        }
+    }
+    return best;
 }
 constexpr int64_t kForwardLeast = 512, kWeightLeast = 256;
 
 static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 template <typename T, bool PT, bool QT, int EPI, bool FAST>
-static void launch_tiles(GemmParams p, hipStream_t st)
+static void launch_tiles(GemmParams p, int32_t tile, hipStream_t st)
 {
-    const bool small = small_tiles(p.rows, p.outs);
-    const int64_t t = small ? 64 : 128;
-    p.row_tiles = (int32_t)ceil_div(p.rows, t);
-    p.out_tiles = (int32_t)ceil_div(p.outs, t);
-    p.split = ceil_div(ceil_div(p.depth, p.splits), kStep) * kStep;
-    const dim3 grid((unsigned)((int64_t)p.row_tiles * p.out_tiles), (unsigned)p.splits);
-    if (small)
+    p.row_tiles = (int32_t)ceil_div(p.rows, tile);
+    p.out_tiles = (int32_t)ceil_div(p.outs, tile);
+    p.split = ceil_div(ceil_div(p.depth, p.splits), 64) * 64;
+    // as many workgroups as are resident at once, a multiple of eight (XCDs)
+    const int64_t most = std::max<int64_t>(8, (tile == 256 ? 256 : tile == 128 ? 512 : 1280) / p.splits / 8 * 8);
+    const dim3 grid((unsigned)std::min((int64_t)p.row_tiles * p.out_tiles, most), (unsigned)p.splits);
+    if (tile == 64)
         hipLaunchKernelGGL((gemm_kernel<T, PT, QT, 64, EPI, FAST>), grid, dim3(256), 0, st, p);
-    else
+    else if (tile == 128)
         hipLaunchKernelGGL((gemm_kernel<T, PT, QT, 128, EPI, FAST>), grid, dim3(256), 0, st, p);
+    else if constexpr (has_256(FAST, EPI))
+        hipLaunchKernelGGL((gemm_kernel<T, PT, QT, 256, EPI, FAST>), grid, dim3(512), 0, st, p);
 }
 
-// FAST: whole 16-byte pieces everywhere, offsets in a tile within 31 bits.
-template <typename T, bool PT, bool QT, int EPI>
-static f3s_status launch_gemm(const GemmParams& p, hipStream_t st)
+// Whole 16-byte pieces everywhere, offsets in a tile within 31 bits.
+static bool fast(const GemmParams& p, bool pt = false, bool qt = false)
 {
     auto rows_ok = [](const char* x, int64_t ld) {
         return ((uintptr_t)x & 15) == 0 && ld % 8 == 0 && ld < (1 << 22);
     };
-    const int64_t pcols = PT ? p.rows : p.depth, qcols = QT ? p.outs : p.depth;
-    const bool fast = rows_ok(p.P, p.ldp) && rows_ok(p.Q, p.ldq) && pcols % 8 == 0 &&
-                      qcols % 8 == 0 && p.outs % 8 == 0 && ((uintptr_t)p.C & 15) == 0 &&
-                      (!p.bias || ((uintptr_t)p.bias & 15) == 0) &&
-                      (!p.R || rows_ok(p.R, p.ldr));
-    if (tiles(p.rows, p.outs, small_tiles(p.rows, p.outs)) >= ((int64_t)1 << 31)) {
+    const int64_t pcols = pt ? p.rows : p.depth, qcols = qt ? p.outs : p.depth;
+    return rows_ok(p.P, p.ldp) && rows_ok(p.Q, p.ldq) && pcols % 8 == 0 && qcols % 8 == 0 &&
+           p.outs % 8 == 0 && ((uintptr_t)p.C & 15) == 0 &&
+           (!p.bias || ((uintptr_t)p.bias & 15) == 0) && (!p.R || rows_ok(p.R, p.ldr));
+}
+
+template <typename T, bool PT, bool QT, int EPI>
+static f3s_status launch_gemm(GemmParams p, const Tiling& t, hipStream_t st)
+{
+    p.splits = t.splits;
+    if (ceil_div(p.rows, t.tile) * ceil_div(p.outs, t.tile) >= ((int64_t)1 << 31)) {
         set_error("linear: too many tiles");
         return F3S_EUNSUPPORTED;
     }
-    if (fast) launch_tiles<T, PT, QT, EPI, true>(p, st);
-    else launch_tiles<T, PT, QT, EPI, false>(p, st);
+    const bool whole = fast(p, PT, QT);
+    const int32_t tile = has_256(whole, EPI) ? t.tile : std::min(t.tile, 128);
+    if (whole) launch_tiles<T, PT, QT, EPI, true>(p, tile, st);
+    else launch_tiles<T, PT, QT, EPI, false>(p, tile, st);
+    F3S_HIP(hipGetLastError());
+    return F3S_OK;
+}
+
+template <typename T, int KF>
+static f3s_status launch_rows(GemmParams p, hipStream_t st)
+{
+    int dev = 0, cus = 0;
+    F3S_HIP(hipGetDevice(&dev));
+    F3S_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
+    constexpr int64_t most = kRowPieces / (4 * KF) / 32 * 32;
+    const int64_t ny = ceil_div(p.outs, most);
+    const int64_t unit = p.outs % 64 == 0 && most % 64 == 0 ? 64 : 32;   // whole lines where M allows
+    p.split = ceil_div(ceil_div(p.outs, ny), unit) * unit;
+    const int64_t need = ceil_div(ceil_div(p.rows, 16), kRowWaves);
+    const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(need, cus / ny)), (unsigned)ny);
+    if (p.R)
+        hipLaunchKernelGGL((rows_kernel<T, KF, true>), grid, dim3(kRowWaves * kWave), 0, st, p);
+    else
+        hipLaunchKernelGGL((rows_kernel<T, KF, false>), grid, dim3(kRowWaves * kWave), 0, st, p);
     F3S_HIP(hipGetLastError());
     return F3S_OK;
 }
@@ -576,6 +827,11 @@ static f3s_status launch_gemm(const GemmParams& p, hipStream_t st)
 template <typename T>
 static f3s_status forward(GemmParams p, void* ws, hipStream_t st)
 {
+    if (p.rows >= kManyRows && p.depth <= 256 && p.outs % 32 == 0 && p.outs <= 8192 && fast(p)) {
+        if (p.depth <= 64) return launch_rows<T, 2>(p, st);
+        if (p.depth <= 128) return launch_rows<T, 4>(p, st);
+        return launch_rows<T, 8>(p, st);
+    }
     if (p.rows <= kFewRows) {
         const bool fast = ((uintptr_t)p.P & 15) == 0 && ((uintptr_t)p.Q & 15) == 0 &&
                           p.depth % 8 == 0 && p.ldp % 8 == 0;
@@ -594,12 +850,13 @@ static f3s_status forward(GemmParams p, void* ws, hipStream_t st)
         F3S_HIP(hipGetLastError());
         return F3S_OK;
     }
-    p.splits = splits_for(p.rows, p.outs, p.depth, kForwardLeast);
-    if (p.splits == 1) return launch_gemm<T, false, false, kEpiForward>(p, st);
+    const Tiling t = tiling(p.rows, p.outs, p.depth, kForwardLeast, false);
+    if (t.splits == 1) return launch_gemm<T, false, false, kEpiForward>(p, t, st);
     GemmParams part = p;
     part.C = static_cast<char*>(ws);
     part.bias = part.R = nullptr;
-    F3S_TRY((launch_gemm<T, false, false, kEpiPart>(part, st)));
+    F3S_TRY((launch_gemm<T, false, false, kEpiPart>(part, t, st)));
+    p.splits = t.splits;
     hipLaunchKernelGGL((join_forward<T>), dim3((unsigned)ceil_div(p.rows * p.outs, 256)), dim3(256),
                        0, st, p, static_cast<const float*>(ws));
     F3S_HIP(hipGetLastError());
@@ -609,7 +866,7 @@ static f3s_status forward(GemmParams p, void* ws, hipStream_t st)
 static size_t forward_bytes(int64_t n, int64_t K, int64_t M)
 {
     if (n <= kFewRows) return 0;
-    const int32_t s = splits_for(n, M, K, kForwardLeast);
+    const int32_t s = tiling(n, M, K, kForwardLeast, false).splits;
     return s == 1 ? 0 : up256(sizeof(float) * (size_t)s * n * M);
 }
 
@@ -617,23 +874,24 @@ static size_t forward_bytes(int64_t n, int64_t K, int64_t M)
 // db's.
 struct BackwardSpace {
     size_t dz = 0, sums = 0, shares = 0, parts = 0, db = 0, bytes = 0;
-    int32_t splits = 1;
+    Tiling slope{}, dx{}, dw{};
     int64_t sum_rows = 0;
 };
 static BackwardSpace backward_space(int64_t n, int64_t K, int64_t M, int32_t act)
 {
     BackwardSpace s;
+    s.dx = tiling(n, K, M, M + 1, false);
     if (act != kActNone) {
-        const int64_t t = small_tiles(n, M) ? 64 : 128;
-        s.sum_rows = 2 * ceil_div(n, t);
+        s.slope = tiling(n, M, K, K + 1, false);
+        s.sum_rows = 2 * ceil_div(n, std::min(s.slope.tile, 64));   // (at most)
         s.dz = 0;
         s.sums = up256(2 * (size_t)n * M);
         s.shares = s.sums + up256(sizeof(float) * (size_t)s.sum_rows * M);
         s.parts = s.shares + up256(sizeof(float) * (size_t)kSumShares * M);
     }
-    s.splits = splits_for(M, K, n, kWeightLeast);
-    s.db = s.parts + up256(sizeof(float) * (size_t)s.splits * M * K);
-    s.bytes = s.db + up256(sizeof(float) * (size_t)s.splits * M);
+    s.dw = tiling(M, K, n, kWeightLeast, true, act == kActNone);
+    s.db = s.parts + up256(sizeof(float) * (size_t)s.dw.splits * M * K);
+    s.bytes = s.db + up256(sizeof(float) * (size_t)s.dw.splits * M);
     return s;
 }
 
@@ -667,16 +925,17 @@ static f3s_status backward(const LinearArgs& a, char* ws, hipStream_t st)
         p.C = ws + s.dz;
         p.sums = a.db ? reinterpret_cast<float*>(ws + s.sums) : nullptr;
         p.act = a.act;
-        p.splits = 1;
-        F3S_TRY((launch_gemm<T, false, false, kEpiSlope>(p, st)));
+        F3S_TRY((launch_gemm<T, false, false, kEpiSlope>(p, s.slope, st)));
         dz = ws + s.dz;
         lddz = a.M;
         if (db_left) {
             float* shares = reinterpret_cast<float*>(ws + s.shares);
-            const int64_t ny = std::min<int64_t>(kSumShares, s.sum_rows);
+            const int32_t tile = has_256(fast(p), kEpiSlope) ? s.slope.tile : std::min(s.slope.tile, 128);
+            const int64_t sum_rows = 2 * ceil_div(a.n, tile);
+            const int64_t ny = std::min<int64_t>(kSumShares, sum_rows);
             const unsigned nx = (unsigned)ceil_div(a.M, 64);
             hipLaunchKernelGGL((column_sums<float>), dim3(nx, (unsigned)ny), dim3(256), 0, st,
-                               p.sums, s.sum_rows, a.M, shares);
+                               p.sums, sum_rows, a.M, shares);
             hipLaunchKernelGGL((column_sums<T>), dim3(nx, 1), dim3(256), 0, st, shares, ny, a.M,
                                reinterpret_cast<T*>(a.db));
             F3S_HIP(hipGetLastError());
@@ -693,8 +952,7 @@ static f3s_status backward(const LinearArgs& a, char* ws, hipStream_t st)
         p.outs = a.K;
         p.depth = a.M;
         p.C = a.dX;
-        p.splits = 1;
-        F3S_TRY((launch_gemm<T, false, true, kEpiPlain>(p, st)));
+        F3S_TRY((launch_gemm<T, false, true, kEpiPlain>(p, s.dx, st)));
     }
     if (a.dW || db_left) {
         GemmParams p{};
@@ -707,11 +965,11 @@ static f3s_status backward(const LinearArgs& a, char* ws, hipStream_t st)
         p.depth = a.n;
         p.C = ws + s.parts;
         p.sums = db_left ? reinterpret_cast<float*>(ws + s.db) : nullptr;
-        p.splits = s.splits;
-        F3S_TRY((launch_gemm<T, true, true, kEpiPart>(p, st)));
+        if (p.sums) F3S_TRY((launch_gemm<T, true, true, kEpiPartSums>(p, s.dw, st)));
+        else F3S_TRY((launch_gemm<T, true, true, kEpiPart>(p, s.dw, st)));
         const int64_t count = a.dW ? a.M * a.K : 0, nsums = db_left ? a.M : 0;
         hipLaunchKernelGGL((join_splits<T>), dim3((unsigned)ceil_div(count + nsums, 256)), dim3(256),
-                           0, st, reinterpret_cast<const float*>(ws + s.parts), count, s.splits,
+                           0, st, reinterpret_cast<const float*>(ws + s.parts), count, s.dw.splits,
                            reinterpret_cast<T*>(a.dW), p.sums, nsums, reinterpret_cast<T*>(a.db));
         F3S_HIP(hipGetLastError());
     }
@@ -776,7 +1034,6 @@ f3s_status f3s_linear_fwd(const uint16_t* X, int64_t x_stride, const uint16_t* W
     p.ldr = r_stride;
     p.C = reinterpret_cast<char*>(Y);
     p.act = act;
-    p.splits = 1;
     if (dtype == F3S_F16) return forward<_Float16>(p, workspace, as_stream(stream));
     return forward<__bf16>(p, workspace, as_stream(stream));
 }

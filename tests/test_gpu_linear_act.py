@@ -12,8 +12,8 @@ F = torch.nn.functional
 ACTS = {None: lambda z: z, "relu": F.relu, "gelu": F.gelu, "silu": F.silu,
         "gelu_tanh": lambda z: F.gelu(z, approximate="tanh")}
 # What is left of an activation's value and slope beside its rounding to float32:
-# erf to 1.5e-7 (half of that in Phi), hardware exponentials and reciprocals to a
-# few units of float32's last place, for |z| up to 2^6 in the exponent.
+# Phi to 2e-7 and z Phi to 6e-7, hardware exponentials and reciprocals to a few
+# units of float32's last place, for |z| up to 2^6 in the exponent.
 ACT_ABS = 2.0 ** -17
 STEP = 2.0 ** -24
 
@@ -86,6 +86,8 @@ SIZES = [
     (300, 2048, 65), (300, 2056, 72),                                      # split contraction
     (1003, 100, 301), (1000, 128, 384), (2000, 333, 64), (515, 512, 1032),
     (4100, 264, 1096), (16400, 72, 512), (33000, 16, 136),                  # 128 x 128 tiles
+    (49_152, 8, 32), (49_167, 64, 96), (50_001, 136, 416), (49_153, 256, 224),   # W in LDS
+    (60_000, 128, 640),
 ]
 
 
