@@ -1157,12 +1157,12 @@ struct PassSpace {
 };
 static PassSpace pass_space(const f3s_plan* plan)
 {
-    PassSpace s;
-    s.odd = 2 * kQueueBytes;
-    s.partials = s.odd;
-    if (plan->masked.team == 1)
-        s.partials += round_up(sizeof(uint32_t) * (size_t)plan->masked.num_items * plan->H);
-    s.bytes = s.partials + partial_bytes(plan);
+    PassSpace s{0, 0, 0};   // (teams merge in LDS)
+    if (plan->masked.team == 1) {
+        s.odd = 2 * kQueueBytes;
+        s.partials = s.odd + round_up(sizeof(uint32_t) * (size_t)plan->masked.num_items * plan->H);
+        s.bytes = s.partials + partial_bytes(plan);
+    }
     return s;
 }
 static void set_space(DiffParams& p, const f3s_plan* plan, char* ws, int pass)
@@ -1234,8 +1234,8 @@ f3s_status f3s_diff_attention_fwd(const f3s_plan* plan, const uint16_t* Q, int64
                     rows_ok(O, o_stride, H) && lam && ((uintptr_t)lse & 7) == 0,
                 "f3s_diff_attention_fwd: NULL or misaligned pointer, or a row stride that is no "
                 "multiple of 8 or below H * 128");
-    F3S_REQUIRE(workspace_bytes >= (int64_t)pass_space(plan).bytes && workspace &&
-                    ((uintptr_t)workspace & 15) == 0,
+    F3S_REQUIRE(workspace_bytes >= (int64_t)pass_space(plan).bytes &&
+                    (workspace || pass_space(plan).bytes == 0) && ((uintptr_t)workspace & 15) == 0,
                 "f3s_diff_attention_fwd: workspace too small");
     F3S_TRY(require_device());
     clear_error();
@@ -1274,7 +1274,8 @@ f3s_status f3s_diff_attention_bwd(const f3s_plan* plan, const f3s_plan* reversed
                 "multiple of 8 or below H * 128");
     int64_t need = 0;
     F3S_TRY(f3s_diff_attention_workspace(plan, reversed, &need));
-    F3S_REQUIRE(workspace_bytes >= need && workspace && ((uintptr_t)workspace & 15) == 0,
+    F3S_REQUIRE(workspace_bytes >= need && (workspace || need == 0) &&
+                    ((uintptr_t)workspace & 15) == 0,
                 "f3s_diff_attention_bwd: workspace too small");
     F3S_TRY(require_device());
     clear_error();

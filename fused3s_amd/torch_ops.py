@@ -53,6 +53,7 @@ if len(_hip_runtimes()) > 1:
                       "): import torch before the first fused3s_amd GPU call")
 
 import ctypes as C
+import functools
 
 from . import _lib
 from .attention import Plan
@@ -61,6 +62,11 @@ from .graph import (DeviceBSF, DeviceCSR, convert_device, converts_once, lists_o
                     most_tiles, window_order_device)
 
 HEAD_DIM = 64
+
+# torch's current stream on a device as a number, without a Stream object around it
+# (a small graph's pass is shorter than making one)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 class _TorchStream(Stream):
@@ -123,6 +129,7 @@ class TorchGraph:
         if masked:
             self.plan.compile(s)
         self.device = torch.cuda.current_device()
+        self._torch_device = torch.device("cuda", self.device)
         self._scheduled: Plan | None = None  # diff_attention's plan, where it is not self.plan
         self._reversed: Plan | None = None   # the reversed edges' (prepare_backward)
         self._workspace = {}
@@ -237,24 +244,26 @@ class TorchGraph:
                 C.byref(need)),
                 "f3s_diff_attention_workspace")
             size = self._workspace[backward] = need.value
-        return torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
+        return torch.empty(size, dtype=torch.uint8, device=self._torch_device) if size else None
 
-    def _check_diff(self, lam, scale, **tensors) -> None:
+    def _check_diff(self, lam, tensors) -> None:
+        """Raises for tensors (by name) that diff_attention does not take."""
         if not self.masked:
             raise ValueError("differential attention is edge-exact: it needs masked=True")
-        if torch.cuda.current_device() != self.device:
+        if _current_device() != self.device:
             raise ValueError(f"the graph is on device {self.device}, which is not the current one")
-        n, H = self.n, self.heads
-        if (lam.dtype != torch.float32 or not lam.is_cuda or lam.device.index != self.device
-                or lam.shape != (H,)):
-            raise ValueError(f"lam must be a float32 tensor of {H} weights on the graph's device")
+        device = self._torch_device
+        if lam.dtype is not torch.float32 or lam.device != device or lam.shape != (self.heads,):
+            raise ValueError(f"lam must be a float32 tensor of {self.heads} weights on the graph's "
+                             "device")
         dtype = None
-        for name, t in tensors.items():
-            if (t.dtype not in _DTYPES or not t.is_cuda or t.device.index != self.device
-                    or (dtype or t.dtype) != t.dtype):
+        for name, t, *shapes in tensors:
+            if t.dtype not in _DTYPES or t.device != device or (dtype or t.dtype) is not t.dtype:
                 raise ValueError(f"{name} must be a float16 or bfloat16 tensor on the graph's "
                                  "device, all of one type")
             dtype = t.dtype
+            if t.shape not in shapes:
+                raise ValueError(f"{name} must have shape {shapes[0]}, got {tuple(t.shape)}")
 
     def diff_attention(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor,
                        scale: float = 1.0) -> torch.Tensor:
@@ -267,11 +276,8 @@ class TorchGraph:
         lam: float32 [H].  Returns [n, H, 128] in q's type: sums in float32,
         rounded once; nodes without edges get 0.  Differentiable in q, k, v and
         lam (once).  A graph serves any number of calls at once."""
-        shape = (self.n, self.heads, 2 * HEAD_DIM)
-        self._check_diff(lam, scale, q=q, k=k, v=v)
-        for name, t in (("q", q), ("k", k), ("v", v)):
-            if t.shape != shape and t.shape != (self.n, self.heads * 2 * HEAD_DIM):
-                raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
+        shape, flat = (self.n, self.heads, 2 * HEAD_DIM), (self.n, self.heads * 2 * HEAD_DIM)
+        self._check_diff(lam, (("q", q, shape, flat), ("k", k, shape, flat), ("v", v, shape, flat)))
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                         or lam.requires_grad):
             self.prepare_backward()
@@ -283,10 +289,7 @@ class TorchGraph:
         """diff_attention() on the [n, 3 * H * 128] output of one projection (q,
         k and v side by side in each row), whose gradient is then one tensor
         too, written in place of its thirds."""
-        self._check_diff(lam, scale, qkv=qkv)
-        if qkv.shape != (self.n, 3 * self.heads * 2 * HEAD_DIM):
-            raise ValueError(f"qkv must have shape {(self.n, 3 * self.heads * 2 * HEAD_DIM)}, "
-                             f"got {tuple(qkv.shape)}")
+        self._check_diff(lam, (("qkv", qkv, (self.n, 3 * self.heads * 2 * HEAD_DIM)),))
         if torch.is_grad_enabled() and (qkv.requires_grad or lam.requires_grad):
             self.prepare_backward()
             return _DiffAttention.apply(self, float(scale), lam, qkv)
@@ -300,6 +303,8 @@ def _rows(t: torch.Tensor, graph: TorchGraph) -> torch.Tensor:
     """[n, width] with each row contiguous, 16-byte aligned: t itself where its
     layout is that already."""
     n, width = graph.n, graph.heads * 2 * HEAD_DIM
+    if t.is_contiguous() and t.stride(0) == width and t.data_ptr() % 16 == 0:
+        return t.view(n, width) if t.dim() == 3 else t
     if t.dim() == 3 and (t.stride(2) != 1 or t.stride(1) != 2 * HEAD_DIM and graph.heads > 1):
         t = t.contiguous()
     if t.dim() == 3:
@@ -323,16 +328,18 @@ def _stride(t: torch.Tensor) -> int:
 
 def _diff_forward(graph: TorchGraph, scale: float, lam, q, k, v, lse=None) -> torch.Tensor:
     n, H = graph.n, graph.heads
-    out = torch.empty((n, H, 2 * HEAD_DIM), dtype=q.dtype, device=q.device)
+    out = q.new_empty((n, H, 2 * HEAD_DIM))
     if n:
+        plan = graph._diff_plan().handle
         ws = graph._diff_workspace(False)
-        lam = lam.contiguous()
+        if not lam.is_contiguous():
+            lam = lam.contiguous()
         check(_lib.hip().f3s_diff_attention_fwd(
-            graph._diff_plan().handle, q.data_ptr(), _stride(q), k.data_ptr(), _stride(k), v.data_ptr(),
-            _stride(v), lam.data_ptr(), out.data_ptr(), H * 2 * HEAD_DIM,
-            lse.data_ptr() if lse is not None else None, _DTYPES[q.dtype], n, H, scale,
-            ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
-            torch.cuda.current_stream().cuda_stream), "f3s_diff_attention_fwd")
+            plan, q.data_ptr(), _stride(q), k.data_ptr(), _stride(k), v.data_ptr(), _stride(v),
+            lam.data_ptr(), out.data_ptr(), H * 2 * HEAD_DIM,
+            None if lse is None else lse.data_ptr(), _DTYPES[q.dtype], n, H, scale,
+            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
+            _raw_stream(graph.device)), "f3s_diff_attention_fwd")
     return out
 
 
@@ -373,7 +380,7 @@ class _DiffAttention(torch.autograd.Function):
                 do.data_ptr(), _stride(do), dq.data_ptr(), _stride(dq), dk.data_ptr(), _stride(dk),
                 dv.data_ptr(), _stride(dv), dlam.data_ptr(), _DTYPES[q.dtype], n, H, ctx.scale,
                 ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
-                torch.cuda.current_stream().cuda_stream), "f3s_diff_attention_bwd")
+                _raw_stream(graph.device)), "f3s_diff_attention_bwd")
         return None, None, dlam, *grads
 
 
@@ -381,11 +388,17 @@ class _DiffAttention(torch.autograd.Function):
 _ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
 
-def _linear_workspace(n, K, M, act, backward, device):
+@functools.lru_cache(maxsize=256)
+def _linear_bytes(n, K, M, act, backward) -> int:
     need = C.c_int64()
     check(_lib.hip().f3s_linear_workspace(n, K, M, act, backward, C.byref(need)),
           "f3s_linear_workspace")
-    return torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+    return need.value
+
+
+def _linear_workspace(n, K, M, act, backward, device):
+    size = _linear_bytes(n, K, M, act, backward)
+    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
 
 
 def _matrix(t: torch.Tensor) -> torch.Tensor:
@@ -396,7 +409,7 @@ def _matrix(t: torch.Tensor) -> torch.Tensor:
 
 def _linear_forward(x, w, b, r, act):
     (n, K), M = x.shape, w.shape[0]
-    y = torch.empty((n, M), dtype=x.dtype, device=x.device)
+    y = x.new_empty((n, M))
     if n:
         ws = _linear_workspace(n, K, M, act, 0, x.device) if n > 64 else None
         check(_lib.hip().f3s_linear_fwd(
@@ -404,7 +417,7 @@ def _linear_forward(x, w, b, r, act):
             r.data_ptr() if r is not None else None, _stride(r) if r is not None else 0,
             y.data_ptr(), n, K, M, act, _DTYPES[x.dtype],
             ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
-            torch.cuda.current_stream().cuda_stream), "f3s_linear_fwd")
+            _raw_stream(x.device.index)), "f3s_linear_fwd")
     return y
 
 
@@ -435,7 +448,7 @@ class _Linear(torch.autograd.Function):
                     b.data_ptr() if b is not None else None, dy.data_ptr(), _stride(dy),
                     *(t.data_ptr() if t is not None else None for t in (dx, dw, db)), n, K, M, act,
                     _DTYPES[x.dtype], ws.data_ptr() if ws is not None else None,
-                    ws.numel() if ws is not None else 0, torch.cuda.current_stream().cuda_stream),
+                    ws.numel() if ws is not None else 0, _raw_stream(x.device.index)),
                     "f3s_linear_bwd")
         return dx, dw, db, grad if needs[3] else None, None
 
@@ -447,7 +460,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     GPU; activation None, "relu", "gelu", "gelu_tanh" or "silu".  Sums and
     epilogue are in float32, the result is rounded once.  Differentiable (once);
     for the backward pass the product is computed again rather than kept."""
-    if activation not in _ACTIVATIONS:
+    act = _ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"activation must be one of {list(_ACTIVATIONS)}, got {activation!r}")
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"x [..., K] and weight [M, K] do not fit: {tuple(x.shape)}, "
@@ -455,33 +469,34 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     M, K = weight.shape
     if M == 0 or K == 0:
         raise ValueError("weight must not be empty")
-    shape = (*x.shape[:-1], M)
-    if bias is not None and bias.shape != (M,):
-        raise ValueError(f"bias must have shape {(M,)}, got {tuple(bias.shape)}")
-    if residual is not None and residual.shape != shape:
-        raise ValueError(f"residual must have shape {shape}, got {tuple(residual.shape)}")
+    dtype, device = x.dtype, x.device
     for name, t in (("x", x), ("weight", weight), ("bias", bias), ("residual", residual)):
-        if t is not None and (t.dtype not in _DTYPES or t.dtype != x.dtype or not t.is_cuda
-                              or t.device != x.device):
+        if t is not None and (t.dtype is not dtype or t.device != device
+                              or dtype not in _DTYPES or not t.is_cuda):
             raise ValueError(f"{name} must be a float16 or bfloat16 tensor on a GPU, of x's type "
                              "and device")
-    if x.device.index != torch.cuda.current_device():
-        with torch.cuda.device(x.device):
+    if bias is not None and bias.shape != (M,):
+        raise ValueError(f"bias must have shape {(M,)}, got {tuple(bias.shape)}")
+    flat = x.dim() == 2
+    shape = (x.shape[0], M) if flat else (*x.shape[:-1], M)
+    if residual is not None and residual.shape != shape:
+        raise ValueError(f"residual must have shape {shape}, got {tuple(residual.shape)}")
+    if device.index != _current_device():
+        with torch.cuda.device(device):
             return linear(x, weight, bias, activation, residual)
-    act = _ACTIVATIONS[activation]
-    x2 = _matrix(x if x.dim() == 2 else x.reshape(-1, K))
+    x2 = _matrix(x if flat else x.reshape(-1, K))
     w = weight if weight.is_contiguous() else weight.contiguous()
     b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
     r = residual
     if r is not None:
-        r = _matrix(r if r.dim() == 2 else r.reshape(-1, M))
+        r = _matrix(r if flat else r.reshape(-1, M))
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
                                     or bias is not None and bias.requires_grad
                                     or residual is not None and residual.requires_grad):
         y = _Linear.apply(x2, w, b, r, act)
     else:
         y = _linear_forward(x2, w, b, r, act)
-    return y if x.dim() == 2 else y.view(shape)
+    return y if flat else y.view(shape)
 
 
 _LINEAR_FORWARD, _LINEAR = torch.nn.Linear.forward, torch.nn.functional.linear
