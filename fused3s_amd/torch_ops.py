@@ -469,18 +469,18 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     M, K = weight.shape
     if M == 0 or K == 0:
         raise ValueError("weight must not be empty")
-    dtype, device = x.dtype, x.device
-    for name, t in (("x", x), ("weight", weight), ("bias", bias), ("residual", residual)):
-        if t is not None and (t.dtype is not dtype or t.device != device
-                              or dtype not in _DTYPES or not t.is_cuda):
-            raise ValueError(f"{name} must be a float16 or bfloat16 tensor on a GPU, of x's type "
-                             "and device")
     if bias is not None and bias.shape != (M,):
         raise ValueError(f"bias must have shape {(M,)}, got {tuple(bias.shape)}")
     flat = x.dim() == 2
     shape = (x.shape[0], M) if flat else (*x.shape[:-1], M)
     if residual is not None and residual.shape != shape:
         raise ValueError(f"residual must have shape {shape}, got {tuple(residual.shape)}")
+    dtype, device = x.dtype, x.device
+    for name, t in (("x", x), ("weight", weight), ("bias", bias), ("residual", residual)):
+        if t is not None and (t.dtype is not dtype or t.device != device
+                              or dtype not in _DTYPES or not t.is_cuda):
+            raise ValueError(f"{name} must be a float16 or bfloat16 tensor on a GPU, of x's type "
+                             "and device")
     if device.index != _current_device():
         with torch.cuda.device(device):
             return linear(x, weight, bias, activation, residual)
