@@ -11,13 +11,13 @@
 //   dx       P = dz [n][M],     Q = W, transposed
 //   dW       P, Q = dz, x, both transposed, n cut into splits whose float32
 //            sums are added in order; db with it
-// A workgroup of four waves owns a block of C and goes through the contraction in
-// steps: both operands' tiles go from memory straight into LDS (16 bytes a lane, no
-// registers), ahead of the products, in an order in which neither plain nor
-// transposing LDS reads meet bank conflicts.  Q is the MFMA's A operand,
-// so a lane holds four consecutive outputs of a row; the epilogue passes them
-// through LDS, 16 rows at a time, so that whole lines are read (residual, dy) and
-// written.
+// A workgroup owns a block of C and goes through the contraction in steps: both
+// operands' tiles go from memory straight into LDS (16 bytes a lane, no registers),
+// ahead of the products, in an order in which neither plain nor transposing LDS
+// reads meet bank conflicts.  Q is the MFMA's A operand, so a lane holds four
+// consecutive outputs of a row; the epilogue passes them through LDS, 16 rows at a
+// time, so that whole lines are read (residual, dy) and written.  Two kernels of
+// their own: a few rows, and many rows of few inputs.
 #include <algorithm>
 
 #include "half_types.hpp"
@@ -42,7 +42,8 @@ struct GemmParams {
     const char* R;        // residual (forward, NULL: none) or dy (slope)
     int64_t ldr;
     char* C;              // [rows][outs]
-    float* sums;          // slope: [row tiles][2][outs]; splits of dW: [splits][rows], NULL: none
+    float* sums;          // NULL: none; slope: [row tiles][2][outs], rows_kernel [workgroups][outs];
+                          // splits of dW: [splits][rows]
     int64_t split;        // contraction steps per split (a multiple of 64)
     int32_t act;
     int32_t row_tiles, out_tiles, splits;
@@ -512,22 +513,62 @@ few_rows_kernel(const GemmParams p)
     }
 }
 
+// Sums over a row's 16 lanes of eight values each: lane r is left with those of
+// values 4 (r & 1) + 2 (r >> 1 & 1) + {0, 1}.
+template <int CTRL>
+__device__ __forceinline__ float from_lane(float x)
+{
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 0xf,
+                                                              0xf, true));
+}
+__device__ __forceinline__ f2 row_sums(const float (&v)[8], int r)
+{
+    constexpr int kXor1 = 0xb1, kXor2 = 0x4e, kRor4 = 0x124, kRor8 = 0x128;
+    float a[4], c[2];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float keep = r & 1 ? v[k + 4] : v[k], give = r & 1 ? v[k] : v[k + 4];
+        a[k] = keep + from_lane<kXor1>(give);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const float keep = r & 2 ? a[k + 2] : a[k], give = r & 2 ? a[k] : a[k + 2];
+        c[k] = keep + from_lane<kXor2>(give);
+        c[k] += from_lane<kRor4>(c[k]);
+        c[k] += from_lane<kRor8>(c[k]);
+    }
+    return f2{c[0], c[1]};
+}
+
 // Many rows of few inputs (K <= 256): W (or as many of its columns as 96 KB hold)
 // is laid out once per workgroup in LDS, in the order the MFMA operands are read,
 // and 16 waves stream blocks of 16 rows past it, their operands loaded straight
 // into registers, one block ahead.  W's rows are dealt to the tiles so that a lane
 // holds eight consecutive outputs of one row (two 16 x 16 tiles side by side); two
 // such pieces go through a small stage so that whole 128-byte lines are stored.
-// Bound by the rows in and out, and by the activation where it has one.
+// MODE: act(z + bias), + R, or dy act'(z + bias) and the sums of its columns (a
+// wave's own in LDS, joined in order at the end).
+// Bound by the rows in and out, and by the activation where it has one (gelu: 20
+// operations' time a value).
+enum RowsMode : int { kRowsAct = 0, kRowsResidual = 1, kRowsSlope = 2 };
 constexpr int kRowWaves = 16, kRowPieces = 6144;
-template <typename T, int KF, bool RES>
+// outputs per workgroup at most
+constexpr int rows_cols(int kf, int mode)
+{
+    const int most = kRowPieces / (4 * kf);
+    return mode == kRowsSlope && most > 384 ? 384 : most;   // (the sums: 64 bytes of LDS each)
+}
+template <typename T, int KF, int MODE>
 __global__ void __launch_bounds__(kRowWaves * kWave) __attribute__((amdgpu_waves_per_eu(4)))
 rows_kernel(const GemmParams p)
 {
+    constexpr bool RES = MODE != kRowsAct, SLOPE = MODE == kRowsSlope;
+    constexpr int kCols = rows_cols(KF, MODE);
     typedef typename Half<T>::v8 v8;
     __shared__ __align__(16) v8 wl[kRowPieces];
-    __shared__ __align__(16) T bl[kRowPieces / (4 * KF)];
+    __shared__ __align__(16) T bl[kCols];
     __shared__ __align__(16) T stage[kRowWaves][16 * kStageRow];
+    __shared__ __align__(16) float sums[SLOPE ? kRowWaves : 1][SLOPE ? kCols : 1];
     const int tid = threadIdx.x, lane = tid % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int g = lane >> 4, r = lane & 15;
@@ -551,11 +592,13 @@ rows_kernel(const GemmParams p)
         wl[i] = k < K ? *reinterpret_cast<const v8*>(W + (int64_t)(m0 + col) * p.ldq + k) : zero;
     }
     for (int i = tid; i < mc; i += kRowWaves * kWave) bl[i] = bias ? bias[m0 + i] : (T)0.f;
+    if constexpr (SLOPE)
+        for (int i = tid; i < kRowWaves * kCols; i += kRowWaves * kWave) sums[0][i] = 0.f;
     __syncthreads();
 
     const int64_t blocks = (p.rows + 15) >> 4, step = (int64_t)gridDim.x * kRowWaves;
     int64_t b = (int64_t)blockIdx.x * kRowWaves + wave;
-    if (b >= blocks) return;
+    if (!SLOPE && b >= blocks) return;
     auto load = [&](int64_t blk, v8 (&x)[KF]) __attribute__((always_inline)) {
         const int64_t row = min(blk * 16 + r, p.rows - 1);   // (past the end: not stored)
         const T* src = X + row * p.ldp + 8 * g;
@@ -576,8 +619,24 @@ rows_kernel(const GemmParams p)
             a1 = Half<T>::mfma(w[(KF + f) * 64], x[f], a1);
         }
         float y[8] = {a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
-        act_values(p.act, y);
-        if constexpr (RES) {
+        if constexpr (SLOPE) {
+            act_slopes(p.act, y);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] *= (float)rest[k];
+            if (p.sums) {
+                float own[8];   // (a row past the end repeats the last one)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) own[k] = b * 16 + r < p.rows ? y[k] : 0.f;
+                const f2 s = row_sums(own, r);
+                if (r < 4) {
+                    f2* to = reinterpret_cast<f2*>(&sums[wave][c + 8 * g + 4 * (r & 1) + (r & 2)]);
+                    *to = f2{(*to)[0] + s[0], (*to)[1] + s[1]};
+                }
+            }
+        } else {
+            act_values(p.act, y);
+        }
+        if constexpr (MODE == kRowsResidual) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) y[k] += (float)rest[k];
         }
@@ -631,6 +690,14 @@ rows_kernel(const GemmParams p)
         }
 #pragma unroll
         for (int f = 0; f < KF; ++f) x[f] = nx[f];
+    }
+    if constexpr (SLOPE) {
+        __syncthreads();
+        if (p.sums && tid < mc) {
+            float s = 0.f;
+            for (int w = 0; w < kRowWaves; ++w) s += sums[w][tid];
+            p.sums[(int64_t)blockIdx.x * M + m0 + tid] = s;
+        }
     }
 }
 
@@ -719,9 +786,10 @@ constexpr bool has_256(bool whole_pieces, int epi) { return whole_pieces && epi 
 // Size of the tiles and splits of the contraction, by what each choice would take:
 // full waves of workgroups at the rate that a large product reaches (900, 760 and
 // 580 TFLOP/s), 128 steps more for a tile's beginning and end, and for splits a
-// launch and their sums' bytes at 8 TB/s (they stay in the Infinity Cache).  (Microseconds with 64, 128, 256, chosen;
-// forward: 8,192 x 1,024 -> 1,024 32, 25, 40, 25; 200,003 x 512 -> 128 53, 55, 84,
-// 53; 2,048 x 2,048 -> 2,048 28, 28, 49, 28; 1,024 x 1,024 -> 1,024 12, 16, 25, 12.)
+// launch and their sums' bytes at 8 TB/s (they stay in the Infinity Cache).
+// (Microseconds with 64, 128, 256, chosen; forward: 8,192 x 1,024 -> 1,024 32, 25,
+// 40, 25; 200,003 x 512 -> 128 53, 55, 84, 53; 2,048 x 2,048 -> 2,048 28, 28, 49, 28;
+// 1,024 x 1,024 -> 1,024 12, 16, 25, 12.)
 struct Tiling {
     int32_t tile, splits;
 };
@@ -804,22 +872,46 @@ static f3s_status launch_gemm(GemmParams p, const Tiling& t, hipStream_t st)
     return F3S_OK;
 }
 
-template <typename T, int KF>
-static f3s_status launch_rows(GemmParams p, hipStream_t st)
+// Many rows of few inputs (rows_kernel; W's columns of a workgroup are no fewer than
+// 192, and the rows are read once for each so many).  Microseconds so and by tiles,
+// no activation, M of 384 to 4,096: 50,000 x 128 -> 384 15 and 20; 100,000 x 256 ->
+// 4,096 304 and 370; 100,000 x 32 -> 4,096 183 and 232; 500,000 x 128 -> 512 136 and
+// 227; but 20,000 x 128 -> 384 13 and 10, 20,000 x 256 -> 256 11.3 and 10.8.  With
+// gelu's slope and its sums: 50,000 x 128 -> 384 38 and 45, 100,000 x 256 -> 4,096 579
+// and 805, 500,000 x 128 -> 512 350 and 511; but 20,000 x 128 -> 384 36 and 23.
+static bool takes_rows(const GemmParams& p)
 {
-    int dev = 0, cus = 0;
-    F3S_HIP(hipGetDevice(&dev));
-    F3S_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
-    constexpr int64_t most = kRowPieces / (4 * KF) / 32 * 32;
+    return p.rows >= kManyRows && p.depth <= 256 && p.outs % 32 == 0 && p.outs <= 8192 && fast(p);
+}
+
+template <typename T, int KF, int MODE>
+static void launch_rows(GemmParams p, int32_t cus, int64_t* workgroups, hipStream_t st)
+{
+    constexpr int64_t most = rows_cols(KF, MODE) / 32 * 32;
     const int64_t ny = ceil_div(p.outs, most);
     const int64_t unit = p.outs % 64 == 0 && most % 64 == 0 ? 64 : 32;   // whole lines where M allows
     p.split = ceil_div(ceil_div(p.outs, ny), unit) * unit;
     const int64_t need = ceil_div(ceil_div(p.rows, 16), kRowWaves);
-    const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(need, cus / ny)), (unsigned)ny);
-    if (p.R)
-        hipLaunchKernelGGL((rows_kernel<T, KF, true>), grid, dim3(kRowWaves * kWave), 0, st, p);
-    else
-        hipLaunchKernelGGL((rows_kernel<T, KF, false>), grid, dim3(kRowWaves * kWave), 0, st, p);
+    *workgroups = std::max<int64_t>(1, std::min<int64_t>(need, cus / ny));
+    hipLaunchKernelGGL((rows_kernel<T, KF, MODE>), dim3((unsigned)*workgroups, (unsigned)ny),
+                       dim3(kRowWaves * kWave), 0, st, p);
+}
+
+template <typename T>
+static f3s_status many_rows(const GemmParams& p, bool slope, int64_t* workgroups, hipStream_t st)
+{
+    int dev = 0, cus = 0;
+    F3S_HIP(hipGetDevice(&dev));
+    F3S_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
+    auto go = [&](auto kf) {
+        constexpr int KF = decltype(kf)::value;
+        if (slope) launch_rows<T, KF, kRowsSlope>(p, cus, workgroups, st);
+        else if (p.R) launch_rows<T, KF, kRowsResidual>(p, cus, workgroups, st);
+        else launch_rows<T, KF, kRowsAct>(p, cus, workgroups, st);
+    };
+    if (p.depth <= 64) go(std::integral_constant<int, 2>{});
+    else if (p.depth <= 128) go(std::integral_constant<int, 4>{});
+    else go(std::integral_constant<int, 8>{});
     F3S_HIP(hipGetLastError());
     return F3S_OK;
 }
@@ -827,10 +919,9 @@ static f3s_status launch_rows(GemmParams p, hipStream_t st)
 template <typename T>
 static f3s_status forward(GemmParams p, void* ws, hipStream_t st)
 {
-    if (p.rows >= kManyRows && p.depth <= 256 && p.outs % 32 == 0 && p.outs <= 8192 && fast(p)) {
-        if (p.depth <= 64) return launch_rows<T, 2>(p, st);
-        if (p.depth <= 128) return launch_rows<T, 4>(p, st);
-        return launch_rows<T, 8>(p, st);
+    if (takes_rows(p)) {
+        int64_t workgroups;
+        return many_rows<T>(p, false, &workgroups, st);
     }
     if (p.rows <= kFewRows) {
         const bool fast = ((uintptr_t)p.P & 15) == 0 && ((uintptr_t)p.Q & 15) == 0 &&
@@ -870,8 +961,8 @@ static size_t forward_bytes(int64_t n, int64_t K, int64_t M)
     return s == 1 ? 0 : up256(sizeof(float) * (size_t)s * n * M);
 }
 
-// Workspace of a backward call: dz, the sums of its columns (act), dW's splits,
-// db's.
+// Workspace of a backward call: dz, the sums of its columns and their shares (act),
+// dW's splits, db's.
 struct BackwardSpace {
     size_t dz = 0, sums = 0, shares = 0, parts = 0, db = 0, bytes = 0;
     Tiling slope{}, dx{}, dw{};
@@ -925,14 +1016,20 @@ static f3s_status backward(const LinearArgs& a, char* ws, hipStream_t st)
         p.C = ws + s.dz;
         p.sums = a.db ? reinterpret_cast<float*>(ws + s.sums) : nullptr;
         p.act = a.act;
-        F3S_TRY((launch_gemm<T, false, false, kEpiSlope>(p, s.slope, st)));
+        int64_t sum_rows;
+        if (takes_rows(p)) {
+            F3S_TRY(many_rows<T>(p, true, &sum_rows, st));
+        } else {
+            const int32_t tile = has_256(fast(p), kEpiSlope) ? s.slope.tile
+                                                             : std::min(s.slope.tile, 128);
+            sum_rows = 2 * ceil_div(a.n, tile);
+            F3S_TRY((launch_gemm<T, false, false, kEpiSlope>(p, s.slope, st)));
+        }
         dz = ws + s.dz;
         lddz = a.M;
         if (db_left) {
             float* shares = reinterpret_cast<float*>(ws + s.shares);
-            const int32_t tile = has_256(fast(p), kEpiSlope) ? s.slope.tile : std::min(s.slope.tile, 128);
-            const int64_t sum_rows = 2 * ceil_div(a.n, tile);
-            const int64_t ny = std::min<int64_t>(kSumShares, sum_rows);
+            const int64_t ny = std::min<int64_t>(kSumShares, ceil_div(sum_rows, 16));
             const unsigned nx = (unsigned)ceil_div(a.M, 64);
             hipLaunchKernelGGL((column_sums<float>), dim3(nx, (unsigned)ny), dim3(256), 0, st,
                                p.sums, sum_rows, a.M, shares);
@@ -961,7 +1058,7 @@ static f3s_status backward(const LinearArgs& a, char* ws, hipStream_t st)
         p.Q = a.X;
         p.ldq = a.ldx;
         p.rows = a.M;
-        p.outs = a.K;
+        p.outs = a.dW ? a.K : std::min<int64_t>(a.K, 8);   // (db alone: one column of tiles)
         p.depth = a.n;
         p.C = ws + s.parts;
         p.sums = db_left ? reinterpret_cast<float*>(ws + s.db) : nullptr;

@@ -119,6 +119,21 @@ def test_some_gradients(gpu):
                 assert torch.equal(g, every[name]), (leaves, name)
 
 
+@pytest.mark.parametrize("dtype", HALF)
+def test_many_rows_gradients(gpu, dtype):
+    """Rows enough for W in LDS, in both passes: blocks of rows that do not divide
+    among the workgroups, outputs that need two turns of 384, a last row alone, no
+    bias, a bias but no gradient of it; every run gives the same bits."""
+    for n, K, M, act, bias in ((49_169, 128, 416, "gelu", True), (70_001, 64, 800, "silu", True),
+                               (49_152, 248, 224, "gelu_tanh", True),
+                               (50_000, 32, 32, "relu", False)):
+        t = make(n, K, M, dtype, bias=bias, residual=False, seed=2)
+        got = step(t, act)
+        check(t, act, got)
+        for name, g in step(t, act, "xw").items():
+            assert torch.equal(g, got[name]), (n, name)
+
+
 @pytest.mark.parametrize("act", [None, "silu"])
 def test_layouts(gpu, act):
     """Rows at a distance, unaligned starts, transposed weights, more dimensions,
