@@ -142,42 +142,87 @@ __device__ __forceinline__ int place_steps(int row)
         return (row & 2) | (((row >> 3) & 1) << 2);
 }
 
-// Loads one operand's tile, rows (or outputs) from `first` and steps from `step`,
-// into LDS at `lds`.  FAST: rows 16-byte aligned, whole pieces inside or outside.
-template <typename T, bool TRANS, int TILE, int WAVES, bool FAST>
-__device__ __forceinline__ void load_tile(const char* base, int64_t ld, int64_t first, int64_t count,
-                                          int64_t step, int64_t end, char* lds, int wave, int lane)
-{
-    constexpr int kPieces = (TRANS ? TILE : kStep) / 8;     // per stored row
-    constexpr int kLoads = TILE * kStep * 2 / 1024 / WAVES;  // 1,024 bytes per wave and load
-    // stored rows and columns from here on
-    const int64_t r0 = TRANS ? step : first, c0 = TRANS ? first : step;
-    const int64_t rows = (TRANS ? end : count) - r0, cols = (TRANS ? count : end) - c0;
-    const char* src = base + (r0 * ld + c0) * 2;
-    const int row_in = lane / kPieces, pos = lane % kPieces;
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-        const int chunk = i * WAVES + wave;
-        const int row = chunk * (64 / kPieces) + row_in;
-        const int piece = pos ^ (TRANS ? place_steps<TILE>(row) : place_rows(row));
-        char* to = lds + chunk * 1024;
-        if constexpr (FAST) {
-            const __amdgpu_buffer_rsrc_t rs = make_rsrc(src, 0x7fffffffu);
-            const bool in = row < rows && piece * 8 < cols;
-            const uint32_t at = in ? (uint32_t)(row * (int32_t)ld + piece * 8) * 2 : 0xffffff00u;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                rs, (__attribute__((address_space(3))) void*)to, 16, (int)at, 0, 0, 0);
-        } else {
-            typename Half<T>::v8 v = {};
-            const T* p = reinterpret_cast<const T*>(src) + row * ld + piece * 8;
-            if (row < rows) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (piece * 8 + k < cols) v[k] = p[k];
-            }
-            *reinterpret_cast<typename Half<T>::v8*>(to + lane * 16) = v;
-        }
+// One operand's tile, rows (or outputs) from `first` and steps from `step`: the
+// places of its pieces.  `in` says whether piece i of a lane is (in part) inside.
+template <bool TRANS, int TILE, int WAVES>
+struct TileAt {
+    static constexpr int pieces = (TRANS ? TILE : kStep) / 8;        // per stored row
+    static constexpr int loads = TILE * kStep * 2 / 1024 / WAVES;    // 1,024 bytes per wave and load
+    int64_t rows, cols;   // stored rows and columns from here on
+    const char* src;
+    __device__ __forceinline__ TileAt(const char* base, int64_t ld, int64_t first, int64_t count,
+                                      int64_t step, int64_t end)
+    {
+        const int64_t r0 = TRANS ? step : first, c0 = TRANS ? first : step;
+        rows = (TRANS ? end : count) - r0;
+        cols = (TRANS ? count : end) - c0;
+        src = base + (r0 * ld + c0) * 2;
     }
+    static __device__ __forceinline__ int chunk(int i, int wave) { return i * WAVES + wave; }
+    static __device__ __forceinline__ int row(int i, int wave, int lane)
+    {
+        return chunk(i, wave) * (64 / pieces) + lane / pieces;
+    }
+    static __device__ __forceinline__ int piece(int row, int lane)
+    {
+        return (lane % pieces) ^ (TRANS ? place_steps<TILE>(row) : place_rows(row));
+    }
+};
+
+// Straight into LDS.  Rows 16-byte aligned, whole pieces inside or outside.
+template <bool TRANS, int TILE, int WAVES>
+__device__ __forceinline__ void load_tile(const TileAt<TRANS, TILE, WAVES>& t, int64_t ld, char* lds,
+                                          int wave, int lane)
+{
+#pragma unroll
+    for (int i = 0; i < t.loads; ++i) {
+        const int row = t.row(i, wave, lane), piece = t.piece(row, lane);
+        const __amdgpu_buffer_rsrc_t rs = make_rsrc(t.src, 0x7fffffffu);
+        const bool in = row < t.rows && piece * 8 < t.cols;
+        const uint32_t at = in ? (uint32_t)(row * (int32_t)ld + piece * 8) * 2 : 0xffffff00u;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rs, (__attribute__((address_space(3))) void*)(lds + t.chunk(i, wave) * 1024), 16, (int)at,
+            0, 0, 0);
+    }
+}
+
+// Any alignment and width: through registers, whose contents go to LDS (put_tile)
+// when the products of the step before are done.  A piece that its row ends in is
+// read whole where another row follows (its address stays inside then), and what is
+// not the row's becomes zero.
+template <typename V>
+struct __attribute__((packed, aligned(2))) Unaligned {
+    V v;
+};
+template <typename T, bool TRANS, int TILE, int WAVES, typename V = typename Half<T>::v8>
+__device__ __forceinline__ void fetch_tile(const TileAt<TRANS, TILE, WAVES>& t, int64_t ld, V* to,
+                                           int wave, int lane)
+{
+#pragma unroll
+    for (int i = 0; i < t.loads; ++i) {
+        const int row = t.row(i, wave, lane), piece = t.piece(row, lane);
+        const T* p = reinterpret_cast<const T*>(t.src) + row * ld + piece * 8;
+        const int64_t left = row < t.rows ? t.cols - piece * 8 : 0;
+        const bool whole = left >= 8 || (left > 0 && ld >= 8 && row + 1 < t.rows);
+        V v = {};
+        if (whole) v = reinterpret_cast<const Unaligned<V>*>(p)->v;
+        if (left < 8) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (!whole && k < left) v[k] = p[k];
+                if (k >= left) v[k] = (T)0.f;
+            }
+        }
+        to[i] = v;
+    }
+}
+template <bool TRANS, int TILE, int WAVES, typename V>
+__device__ __forceinline__ void put_tile(const V* from, char* lds, int wave, int lane)
+{
+    typedef TileAt<TRANS, TILE, WAVES> At;
+#pragma unroll
+    for (int i = 0; i < At::loads; ++i)
+        *reinterpret_cast<V*>(lds + At::chunk(i, wave) * 1024 + lane * 16) = from[i];
 }
 
 // Operand fragment: 16 rows from 16 t, contraction 32 f + 8 g ..
@@ -316,16 +361,34 @@ gemm_kernel(const GemmParams p)
     }
 
     int32_t rt, ot;
+    typedef TileAt<PT, SIZE, S::waves> AtP;
+    typedef TileAt<QT, SIZE, S::waves> AtQ;
+    v8 held_p[FAST ? 1 : AtP::loads], held_q[FAST ? 1 : AtQ::loads];
+    // step c's tiles into buffer buf; not FAST: on their way, put() brings them there
     auto load = [&](int64_t c, int buf) __attribute__((always_inline)) {
-        load_tile<T, PT, SIZE, S::waves, FAST>(p.P, p.ldp, (int64_t)rt * SIZE, p.rows, c, end,
-                                               lds[buf][0], wave, lane);
-        load_tile<T, QT, SIZE, S::waves, FAST>(p.Q, p.ldq, (int64_t)ot * SIZE, p.outs, c, end,
-                                               lds[buf][1], wave, lane);
+        const AtP at_p(p.P, p.ldp, (int64_t)rt * SIZE, p.rows, c, end);
+        const AtQ at_q(p.Q, p.ldq, (int64_t)ot * SIZE, p.outs, c, end);
+        if constexpr (FAST) {
+            load_tile(at_p, p.ldp, lds[buf][0], wave, lane);
+            load_tile(at_q, p.ldq, lds[buf][1], wave, lane);
+        } else {
+            fetch_tile<T>(at_p, p.ldp, held_p, wave, lane);
+            fetch_tile<T>(at_q, p.ldq, held_q, wave, lane);
+        }
+    };
+    auto put = [&](int buf) __attribute__((always_inline)) {
+        if constexpr (!FAST) {
+            put_tile<PT, SIZE, S::waves>(held_p, lds[buf][0], wave, lane);
+            put_tile<QT, SIZE, S::waves>(held_q, lds[buf][1], wave, lane);
+        }
     };
     int buf = 0;
     int64_t tile = blockIdx.x;
     tile_of(p, tile, rt, ot);
-    if (begin < end) load(begin, 0);
+    if (begin < end) {
+        load(begin, 0);
+        put(0);
+    }
     // A workgroup's tiles one after another: the next one's first step is on its
     // way during the epilogue.
     for (; tile < total; tile += gridDim.x) {
@@ -379,6 +442,7 @@ gemm_kernel(const GemmParams p)
                 }
                 if constexpr (SIZE == 256) __builtin_amdgcn_s_setprio(0);
             }
+            if (c + kStep < end) put(buf ^ 1);
         }
         // the next tile's first step goes to `buf`, the epilogue's stages to the other
         __syncthreads();
@@ -445,6 +509,7 @@ gemm_kernel(const GemmParams p)
                 }
             }
         }
+        if (tile + gridDim.x < total && begin < end) put(buf);
     }
 }
 
@@ -720,6 +785,38 @@ join_splits(const float* __restrict__ parts, int64_t count, int32_t splits, T* _
     }
 }
 
+// The same for the slope pass: dz, and the sums of the columns of blockIdx.y's share
+// of the rows; 64 columns per workgroup.
+template <typename T>
+__global__ void __launch_bounds__(256)
+join_slope(const GemmParams p, const float* __restrict__ parts)
+{
+    __shared__ float lds[4][64];
+    const int64_t col = (int64_t)blockIdx.x * 64 + threadIdx.x % 64, count = p.rows * p.outs;
+    const int part = threadIdx.x / 64;
+    const int64_t per = (p.rows + gridDim.y - 1) / gridDim.y;
+    const int64_t r0 = blockIdx.y * per, r1 = min(p.rows, r0 + per);
+    float sum = 0.f;
+    if (col < p.outs) {
+        const float bias = p.bias ? (float)reinterpret_cast<const T*>(p.bias)[col] : 0.f;
+        for (int64_t row = r0 + part; row < r1; row += 4) {
+            float z[1] = {0.f};
+            for (int32_t k = 0; k < p.splits; ++k) z[0] += parts[k * count + row * p.outs + col];
+            z[0] += bias;
+            act_slopes(p.act, z);
+            z[0] *= (float)reinterpret_cast<const T*>(p.R)[row * p.ldr + col];
+            sum += z[0];
+            reinterpret_cast<T*>(p.C)[row * p.outs + col] = (T)z[0];
+        }
+    }
+    lds[part][threadIdx.x % 64] = sum;
+    __syncthreads();
+    if (p.sums && part == 0 && col < p.outs) {
+        const int t = threadIdx.x;
+        p.sums[blockIdx.y * p.outs + col] = (lds[0][t] + lds[1][t]) + (lds[2][t] + lds[3][t]);
+    }
+}
+
 // The same, finished as the forward pass is (a short, deep product).
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -962,7 +1059,7 @@ static size_t forward_bytes(int64_t n, int64_t K, int64_t M)
 }
 
 // Workspace of a backward call: dz, the sums of its columns and their shares (act),
-// dW's splits, db's.
+// the splits of the products (one after another), db's.
 struct BackwardSpace {
     size_t dz = 0, sums = 0, shares = 0, parts = 0, db = 0, bytes = 0;
     Tiling slope{}, dx{}, dw{};
@@ -971,9 +1068,12 @@ struct BackwardSpace {
 static BackwardSpace backward_space(int64_t n, int64_t K, int64_t M, int32_t act)
 {
     BackwardSpace s;
-    s.dx = tiling(n, K, M, M + 1, false);
+    s.dx = tiling(n, K, M, kForwardLeast, false);
+    size_t parts = s.dx.splits > 1 ? sizeof(float) * (size_t)s.dx.splits * n * K : 0;
     if (act != kActNone) {
-        s.slope = tiling(n, M, K, K + 1, false);
+        s.slope = tiling(n, M, K, kForwardLeast, false);
+        if (s.slope.splits > 1)
+            parts = std::max(parts, sizeof(float) * (size_t)s.slope.splits * n * M);
         s.sum_rows = 2 * ceil_div(n, std::min(s.slope.tile, 64));   // (at most)
         s.dz = 0;
         s.sums = up256(2 * (size_t)n * M);
@@ -981,7 +1081,8 @@ static BackwardSpace backward_space(int64_t n, int64_t K, int64_t M, int32_t act
         s.parts = s.shares + up256(sizeof(float) * (size_t)kSumShares * M);
     }
     s.dw = tiling(M, K, n, kWeightLeast, true, act == kActNone);
-    s.db = s.parts + up256(sizeof(float) * (size_t)s.dw.splits * M * K);
+    parts = std::max(parts, sizeof(float) * (size_t)s.dw.splits * M * K);
+    s.db = s.parts + up256(parts);
     s.bytes = s.db + up256(sizeof(float) * (size_t)s.dw.splits * M);
     return s;
 }
@@ -993,6 +1094,17 @@ struct LinearArgs {
     int64_t n, K, M;
     int32_t act;
 };
+
+template <typename T>
+static f3s_status join(const char* parts, int64_t count, int32_t splits, char* out, const float* sums,
+                       int64_t nsums, char* db, hipStream_t st)
+{
+    hipLaunchKernelGGL((join_splits<T>), dim3((unsigned)ceil_div(count + nsums, 256)), dim3(256), 0,
+                       st, reinterpret_cast<const float*>(parts), count, splits,
+                       reinterpret_cast<T*>(out), sums, nsums, reinterpret_cast<T*>(db));
+    F3S_HIP(hipGetLastError());
+    return F3S_OK;
+}
 
 template <typename T>
 static f3s_status backward(const LinearArgs& a, char* ws, hipStream_t st)
@@ -1019,6 +1131,16 @@ static f3s_status backward(const LinearArgs& a, char* ws, hipStream_t st)
         int64_t sum_rows;
         if (takes_rows(p)) {
             F3S_TRY(many_rows<T>(p, true, &sum_rows, st));
+        } else if (s.slope.splits > 1) {
+            GemmParams part = p;
+            part.C = ws + s.parts;
+            part.bias = part.R = nullptr;
+            F3S_TRY((launch_gemm<T, false, false, kEpiPart>(part, s.slope, st)));
+            p.splits = s.slope.splits;
+            sum_rows = ceil_div(a.n, 32);
+            hipLaunchKernelGGL((join_slope<T>), dim3((unsigned)ceil_div(a.M, 64), (unsigned)sum_rows),
+                               dim3(256), 0, st, p, reinterpret_cast<const float*>(ws + s.parts));
+            F3S_HIP(hipGetLastError());
         } else {
             const int32_t tile = has_256(fast(p), kEpiSlope) ? s.slope.tile
                                                              : std::min(s.slope.tile, 128);
@@ -1049,7 +1171,13 @@ static f3s_status backward(const LinearArgs& a, char* ws, hipStream_t st)
         p.outs = a.K;
         p.depth = a.M;
         p.C = a.dX;
-        F3S_TRY((launch_gemm<T, false, true, kEpiPlain>(p, s.dx, st)));
+        if (s.dx.splits == 1) {
+            F3S_TRY((launch_gemm<T, false, true, kEpiPlain>(p, s.dx, st)));
+        } else {
+            p.C = ws + s.parts;
+            F3S_TRY((launch_gemm<T, false, true, kEpiPart>(p, s.dx, st)));
+            F3S_TRY((join<T>(ws + s.parts, a.n * a.K, s.dx.splits, a.dX, nullptr, 0, nullptr, st)));
+        }
     }
     if (a.dW || db_left) {
         GemmParams p{};
@@ -1065,10 +1193,7 @@ static f3s_status backward(const LinearArgs& a, char* ws, hipStream_t st)
         if (p.sums) F3S_TRY((launch_gemm<T, true, true, kEpiPartSums>(p, s.dw, st)));
         else F3S_TRY((launch_gemm<T, true, true, kEpiPart>(p, s.dw, st)));
         const int64_t count = a.dW ? a.M * a.K : 0, nsums = db_left ? a.M : 0;
-        hipLaunchKernelGGL((join_splits<T>), dim3((unsigned)ceil_div(count + nsums, 256)), dim3(256),
-                           0, st, reinterpret_cast<const float*>(ws + s.parts), count, s.dw.splits,
-                           reinterpret_cast<T*>(a.dW), p.sums, nsums, reinterpret_cast<T*>(a.db));
-        F3S_HIP(hipGetLastError());
+        F3S_TRY((join<T>(ws + s.parts, count, s.dw.splits, a.dW, p.sums, nsums, a.db, st)));
     }
     return F3S_OK;
 }
