@@ -461,7 +461,8 @@ __device__ __forceinline__ void diff_finish(const DiffParams& p, DiffState& st, 
     const uint32_t head_off = (uint32_t)h * kHeadBytes;
     if constexpr (PASS == kDiffForward) {
         const float l1 = over_groups(st.y[0]), l2 = over_groups(st.y[1]);
-        const bool some = l1 != 0.f;   // (a row of NaN is some)
+        // (a row of NaN is some; one map's logits all -inf: 0 / 0)
+        const bool some = l1 != 0.f || l2 != 0.f;
         const float f1 = some ? 1.f / l1 : 0.f, f2 = some ? lam / l2 : 0.f;
         store_rows<T>(p.out1, stage, w, p.n, head_off, lane, [&](int t) {
             const f4 o = st.acc[t] * f1 - st.acc[8 + t] * f2;

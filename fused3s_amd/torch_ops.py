@@ -52,6 +52,7 @@ if len(_hip_runtimes()) > 1:
     raise ImportError("two HIP runtimes are loaded (" + ", ".join(sorted(_hip_runtimes())) +
                       "): import torch before the first fused3s_amd GPU call")
 
+import contextlib
 import ctypes as C
 import functools
 
@@ -67,6 +68,14 @@ HEAD_DIM = 64
 # (a small graph's pass is shorter than making one)
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
+
+
+_NO_CONTEXT = contextlib.nullcontext()
+
+
+def _on(device: int):
+    """The device as the current one (an autograd thread's own is that already)."""
+    return _NO_CONTEXT if _current_device() == device else torch.cuda.device(device)
 
 
 class _TorchStream(Stream):
@@ -192,7 +201,9 @@ class TorchGraph:
     def prepare_backward(self) -> "TorchGraph":
         """Builds what the gradient of diff_attention reads, a compiled plan of
         the reversed edges; the first call that needs it does so otherwise.
-        Waits for the GPU, so before a capture."""
+        Waits for the GPU, so before a capture.  (The leaves of a captured step
+        must not belong to an eager step that is still alive, as with torch's
+        own operators: capture with detached ones.)"""
         if self._reversed is None:
             if not self.masked:
                 raise ValueError("a gradient needs the masked (edge-exact) semantics")
@@ -365,14 +376,14 @@ class _DiffAttention(torch.autograd.Function):
         lam, lse, *tensors = ctx.saved_tensors
         packed = len(tensors) == 1
         q, k, v = _thirds(tensors[0], graph) if packed else (_rows(t, graph) for t in tensors)
-        grads = [torch.empty(shape, dtype=q.dtype, device=q.device) for shape in ctx.shapes]
+        grads = [q.new_empty(shape) for shape in ctx.shapes]
         if packed:
             dq, dk, dv = (grads[0][:, i * width:(i + 1) * width] for i in range(3))
         else:
             dq, dk, dv = (t.view(n, width) for t in grads)
         dlam = torch.empty_like(lam)
         do = _rows(grad, graph)
-        with torch.cuda.device(graph.device):
+        with _on(graph.device):
             ws = graph._diff_workspace(True)
             check(_lib.hip().f3s_diff_attention_bwd(
                 graph._diff_plan().handle, graph._reversed.handle, q.data_ptr(), _stride(q),
@@ -436,12 +447,11 @@ class _Linear(torch.autograd.Function):
         x, w, b = ctx.saved_tensors
         (n, K), M, act = x.shape, w.shape[0], ctx.act
         needs = ctx.needs_input_grad
-        empty = lambda wanted, *shape: (torch.empty(shape, dtype=x.dtype, device=x.device)
-                                        if wanted else None)
+        empty = lambda wanted, *shape: x.new_empty(shape) if wanted else None
         dx, dw, db = empty(needs[0], n, K), empty(needs[1], M, K), empty(needs[2], M)
         if any(needs[:3]):
             dy = _matrix(grad)
-            with torch.cuda.device(x.device):
+            with _on(x.device.index):
                 ws = _linear_workspace(n, K, M, act, 1, x.device)
                 check(_lib.hip().f3s_linear_bwd(
                     x.data_ptr(), _stride(x), w.data_ptr(),

@@ -185,6 +185,34 @@ def test_odd_values_stay_with_their_edges(gpu, value, H, n):
             assert not torch.isfinite(got["o"][sources, H - 1]).any()
 
 
+@pytest.mark.parametrize("n", [40, 4000])
+def test_logits_of_minus_infinity(gpu, n):
+    """Every logit of a row -inf: NaN where one map's are, in either place, 0 where
+    both maps' are, and rows with a finite logit among theirs as if it were alone."""
+    from fused3s_amd.torch_ops import TorchGraph
+    rp = np.arange(0, 2 * n + 1, 2, dtype=np.int32)      # row i: i and i + 1
+    ci = np.sort(np.stack([np.arange(n), (np.arange(n) + 1) % n], 1), 1).reshape(-1).astype(np.int32)
+    graph = TorchGraph(rp, ci, heads=1)
+    q, k, v, lam, _ = inputs(n, 1, torch.float16, 5)
+    q = q.abs() + 0.125
+    at = {1: slice(0, 64), 2: slice(64, 128), 3: slice(0, 128)}
+    for first, maps in ((4, 1), (12, 2), (20, 3)):       # nodes first .. first + 2
+        k[first:first + 3, 0, at[maps]] = -float("inf")
+    o = graph.diff_attention(q, k, v, lam, 0.125)
+    nan = torch.isnan(o).flatten(1).all(1)
+    assert nan[[4, 5, 12, 13]].all() and int(nan.sum()) == 4
+    assert not o[20:22].any() and bool(torch.isfinite(o[~nan]).all())
+    # row 3 attends nodes 3 and 4, node 4 by its second map only
+    w = torch.softmax(torch.stack([(q[3, 0, 64:].double() * k[j, 0, 64:].double()).sum() * 0.125
+                                   for j in (3, 4)]), 0)
+    want = v[3, 0].double() - lam.double() * (w[0] * v[3, 0].double() + w[1] * v[4, 0].double())
+    size = v[3, 0].double().abs() + lam.abs() * v[3:5, 0].double().abs().sum(0)
+    # 64 products and 3 more roundings of 2^-24 in a logit of at most 16, twice
+    # that as a weight's relative error, and the output's rounding
+    bound = 2 * 67 * 2.0 ** -24 * 16 * size + want.abs() * 2.0 ** -11 + 2.0 ** -25
+    assert bool(((o[3, 0].double() - want).abs() <= bound).all())
+
+
 def test_linear_in_values_and_weights(gpu):
     """o is linear in v and in lam, so its differences there are its derivatives
     times the step, up to the rounding of the two o's."""
