@@ -127,6 +127,11 @@ __device__ __forceinline__ void act_slopes(int act, float (&z)[N])
 
 constexpr int kStep = 64;   // contraction steps per tile
 
+template <typename V>
+struct __attribute__((packed, aligned(2))) Unaligned {
+    V v;
+};
+
 // Where piece p (16 bytes) of a stored row lies in LDS, by exclusive or.  Row by
 // row, 128 bytes each: the pieces of one number that 16 rows' lanes read together
 // lie in distinct banks.
@@ -190,10 +195,6 @@ __device__ __forceinline__ void load_tile(const TileAt<TRANS, TILE, WAVES>& t, i
 // when the products of the step before are done.  A piece that its row ends in is
 // read whole where another row follows (its address stays inside then), and what is
 // not the row's becomes zero.
-template <typename V>
-struct __attribute__((packed, aligned(2))) Unaligned {
-    V v;
-};
 template <typename T, bool TRANS, int TILE, int WAVES, typename V = typename Half<T>::v8>
 __device__ __forceinline__ void fetch_tile(const TileAt<TRANS, TILE, WAVES>& t, int64_t ld, V* to,
                                            int wave, int lane)
@@ -269,57 +270,61 @@ __device__ __forceinline__ void tile_of(const GemmParams& p, int64_t b, int32_t&
     out = (int32_t)(in / size);
 }
 
-// Eight values at C's (row, out ..) from float32: bias, activation, residual, rounding.
+// Eight values of an operand from `out` of `left` there are.
+template <typename T, bool FAST>
+__device__ __forceinline__ typename Half<T>::v8 load8(const T* src, int64_t left)
+{
+    typename Half<T>::v8 v = {};
+    if constexpr (FAST) {   // (whole pieces)
+        if (left > 0) v = *reinterpret_cast<const typename Half<T>::v8*>(src);
+    } else if (left >= 8) {
+        v = reinterpret_cast<const Unaligned<typename Half<T>::v8>*>(src)->v;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < left) v[k] = src[k];
+    }
+    return v;
+}
+
+// Eight values at C's (row, out ..) from float32: bias, activation, residual (or dy),
+// rounding.
 template <typename T, int EPI, bool FAST>
 __device__ __forceinline__ void finish8(const GemmParams& p, int64_t row, int64_t out, f4 lo, f4 hi,
+                                        typename Half<T>::v8 bias, typename Half<T>::v8 r,
                                         float (&sum)[8])
 {
     typedef typename Half<T>::v8 v8;
     float z[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     const int64_t left = p.outs - out;
     if (row >= p.rows || left <= 0) return;
-    const int many = FAST ? 8 : (int)min((int64_t)8, left);   // (FAST: outs % 8 == 0)
-    auto load = [&](const T* src, float (&x)[8]) __attribute__((always_inline)) {
-        if constexpr (FAST) {
-            const v8 v = *reinterpret_cast<const v8*>(src);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] = (float)v[k];
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] = k < many ? (float)src[k] : 0.f;
-        }
-    };
     if constexpr (EPI == kEpiForward || EPI == kEpiSlope) {
-        if (p.bias) {
-            float b[8];
-            load(reinterpret_cast<const T*>(p.bias) + out, b);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) z[k] += b[k];
-        }
-        float r[8] = {};
-        if (p.R) load(reinterpret_cast<const T*>(p.R) + row * p.ldr + out, r);
+        for (int k = 0; k < 8; ++k) z[k] += (float)bias[k];
         if constexpr (EPI == kEpiForward) {
             act_values(p.act, z);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) z[k] += r[k];
+            for (int k = 0; k < 8; ++k) z[k] += (float)r[k];
         } else {
             act_slopes(p.act, z);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                z[k] *= r[k];
+                z[k] *= (float)r[k];
                 sum[k] += z[k];
             }
         }
     }
     T* dst = reinterpret_cast<T*>(p.C) + row * p.outs + out;
+    typedef float f8 __attribute__((ext_vector_type(8)));
+    const v8 y = __builtin_convertvector((f8{z[0], z[1], z[2], z[3], z[4], z[5], z[6], z[7]}), v8);
     if constexpr (FAST) {
-        typedef float f8 __attribute__((ext_vector_type(8)));
-        *reinterpret_cast<v8*>(dst) = __builtin_convertvector(
-            (f8{z[0], z[1], z[2], z[3], z[4], z[5], z[6], z[7]}), v8);
+        *reinterpret_cast<v8*>(dst) = y;
+    } else if (left >= 8) {
+        reinterpret_cast<Unaligned<v8>*>(dst)->v = y;
     } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-            if (k < many) dst[k] = (T)z[k];
+            if (k < left) dst[k] = y[k];
     }
 }
 
@@ -444,6 +449,33 @@ gemm_kernel(const GemmParams p)
             }
             if (c + kStep < end) put(buf ^ 1);
         }
+        constexpr int kLanes = S::outs / 8;      // lanes per row of the block, 8 outputs each
+        constexpr int kRowsAtOnce = kWave / kLanes, kTurns = 16 / kRowsAtOnce;
+        const int64_t out = out0 + S::outs * wo + 8 * (lane % kLanes);
+        auto row_of = [&](int j, int v) __attribute__((always_inline)) -> int64_t {
+            return row0 + S::rows * wr + 16 * j + v * kRowsAtOnce + lane / kLanes;
+        };
+        // The residual's (dy's) rows, 64 asked for ahead (a wait for each 16 rows:
+        // 32,768 x 1,024 -> 4,096, gelu's slope 444 us); not FAST: where they are used,
+        // the next step holds the registers.
+        constexpr bool kEnds = EPI == kEpiForward || EPI == kEpiSlope;
+        constexpr int kAhead = !(kEnds && FAST) ? 1 : kNr < 4 ? kNr : 4;
+        v8 bias = {}, res[kAhead][kTurns] = {};
+        auto residual = [&](int j, int v) __attribute__((always_inline)) -> v8 {
+            const int64_t row = row_of(j, v);
+            if (!p.R || row >= p.rows) return v8{};
+            return load8<T, FAST>(reinterpret_cast<const T*>(p.R) + row * p.ldr + out, p.outs - out);
+        };
+        if constexpr (kEnds) {
+            if (p.bias)
+                bias = load8<T, FAST>(reinterpret_cast<const T*>(p.bias) + out, p.outs - out);
+            if constexpr (FAST) {
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+                    for (int v = 0; v < kTurns; ++v) res[j][v] = residual(j, v);
+            }
+        }
         // the next tile's first step goes to `buf`, the epilogue's stages to the other
         __syncthreads();
         if (tile + gridDim.x < total) {
@@ -453,9 +485,6 @@ gemm_kernel(const GemmParams p)
 
         float* stage = reinterpret_cast<float*>(&lds[buf ^ 1][0][0]) + wave * 16 * kOutRow;
         float sum[8] = {};
-        constexpr int kLanes = S::outs / 8;      // lanes per row of the block, 8 outputs each
-        constexpr int kRowsAtOnce = kWave / kLanes;
-        const int64_t out = out0 + S::outs * wo + 8 * (lane % kLanes);
         float* part = kPart ? reinterpret_cast<float*>(p.C) + (int64_t)blockIdx.y * p.rows * p.outs
                             : nullptr;
 #pragma unroll
@@ -466,11 +495,11 @@ gemm_kernel(const GemmParams p)
                 *reinterpret_cast<f4*>(&stage[r * kOutRow + 16 * i + 4 * g]) = acc[i][j];
             wave_lds_order();
 #pragma unroll
-            for (int v = 0; v < 16 / kRowsAtOnce; ++v) {
+            for (int v = 0; v < kTurns; ++v) {
                 const int rr = v * kRowsAtOnce + lane / kLanes;
                 const float* src = &stage[rr * kOutRow + 8 * (lane % kLanes)];
                 const f4 lo = *reinterpret_cast<const f4*>(src), hi = *reinterpret_cast<const f4*>(src + 4);
-                const int64_t row = row0 + S::rows * wr + 16 * j + rr;
+                const int64_t row = row_of(j, v);
                 if constexpr (kPart) {
                     if (row < p.rows && out < p.outs) {
                         float* dst = part + row * p.outs + out;
@@ -484,7 +513,14 @@ gemm_kernel(const GemmParams p)
                         }
                     }
                 } else {
-                    finish8<T, EPI, FAST>(p, row, out, lo, hi, sum);
+                    v8 other = {};
+                    if constexpr (kEnds && FAST) {
+                        other = res[j % kAhead][v];
+                        if (j + kAhead < kNr) res[j % kAhead][v] = residual(j + kAhead, v);
+                    } else if constexpr (kEnds) {
+                        other = residual(j, v);
+                    }
+                    finish8<T, EPI, FAST>(p, row, out, lo, hi, bias, other, sum);
                 }
             }
         }
@@ -766,23 +802,45 @@ rows_kernel(const GemmParams p)
     }
 }
 
-// Splits of a product added in their order; `rows x outs` values, and (db) the
-// sums that came with them.
-template <typename T>
+// Splits of a product added: `count` values, and (db) the sums that came with them.
+// WAYS 1: a thread for each value; 4: a wave for each quarter of the splits of 64
+// values, the quarters added in order.  (50 splits of 128 x 512: 26 us and 10; one of
+// 4,096 x 4,096: 35 and 90.  So 4 from 9 splits on, more than one turn of loads.)
+__device__ __forceinline__ float split_sum(const float* __restrict__ at, int64_t stride,
+                                           int32_t first, int32_t end)
+{
+    float s = 0.f;
+    for (int32_t k = first; k < end; k += 8) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = k + i < end ? at[(k + i) * stride] : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += x[i];
+    }
+    return s;
+}
+template <typename T, int WAYS>
 __global__ void __launch_bounds__(256)
 join_splits(const float* __restrict__ parts, int64_t count, int32_t splits, T* __restrict__ out,
             const float* __restrict__ sums, int64_t nsums, T* __restrict__ db)
 {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < count) {
-        float s = 0.f;
-        for (int32_t k = 0; k < splits; ++k) s += parts[k * count + i];
-        out[i] = (T)s;
-    } else if (i < count + nsums) {
-        float s = 0.f;
-        for (int32_t k = 0; k < splits; ++k) s += sums[k * nsums + i - count];
-        db[i - count] = (T)s;
+    constexpr int kValues = 256 / WAYS;
+    const int t = threadIdx.x % kValues, way = threadIdx.x / kValues;
+    const int64_t i = (int64_t)blockIdx.x * kValues + t;
+    const int32_t per = (splits + WAYS - 1) / WAYS, first = way * per, end = min(splits, first + per);
+    float s = 0.f;
+    if (i < count) s = split_sum(parts + i, count, first, end);
+    else if (i < count + nsums) s = split_sum(sums + i - count, nsums, first, end);
+    if constexpr (WAYS > 1) {
+        __shared__ float lds[WAYS][kValues];
+        lds[way][t] = s;
+        __syncthreads();
+        if (way) return;
+#pragma unroll
+        for (int w = 1; w < WAYS; ++w) s += lds[w][t];
     }
+    if (i < count) out[i] = (T)s;
+    else if (i < count + nsums) db[i - count] = (T)s;
 }
 
 // The same for the slope pass: dz, and the sums of the columns of blockIdx.y's share
@@ -1099,9 +1157,15 @@ template <typename T>
 static f3s_status join(const char* parts, int64_t count, int32_t splits, char* out, const float* sums,
                        int64_t nsums, char* db, hipStream_t st)
 {
-    hipLaunchKernelGGL((join_splits<T>), dim3((unsigned)ceil_div(count + nsums, 256)), dim3(256), 0,
-                       st, reinterpret_cast<const float*>(parts), count, splits,
-                       reinterpret_cast<T*>(out), sums, nsums, reinterpret_cast<T*>(db));
+    auto go = [&](auto ways) {
+        constexpr int kWays = decltype(ways)::value;
+        hipLaunchKernelGGL((join_splits<T, kWays>),
+                           dim3((unsigned)ceil_div(count + nsums, 256 / kWays)), dim3(256), 0, st,
+                           reinterpret_cast<const float*>(parts), count, splits,
+                           reinterpret_cast<T*>(out), sums, nsums, reinterpret_cast<T*>(db));
+    };
+    if (splits <= 8) go(std::integral_constant<int, 1>{});
+    else go(std::integral_constant<int, 4>{});
     F3S_HIP(hipGetLastError());
     return F3S_OK;
 }
