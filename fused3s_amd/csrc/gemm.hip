@@ -342,12 +342,15 @@ struct Shape {
     static constexpr int tile_bytes = SIZE * kStep * 2;
 };
 
-template <typename T, bool PT, bool QT, int SIZE, int EPI, bool FAST>
+// kWhole: whole 16-byte pieces everywhere; kTiles: of the operands' rows; kAny.
+enum Way : int { kAny = 0, kTiles = 1, kWhole = 2 };
+template <typename T, bool PT, bool QT, int SIZE, int EPI, int WAY>
 __global__ void __launch_bounds__(Shape<SIZE>::waves * kWave) __attribute__((amdgpu_waves_per_eu(2)))
 gemm_kernel(const GemmParams p)
 {
     typedef typename Half<T>::v8 v8;
     typedef Shape<SIZE> S;
+    constexpr bool LOADS = WAY != kAny, FAST = WAY == kWhole;   // tiles; C, bias and R
     constexpr int kNo = S::outs / 16, kNr = S::rows / 16;
     constexpr int kOutRow = S::outs + 4;      // floats of a staged row
     __shared__ __align__(256) char lds[2][2][S::tile_bytes];   // [buffer][P, Q]
@@ -368,12 +371,12 @@ gemm_kernel(const GemmParams p)
     int32_t rt, ot;
     typedef TileAt<PT, SIZE, S::waves> AtP;
     typedef TileAt<QT, SIZE, S::waves> AtQ;
-    v8 held_p[FAST ? 1 : AtP::loads], held_q[FAST ? 1 : AtQ::loads];
-    // step c's tiles into buffer buf; not FAST: on their way, put() brings them there
+    v8 held_p[LOADS ? 1 : AtP::loads], held_q[LOADS ? 1 : AtQ::loads];
+    // step c's tiles into buffer buf; not LOADS: on their way, put() brings them there
     auto load = [&](int64_t c, int buf) __attribute__((always_inline)) {
         const AtP at_p(p.P, p.ldp, (int64_t)rt * SIZE, p.rows, c, end);
         const AtQ at_q(p.Q, p.ldq, (int64_t)ot * SIZE, p.outs, c, end);
-        if constexpr (FAST) {
+        if constexpr (LOADS) {
             load_tile(at_p, p.ldp, lds[buf][0], wave, lane);
             load_tile(at_q, p.ldq, lds[buf][1], wave, lane);
         } else {
@@ -382,7 +385,7 @@ gemm_kernel(const GemmParams p)
         }
     };
     auto put = [&](int buf) __attribute__((always_inline)) {
-        if constexpr (!FAST) {
+        if constexpr (!LOADS) {
             put_tile<PT, SIZE, S::waves>(held_p, lds[buf][0], wave, lane);
             put_tile<QT, SIZE, S::waves>(held_q, lds[buf][1], wave, lane);
         }
@@ -423,7 +426,7 @@ gemm_kernel(const GemmParams p)
                 for (int j = 0; j < kNr; ++j) b[f][j] = fragment<T, PT, SIZE>(pt, kNr * wr + j, f, lane);
             };
             // both halves' operands at once (128: 4 % faster) where there are registers
-            constexpr bool kBoth = SIZE != 256 && FAST;
+            constexpr bool kBoth = SIZE != 256 && LOADS;
             read(0);
             if constexpr (kBoth) {
                 __builtin_amdgcn_sched_barrier(0);
@@ -456,10 +459,10 @@ gemm_kernel(const GemmParams p)
             return row0 + S::rows * wr + 16 * j + v * kRowsAtOnce + lane / kLanes;
         };
         // The residual's (dy's) rows, 64 asked for ahead (a wait for each 16 rows:
-        // 32,768 x 1,024 -> 4,096, gelu's slope 444 us); not FAST: where they are used,
-        // the next step holds the registers.
+        // 32,768 x 1,024 -> 4,096, gelu's slope 444 us, 379 so); not LOADS: where they
+        // are used, the next step holds the registers.
         constexpr bool kEnds = EPI == kEpiForward || EPI == kEpiSlope;
-        constexpr int kAhead = !(kEnds && FAST) ? 1 : kNr < 4 ? kNr : 4;
+        constexpr int kAhead = !(kEnds && LOADS) ? 1 : kNr < 4 ? kNr : 4;
         v8 bias = {}, res[kAhead][kTurns] = {};
         auto residual = [&](int j, int v) __attribute__((always_inline)) -> v8 {
             const int64_t row = row_of(j, v);
@@ -469,7 +472,7 @@ gemm_kernel(const GemmParams p)
         if constexpr (kEnds) {
             if (p.bias)
                 bias = load8<T, FAST>(reinterpret_cast<const T*>(p.bias) + out, p.outs - out);
-            if constexpr (FAST) {
+            if constexpr (LOADS) {
 #pragma unroll
                 for (int j = 0; j < kAhead; ++j)
 #pragma unroll
@@ -514,7 +517,7 @@ gemm_kernel(const GemmParams p)
                     }
                 } else {
                     v8 other = {};
-                    if constexpr (kEnds && FAST) {
+                    if constexpr (kEnds && LOADS) {
                         other = res[j % kAhead][v];
                         if (j + kAhead < kNr) res[j % kAhead][v] = residual(j + kAhead, v);
                     } else if constexpr (kEnds) {
@@ -936,7 +939,7 @@ constexpr int64_t kSumShares = 64;
 
 // Where the tiles of 256 serve: elsewhere they would need more registers than
 // there are.
-constexpr bool has_256(bool whole_pieces, int epi) { return whole_pieces && epi != kEpiPartSums; }
+constexpr bool has_256(int way, int epi) { return way != kAny && epi != kEpiPartSums; }
 
 // Size of the tiles and splits of the contraction, by what each choice would take:
 // full waves of workgroups at the rate that a large product reaches (900, 760 and
@@ -982,7 +985,7 @@ constexpr int64_t kForwardLeast = 512, kWeightLeast = 256;
 
 static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-template <typename T, bool PT, bool QT, int EPI, bool FAST>
+template <typename T, bool PT, bool QT, int EPI, int WAY>
 static void launch_tiles(GemmParams p, int32_t tile, hipStream_t st)
 {
     p.row_tiles = (int32_t)ceil_div(p.rows, tile);
@@ -992,23 +995,27 @@ static void launch_tiles(GemmParams p, int32_t tile, hipStream_t st)
     const int64_t most = std::max<int64_t>(8, (tile == 256 ? 256 : tile == 128 ? 512 : 1280) / p.splits / 8 * 8);
     const dim3 grid((unsigned)std::min((int64_t)p.row_tiles * p.out_tiles, most), (unsigned)p.splits);
     if (tile == 64)
-        hipLaunchKernelGGL((gemm_kernel<T, PT, QT, 64, EPI, FAST>), grid, dim3(256), 0, st, p);
+        hipLaunchKernelGGL((gemm_kernel<T, PT, QT, 64, EPI, WAY>), grid, dim3(256), 0, st, p);
     else if (tile == 128)
-        hipLaunchKernelGGL((gemm_kernel<T, PT, QT, 128, EPI, FAST>), grid, dim3(256), 0, st, p);
-    else if constexpr (has_256(FAST, EPI))
-        hipLaunchKernelGGL((gemm_kernel<T, PT, QT, 256, EPI, FAST>), grid, dim3(512), 0, st, p);
+        hipLaunchKernelGGL((gemm_kernel<T, PT, QT, 128, EPI, WAY>), grid, dim3(256), 0, st, p);
+    else if constexpr (has_256(WAY, EPI))
+        hipLaunchKernelGGL((gemm_kernel<T, PT, QT, 256, EPI, WAY>), grid, dim3(512), 0, st, p);
 }
 
-// Whole 16-byte pieces everywhere, offsets in a tile within 31 bits.
-static bool fast(const GemmParams& p, bool pt = false, bool qt = false)
+// Offsets in a tile within 31 bits, and kWay's pieces.  (kTiles for forward products
+// only, 2,000 x 2,000 -> 2,001 39 us so, 68 as kAny: in the others the outputs' number is
+// that of an operand's columns.)
+static Way way_of(const GemmParams& p, bool pt = false, bool qt = false)
 {
     auto rows_ok = [](const char* x, int64_t ld) {
         return ((uintptr_t)x & 15) == 0 && ld % 8 == 0 && ld < (1 << 22);
     };
     const int64_t pcols = pt ? p.rows : p.depth, qcols = qt ? p.outs : p.depth;
-    return rows_ok(p.P, p.ldp) && rows_ok(p.Q, p.ldq) && pcols % 8 == 0 && qcols % 8 == 0 &&
-           p.outs % 8 == 0 && ((uintptr_t)p.C & 15) == 0 &&
-           (!p.bias || ((uintptr_t)p.bias & 15) == 0) && (!p.R || rows_ok(p.R, p.ldr));
+    if (!rows_ok(p.P, p.ldp) || !rows_ok(p.Q, p.ldq) || pcols % 8 != 0 || qcols % 8 != 0) return kAny;
+    if (p.outs % 8 == 0 && ((uintptr_t)p.C & 15) == 0 && (!p.bias || ((uintptr_t)p.bias & 15) == 0) &&
+        (!p.R || rows_ok(p.R, p.ldr)))
+        return kWhole;
+    return pt || qt ? kAny : kTiles;
 }
 
 template <typename T, bool PT, bool QT, int EPI>
@@ -1019,10 +1026,11 @@ static f3s_status launch_gemm(GemmParams p, const Tiling& t, hipStream_t st)
         set_error("linear: too many tiles");
         return F3S_EUNSUPPORTED;
     }
-    const bool whole = fast(p, PT, QT);
-    const int32_t tile = has_256(whole, EPI) ? t.tile : std::min(t.tile, 128);
-    if (whole) launch_tiles<T, PT, QT, EPI, true>(p, tile, st);
-    else launch_tiles<T, PT, QT, EPI, false>(p, tile, st);
+    const Way way = way_of(p, PT, QT);
+    const int32_t tile = has_256(way, EPI) ? t.tile : std::min(t.tile, 128);
+    if (way == kWhole) launch_tiles<T, PT, QT, EPI, kWhole>(p, tile, st);
+    else if (way == kAny) launch_tiles<T, PT, QT, EPI, kAny>(p, tile, st);
+    else if constexpr (!PT && !QT) launch_tiles<T, PT, QT, EPI, kTiles>(p, tile, st);
     F3S_HIP(hipGetLastError());
     return F3S_OK;
 }
@@ -1036,7 +1044,8 @@ static f3s_status launch_gemm(GemmParams p, const Tiling& t, hipStream_t st)
 // and 805, 500,000 x 128 -> 512 350 and 511; but 20,000 x 128 -> 384 36 and 23.
 static bool takes_rows(const GemmParams& p)
 {
-    return p.rows >= kManyRows && p.depth <= 256 && p.outs % 32 == 0 && p.outs <= 8192 && fast(p);
+    return p.rows >= kManyRows && p.depth <= 256 && p.outs % 32 == 0 && p.outs <= 8192 &&
+           way_of(p) == kWhole;
 }
 
 template <typename T, int KF, int MODE>
@@ -1206,7 +1215,7 @@ static f3s_status backward(const LinearArgs& a, char* ws, hipStream_t st)
                                dim3(256), 0, st, p, reinterpret_cast<const float*>(ws + s.parts));
             F3S_HIP(hipGetLastError());
         } else {
-            const int32_t tile = has_256(fast(p), kEpiSlope) ? s.slope.tile
+            const int32_t tile = has_256(way_of(p), kEpiSlope) ? s.slope.tile
                                                              : std::min(s.slope.tile, 128);
             sum_rows = 2 * ceil_div(a.n, tile);
             F3S_TRY((launch_gemm<T, false, false, kEpiSlope>(p, s.slope, st)));
