@@ -47,6 +47,7 @@ struct GemmParams {
     int64_t split;        // contraction steps per split (a multiple of 64)
     int32_t act;
     int32_t row_tiles, out_tiles, splits;
+    bool q_steps;         // rows_kernel: Q lies contraction by contraction
 };
 
 __device__ __forceinline__ float logistic(float z)
@@ -693,7 +694,14 @@ rows_kernel(const GemmParams p)
         const int row = l & 15;
         const int col = (tile >> 1) * 32 + 8 * (row >> 2) + 4 * (tile & 1) + (row & 3);
         const int k = 32 * f + 8 * (l >> 4);
-        wl[i] = k < K ? *reinterpret_cast<const v8*>(W + (int64_t)(m0 + col) * p.ldq + k) : zero;
+        v8 w = zero;
+        if (k < K && !p.q_steps) {
+            w = *reinterpret_cast<const v8*>(W + (int64_t)(m0 + col) * p.ldq + k);
+        } else if (k < K) {   // (dx; once per workgroup)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = W[(k + e) * p.ldq + m0 + col];
+        }
+        wl[i] = w;
     }
     for (int i = tid; i < mc; i += kRowWaves * kWave) bl[i] = bias ? bias[m0 + i] : (T)0.f;
     if constexpr (SLOPE)
@@ -1042,10 +1050,12 @@ static f3s_status launch_gemm(GemmParams p, const Tiling& t, hipStream_t st)
 // 227; but 20,000 x 128 -> 384 13 and 10, 20,000 x 256 -> 256 11.3 and 10.8.  With
 // gelu's slope and its sums: 50,000 x 128 -> 384 38 and 45, 100,000 x 256 -> 4,096 579
 // and 805, 500,000 x 128 -> 512 350 and 511; but 20,000 x 128 -> 384 36 and 23.
+// dx (W's values one by one, once per workgroup): 200,003 x 128 -> 512 48 and 62,
+// 100,000 x 256 -> 4,096 327 and 360; but 65,536 x 256 -> 512 37 and 30.
 static bool takes_rows(const GemmParams& p)
 {
-    return p.rows >= kManyRows && p.depth <= 256 && p.outs % 32 == 0 && p.outs <= 8192 &&
-           way_of(p) == kWhole;
+    return p.rows >= (p.q_steps ? 2 : 1) * kManyRows && p.depth <= 256 && p.outs % 32 == 0 &&
+           p.outs <= 8192 && way_of(p, false, p.q_steps) == kWhole;
 }
 
 template <typename T, int KF, int MODE>
@@ -1244,7 +1254,11 @@ static f3s_status backward(const LinearArgs& a, char* ws, hipStream_t st)
         p.outs = a.K;
         p.depth = a.M;
         p.C = a.dX;
-        if (s.dx.splits == 1) {
+        p.q_steps = true;
+        int64_t workgroups;
+        if (takes_rows(p)) {
+            F3S_TRY(many_rows<T>(p, false, &workgroups, st));
+        } else if (s.dx.splits == 1) {
             F3S_TRY((launch_gemm<T, false, true, kEpiPlain>(p, s.dx, st)));
         } else {
             p.C = ws + s.parts;

@@ -126,6 +126,7 @@ def test_many_rows_gradients(gpu, dtype):
     bias, a bias but no gradient of it; every run gives the same bits."""
     for n, K, M, act, bias in ((49_169, 128, 416, "gelu", True), (70_001, 64, 800, "silu", True),
                                (49_152, 248, 224, "gelu_tanh", True),
+                               (98_304, 416, 136, None, True), (98_321, 32, 256, "relu", True),
                                (50_000, 32, 32, "relu", False)):
         t = make(n, K, M, dtype, bias=bias, residual=False, seed=2)
         got = step(t, act)
