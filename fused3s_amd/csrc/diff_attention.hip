@@ -1031,9 +1031,9 @@ diff_dlam_kernel(const float* __restrict__ parts, int32_t W, float* __restrict__
     for (int32_t i = threadIdx.x; i < W; i += 32 * 1024) {
         float x[32];   // (in one batch: the loads' latency is all there is)
 #pragma unroll
-        for (int k = 0; k < 32; ++k) x[k] = i + k * 1024 < W ? src[i + k * 1024] : 0.f;
+        for (int k = 0; k < 32; ++k) x[k] = src[min(i + k * 1024, W - 1)];
 #pragma unroll
-        for (int k = 0; k < 32; ++k) s += x[k];
+        for (int k = 0; k < 32; ++k) s += i + k * 1024 < W ? x[k] : 0.f;
     }
     s = wave_sum(s);
     if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = s;
