@@ -31,6 +31,7 @@ enum Epilogue : int {
     kEpiPlain = 2,     // z
     kEpiPart = 3,      // z in float32, one slice per split
     kEpiPartSums = 4,  // and the sums of P's rows (dW: db)
+    kEpiPlainSums = 5, // z, and those sums
 };
 
 struct GemmParams {
@@ -362,7 +363,8 @@ gemm_kernel(const GemmParams p)
     const int wr = wave / S::wave_outs, wo = wave % S::wave_outs;
     const int64_t begin = (int64_t)blockIdx.y * p.split, end = min(p.depth, begin + p.split);
     const int64_t total = (int64_t)p.row_tiles * p.out_tiles;
-    constexpr bool kSums = EPI == kEpiPartSums, kPart = EPI == kEpiPart || kSums;
+    constexpr bool kSums = EPI == kEpiPartSums || EPI == kEpiPlainSums;
+    constexpr bool kPart = EPI == kEpiPart || EPI == kEpiPartSums;
     v8 ones;
     if constexpr (kSums) {
 #pragma unroll
@@ -915,7 +917,13 @@ column_sums(const float* __restrict__ in, int64_t rows, int64_t cols, OUT* __res
     const int64_t r0 = blockIdx.y * per, r1 = min(rows, r0 + per);
     float s = 0.f;
     if (col < cols)
-        for (int64_t i = r0 + part; i < r1; i += 4) s += in[i * cols + col];
+        for (int64_t i = r0 + part; i < r1; i += 64) {
+            float x[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) x[k] = in[min(i + 4 * k, r1 - 1) * cols + col];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) s += i + 4 * k < r1 ? x[k] : 0.f;
+        }
     lds[part][threadIdx.x % 64] = s;
     __syncthreads();
     if (part == 0 && col < cols) {
@@ -943,24 +951,28 @@ hipError_t warm_gemm(hipStream_t s)
 // ------------------------------------------------------------------ launches
 
 constexpr int64_t kFewRows = 64, kManyRows = 48 * 1024;
-constexpr int64_t kSumShares = 64;
+constexpr int64_t kSumShares = 64, kSumRows = 512;
 
 // Where the tiles of 256 serve: elsewhere they would need more registers than
 // there are.
-constexpr bool has_256(int way, int epi) { return way != kAny && epi != kEpiPartSums; }
+constexpr bool has_256(int way, int epi)
+{
+    return way != kAny && epi != kEpiPartSums && epi != kEpiPlainSums;
+}
 
 // Size of the tiles and splits of the contraction, by what each choice would take:
 // full waves of workgroups at the rate that a large product reaches (900, 760 and
 // 580 TFLOP/s), 128 steps more for a tile's beginning and end, and for splits a
-// launch and their sums' bytes at 8 TB/s (they stay in the Infinity Cache).
+// launch and their sums' bytes at 8 TB/s (they stay in the Infinity Cache); twice the
+// time where an operand's rows are no whole pieces.
 // (Microseconds with 64, 128, 256, chosen; forward: 8,192 x 1,024 -> 1,024 32, 25,
 // 40, 25; 200,003 x 512 -> 128 53, 55, 84, 53; 2,048 x 2,048 -> 2,048 28, 28, 49, 28;
 // 1,024 x 1,024 -> 1,024 12, 16, 25, 12.)
 struct Tiling {
     int32_t tile, splits;
 };
-static Tiling tiling(int64_t rows, int64_t outs, int64_t depth, int64_t least, bool weights,
-                     bool sums = false)
+static Tiling tiling(int64_t rows, int64_t outs, int64_t depth, int64_t least, bool odd,
+                     bool weights, bool sums = false)
 {
     struct Kind {
         int32_t tile;
@@ -973,14 +985,15 @@ static Tiling tiling(int64_t rows, int64_t outs, int64_t depth, int64_t least, b
     Tiling best{64, 1};
     double best_time = 1e300;
     for (const Kind& k : kinds) {
-        if (weights && k.tile == 256 && sums) continue;
+        if (k.tile == 256 && (odd || (weights && sums))) continue;
         const int64_t n = ceil_div(rows, k.tile) * ceil_div(outs, k.tile);
         for (int64_t s = 1; s <= 256 && (s == 1 || depth / s >= least); s += s < 4 ? 1 : s / 4) {
             // (a wave that is not full is shorter as far as workgroups share CUs)
             const double part = (double)(n * s % k.slots) / k.slots;
             const double waves = (double)(n * s / k.slots) + (part > 0 ? std::max(part, k.alone) : 0);
             double time = waves * k.slots * k.tile * k.tile * ((double)depth / s + 128) / k.rate;
-            if (weights || s > 1) time += 3.0 + (double)rows * outs * (8 * s + 2) / 8e6;
+            if (odd) time *= 2;   // (rows that are no whole pieces)
+            if (s > 1) time += 3.0 + (double)rows * outs * (8 * s + 2) / 8e6;
             if (time < best_time) {
                 best_time = time;
                 best = Tiling{k.tile, (int32_t)s};
@@ -1115,7 +1128,7 @@ static f3s_status forward(GemmParams p, void* ws, hipStream_t st)
         F3S_HIP(hipGetLastError());
         return F3S_OK;
     }
-    const Tiling t = tiling(p.rows, p.outs, p.depth, kForwardLeast, false);
+    const Tiling t = tiling(p.rows, p.outs, p.depth, kForwardLeast, p.depth % 8 != 0, false);
     if (t.splits == 1) return launch_gemm<T, false, false, kEpiForward>(p, t, st);
     GemmParams part = p;
     part.C = static_cast<char*>(ws);
@@ -1131,7 +1144,7 @@ static f3s_status forward(GemmParams p, void* ws, hipStream_t st)
 static size_t forward_bytes(int64_t n, int64_t K, int64_t M)
 {
     if (n <= kFewRows) return 0;
-    const int32_t s = tiling(n, M, K, kForwardLeast, false).splits;
+    const int32_t s = tiling(n, M, K, kForwardLeast, K % 8 != 0, false).splits;
     return s == 1 ? 0 : up256(sizeof(float) * (size_t)s * n * M);
 }
 
@@ -1145,10 +1158,11 @@ struct BackwardSpace {
 static BackwardSpace backward_space(int64_t n, int64_t K, int64_t M, int32_t act)
 {
     BackwardSpace s;
-    s.dx = tiling(n, K, M, kForwardLeast, false);
+    const bool odd_k = K % 8 != 0, odd = odd_k || M % 8 != 0;
+    s.dx = tiling(n, K, M, kForwardLeast, odd, false);
     size_t parts = s.dx.splits > 1 ? sizeof(float) * (size_t)s.dx.splits * n * K : 0;
     if (act != kActNone) {
-        s.slope = tiling(n, M, K, kForwardLeast, false);
+        s.slope = tiling(n, M, K, kForwardLeast, odd_k, false);
         if (s.slope.splits > 1)
             parts = std::max(parts, sizeof(float) * (size_t)s.slope.splits * n * M);
         s.sum_rows = 2 * ceil_div(n, std::min(s.slope.tile, 64));   // (at most)
@@ -1157,7 +1171,7 @@ static BackwardSpace backward_space(int64_t n, int64_t K, int64_t M, int32_t act
         s.shares = s.sums + up256(sizeof(float) * (size_t)s.sum_rows * M);
         s.parts = s.shares + up256(sizeof(float) * (size_t)kSumShares * M);
     }
-    s.dw = tiling(M, K, n, kWeightLeast, true, act == kActNone);
+    s.dw = tiling(M, K, n, kWeightLeast, odd, true, act == kActNone);
     parts = std::max(parts, sizeof(float) * (size_t)s.dw.splits * M * K);
     s.db = s.parts + up256(parts);
     s.bytes = s.db + up256(sizeof(float) * (size_t)s.dw.splits * M);
@@ -1233,12 +1247,17 @@ static f3s_status backward(const LinearArgs& a, char* ws, hipStream_t st)
         dz = ws + s.dz;
         lddz = a.M;
         if (db_left) {
-            float* shares = reinterpret_cast<float*>(ws + s.shares);
-            const int64_t ny = std::min<int64_t>(kSumShares, ceil_div(sum_rows, 16));
+            const float* sums = p.sums;
             const unsigned nx = (unsigned)ceil_div(a.M, 64);
-            hipLaunchKernelGGL((column_sums<float>), dim3(nx, (unsigned)ny), dim3(256), 0, st,
-                               p.sums, sum_rows, a.M, shares);
-            hipLaunchKernelGGL((column_sums<T>), dim3(nx, 1), dim3(256), 0, st, shares, ny, a.M,
+            if (sum_rows > kSumRows) {   // shares of them first
+                float* shares = reinterpret_cast<float*>(ws + s.shares);
+                const int64_t ny = std::min<int64_t>(kSumShares, ceil_div(sum_rows, 64));
+                hipLaunchKernelGGL((column_sums<float>), dim3(nx, (unsigned)ny), dim3(256), 0, st,
+                                   sums, sum_rows, a.M, shares);
+                sums = shares;
+                sum_rows = ny;
+            }
+            hipLaunchKernelGGL((column_sums<T>), dim3(nx, 1), dim3(256), 0, st, sums, sum_rows, a.M,
                                reinterpret_cast<T*>(a.db));
             F3S_HIP(hipGetLastError());
             db_left = false;
@@ -1275,12 +1294,17 @@ static f3s_status backward(const LinearArgs& a, char* ws, hipStream_t st)
         p.rows = a.M;
         p.outs = a.dW ? a.K : std::min<int64_t>(a.K, 8);   // (db alone: one column of tiles)
         p.depth = a.n;
-        p.C = ws + s.parts;
         p.sums = db_left ? reinterpret_cast<float*>(ws + s.db) : nullptr;
-        if (p.sums) F3S_TRY((launch_gemm<T, true, true, kEpiPartSums>(p, s.dw, st)));
+        // (one split: no sums to join; 4,096 x 4,096 of 4,096 rows 145 us, 181 with them)
+        const bool whole = a.dW && s.dw.splits == 1;
+        p.C = whole ? a.dW : ws + s.parts;
+        if (whole && p.sums) F3S_TRY((launch_gemm<T, true, true, kEpiPlainSums>(p, s.dw, st)));
+        else if (whole) F3S_TRY((launch_gemm<T, true, true, kEpiPlain>(p, s.dw, st)));
+        else if (p.sums) F3S_TRY((launch_gemm<T, true, true, kEpiPartSums>(p, s.dw, st)));
         else F3S_TRY((launch_gemm<T, true, true, kEpiPart>(p, s.dw, st)));
-        const int64_t count = a.dW ? a.M * a.K : 0, nsums = db_left ? a.M : 0;
-        F3S_TRY((join<T>(ws + s.parts, count, s.dw.splits, a.dW, p.sums, nsums, a.db, st)));
+        const int64_t count = a.dW && !whole ? a.M * a.K : 0, nsums = db_left ? a.M : 0;
+        if (count + nsums > 0)
+            F3S_TRY((join<T>(ws + s.parts, count, s.dw.splits, a.dW, p.sums, nsums, a.db, st)));
     }
     return F3S_OK;
 }

@@ -119,6 +119,19 @@ def test_some_gradients(gpu):
                 assert torch.equal(g, every[name]), (leaves, name)
 
 
+@pytest.mark.parametrize("n,K,M", [
+    (404, 45, 4037), (66, 4104, 520), (500, 4096, 72),       # deep dx, deep z: split
+    (3000, 512, 517), (9000, 1024, 1030), (70, 8, 8200),     # operands whole, outputs odd
+    (2500, 2048, 2056), (300, 1027, 1025)])
+def test_products_of_a_step(gpu, n, K, M):
+    """Every way a step's products take through tiles, with and without the sums
+    that a bias needs."""
+    for i, dtype in enumerate(HALF):
+        for act, bias in ((None, bool(i)), ("silu" if i else "gelu", True)):
+            t = make(n, K, M, dtype, bias=bias, residual=bias, seed=4)
+            check(t, act, step(t, act))
+
+
 @pytest.mark.parametrize("dtype", HALF)
 def test_many_rows_gradients(gpu, dtype):
     """Rows enough for W in LDS, in both passes: blocks of rows that do not divide
