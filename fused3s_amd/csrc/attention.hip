@@ -1029,13 +1029,19 @@ static f3s_status launch_schedule(const int32_t* d_window_offsets, const int32_t
 // on config 4 (15.9 M tiles, one head) ran flat from 3,584 to 6,144 tiles
 // (546-549 us) against 557 us at 1/8192 (1,936 tiles) and 571 us at 1,024:
 // the heaviest windows, which the descending order starts first, need few
-// segments.  seg[0] serves masked passes, seg[1] tile-dense ones.
-__host__ __device__ __forceinline__ void auto_segments(int64_t T, int32_t W, int32_t H,
+// segments.  seg[0] serves masked passes, seg[1] tile-dense ones.  `fine`, for
+// plans of differential attention, whose chunks take several times as long (a
+// window alone on its wave is what a mid-sized graph then waits for): 1.5 x the
+// mean window.  (A step, microseconds with 4, 2, 1.5 and 1 x; powerlaw, 14 edges a
+// node, two heads: 20,011 nodes 212, 191, 194, 237; 40,000 405, 363, 346, 344;
+// 60,000 482, 455, 444, 456; 12,000 of communities, 40 edges 196, 200, 194, 286.)
+__host__ __device__ __forceinline__ void auto_segments(int64_t T, int32_t W, int32_t H, bool fine,
                                                        int64_t seg[2])
 {
     const int64_t mean = W > 0 ? (T + W - 1) / W : 0;
-    int64_t m = 256, dd = 16;
-    if (4 * mean > m) m = 4 * mean;
+    int64_t m = fine ? 128 : 256, dd = 16;
+    const int64_t most = fine ? 3 * mean / 2 : 4 * mean;
+    if (most > m) m = most;
     if ((T * H + 3071) / 3072 > m) m = (T * H + 3071) / 3072;
     if (2 * mean > dd) dd = 2 * mean;
     if ((T * H + 51199) / 51200 > dd) dd = (T * H + 51199) / 51200;
@@ -1052,6 +1058,7 @@ struct PlanSeq {
     const int32_t* offs;
     const int32_t* order;
     int32_t W, P, H, seg_fixed, nsets, team[2];
+    bool fine;
 };
 constexpr int kPlanArrays = 6;
 
@@ -1061,7 +1068,7 @@ __device__ __forceinline__ int32_t plan_segments(const PlanSeq& q, int64_t seg[2
     if (q.seg_fixed > 0)
         seg[0] = seg[1] = q.seg_fixed;
     else
-        auto_segments(T, q.W, q.H, seg);
+        auto_segments(T, q.W, q.H, q.fine, seg);
     return T;
 }
 
@@ -1337,7 +1344,7 @@ static f3s_status build_plan_sets(f3s_plan* p, const int32_t* d_window_offsets,
     StagingGuard staging(st);
     // [0] T, [1..2] segment sizes, [3..] totals
     int64_t* info = pinned ? h : reinterpret_cast<int64_t*>(mem);
-    const PlanSeq q{d_window_offsets, seq, W, P, H, seg_tiles, nsets, {team_m, team_d}};
+    const PlanSeq q{d_window_offsets, seq, W, P, H, seg_tiles, nsets, {team_m, team_d}, by_schedule};
     if (nb > 1)
         hipLaunchKernelGGL(plan_sums, dim3((unsigned)nb), dim3(kPlanThreads), 0, st, q, sums);
     hipLaunchKernelGGL(plan_bases, dim3((unsigned)nb), dim3(kPlanThreads), 0, st, q, sums, bases,
