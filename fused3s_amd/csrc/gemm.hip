@@ -335,8 +335,9 @@ __device__ __forceinline__ void finish8(const GemmParams& p, int64_t row, int64_
 // 256: eight waves of 128 rows by 64 outputs.  (What bounds the small ones is the
 // way from L2 to LDS, 64 bytes per clock and CU: 128 x 128 x 64 products take its
 // time as long as the matrix cores'; 256 x 256 x 64 half of it.  32,768 x 1,024 ->
-// 4,096, TFLOP/s: 64 560, 128 737, 256 839; three steps of 32 with the next one's
-// operands read ahead into registers, 256 x 256 743, 256 x 128 698.)
+// 4,096, TFLOP/s: 64 560, 128 737, 256 880; 256 by four waves of 128 x 128, a wave
+// per SIMD, 776; three steps of 32 with the next one's operands read ahead into
+// registers, 256 x 256 743, 256 x 128 698.)
 template <int SIZE>
 struct Shape {
     static constexpr int wave_rows = 2, wave_outs = SIZE == 256 ? 4 : 2, waves = wave_rows * wave_outs;
