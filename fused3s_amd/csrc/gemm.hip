@@ -335,7 +335,7 @@ __device__ __forceinline__ void finish8(const GemmParams& p, int64_t row, int64_
 // 256: eight waves of 128 rows by 64 outputs.  (What bounds the small ones is the
 // way from L2 to LDS, 64 bytes per clock and CU: 128 x 128 x 64 products take its
 // time as long as the matrix cores'; 256 x 256 x 64 half of it.  32,768 x 1,024 ->
-// 4,096, TFLOP/s: 64 560, 128 737, 256 880; 256 by four waves of 128 x 128, a wave
+// 4,096, TFLOP/s: 64 560, 128 737, 256 910; 256 by four waves of 128 x 128, a wave
 // per SIMD, 776; three steps of 32 with the next one's operands read ahead into
 // registers, 256 x 256 743, 256 x 128 698.)
 template <int SIZE>
@@ -429,30 +429,42 @@ gemm_kernel(const GemmParams p)
 #pragma unroll
                 for (int j = 0; j < kNr; ++j) b[f][j] = fragment<T, PT, SIZE>(pt, kNr * wr + j, f, lane);
             };
-            // both halves' operands at once (128: 4 % faster) where there are registers
-            constexpr bool kBoth = SIZE != 256 && LOADS;
+            // both halves' operands at once (128: 4 % faster) where there are registers;
+            // 256: the second half's between the first half's products (4,096 x 4,096 of
+            // 4,096 rows 111 us, 120 one after another; dW's take too many registers)
+            constexpr bool kBoth = SIZE != 256 && LOADS, kBetween = SIZE == 256 && !PT;
             read(0);
-            if constexpr (kBoth) {
+            if constexpr (kBoth || kBetween) {
                 __builtin_amdgcn_sched_barrier(0);
                 read(1);
-                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (kBoth) __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
             for (int f = 0; f < kStep / 32; ++f) {
-                if (!kBoth && f) read(f);
-                if constexpr (SIZE == 256) __builtin_amdgcn_s_setprio(1);   // (4 % faster so)
+                if (!kBoth && !kBetween && f) read(f);
+                if constexpr (SIZE == 256 && PT) __builtin_amdgcn_s_setprio(1);   // (4 % faster so)
 #pragma unroll
                 for (int j = 0; j < kNr; ++j)
 #pragma unroll
                     for (int i = 0; i < kNo; ++i)
                         acc[i][j] = Half<T>::mfma(a[f][i], b[f][j], acc[i][j]);
+                if constexpr (kBetween) {
+                    if (f == 0) {
+#pragma unroll
+                        for (int q = 0; q < kNo + kNr; ++q) {
+                            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // an LDS read
+                            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);   // two products
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
                 if constexpr (kSums) {
                     if (with_sums) {
 #pragma unroll
                         for (int j = 0; j < kNr; ++j) col[j] = Half<T>::mfma(ones, b[f][j], col[j]);
                     }
                 }
-                if constexpr (SIZE == 256) __builtin_amdgcn_s_setprio(0);
+                if constexpr (SIZE == 256 && PT) __builtin_amdgcn_s_setprio(0);
             }
             if (c + kStep < end) put(buf ^ 1);
         }
