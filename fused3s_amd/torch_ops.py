@@ -469,7 +469,10 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     weight [M, K], bias [M], residual [..., M], all float16 or all bfloat16 on one
     GPU; activation None, "relu", "gelu", "gelu_tanh" or "silu".  Sums and
     epilogue are in float32, the result is rounded once.  Differentiable (once);
-    for the backward pass the product is computed again rather than kept."""
+    for the backward pass the product z is computed again rather than kept, and
+    dz = dy * activation'(z) is rounded to the type, as between torch's own
+    modules, before the gradients of x and weight are made of it: those two are
+    rounded twice, bias's gradient (and all of them without an activation) once."""
     act = _ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation must be one of {list(_ACTIVATIONS)}, got {activation!r}")

@@ -322,7 +322,10 @@ f3s_status f3s_linear_fwd(const uint16_t* X, int64_t x_stride, const uint16_t* W
                           void* workspace, int64_t workspace_bytes, void* stream);
 /* Its gradient: dX[n][K], dW[M][K], db[M] (contiguous; NULL: not wanted) from
  * dY, whose rows are dy_stride values apart (dR is dY).  With an activation z is
- * computed again from X, W and bias: the forward call keeps nothing. */
+ * computed again from X, W and bias: the forward call keeps nothing.  Sums are
+ * float32.  dZ = dY act'(Z) is rounded to `dtype` before dX = dZ W and dW = dZ^T X
+ * are made of it, so these two carry its rounding and their own; db is summed
+ * before that.  Without an activation dZ is dY: one rounding each. */
 f3s_status f3s_linear_bwd(const uint16_t* X, int64_t x_stride, const uint16_t* W,
                           const uint16_t* bias, const uint16_t* dY, int64_t dy_stride, uint16_t* dX,
                           uint16_t* dW, uint16_t* db, int64_t n, int64_t K, int64_t M, int32_t act,
