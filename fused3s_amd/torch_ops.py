@@ -72,6 +72,42 @@ _current_device = torch._C._cuda_getDevice
 
 _NO_CONTEXT = contextlib.nullcontext()
 
+_dispatch_modes, _is_tracing = torch._C._len_torch_dispatch_stack, torch._C._is_tracing
+_key_included, _PRE_DISPATCH = (torch._C._dispatch_tls_is_dispatch_key_included,
+                                torch._C.DispatchKey.PreDispatch)
+_transform, _dynamo = torch._C._functorch.peek_interpreter_stack, torch.compiler.is_dynamo_compiling
+
+
+def _records_or_replaces() -> bool:
+    """Whether a dispatch mode that records a program or stands in for its memory
+    is active (make_fx, export, fake tensors; one that only looks on is neither)."""
+    key = torch._C._TorchDispatchModeKey
+    return any(torch._C._get_dispatch_mode(k) is not None
+               for k in (key.PROXY, key.FAKE, key.FUNCTIONAL))
+
+
+def _transformed(tensors) -> bool:
+    f = torch._C._functorch
+    return (any(t is not None and f.is_functorch_wrapped_tensor(t) for t in tensors)
+            or any(i.key() == f.TransformType.Functionalize for i in f.get_interpreter_stack()))
+
+
+def _refuse_unseen(who: str, *tensors) -> None:
+    """Raises where torch does not see what a kernel called on data pointers does,
+    and would go on without it: a forward-mode derivative would be lost, a traced
+    program hold the output's allocation and nothing that fills it.  (Some 0.6 us.)"""
+    compiled = _dynamo()   # (it sees the level, not the tangents)
+    if forward_ad._current_level >= 0 and (compiled or any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)):
+        raise RuntimeError(f"{who} has no forward-mode derivative")
+    if compiled:
+        return   # (its graph breaks at the library's call, which then runs, or it raises)
+    if (_is_tracing() or _key_included(_PRE_DISPATCH)
+            or _dispatch_modes() > 0 and _records_or_replaces()
+            or _transform() is not None and _transformed(tensors)):
+        raise RuntimeError(f"{who} cannot be traced or transformed: its kernel is not an operator "
+                           "that torch sees")
+
 
 def _on(device: int):
     """The device as the current one (an autograd thread's own is that already)."""
@@ -148,6 +184,7 @@ class TorchGraph:
         """softmax over each node's neighbours of scale * q.k, weights applied
         to v; [n, H, 64] fp16 contiguous CUDA tensors in, [n, H, 64] fp32 out.
         masked=False gives the reference's tile-dense semantics instead."""
+        _refuse_unseen("attention", q, k, v)
         n, H = self.n, self.heads
         shape = (n, H, HEAD_DIM)
         for name, t in (("q", q), ("k", k), ("v", v)):
@@ -181,6 +218,7 @@ class TorchGraph:
         """attention() on the [n, 3 * H * 64] fp16 output of one projection
         (q, k and v side by side in each row, no copies made), O [n, H, 64]
         in float32 or float16 (f3s_attention_fwd_packed)."""
+        _refuse_unseen("attention_packed", qkv)
         if qkv.requires_grad:
             raise RuntimeError("the fused pass is forward-only (no autograd)")
         if qkv.dtype != torch.float16 or not qkv.is_cuda or not qkv.is_contiguous():
@@ -286,7 +324,9 @@ class TorchGraph:
         projection's output is taken as it is; other layouts are copied);
         lam: float32 [H].  Returns [n, H, 128] in q's type: sums in float32,
         rounded once; nodes without edges get 0.  Differentiable in q, k, v and
-        lam (once).  A graph serves any number of calls at once."""
+        lam (once); tracing, functorch's transforms and forward-mode differentiation
+        are refused.  A graph serves any number of calls at once."""
+        _refuse_unseen("diff_attention", q, k, v, lam)
         shape, flat = (self.n, self.heads, 2 * HEAD_DIM), (self.n, self.heads * 2 * HEAD_DIM)
         self._check_diff(lam, (("q", q, shape, flat), ("k", k, shape, flat), ("v", v, shape, flat)))
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
@@ -300,6 +340,7 @@ class TorchGraph:
         """diff_attention() on the [n, 3 * H * 128] output of one projection (q,
         k and v side by side in each row), whose gradient is then one tensor
         too, written in place of its thirds."""
+        _refuse_unseen("diff_attention_packed", qkv, lam)
         self._check_diff(lam, (("qkv", qkv, (self.n, 3 * self.heads * 2 * HEAD_DIM)),))
         if torch.is_grad_enabled() and (qkv.requires_grad or lam.requires_grad):
             self.prepare_backward()
@@ -472,7 +513,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     for the backward pass the product z is computed again rather than kept, and
     dz = dy * activation'(z) is rounded to the type, as between torch's own
     modules, before the gradients of x and weight are made of it: those two are
-    rounded twice, bias's gradient (and all of them without an activation) once."""
+    rounded twice, bias's gradient (and all of them without an activation) once.
+    Tracing, functorch's transforms and forward-mode differentiation are refused."""
+    _refuse_unseen("linear", x, weight, bias, residual)
     act = _ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation must be one of {list(_ACTIVATIONS)}, got {activation!r}")

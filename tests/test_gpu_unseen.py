@@ -1,0 +1,55 @@
+"""On a device: what torch cannot see is refused by the layers too, and what only
+looks on, or compiles around the calls, gets their results."""
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+from conftest import random_csr
+
+pytestmark = pytest.mark.gpu
+
+
+def layers():
+    from fused3s_amd.torch_ops import (DiffGraphTransformerLayer, GraphTransformerLayer,
+                                       TorchGraph)
+    rp, ci = random_csr(300, 5, 2)
+    torch.manual_seed(0)
+    x = torch.randn(300, 64, device="cuda").half()
+    graph = TorchGraph(rp, ci, heads=2).prepare_backward()
+    for kind, more in ((GraphTransformerLayer, {}), (DiffGraphTransformerLayer, {"ffn_dim": 128})):
+        yield kind(64, heads=2, **more).cuda().half(), graph, x
+
+
+def test_layers_refuse(gpu):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    for layer, graph, x in layers():
+        layer.requires_grad_(False)
+        for grad in (torch.no_grad, torch.enable_grad):
+            with grad():
+                with forward_ad.dual_level():
+                    with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                        layer(forward_ad.make_dual(x, torch.ones_like(x)), graph)
+                with pytest.raises(RuntimeError, match="cannot be traced"):
+                    make_fx(lambda t: layer(t, graph))(x)
+                with pytest.raises(RuntimeError, match="cannot be traced"):
+                    torch.jit.trace(lambda t: layer(t, graph), x, check_trace=False)
+
+
+def test_onlookers_see_the_results(gpu):
+    from torch.utils.flop_counter import FlopCounterMode
+
+    from fused3s_amd.torch_ops import linear
+    for layer, graph, x in layers():
+        want = layer(x, graph)
+        bound = 2.0 ** -8 * want.abs().max()   # (projections by torch, rounded between)
+        with FlopCounterMode(display=False):
+            assert (layer(x, graph) - want).abs().max() <= bound
+    compiled = torch.compile(layer, backend="eager")   # (the trainable one)
+    assert (compiled(x, graph) - want).abs().max() <= bound
+    w = torch.randn(40, 64, device="cuda").half().requires_grad_()
+    want = linear(x, w, None, "silu")
+    assert torch.equal(torch.compile(lambda t: linear(t, w, None, "silu"), backend="eager")(x), want)
+    with FlopCounterMode(display=False), torch.inference_mode():
+        assert torch.equal(linear(x, w, None, "silu"), want)
