@@ -92,10 +92,20 @@ def _transformed(tensors) -> bool:
             or any(i.key() == f.TransformType.Functionalize for i in f.get_interpreter_stack()))
 
 
+_PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, type(None)))
+
+
+def _stands_for_others(t: torch.Tensor) -> bool:
+    """Whether t is of a subclass that dispatches its operations itself: its own
+    data pointer is not what it stands for."""
+    return type(t).__torch_dispatch__ is not torch.Tensor.__torch_dispatch__
+
+
 def _refuse_unseen(who: str, *tensors) -> None:
     """Raises where torch does not see what a kernel called on data pointers does,
     and would go on without it: a forward-mode derivative would be lost, a traced
-    program hold the output's allocation and nothing that fills it.  (Some 0.6 us.)"""
+    program hold the output's allocation and nothing that fills it, a wrapper's
+    tensor be left out.  (Some 0.7 us.)"""
     compiled = _dynamo()   # (it sees the level, not the tangents)
     if forward_ad._current_level >= 0 and (compiled or any(
             t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)):
@@ -107,6 +117,9 @@ def _refuse_unseen(who: str, *tensors) -> None:
             or _transform() is not None and _transformed(tensors)):
         raise RuntimeError(f"{who} cannot be traced or transformed: its kernel is not an operator "
                            "that torch sees")
+    for t in tensors:
+        if type(t) not in _PLAIN and _stands_for_others(t):
+            raise TypeError(f"{who} takes no {type(t).__name__}: it has no memory of its own")
 
 
 def _on(device: int):
@@ -602,8 +615,8 @@ def _project(m: torch.nn.Module, x: torch.Tensor, watched: bool) -> torch.Tensor
                 and (K <= 128 or M <= 128 or x.shape[0] >= 65536)
                 and w.dtype is torch.float16 and w.device == x.device and w.is_contiguous()
                 and type(w) is torch.nn.Parameter
-                and (b is None or (b.dtype is torch.float16 and b.device == x.device
-                                   and b.is_contiguous()))
+                and (b is None or (type(b) is torch.nn.Parameter and b.dtype is torch.float16
+                                   and b.device == x.device and b.is_contiguous()))
                 and (x.data_ptr() | w.data_ptr()) % 16 == 0
                 and x.device.index == torch.cuda.current_device()):
             y = torch.empty((x.shape[0], M), dtype=torch.float16, device=x.device)
@@ -669,9 +682,11 @@ _TORCH_ACTIVATIONS = {
 
 def _dense(m: torch.nn.Module, x: torch.Tensor, watched: bool, activation: str | None = None,
            residual: torch.Tensor | None = None) -> torch.Tensor:
-    """activation(m(x)) + residual: linear() where m is a plain Linear of a type
-    it takes and nothing watches the call, else torch's own operations."""
+    """activation(m(x)) + residual: linear() where m is a plain Linear of plain tensors
+    of a type it takes and nothing watches the call, else torch's own operations."""
     if (not watched and _is_plain_linear(m) and type(x) is torch.Tensor and x.is_cuda
+            and type(m.weight) in _PLAIN and type(m.bias) in _PLAIN
+            and (residual is None or type(residual) is torch.Tensor)
             and x.dtype in _DTYPES and m.weight.dtype == x.dtype and m.weight.device == x.device
             and (residual is None or residual.dtype == x.dtype)):
         return linear(x, m.weight, m.bias, activation, residual)

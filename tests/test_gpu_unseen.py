@@ -53,3 +53,34 @@ def test_onlookers_see_the_results(gpu):
     assert torch.equal(torch.compile(lambda t: linear(t, w, None, "silu"), backend="eager")(x), want)
     with FlopCounterMode(display=False), torch.inference_mode():
         assert torch.equal(linear(x, w, None, "silu"), want)
+
+
+class Counted(torch.Tensor):
+    """A weight whose class sees its uses."""
+
+    seen = []
+
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):
+        Counted.seen.append(func)
+        return super().__torch_function__(func, types, args, kwargs or {})
+
+
+def test_weights_of_a_subclass_are_torchs(gpu):
+    """A projection whose weight or bias is of a tensor subclass is torch's own, as
+    the forward-only layer's is: the subclass sees the product."""
+    for layer, graph, x in layers():
+        with torch.no_grad():
+            want = layer(x, graph).as_subclass(torch.Tensor)
+            for name, p in list(layer.named_parameters()):
+                module, _, leaf = name.rpartition(".")
+                if leaf not in ("weight", "bias"):
+                    continue
+                owner = layer.get_submodule(module)
+                setattr(owner, leaf, torch.nn.Parameter(p.detach().as_subclass(Counted),
+                                                        requires_grad=False))
+                Counted.seen.clear()
+                y = layer(x, graph).as_subclass(torch.Tensor)
+                assert torch.nn.functional.linear in Counted.seen, name
+                assert (y - want).abs().max() <= 2.0 ** -8 * want.abs().max(), name
+                setattr(owner, leaf, p)

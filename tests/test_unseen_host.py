@@ -108,3 +108,33 @@ def test_compiled_calls():
             f(x)
         with forward_ad.dual_level(), pytest.raises(RuntimeError, match="no forward-mode"):
             f(forward_ad.make_dual(x, torch.ones_like(x)))
+
+
+class Wrapper(torch.Tensor):
+    """A tensor that stands for another one and has no memory of its own."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        t = torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype,
+                                                device=inner.device)
+        t.inner = inner
+        return t
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        inner = lambda t: t.inner if isinstance(t, Wrapper) else t
+        return func(*map(inner, args), **(kwargs or {}))
+
+
+class Named(torch.Tensor):
+    """A subclass that is its own memory."""
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_wrappers_are_refused(name):
+    """(A wrapper's data pointer is NULL: as bias or residual it would be left out.)"""
+    call, x = calls()[name]
+    with pytest.raises(TypeError, match="takes no Wrapper"):
+        call(Wrapper(x))
+    with pytest.raises(ValueError):
+        call(x.as_subclass(Named))
