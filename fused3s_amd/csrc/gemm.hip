@@ -96,7 +96,7 @@ __device__ __forceinline__ void each(float (&z)[N], F f)
 #pragma unroll
     for (int k = 0; k < N; ++k) z[k] = f(z[k]);
 }
-// z -> act(z), and z -> act'(z); act is uniform.
+// z -> act(z), and (smooth activations) z -> act'(z); act is uniform.
 template <int N>
 __device__ __forceinline__ void act_values(int act, float (&z)[N])
 {
@@ -112,7 +112,6 @@ template <int N>
 __device__ __forceinline__ void act_slopes(int act, float (&z)[N])
 {
     switch (act) {
-    case kActRelu: each(z, [](float x) { return x > 0.f ? 1.f : x == x ? 0.f : x; }); break;
     case kActGelu:   // Phi + x phi
         each(z, [](float x) {
             return __builtin_fmaf(0.39894228f * x, fast_exp2(-0.72134752f * x * x), normal_cdf(x));
@@ -132,6 +131,19 @@ __device__ __forceinline__ void act_slopes(int act, float (&z)[N])
         break;
     default: each(z, [](float) { return 1.f; }); break;
     }
+}
+// z -> dy act'(z).  relu passes dy on or not: 0 x inf is no gradient of a unit that is off.
+template <int N>
+__device__ __forceinline__ void act_gradients(int act, float (&z)[N], const float (&dy)[N])
+{
+    if (act == kActRelu) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) z[k] = z[k] > 0.f ? dy[k] : z[k] == z[k] ? 0.f : z[k];
+        return;
+    }
+    act_slopes(act, z);
+#pragma unroll
+    for (int k = 0; k < N; ++k) z[k] *= dy[k];
 }
 
 constexpr int kStep = 64;   // contraction steps per tile
@@ -315,12 +327,12 @@ __device__ __forceinline__ void finish8(const GemmParams& p, int64_t row, int64_
 #pragma unroll
             for (int k = 0; k < 8; ++k) z[k] += (float)r[k];
         } else {
-            act_slopes(p.act, z);
+            float dy[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                z[k] *= (float)r[k];
-                sum[k] += z[k];
-            }
+            for (int k = 0; k < 8; ++k) dy[k] = (float)r[k];
+            act_gradients(p.act, z, dy);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sum[k] += z[k];
         }
     }
     T* dst = reinterpret_cast<T*>(p.C) + row * p.outs + out;
@@ -754,9 +766,10 @@ rows_kernel(const GemmParams p)
         }
         float y[8] = {a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
         if constexpr (SLOPE) {
-            act_slopes(p.act, y);
+            float dy[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) y[k] *= (float)rest[k];
+            for (int k = 0; k < 8; ++k) dy[k] = (float)rest[k];
+            act_gradients(p.act, y, dy);
             if (p.sums) {
                 float own[8];   // (a row past the end repeats the last one)
 #pragma unroll
@@ -894,8 +907,8 @@ join_slope(const GemmParams p, const float* __restrict__ parts)
             float z[1] = {0.f};
             for (int32_t k = 0; k < p.splits; ++k) z[0] += parts[k * count + row * p.outs + col];
             z[0] += bias;
-            act_slopes(p.act, z);
-            z[0] *= (float)reinterpret_cast<const T*>(p.R)[row * p.ldr + col];
+            const float dy[1] = {(float)reinterpret_cast<const T*>(p.R)[row * p.ldr + col]};
+            act_gradients(p.act, z, dy);
             sum += z[0];
             reinterpret_cast<T*>(p.C)[row * p.outs + col] = (T)z[0];
         }

@@ -1,0 +1,60 @@
+"""linear()'s gradient where z or dy are infinite, NaN or at the type's ends, in
+each kernel that a backward pass takes."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_gpu_linear_act import ACTS, HALF, make, step
+
+pytestmark = pytest.mark.gpu
+
+# the slope's kernel: split z and its join, whole tiles, tiles with operands through
+# registers, W in LDS
+SIZES = [(70, 4104, 72), (400, 96, 160), (401, 97, 161), (49_170, 64, 96)]
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("n,K,M", SIZES)
+def test_relu_passes_on_or_not(gpu, n, K, M, dtype):
+    """An off unit's gradient is 0 whatever dy is; an on unit's is dy, infinite or
+    not, and reaches its own row of dx and its own output's dw and db."""
+    t = make(n, K, M, dtype, residual=False, seed=1)
+    t["b"][0], t["b"][1], t["b"][8] = -1000.0, 1000.0, -1000.0   # off, on, off in every row
+    clean = step(t, "relu")
+    for value in (float("inf"), float("nan")):
+        bad = {**t, "dy": t["dy"].clone()}
+        bad["dy"][3, 0] = bad["dy"][n - 1, 8] = value
+        assert torch.equal(bad["x"], t["x"])
+        got = step(bad, "relu")
+        for name in got:
+            assert torch.equal(got[name], clean[name]), (name, value)
+        bad["dy"][5, 1] = value
+        got = step(bad, "relu")
+        rows = torch.arange(n, device="cuda") != 5
+        outs = torch.arange(M, device="cuda") != 1
+        assert torch.equal(got["dx"][rows], clean["dx"][rows])
+        assert torch.equal(got["dw"][outs], clean["dw"][outs])
+        assert torch.equal(got["db"][outs], clean["db"][outs])
+        assert not torch.isfinite(got["dx"][5]).any() and not torch.isfinite(got["db"][1])
+
+
+@pytest.mark.parametrize("act", list(ACTS))
+@pytest.mark.parametrize("n,K,M", SIZES)
+def test_odd_rows_stay_alone(gpu, n, K, M, act):
+    """A NaN or infinite value in one row of x or dy: the other rows of dx are bit
+    for bit what they are without it."""
+    t = make(n, K, M, torch.float16, residual=False, seed=2)
+    clean = step(t, act)
+    rows = torch.arange(n, device="cuda") != 7
+    for name in ("x", "dy"):
+        for value in (float("inf"), float("nan")):
+            bad = {**t, name: t[name].clone()}
+            bad[name][7, 3] = value
+            got = step(bad, act)
+            assert torch.equal(got["dx"][rows], clean["dx"][rows]), (name, value)
+            assert torch.equal(got["y"][rows], clean["y"][rows]), (name, value)
+            if name == "dy":
+                outs = torch.arange(M, device="cuda") != 3
+                assert torch.equal(got["dw"][outs], clean["dw"][outs]), value
+                assert torch.equal(got["db"][outs], clean["db"][outs]), value
