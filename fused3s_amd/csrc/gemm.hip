@@ -120,7 +120,9 @@ __device__ __forceinline__ void act_slopes(int act, float (&z)[N])
     case kActGeluTanh:
         each(z, [](float x) {
             const float s = gelu_tanh_cdf(x);
-            return s + x * s * (1.f - s) * 2.f * kTanhA * __builtin_fmaf(3.f * kTanhB * x, x, 1.f);
+            // (s (1 - s) is 0 from |x| = 10 on; x x overflows from 2^64 on)
+            const float t = __builtin_fminf(x * x, 1e4f);
+            return s + x * s * (1.f - s) * 2.f * kTanhA * __builtin_fmaf(3.f * kTanhB, t, 1.f);
         });
         break;
     case kActSilu:

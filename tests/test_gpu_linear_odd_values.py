@@ -58,3 +58,25 @@ def test_odd_rows_stay_alone(gpu, n, K, M, act):
                 outs = torch.arange(M, device="cuda") != 3
                 assert torch.equal(got["dw"][outs], clean["dw"][outs]), value
                 assert torch.equal(got["db"][outs], clean["db"][outs]), value
+
+
+@pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("n,K,M", SIZES)
+def test_gradient_of_large_products(gpu, n, K, M, act):
+    """z of any finite size (bfloat16 reaches 2^127): the slope is 0 or 1, not what an
+    overflow on the way makes of it."""
+    t = make(n, K, M, torch.bfloat16, residual=False, seed=3)
+    t["w"] = t["w"] * 2.0 ** -60          # (the columns below are their bias)
+    exps = [10, 20, 40, 63, 64, 65, 90, 120]
+    for i, e in enumerate(exps):
+        t["b"][2 * i], t["b"][2 * i + 1] = 2.0 ** e, -2.0 ** e
+    got = step(t, act)
+    on, off = slice(0, 2 * len(exps), 2), slice(1, 2 * len(exps), 2)
+    assert torch.isfinite(got["y"]).all()
+    assert torch.equal(got["y"][:, on], t["b"][on].expand(n, -1)) and not got["y"][:, off].any()
+    # db: n values of dy summed in float32, rounded once
+    dy = t["dy"][:, on].double()
+    bound = (n + 2) * 2.0 ** -24 * dy.abs().sum(0) + 2.0 ** -8 * dy.sum(0).abs()
+    assert ((got["db"][on].double() - dy.sum(0)).abs() <= bound).all()
+    assert not got["db"][off].any()
+    assert all(torch.isfinite(g).all() for g in got.values())
