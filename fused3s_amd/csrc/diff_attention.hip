@@ -25,7 +25,10 @@
 // Every 16-bit weight (p, p g, ds) is the sum of two (split8), two MFMAs
 // instead of one: p_1 and p_2 nearly cancel where lam is near 1 and the maps
 // are alike, and what a single rounding of each leaves is then large beside
-// their difference.  Sums and softmax statistics are in float32.
+// their difference.  binary16's two halves end at 2^-25, so what can be far below 1
+// is scaled: p g and ds by a power of two per row that follows them
+// (range_update), p_1 - lam p_2 of the columns by a fixed 2^14 (kLift).  Sums and
+// softmax statistics are in float32.
 //
 // A value that is infinite or NaN reaches, through the matrix cores, rows of its
 // window that have no edge to it (0 x inf).  So a window whose sums are not
@@ -392,6 +395,13 @@ __device__ __forceinline__ void map_update(DiffState& st, int m, const f4 s0, co
     }
 }
 
+// Weights of a size of 1 at most, in binary16: with |w| <= 2 they stay below 2^15, and
+// their halves end at 2^-39.  (A node that a row hardly attends, or that only rows of
+// very many edges do, has weights of 2^-17 and less alone: unscaled, 2^-20 was off by
+// 2^-6 of itself.)
+template <typename T>
+constexpr float kLift = Half<T>::kRange ? 16384.f : 1.f;
+
 // Scales weights of unknown size into binary16: a power of two per row, st.x[m],
 // moved (and the sums that it scales with it) when a weight would come within a
 // factor of four of the type's end, to put that weight at 2^3 to 2^4.
@@ -496,7 +506,8 @@ __device__ __forceinline__ void diff_finish(const DiffParams& p, DiffState& st, 
         if (lane == 0) p.dlam_parts[(int64_t)h * p.W + w] = s;
     } else {
         const float f1 = fast_exp2(st.x[0]), f2 = fast_exp2(st.x[1]);
-        const float back = Half<T>::kRange ? __builtin_fmaxf(1.f, __builtin_fabsf(lam)) : 1.f;
+        const float back =
+            Half<T>::kRange ? __builtin_fmaxf(1.f, __builtin_fabsf(lam)) * (1.f / kLift<T>) : 1.f;
         store_rows<T>(p.out1, stage, w, p.n, head_off, lane, [&](int t) {
             return t < 4 ? p.scale * (st.acc[t] * f1) : -lam * p.scale * (st.acc[t] * f2);
         });
@@ -750,10 +761,10 @@ diff_kernel(const DiffParams p)
                 return c + kBlockRecs < u.ce ? fetch(c + kBlockRecs) : fetch(go_on ? next.cb : u.cb);
             };
             if (u.cb < u.ce) blk = fetch_after(u.cb);
-            // |p_1 - lam p_2| <= 1 + |lam|: binary16's range needs lam out of it
+            // |p_1 - lam p_2| <= 1 + |lam|: binary16's range needs lam out of it, and kLift
             float fit = 1.f, fit_lam = u.lam;   // (uniform)
             if constexpr (PASS == kDiffColumns && Half<T>::kRange) {
-                fit = uniform(1.f / __builtin_fmaxf(1.f, __builtin_fabsf(u.lam)));
+                fit = uniform(kLift<T> / __builtin_fmaxf(1.f, __builtin_fabsf(u.lam)));
                 fit_lam = uniform(fit * u.lam);
             }
             if constexpr (PASS == kDiffRows) {
