@@ -27,8 +27,8 @@
 // are alike, and what a single rounding of each leaves is then large beside
 // their difference.  binary16's two halves end at 2^-25, so what can be far below 1
 // is scaled: p g and ds by a power of two per row that follows them
-// (range_update), p_1 - lam p_2 of the columns by a fixed 2^14 (kLift).  Sums and
-// softmax statistics are in float32.
+// (range_update), p of the rows and p_1 - lam p_2 of the columns by a fixed 2^14
+// (kLift).  Sums and softmax statistics are in float32.
 //
 // A value that is infinite or NaN reaches, through the matrix cores, rows of its
 // window that have no edge to it (0 x inf).  So a window whose sums are not
@@ -399,8 +399,21 @@ __device__ __forceinline__ void map_update(DiffState& st, int m, const f4 s0, co
 // their halves end at 2^-39.  (A node that a row hardly attends, or that only rows of
 // very many edges do, has weights of 2^-17 and less alone: unscaled, 2^-20 was off by
 // 2^-6 of itself.)
+// (In the rows' pass as an addend of the exponent: all its sums are divided by the
+// weights' own.  A row of 10^5 equal edges has weights of 2^-17, all rounded the same
+// way: dq, a difference of two sums of them, was off by 2^-8 of either.)
 template <typename T>
 constexpr float kLift = Half<T>::kRange ? 16384.f : 1.f;
+template <typename T>
+constexpr float kLiftLog2 = Half<T>::kRange ? 14.f : 0.f;
+// Such a weight's exponent.  A weight is at most 1, but for what a log-sum-exp of 24
+// bits leaves (logits past 2^24 come out as 2^2 and more): kept at 2 (rows, lifted) and
+// at 1 (columns), inside the type.  NaN stays.
+template <typename T>
+__device__ __forceinline__ float lifted(float x, float most)
+{
+    return Half<T>::kRange ? __builtin_elementwise_minimum(x, most) : x;
+}
 
 // Scales weights of unknown size into binary16: a power of two per row, st.x[m],
 // moved (and the sums that it scales with it) when a weight would come within a
@@ -773,6 +786,8 @@ diff_kernel(const DiffParams p)
                 // (the columns' pass finds them beside D)
                 if (l < 16 && row < n && (MODE != kDiffTeam || wave == 0))
                     *reinterpret_cast<float2*>(p.stats + ((int64_t)row * H + u.h) * 4) = lse;
+                lse.x -= kLiftLog2<T>;
+                lse.y -= kLiftLog2<T>;
                 // The matrix cores' sums are rounded towards one side, by some 2^-30 of
                 // g: nothing, but for dlam, where it adds up over all rows (500,000 of
                 // them: 1.4e-5 of it).  Odd rows take -do, and their sums of p g are
@@ -867,8 +882,10 @@ diff_kernel(const DiffParams p)
                             float pw[1][8], pg[1][8];
 #pragma unroll
                             for (int j = 0; j < 8; ++j) {
-                                const float e = fast_exp2(__builtin_fmaf(
-                                    sm[j >> 2][j & 3], p.scale_log2, m ? -lse.y : -lse.x));
+                                const float e = fast_exp2(lifted<T>(
+                                    __builtin_fmaf(sm[j >> 2][j & 3], p.scale_log2,
+                                                   m ? -lse.y : -lse.x),
+                                    kLiftLog2<T> + 1.f));
                                 pw[0][j] = where(on[j], e);
                                 st.z[m] += pw[0][j];
                             }
@@ -901,9 +918,11 @@ diff_kernel(const DiffParams p)
                             attends(masks, lane, on);
 #pragma unroll
                             for (int j = 0; j < 8; ++j)
-                                pw[m][j] = where(on[j], fast_exp2(__builtin_fmaf(
-                                                            s[m][j >> 2][j & 3], p.scale_log2,
-                                                            -L.stats[4 * slot_of(g, j) + m])));
+                                pw[m][j] = where(
+                                    on[j], fast_exp2(lifted<T>(
+                                               __builtin_fmaf(s[m][j >> 2][j & 3], p.scale_log2,
+                                                              -L.stats[4 * slot_of(g, j) + m]),
+                                               0.f)));
                         }
                         __builtin_amdgcn_sched_barrier(0);
                         if (kLate && more) load2(ahead, ahead_h);

@@ -353,7 +353,8 @@ f3s_status f3s_reverse_csr(const int32_t* d_row_ptr, const int32_t* d_col_idx, i
  * statistics are float32, O is rounded once.  An infinite or NaN value reaches
  * the rows with an edge to its node only (an infinite value of V makes their
  * sums NaN).  A row whose logits are all -inf is 0 if both maps' are, as one
- * without edges, else NaN.  Deterministic.
+ * without edges, else NaN.  Logits past 2^26 in size may come out as NaN: float32
+ * holds them to whole units only.  Deterministic.
  * workspace: f3s_diff_attention_workspace bytes (reversed NULL), 16-byte
  * aligned, this call's alone until it is done; nothing else is allocated or
  * kept, so calls may overlap and be captured.  Asynchronous on `stream`. */
