@@ -1299,8 +1299,9 @@ namespace f3s {
 // host round trip for their totals (and, for automatic plans, T and the
 // segment sizes computed on the device), then the item lists; the partial
 // buffer is shared by the sets (a plan serves one pass at a time).  From
-// kSchedOrderedMin window-heads on, with one wave per item (no teams), the
-// items follow the drop-in launch's schedule (classes of tile count,
+// kSchedOrderedMin window-heads on, with one wave per item (no teams), and
+// from kHeavyMaxWindows + 1 windows on where masked passes run no teams if
+// `by_schedule` asks for it, the items follow the drop-in launch's schedule (classes of tile count,
 // heaviest first, eight interleaved XCD shares; no team list: heavy windows
 // are split into segments), dealt round-robin, whatever the window order;
 // otherwise they follow the order's sequence.  (On config 4, 62,500
@@ -1314,9 +1315,16 @@ static f3s_status build_plan_sets(f3s_plan* p, const int32_t* d_window_offsets,
     const int32_t W = p->W, H = p->H;
     const bool automatic = seg_tiles == 0;
     const int32_t team_m = automatic ? team_for(W, H, true) : 1;
-    const int32_t team_d = automatic ? team_for(W, H, false) : 1;
+    // (by_schedule: such a plan is made for masked passes; the teams that tile-dense
+    // ones would run up to 2,048 window-heads do not decide its sequence)
+    const int32_t team_d =
+        automatic && !(by_schedule && team_m == 1) ? team_for(W, H, false) : 1;
     const int32_t nsets = automatic ? 2 : 1;
     const int arrays = 3 * nsets;
+    // (Few windows of many heads go without: a window's heads share a workgroup, and the
+    // heaviest of them a CU then.  Differential attention's forward pass, microseconds
+    // scheduled, in natural and in descending order, powerlaw, 14 edges a node: 8,000
+    // nodes, four heads 61, 44, 45; 9,000, two 36, 37, 41; 30,000, one 37, 46, 57.)
     const bool scheduled = W > kHeavyMaxWindows && team_m == 1 && team_d == 1 &&
                            (by_schedule || (int64_t)W * H >= kSchedOrderedMin);
     StreamBuffer sbuf(st);

@@ -275,8 +275,9 @@ class TorchGraph:
         return self
 
     def _compiled(self, bsf: DeviceBSF, s: Stream) -> Plan:
-        """A compiled plan in the library's sequence; small graphs' teams are the
-        same in every sequence."""
+        """A compiled plan in the library's sequence (in natural order up to 512
+        windows), its windows cut finer; small graphs' teams are the same in every
+        sequence."""
         plan = Plan(bsf, H=self.heads, stream=s, scheduled=True)
         plan.compile(s)
         plan.bsf = None   # the compiled lists are all that is read
@@ -284,8 +285,8 @@ class TorchGraph:
 
     def _diff_plan(self) -> Plan:
         """The plan of diff_attention: self.plan, where that follows the
-        library's sequence or the windows run on teams; else one that does, made
-        by the first call.  (Waits for the GPU then, so before a capture.)"""
+        library's sequence or the windows run on teams; else one made for it by the
+        first call (_compiled).  (Waits for the GPU then, so before a capture.)"""
         if self._scheduled is None:
             W = self.bsf.W
             if W * self.heads <= 1024 or W * self.heads >= 2**18:

@@ -248,10 +248,11 @@ f3s_status f3s_plan_create(const int32_t* d_window_offsets, const int32_t* d_win
                            int32_t W, int32_t H, int32_t seg_tiles, void* stream,
                            f3s_plan** plan_out);
 /* f3s_plan_create (automatic segments) whose items follow the library's
- * schedule from 513 windows on, where no teams run, not only from 2^18
- * window-heads: each class's windows in eight contiguous shares, one for each
- * XCD.  For passes of longer rows, which gain more from a community-ordered
- * graph's L2 reuse (f3s_diff_attention_fwd). */
+ * schedule from 513 windows on, wherever masked passes run no teams (past 1,024
+ * window-heads), not only from 2^18 window-heads: each class's windows in eight
+ * contiguous shares, one for each XCD.  Fewer windows keep their natural order.
+ * For passes of longer rows, which gain more from a community-ordered graph's
+ * L2 reuse (f3s_diff_attention_fwd). */
 f3s_status f3s_plan_create_scheduled(const int32_t* d_window_offsets, int32_t W, int32_t H,
                                      void* stream, f3s_plan** plan_out);
 f3s_status f3s_plan_destroy(f3s_plan* plan);
