@@ -1038,6 +1038,7 @@ static Tiling tiling(int64_t rows, int64_t outs, int64_t depth, int64_t least, b
     return best;
 }
 constexpr int64_t kForwardLeast = 512, kWeightLeast = 256;
+constexpr int64_t kDbOuts = 8;   // columns of the product that db alone takes
 
 static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
@@ -1206,8 +1207,13 @@ static BackwardSpace backward_space(int64_t n, int64_t K, int64_t M, int32_t act
         s.shares = s.sums + up256(sizeof(float) * (size_t)s.sum_rows * M);
         s.parts = s.shares + up256(sizeof(float) * (size_t)kSumShares * M);
     }
+    // dW of one split is written at once; db alone (no activation) still has a product,
+    // of at most eight columns, whose sums are all that is read
     s.dw = tiling(M, K, n, kWeightLeast, odd, true, act == kActNone);
-    parts = std::max(parts, sizeof(float) * (size_t)s.dw.splits * M * K);
+    if (s.dw.splits > 1)
+        parts = std::max(parts, sizeof(float) * (size_t)s.dw.splits * M * K);
+    else if (act == kActNone)
+        parts = std::max(parts, sizeof(float) * (size_t)M * std::min<int64_t>(K, kDbOuts));
     s.db = s.parts + up256(parts);
     s.bytes = s.db + up256(sizeof(float) * (size_t)s.dw.splits * M);
     return s;
@@ -1327,7 +1333,7 @@ static f3s_status backward(const LinearArgs& a, char* ws, hipStream_t st)
         p.Q = a.X;
         p.ldq = a.ldx;
         p.rows = a.M;
-        p.outs = a.dW ? a.K : std::min<int64_t>(a.K, 8);   // (db alone: one column of tiles)
+        p.outs = a.dW ? a.K : std::min<int64_t>(a.K, kDbOuts);   // (db alone: one column of tiles)
         p.depth = a.n;
         p.sums = db_left ? reinterpret_cast<float*>(ws + s.db) : nullptr;
         // (one split: no sums to join; 4,096 x 4,096 of 4,096 rows 145 us, 181 with them)
