@@ -70,6 +70,8 @@ HIP_API = {
                                          c_vp]),
     "f3s_linear_f16": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_i64, c_i32, c_i32, c_vp]),
     "f3s_linear_workspace": (c_i32, [c_i64, c_i64, c_i64, c_i32, c_i32, P_i64]),
+    "f3s_linear_tiling": (c_i32, [c_i64, c_i64, c_i64, c_i32, c_i32, c_i32, P_i32, P_i32, P_i32,
+                                  P_i64, P_i64, P_i32]),
     "f3s_linear_fwd": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64,
                                c_i32, c_i32, c_vp, c_i64, c_vp]),
     "f3s_linear_bwd": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64,

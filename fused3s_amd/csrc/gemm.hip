@@ -1042,15 +1042,26 @@ constexpr int64_t kDbOuts = 8;   // columns of the product that db alone takes
 
 static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
+static int32_t tile_size(const Tiling& t, int way, int epi)
+{
+    return has_256(way, epi) ? t.tile : std::min(t.tile, 128);
+}
+
+// Workgroups of each split: as many as are resident at once, a multiple of eight (XCDs).
+static int64_t workgroups_of(int64_t tiles, int32_t tile, int32_t splits)
+{
+    const int64_t resident = tile == 256 ? 256 : tile == 128 ? 512 : 1280;
+    return std::min(tiles, std::max<int64_t>(8, resident / splits / 8 * 8));
+}
+
 template <typename T, bool PT, bool QT, int EPI, int WAY>
 static void launch_tiles(GemmParams p, int32_t tile, hipStream_t st)
 {
     p.row_tiles = (int32_t)ceil_div(p.rows, tile);
     p.out_tiles = (int32_t)ceil_div(p.outs, tile);
     p.split = ceil_div(ceil_div(p.depth, p.splits), 64) * 64;
-    // as many workgroups as are resident at once, a multiple of eight (XCDs)
-    const int64_t most = std::max<int64_t>(8, (tile == 256 ? 256 : tile == 128 ? 512 : 1280) / p.splits / 8 * 8);
-    const dim3 grid((unsigned)std::min((int64_t)p.row_tiles * p.out_tiles, most), (unsigned)p.splits);
+    const dim3 grid((unsigned)workgroups_of((int64_t)p.row_tiles * p.out_tiles, tile, p.splits),
+                    (unsigned)p.splits);
     if (tile == 64)
         hipLaunchKernelGGL((gemm_kernel<T, PT, QT, 64, EPI, WAY>), grid, dim3(256), 0, st, p);
     else if (tile == 128)
@@ -1084,7 +1095,7 @@ static f3s_status launch_gemm(GemmParams p, const Tiling& t, hipStream_t st)
         return F3S_EUNSUPPORTED;
     }
     const Way way = way_of(p, PT, QT);
-    const int32_t tile = has_256(way, EPI) ? t.tile : std::min(t.tile, 128);
+    const int32_t tile = tile_size(t, way, EPI);
     if (way == kWhole) launch_tiles<T, PT, QT, EPI, kWhole>(p, tile, st);
     else if (way == kAny) launch_tiles<T, PT, QT, EPI, kAny>(p, tile, st);
     else if constexpr (!PT && !QT) launch_tiles<T, PT, QT, EPI, kTiles>(p, tile, st);
@@ -1280,9 +1291,7 @@ static f3s_status backward(const LinearArgs& a, char* ws, hipStream_t st)
                                dim3(256), 0, st, p, reinterpret_cast<const float*>(ws + s.parts));
             F3S_HIP(hipGetLastError());
         } else {
-            const int32_t tile = has_256(way_of(p), kEpiSlope) ? s.slope.tile
-                                                             : std::min(s.slope.tile, 128);
-            sum_rows = 2 * ceil_div(a.n, tile);
+            sum_rows = 2 * ceil_div(a.n, tile_size(s.slope, way_of(p), kEpiSlope));
             F3S_TRY((launch_gemm<T, false, false, kEpiSlope>(p, s.slope, st)));
         }
         dz = ws + s.dz;
@@ -1378,6 +1387,54 @@ f3s_status f3s_linear_workspace(int64_t n, int64_t K, int64_t M, int32_t act, in
     F3S_TRY(check_linear(n, K, M, act, F3S_F16, "f3s_linear_workspace"));
     *bytes = (int64_t)(n == 0 ? 0 : backward_pass ? backward_space(n, K, M, act).bytes
                                                   : forward_bytes(n, K, M));
+    return F3S_OK;
+}
+
+f3s_status f3s_linear_tiling(int64_t n, int64_t K, int64_t M, int32_t act, int32_t bias,
+                             int32_t product, int32_t* kernel, int32_t* tile, int32_t* splits,
+                             int64_t* tiles, int64_t* workgroups, int32_t* pieces)
+{
+    F3S_TRY(check_linear(n, K, M, act, F3S_F16, "f3s_linear_tiling"));
+    F3S_REQUIRE(n > 0 && product >= F3S_LINEAR_FORWARD && product <= F3S_LINEAR_DW,
+                "f3s_linear_tiling: no rows, or an unknown product");
+    const char* aligned = reinterpret_cast<const char*>((uintptr_t)256);
+    const BackwardSpace s = backward_space(n, K, M, act);
+    const bool dx = product == F3S_LINEAR_DX, dw = product == F3S_LINEAR_DW;
+    const bool sums = dw && bias && act == kActNone;   // db beside dW
+    GemmParams p{};
+    p.P = p.Q = aligned;
+    p.C = const_cast<char*>(aligned);
+    p.rows = dw ? M : n;
+    p.outs = dx || dw ? K : M;
+    p.depth = dx ? M : dw ? n : K;
+    p.ldp = dx || dw ? M : K;
+    p.ldq = K;
+    p.q_steps = dx;
+    if (product == F3S_LINEAR_SLOPE) {
+        p.R = aligned;
+        p.ldr = M;
+    }
+    const Tiling t = dx ? s.dx : dw ? s.dw
+                                    : tiling(n, M, K, kForwardLeast, K % 8 != 0, false);
+    const Way way = way_of(p, dw, dx || dw);
+    const bool parts = t.splits > 1;
+    const int epi = dw ? (sums ? (parts ? kEpiPartSums : kEpiPlainSums)
+                               : parts ? kEpiPart : kEpiPlain)
+                       : parts ? kEpiPart
+                               : dx ? kEpiPlain
+                                    : product == F3S_LINEAR_SLOPE ? kEpiSlope : kEpiForward;
+    const int32_t kind = !dw && takes_rows(p) ? F3S_LINEAR_W_IN_LDS
+                         : product == F3S_LINEAR_FORWARD && n <= kFewRows ? F3S_LINEAR_FEW_ROWS
+                                                                          : F3S_LINEAR_TILES;
+    const bool tiled = kind == F3S_LINEAR_TILES;
+    const int32_t size = tiled ? tile_size(t, way, epi) : 0;
+    const int64_t count = tiled ? ceil_div(p.rows, size) * ceil_div(p.outs, size) : 0;
+    if (kernel) *kernel = kind;
+    if (tile) *tile = size;
+    if (splits) *splits = tiled ? t.splits : 1;
+    if (tiles) *tiles = count;
+    if (workgroups) *workgroups = tiled ? workgroups_of(count, size, t.splits) : 0;
+    if (pieces) *pieces = way;
     return F3S_OK;
 }
 

@@ -317,6 +317,22 @@ f3s_status f3s_linear_f16(const uint16_t* X, const uint16_t* W, const uint16_t* 
 #define F3S_ACT_SILU 4
 f3s_status f3s_linear_workspace(int64_t n, int64_t K, int64_t M, int32_t act, int32_t backward_pass,
                                 int64_t* bytes);
+/* How a product of such a call runs, for tests and measurements: F3S_LINEAR_FORWARD, the
+ * backward pass's SLOPE (z again; with an activation), DX or DW (`bias`: with db), of
+ * contiguous 16-byte-aligned tensors.  kernel: up to 64 rows, W held in LDS, or tiles;
+ * tiles only: their side, splits of the contraction, tiles and workgroups of each split
+ * (fewer workgroups take several tiles each); pieces: 2 whole 16-byte pieces everywhere,
+ * 1 in the operands' rows, 0 neither.  Any output may be NULL. */
+#define F3S_LINEAR_FORWARD 0
+#define F3S_LINEAR_SLOPE 1
+#define F3S_LINEAR_DX 2
+#define F3S_LINEAR_DW 3
+#define F3S_LINEAR_FEW_ROWS 0
+#define F3S_LINEAR_W_IN_LDS 1
+#define F3S_LINEAR_TILES 2
+f3s_status f3s_linear_tiling(int64_t n, int64_t K, int64_t M, int32_t act, int32_t bias,
+                             int32_t product, int32_t* kernel, int32_t* tile, int32_t* splits,
+                             int64_t* tiles, int64_t* workgroups, int32_t* pieces);
 f3s_status f3s_linear_fwd(const uint16_t* X, int64_t x_stride, const uint16_t* W,
                           const uint16_t* bias, const uint16_t* R, int64_t r_stride, uint16_t* Y,
                           int64_t n, int64_t K, int64_t M, int32_t act, int32_t dtype,
