@@ -31,6 +31,7 @@ from __future__ import annotations
 import numpy as np
 import torch
 from torch.autograd import forward_ad
+from torch.fx import _symbolic_trace
 from torch.utils._device import DeviceContext
 
 # torch ships its own HIP runtime (torch/lib/libamdhip64.so, soname
@@ -73,8 +74,6 @@ _current_device = torch._C._cuda_getDevice
 _NO_CONTEXT = contextlib.nullcontext()
 
 _dispatch_modes, _is_tracing = torch._C._len_torch_dispatch_stack, torch._C._is_tracing
-_key_included, _PRE_DISPATCH = (torch._C._dispatch_tls_is_dispatch_key_included,
-                                torch._C.DispatchKey.PreDispatch)
 _transform, _dynamo = torch._C._functorch.peek_interpreter_stack, torch.compiler.is_dynamo_compiling
 
 
@@ -112,7 +111,7 @@ def _refuse_unseen(who: str, *tensors) -> None:
         raise RuntimeError(f"{who} has no forward-mode derivative")
     if compiled:
         return   # (its graph breaks at the library's call, which then runs, or it raises)
-    if (_is_tracing() or _key_included(_PRE_DISPATCH)
+    if (_is_tracing() or _symbolic_trace._is_fx_tracing_flag
             or _dispatch_modes() > 0 and _records_or_replaces()
             or _transform() is not None and _transformed(tensors)):
         raise RuntimeError(f"{who} cannot be traced or transformed: its kernel is not an operator "
