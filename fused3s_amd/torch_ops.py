@@ -374,21 +374,23 @@ def _rows(t: torch.Tensor, graph: TorchGraph) -> torch.Tensor:
         t = t.contiguous()
     if t.dim() == 3:
         t = t.as_strided((n, width), (t.stride(0), 1))
-    if t.stride(1) != 1 or t.stride(0) % 8 or t.stride(0) < width or t.data_ptr() % 16:
+    if t.stride(1) != 1 or t.data_ptr() % 16 or n > 1 and (t.stride(0) % 8
+                                                           or t.stride(0) < width):
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
 def _thirds(qkv: torch.Tensor, graph: TorchGraph):
     width = graph.heads * 2 * HEAD_DIM
-    if qkv.stride(-1) != 1 or qkv.stride(0) % 8 or qkv.data_ptr() % 16 or (
-            graph.n > 1 and qkv.stride(0) < 3 * width):
+    if qkv.stride(-1) != 1 or qkv.data_ptr() % 16 or (
+            graph.n > 1 and (qkv.stride(0) % 8 or qkv.stride(0) < 3 * width)):
         qkv = qkv.clone(memory_format=torch.contiguous_format)
     return tuple(qkv[:, i * width:(i + 1) * width] for i in range(3))
 
 
 def _stride(t: torch.Tensor) -> int:
-    return max(t.stride(0), t.shape[1])
+    """Values between rows (a single row's stride is of any size and not used)."""
+    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
 
 
 def _diff_forward(graph: TorchGraph, scale: float, lam, q, k, v, lse=None) -> torch.Tensor:

@@ -80,3 +80,27 @@ def test_gradient_of_large_products(gpu, n, K, M, act):
     assert ((got["db"][on].double() - dy.sum(0)).abs() <= bound).all()
     assert not got["db"][off].any()
     assert all(torch.isfinite(g).all() for g in got.values())
+
+
+def test_one_row_of_any_stride(gpu):
+    """A single row's stride means nothing, however large or odd."""
+    from fused3s_amd.torch_ops import TorchGraph, linear
+    import numpy as np
+    t = make(1, 64, 72, torch.float16)
+    want = step(t, "silu")
+    graph = TorchGraph(np.array([0, 1], np.int32), np.zeros(1, np.int32), heads=1)
+    row = torch.randn(1, 3 * 128, device="cuda").half()
+    lam = torch.tensor([0.5], device="cuda")
+    o = graph.diff_attention_packed(row, lam, 0.125)
+    for stride in (0, 1, 7, 2 ** 22, 2 ** 30, 2 ** 31 + 1):
+        x, r = (t[k].as_strided(t[k].shape, (stride, 1)) for k in "xr")
+        assert torch.equal(linear(x, t["w"], t["b"], "silu", r), want["y"]), stride
+        odd = row.as_strided(row.shape, (stride, 1))
+        leaf = odd.detach().requires_grad_()
+        again = graph.diff_attention_packed(leaf, lam, 0.125)
+        assert torch.equal(again, o), stride
+        again.sum().backward()
+        q, k, v = (odd[:, 128 * i:128 * i + 128] for i in range(3))
+        assert torch.equal(graph.diff_attention(q, k, v, lam, 0.125), o), stride
+        q = q.view(1, 1, 128).as_strided((1, 1, 128), (stride, 3, 1))
+        assert torch.equal(graph.diff_attention(q, k, v, lam, 0.125), o), stride
