@@ -547,11 +547,13 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     if residual is not None and residual.shape != shape:
         raise ValueError(f"residual must have shape {shape}, got {tuple(residual.shape)}")
     dtype, device = x.dtype, x.device
-    for name, t in (("x", x), ("weight", weight), ("bias", bias), ("residual", residual)):
-        if t is not None and (t.dtype is not dtype or t.device != device
-                              or dtype not in _DTYPES or not t.is_cuda):
-            raise ValueError(f"{name} must be a float16 or bfloat16 tensor on a GPU, of x's type "
-                             "and device")
+    if (dtype not in _DTYPES or not x.is_cuda
+            or weight.dtype is not dtype or weight.device != device
+            or bias is not None and (bias.dtype is not dtype or bias.device != device)
+            or residual is not None and (residual.dtype is not dtype
+                                         or residual.device != device)):
+        raise ValueError("x, weight, bias and residual must be float16 or bfloat16 tensors on a "
+                         "GPU, all of one type and on one device")
     if device.index != _current_device():
         with torch.cuda.device(device):
             return linear(x, weight, bias, activation, residual)
