@@ -6,8 +6,8 @@ graph's edges, and an output projection.  Here torch supplies the device
 memory and the stream; the attention is the HIP library's planned pass
 (f3s_attention_fwd_planned), called on torch's current stream with the
 tensors' device pointers, and the layer's projections are its f3s_linear_f16
-(torch.nn.Linear's own product where that kernel is not the better one).  There is no CPU fallback, and
-that pass is forward-only: calling it on tensors that require grad raises.
+(torch.nn.Linear's own product where that kernel is not the better one).  There
+is no CPU fallback, and that pass is forward-only: calling it on tensors that require grad raises.
 Differential attention (two softmax maps per head and their difference) and
 linear(), a projection with bias, activation and residual, have gradients.
 
@@ -388,9 +388,9 @@ def _thirds(qkv: torch.Tensor, graph: TorchGraph):
     return tuple(qkv[:, i * width:(i + 1) * width] for i in range(3))
 
 
-def _stride(t: torch.Tensor) -> int:
-    """Values between rows (a single row's stride is of any size and not used)."""
-    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+def _stride(t: torch.Tensor, n: int) -> int:
+    """Values between the n rows (a single row's stride is of any size and not used)."""
+    return t.stride(0) if n > 1 else t.shape[1]
 
 
 def _diff_forward(graph: TorchGraph, scale: float, lam, q, k, v, lse=None) -> torch.Tensor:
@@ -402,8 +402,8 @@ def _diff_forward(graph: TorchGraph, scale: float, lam, q, k, v, lse=None) -> to
         if not lam.is_contiguous():
             lam = lam.contiguous()
         check(_lib.hip().f3s_diff_attention_fwd(
-            plan, q.data_ptr(), _stride(q), k.data_ptr(), _stride(k), v.data_ptr(), _stride(v),
-            lam.data_ptr(), out.data_ptr(), H * 2 * HEAD_DIM,
+            plan, q.data_ptr(), _stride(q, n), k.data_ptr(), _stride(k, n), v.data_ptr(),
+            _stride(v, n), lam.data_ptr(), out.data_ptr(), H * 2 * HEAD_DIM,
             None if lse is None else lse.data_ptr(), _DTYPES[q.dtype], n, H, scale,
             None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
             _raw_stream(graph.device)), "f3s_diff_attention_fwd")
@@ -442,10 +442,11 @@ class _DiffAttention(torch.autograd.Function):
         with _on(graph.device):
             ws = graph._diff_workspace(True)
             check(_lib.hip().f3s_diff_attention_bwd(
-                graph._diff_plan().handle, graph._reversed.handle, q.data_ptr(), _stride(q),
-                k.data_ptr(), _stride(k), v.data_ptr(), _stride(v), lam.data_ptr(), lse.data_ptr(),
-                do.data_ptr(), _stride(do), dq.data_ptr(), _stride(dq), dk.data_ptr(), _stride(dk),
-                dv.data_ptr(), _stride(dv), dlam.data_ptr(), _DTYPES[q.dtype], n, H, ctx.scale,
+                graph._diff_plan().handle, graph._reversed.handle, q.data_ptr(), _stride(q, n),
+                k.data_ptr(), _stride(k, n), v.data_ptr(), _stride(v, n), lam.data_ptr(),
+                lse.data_ptr(), do.data_ptr(), _stride(do, n), dq.data_ptr(), _stride(dq, n),
+                dk.data_ptr(), _stride(dk, n), dv.data_ptr(), _stride(dv, n), dlam.data_ptr(),
+                _DTYPES[q.dtype], n, H, ctx.scale,
                 ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
                 _raw_stream(graph.device)), "f3s_diff_attention_bwd")
         return None, None, dlam, *grads
@@ -480,8 +481,8 @@ def _linear_forward(x, w, b, r, act):
     if n:
         ws = _linear_workspace(n, K, M, act, 0, x.device) if n > 64 else None
         check(_lib.hip().f3s_linear_fwd(
-            x.data_ptr(), _stride(x), w.data_ptr(), b.data_ptr() if b is not None else None,
-            r.data_ptr() if r is not None else None, _stride(r) if r is not None else 0,
+            x.data_ptr(), _stride(x, n), w.data_ptr(), b.data_ptr() if b is not None else None,
+            r.data_ptr() if r is not None else None, _stride(r, n) if r is not None else 0,
             y.data_ptr(), n, K, M, act, _DTYPES[x.dtype],
             ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
             _raw_stream(x.device.index)), "f3s_linear_fwd")
@@ -510,8 +511,8 @@ class _Linear(torch.autograd.Function):
             with _on(x.device.index):
                 ws = _linear_workspace(n, K, M, act, 1, x.device)
                 check(_lib.hip().f3s_linear_bwd(
-                    x.data_ptr(), _stride(x), w.data_ptr(),
-                    b.data_ptr() if b is not None else None, dy.data_ptr(), _stride(dy),
+                    x.data_ptr(), _stride(x, n), w.data_ptr(),
+                    b.data_ptr() if b is not None else None, dy.data_ptr(), _stride(dy, n),
                     *(t.data_ptr() if t is not None else None for t in (dx, dw, db)), n, K, M, act,
                     _DTYPES[x.dtype], ws.data_ptr() if ws is not None else None,
                     ws.numel() if ws is not None else 0, _raw_stream(x.device.index)),
