@@ -356,9 +356,10 @@ __device__ __forceinline__ void finish8(const GemmParams& p, int64_t row, int64_
 // 256: eight waves of 128 rows by 64 outputs.  (What bounds the small ones is the
 // way from L2 to LDS, 64 bytes per clock and CU: 128 x 128 x 64 products take its
 // time as long as the matrix cores'; 256 x 256 x 64 half of it.  32,768 x 1,024 ->
-// 4,096, TFLOP/s: 64 560, 128 737, 256 910; 256 by four waves of 128 x 128, a wave
-// per SIMD, 776; three steps of 32 with the next one's operands read ahead into
-// registers, 256 x 256 743, 256 x 128 698.)
+// 4,096, TFLOP/s: 64 560, 128 737, 256 910 and, since its second half's operands are
+// read between the first half's products, 1,020; beside the 910, 256 by four waves of
+// 128 x 128, a wave per SIMD, 776; three steps of 32 with the next one's operands read
+// ahead into registers, 256 x 256 743, 256 x 128 698.)
 template <int SIZE>
 struct Shape {
     static constexpr int wave_rows = 2, wave_outs = SIZE == 256 ? 4 : 2, waves = wave_rows * wave_outs;
@@ -691,6 +692,12 @@ __device__ __forceinline__ f2 row_sums(const float (&v)[8], int r)
 // wave's own in LDS, joined in order at the end).
 // Bound by the rows in and out, and by the activation where it has one (gelu: 20
 // operations' time a value).
+// (f3s_linear_f16's linear_kernel (linear.hip) streams rows past W in the same order, in
+// binary16, without strides or an epilogue; from 48 K rows on both give the same bits.
+// It stays for the forward-only layer: 50,000 x 64 -> 192 7.2 us against 8.0 here, where
+// the activation is looked at for every piece; 50,000 x 128 -> 384 14.7 and 15.1,
+// 500,000 x 128 -> 512 133 and 134; and below 48 K rows its callers keep the bits they
+// have, which tiles do not give.)
 enum RowsMode : int { kRowsAct = 0, kRowsResidual = 1, kRowsSlope = 2 };
 constexpr int kRowWaves = 16, kRowPieces = 6144;
 // outputs per workgroup at most
@@ -1002,7 +1009,9 @@ constexpr bool has_256(int way, int epi)
 // time where an operand's rows are no whole pieces.
 // (Microseconds with 64, 128, 256, chosen; forward: 8,192 x 1,024 -> 1,024 32, 25,
 // 40, 25; 200,003 x 512 -> 128 53, 55, 84, 53; 2,048 x 2,048 -> 2,048 28, 28, 49, 28;
-// 1,024 x 1,024 -> 1,024 12, 16, 25, 12.)
+// 1,024 x 1,024 -> 1,024 12, 16, 25, 12.  The rates are those at which these choices
+// were measured; tiles of 256 have become faster since, so that their estimates are high:
+// 344 us for 32,768 x 1,024 -> 4,096, which takes 268, and 157 for 4,096 cubed, 112.)
 struct Tiling {
     int32_t tile, splits;
 };

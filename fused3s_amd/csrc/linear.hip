@@ -14,6 +14,9 @@
 // 193 us in the library; non-temporal stores 92 us, but the fused pass then
 // finds nothing of its Q, K and V in the caches: layer 627 against 635 us).
 // 32 rows per wave, halving the LDS reads, changed nothing: they do not bound it.
+// (The product with an epilogue, gemm.hip, has a kernel of this order for many rows
+// too, with bfloat16, strides, activation, residual and slope; what both take is said
+// there.)
 #include <algorithm>
 
 #include "attn_common.hpp"

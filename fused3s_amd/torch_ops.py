@@ -253,7 +253,8 @@ class TorchGraph:
         the reversed edges; the first call that needs it does so otherwise.
         Waits for the GPU, so before a capture.  (The leaves of a captured step
         must not belong to an eager step that is still alive, as with torch's
-        own operators: capture with detached ones.)"""
+        own operators: capture with detached ones.  A captured call reads this
+        object's lists, so it has to outlive the replays.)"""
         if self._reversed is None:
             if not self.masked:
                 raise ValueError("a gradient needs the masked (edge-exact) semantics")
