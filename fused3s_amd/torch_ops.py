@@ -337,7 +337,8 @@ class TorchGraph:
         contiguous, rows at any distance of a multiple of 8 values (a slice of a
         projection's output is taken as it is; other layouts are copied);
         lam: float32 [H].  Returns [n, H, 128] in q's type: sums in float32,
-        rounded once; nodes without edges get 0.  Differentiable in q, k, v and
+        rounded once; nodes without edges get 0.  (Logits are float32: past 2^24 in
+        size the weights are not resolved.)  Differentiable in q, k, v and
         lam (once); tracing, functorch's transforms and forward-mode differentiation
         are refused.  A graph serves any number of calls at once."""
         _refuse_unseen("diff_attention", q, k, v, lam)
