@@ -12,8 +12,8 @@
 //            rounding beside their own, 1.41 x the error of one (32,768 x 1,024 ->
 //            4,096, gelu, bfloat16, against 64 bits in the 2-norm: 2.34e-3, where
 //            rounding the result alone is 1.66e-3).  Two 16-bit values for each
-//            would take twice the matrix instructions of both products, two thirds
-//            of a step.  db is summed before the rounding.  Without an activation
+//            would take twice the matrix instructions of both (six products' for a
+//            step's four).  db is summed before the rounding.  Without an activation
 //            dz is dy, and every result is rounded once.
 //   dx       P = dz [n][M],     Q = W, transposed
 //   dW       P, Q = dz, x, both transposed, n cut into splits whose float32

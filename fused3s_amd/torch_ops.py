@@ -217,7 +217,7 @@ class TorchGraph:
         check(_lib.hip().f3s_attention_fwd_planned(
             self.plan.handle, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
             bsf.block_col.ptr, bsf.tile_mask.ptr if self.masked else None, n, HEAD_DIM, H, scale,
-            torch.cuda.current_stream().cuda_stream), "f3s_attention_fwd_planned")
+            _raw_stream(_current_device())), "f3s_attention_fwd_planned")
         return out
 
     def takes_packed(self) -> bool:
@@ -245,7 +245,7 @@ class TorchGraph:
             check(_lib.hip().f3s_attention_fwd_packed(
                 self.plan.handle, qkv.data_ptr(), out.data_ptr(), int(dtype == torch.float16),
                 self.n, HEAD_DIM, self.heads, float(scale),
-                torch.cuda.current_stream().cuda_stream), "f3s_attention_fwd_packed")
+                _raw_stream(_current_device())), "f3s_attention_fwd_packed")
         return out
 
     def prepare_backward(self) -> "TorchGraph":

@@ -84,3 +84,26 @@ def test_weights_of_a_subclass_are_torchs(gpu):
                 assert torch.nn.functional.linear in Counted.seen, name
                 assert (y - want).abs().max() <= 2.0 ** -8 * want.abs().max(), name
                 setattr(owner, leaf, p)
+
+
+def test_attention_follows_the_current_stream(gpu):
+    """The forward-only passes run on torch's current stream: behind work that is
+    still ahead of them there."""
+    for layer, graph, x in layers():
+        q = torch.randn(300, 2, 64, device="cuda").half()
+        qkv = torch.randn(300, 384, device="cuda").half()
+        want = graph.attention(q, q, q, 0.125), graph.attention_packed(qkv, 0.125)
+        torch.cuda.synchronize()
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            busy = torch.randn(4096, 4096, device="cuda")
+            for _ in range(20):
+                busy = busy @ busy * 1e-2
+            late = q * 0, qkv * 0
+            late[0].copy_(q)
+            late[1].copy_(qkv)
+            got = graph.attention(late[0], late[0], late[0], 0.125), graph.attention_packed(late[1], 0.125)
+        side.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+        break
