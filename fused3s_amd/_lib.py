@@ -76,6 +76,11 @@ HIP_API = {
                                c_i32, c_i32, c_vp, c_i64, c_vp]),
     "f3s_linear_bwd": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64,
                                c_i64, c_i64, c_i32, c_i32, c_vp, c_i64, c_vp]),
+    "f3s_layer_norm_fwd": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_f32, c_i32,
+                                   c_i32, c_vp]),
+    "f3s_layer_norm_workspace": (c_i32, [c_i64, c_i64, c_i32, P_i64]),
+    "f3s_layer_norm_bwd": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64,
+                                   c_i64, c_i32, c_i32, c_vp, c_i64, c_vp]),
     "f3s_reverse_csr": (c_i32, [c_vp, c_vp, c_i32, c_i64, c_vp, c_vp, c_vp]),
     "f3s_diff_attention_workspace": (c_i32, [c_vp, c_vp, P_i64]),
     "f3s_diff_attention_fwd": (c_i32, [c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp,

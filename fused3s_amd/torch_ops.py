@@ -575,6 +575,104 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     return y if flat else y.view(shape)
 
 
+_NORM_DTYPES = {**_DTYPES, torch.float32: 2}   # F3S_F32
+
+
+@functools.lru_cache(maxsize=256)
+def _norm_bytes(n, width, dtype) -> int:
+    need = C.c_int64()
+    check(_lib.hip().f3s_layer_norm_workspace(n, width, dtype, C.byref(need)),
+          "f3s_layer_norm_workspace")
+    return need.value
+
+
+def _norm_forward(x, w, b, eps, stats=None):
+    n, width = x.shape
+    y = x.new_empty((n, width))
+    if n:
+        dtype = _NORM_DTYPES[x.dtype]
+        of = w if w is not None else b
+        check(_lib.hip().f3s_layer_norm_fwd(
+            x.data_ptr(), _stride(x, n), w.data_ptr() if w is not None else None,
+            b.data_ptr() if b is not None else None, y.data_ptr(),
+            stats.data_ptr() if stats is not None else None, n, width, eps, dtype,
+            dtype if of is None else _NORM_DTYPES[of.dtype], _raw_stream(x.device.index)),
+            "f3s_layer_norm_fwd")
+    return y
+
+
+class _LayerNorm(torch.autograd.Function):
+    """layer_norm()'s matrix and its gradients."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, eps):
+        stats = torch.empty((x.shape[0], 2), dtype=torch.float32, device=x.device)
+        ctx.of = None if b is None else b.dtype
+        ctx.save_for_backward(x, w, stats)
+        return _norm_forward(x, w, b, eps, stats)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, w, stats = ctx.saved_tensors
+        n, width = x.shape
+        needs = ctx.needs_input_grad
+        of = ctx.of if w is None else w.dtype
+        dx = x.new_empty((n, width)) if needs[0] else None
+        dw, db = (x.new_empty(width, dtype=of) if wanted else None for wanted in needs[1:3])
+        if any(needs[:3]):
+            dtype = _NORM_DTYPES[x.dtype]
+            dy = _matrix(grad)
+            with _on(x.device.index):
+                ws = (torch.empty(_norm_bytes(n, width, dtype), dtype=torch.uint8, device=x.device)
+                      if needs[1] or needs[2] else None)
+                check(_lib.hip().f3s_layer_norm_bwd(
+                    x.data_ptr(), _stride(x, n), w.data_ptr() if w is not None else None,
+                    stats.data_ptr(), dy.data_ptr(), _stride(dy, n),
+                    *(t.data_ptr() if t is not None else None for t in (dx, dw, db)), n, width,
+                    dtype, dtype if of is None else _NORM_DTYPES[of],
+                    ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
+                    _raw_stream(x.device.index)), "f3s_layer_norm_bwd")
+        return dx, dw, db, None
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
+               bias: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
+    """(x - mean) / sqrt(variance + eps) * weight + bias over the last dimension: x
+    [..., width] float16, bfloat16 or float32 on a GPU, weight and bias [width], both of
+    x's type or both float32.  Returns x's type; sums are float32, every result is
+    rounded once.  Differentiable (once) in all three; the gradients of weight and
+    bias are the same from run to run.  Tracing, functorch's transforms and
+    forward-mode differentiation are refused."""
+    _refuse_unseen("layer_norm", x, weight, bias)
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"x must have a last dimension of at least 1, got {tuple(x.shape)}")
+    width, dtype, device = x.shape[-1], x.dtype, x.device
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and t.shape != (width,):
+            raise ValueError(f"{name} must have shape {(width,)}, got {tuple(t.shape)}")
+    of = weight if weight is not None else bias
+    if (dtype not in _NORM_DTYPES or not x.is_cuda
+            or of is not None and ((of.dtype is not dtype and of.dtype is not torch.float32)
+                                   or of.device != device)
+            or weight is not None and bias is not None and (bias.dtype is not weight.dtype
+                                                            or bias.device != device)):
+        raise ValueError("x must be a float16, bfloat16 or float32 tensor on a GPU, weight and bias "
+                         "both of its type or both float32, on its device")
+    if device.index != _current_device():
+        with torch.cuda.device(device):
+            return layer_norm(x, weight, bias, eps)
+    x2 = _matrix(x if x.dim() == 2 else x.reshape(-1, width))
+    w = weight if weight is None or weight.is_contiguous() else weight.contiguous()
+    b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or weight is not None and weight.requires_grad
+                                    or bias is not None and bias.requires_grad):
+        y = _LayerNorm.apply(x2, w, b, float(eps))
+    else:
+        y = _norm_forward(x2, w, b, float(eps))
+    return y if x.dim() == 2 else y.view(x.shape)
+
+
 _LINEAR_FORWARD, _LINEAR = torch.nn.Linear.forward, torch.nn.functional.linear
 
 

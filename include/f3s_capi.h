@@ -49,6 +49,7 @@ typedef int32_t f3s_status;
 /* 16-bit types of the calls that take both. */
 #define F3S_F16 0           /* IEEE binary16 */
 #define F3S_BF16 1          /* bfloat16 */
+#define F3S_F32 2           /* float32, where a call says that it takes it */
 
 /* Semantics of f3s_attention_fwd*: tile_mask == NULL selects TILE_DENSE
  * (every column < n of every active tile is attended: the reference kernel
@@ -347,6 +348,28 @@ f3s_status f3s_linear_bwd(const uint16_t* X, int64_t x_stride, const uint16_t* W
                           const uint16_t* bias, const uint16_t* dY, int64_t dy_stride, uint16_t* dX,
                           uint16_t* dW, uint16_t* db, int64_t n, int64_t K, int64_t M, int32_t act,
                           int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Layer norm of rows of `width` values (no reference counterpart):
+ *   Y = (X - m) r W + B,  m the row's mean, r = 1 / sqrt(its variance + eps)
+ * X and Y in `dtype` (F3S_F16, F3S_BF16 or F3S_F32), W and B (NULL: ones, zeros)
+ * in weight_dtype: the same or F3S_F32.  Sums are float32, results rounded once.
+ * Rows of X are x_stride values apart, Y is contiguous; no alignment is needed
+ * beyond the types' own.  stats, where not NULL, receives [n][2] float32 (m, r)
+ * for the gradient.  width < 2^24, n < 2^40.  Asynchronous on `stream`, nothing
+ * allocated. */
+f3s_status f3s_layer_norm_fwd(const void* X, int64_t x_stride, const void* W, const void* B, void* Y,
+                              float* stats, int64_t n, int64_t width, float eps, int32_t dtype,
+                              int32_t weight_dtype, void* stream);
+/* Its gradient: dX[n][width] in `dtype`, dW and dB [width] in weight_dtype
+ * (contiguous; NULL: not wanted) from dY, whose rows are dy_stride values apart, and
+ * the forward call's stats.  Deterministic.  workspace (for dW or dB):
+ * f3s_layer_norm_workspace bytes, 16-byte aligned, this call's alone until it is
+ * done; calls may overlap and be captured. */
+f3s_status f3s_layer_norm_workspace(int64_t n, int64_t width, int32_t dtype, int64_t* bytes);
+f3s_status f3s_layer_norm_bwd(const void* X, int64_t x_stride, const void* W, const float* stats,
+                              const void* dY, int64_t dy_stride, void* dX, void* dW, void* dB,
+                              int64_t n, int64_t width, int32_t dtype, int32_t weight_dtype,
+                              void* workspace, int64_t workspace_bytes, void* stream);
 
 /* The reversed edges of a CSR (no reference counterpart): entry (i, j) becomes
  * (j, i).  d_out_row_ptr holds n + 1 entries, d_out_col_idx nnz.  The order of
