@@ -41,8 +41,7 @@
 #include <cmath>
 #include <cstddef>
 
-#include "attn_plan.hpp"
-#include "half_types.hpp"
+#include "edge_stream.hpp"
 
 namespace f3s {
 
@@ -56,28 +55,12 @@ constexpr int kHeadBytes = kHeadD * 2;
 constexpr int kRowHalves = kHeadD;
 __device__ __forceinline__ int swizzle(int row) { return ((row & 7) << 1) | ((row >> 3) & 1); }
 
-// The lane again, for the compiler a new value: what is derived from it is then made
-// where it is used and not held in registers through the chunk loop.
-__device__ __forceinline__ int anew(int lane)
-{
-    asm volatile("" : "+v"(lane));
-    return lane;
-}
-
 enum DiffPass : int { kDiffForward = 0, kDiffRows = 1, kDiffColumns = 2 };
 
-// Rows r of a tensor start `stride` bytes apart; a head's 256 bytes are
-// contiguous, heads adjacent.
-struct DiffRows {
-    const char* ptr;
-    uint64_t stride;
-    uint32_t bytes;   // narrow launches: end of the last row (loads past it read 0)
-};
-
 struct DiffParams {
-    DiffRows x1, x2;        // streamed: k and v; q and do on the reversed edges
-    DiffRows own1, own2;    // the window's own rows: q and do; k and v
-    DiffRows out1, out2;    // o; dq; dk and dv
+    EdgeRows x1, x2;        // streamed: k and v; q and do on the reversed edges
+    EdgeRows own1, own2;    // the window's own rows: q and do; k and v
+    EdgeRows out1, out2;    // o; dq; dk and dv
     const float* lam;       // [H]
     float* lse;             // [n][H][2], log2; forward: written (NULL: not)
     float* stats;           // [n][H][4]: lse_1, lse_2, D_1, D_2
@@ -195,7 +178,7 @@ static_assert(sizeof(DiffLds) >= sizeof(float) * kDiffPartial,
 
 template <typename T, bool WIDE>
 __device__ __forceinline__ typename Half<T>::v8 diff_load(__amdgpu_buffer_rsrc_t rs,
-                                                          const DiffRows& x, uint32_t at,
+                                                          const EdgeRows& x, uint32_t at,
                                                           uint32_t extra)
 {
     if constexpr (!WIDE) {
@@ -207,18 +190,6 @@ __device__ __forceinline__ typename Half<T>::v8 diff_load(__amdgpu_buffer_rsrc_t
             v = *reinterpret_cast<const typename Half<T>::v8*>(x.ptr + at * x.stride + extra);
         return v;
     }
-}
-
-typedef __attribute__((address_space(3))) char* LdsPtr;
-template <typename V>
-__device__ __forceinline__ V lds_read(uint32_t at)
-{
-    return *(__attribute__((address_space(3))) V*)(LdsPtr)(uintptr_t)at;
-}
-template <typename V>
-__device__ __forceinline__ void lds_write(uint32_t at, V v)
-{
-    *(__attribute__((address_space(3))) V*)(LdsPtr)(uintptr_t)at = v;
 }
 
 // Where a lane reads and writes in a stage (addresses in LDS).  A piece's place
@@ -334,29 +305,6 @@ __device__ __forceinline__ void replace_odd(const Places& p, uint32_t stage, uin
     wave_lds_order();
 }
 
-// Which of the lane's eight slots row r attends: all bits or none.
-typedef uint32_t Attends[8];
-__device__ __forceinline__ float where(uint32_t on, float x, float other)
-{
-    return __uint_as_float((__float_as_uint(x) & on) | (__float_as_uint(other) & ~on));
-}
-__device__ __forceinline__ float where(uint32_t on, float x)
-{
-    return __uint_as_float(__float_as_uint(x) & on);
-}
-
-// From a record's masks at `masks`, anew wherever they are used: two LDS reads,
-// where eight registers would be held.
-__device__ __forceinline__ void attends(uint32_t masks, int lane, Attends& on)
-{
-    const int l = anew(lane), r = l & 15, rbit = (r & 1) ? 16 + (r >> 1) : (r >> 1);
-    const uint32_t at = masks + 16 * (l >> 4);   // slots 4 g .. and 16 + 4 g ..
-    const u4 a = lds_read<u4>(at), b = lds_read<u4>(at + 64);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-        on[j] = (uint32_t)__builtin_amdgcn_sbfe((int)(j < 4 ? a[j & 3] : b[j & 3]), rbit, 1);
-}
-
 template <int N>
 __device__ __forceinline__ void edge_weights(float (&w)[N][8], const Attends& on)
 {
@@ -395,26 +343,6 @@ __device__ __forceinline__ void map_update(DiffState& st, int m, const f4 s0, co
     }
 }
 
-// Weights of a size of 1 at most, in binary16: with |w| <= 2 they stay below 2^15, and
-// their halves end at 2^-39.  (A node that a row hardly attends, or that only rows of
-// very many edges do, has weights of 2^-17 and less alone: unscaled, 2^-20 was off by
-// 2^-6 of itself.)
-// (In the rows' pass as an addend of the exponent: all its sums are divided by the
-// weights' own.  A row of 10^5 equal edges has weights of 2^-17, all rounded the same
-// way: dq, a difference of two sums of them, was off by 2^-8 of either.)
-template <typename T>
-constexpr float kLift = Half<T>::kRange ? 16384.f : 1.f;
-template <typename T>
-constexpr float kLiftLog2 = Half<T>::kRange ? 14.f : 0.f;
-// Such a weight's exponent.  A weight is at most 1, but for what a log-sum-exp of 24
-// bits leaves (logits past 2^24 come out as 2^2 and more): kept at 2 (rows, lifted) and
-// at 1 (columns), inside the type.  NaN stays.
-template <typename T>
-__device__ __forceinline__ float lifted(float x, float most)
-{
-    return Half<T>::kRange ? __builtin_elementwise_minimum(x, most) : x;
-}
-
 // Scales weights of unknown size into binary16: a power of two per row, st.x[m],
 // moved (and the sums that it scales with it) when a weight would come within a
 // factor of four of the type's end, to put that weight at 2^3 to 2^4.
@@ -444,7 +372,7 @@ __device__ __forceinline__ void range_update(DiffState& st, int m, float (&w)[8]
 // Rows of 128 values leave whole, through a stage: val(t) is the lane's part of
 // tile t, dims 16 t + 4 g .. + 3.
 template <typename T, typename F>
-__device__ __forceinline__ void store_rows(const DiffRows& out, _Float16* stage, int32_t w,
+__device__ __forceinline__ void store_rows(const EdgeRows& out, _Float16* stage, int32_t w,
                                            int32_t n, uint32_t head_off, int lane, F val)
 {
     typedef typename Half<T>::v8 v8;
@@ -465,12 +393,6 @@ __device__ __forceinline__ void store_rows(const DiffRows& out, _Float16* stage,
                                    16 * r) = x;
     }
     wave_lds_order();
-}
-
-__device__ __forceinline__ float over_groups(float x)
-{
-    x += __shfl_xor(x, 16, kWave);
-    return x + __shfl_xor(x, 32, kWave);
 }
 
 // A window's results from its sums.  `stage`: 2 x 16 rows.
@@ -548,18 +470,6 @@ struct Unit {
     bool there, end;
 };
 
-__device__ __forceinline__ float uniform(float x)
-{
-    return __uint_as_float(__builtin_amdgcn_readfirstlane((int)__float_as_uint(x)));
-}
-
-template <typename V>
-__device__ __forceinline__ V scalar_load(const V* at)
-{
-    typedef const __attribute__((address_space(4))) V* Constant;
-    return *(Constant)(uintptr_t)at;
-}
-
 // Large graphs' waves take unit after unit from a queue, their chunks one stream:
 // the records, own rows and first chunk of a unit are loaded while the one before
 // it is still being computed.  (A window has some 7 to 20 chunks; a wave of its
@@ -629,7 +539,7 @@ diff_kernel(const DiffParams p)
 
     // ---- the window's own rows, in operand order: dims 32 f + 8 g .. of row r
     // (rows past the last are not stored) ----
-    auto own_load = [&](const DiffRows& x, const Unit& u, v8 (&f)[4]) __attribute__((always_inline)) {
+    auto own_load = [&](const EdgeRows& x, const Unit& u, v8 (&f)[4]) __attribute__((always_inline)) {
         const int l = anew(lane);
         const int32_t row = min(max(u.w, 0) * 16 + (l & 15), n - 1);
         const char* src = x.ptr + row * x.stride + (uint32_t)u.h * kHeadBytes + 16 * (l >> 4);
@@ -1147,7 +1057,7 @@ static f3s_status launch_pass(DiffParams p, const f3s_plan* plan, int32_t dtype,
                 "differential attention: too many work items");
     // Offsets of 32 bits where every streamed tensor ends below kNoRow.
     const int64_t head = (int64_t)p.H * kHeadBytes;
-    auto end = [&](const DiffRows& x) { return (int64_t)(p.n - 1) * (int64_t)x.stride + head; };
+    auto end = [&](const EdgeRows& x) { return (int64_t)(p.n - 1) * (int64_t)x.stride + head; };
     const bool wide = end(p.x1) > (int64_t)kNoRow || end(p.x2) > (int64_t)kNoRow;
     if (!wide) {
         p.x1.bytes = (uint32_t)end(p.x1);
@@ -1171,8 +1081,6 @@ static f3s_status launch_pass(DiffParams p, const f3s_plan* plan, int32_t dtype,
     F3S_HIP(hipGetLastError());
     return F3S_OK;
 }
-
-static size_t round_up(size_t x) { return (x + 255) & ~(size_t)255; }
 
 static size_t partial_bytes(const f3s_plan* plan)
 {
@@ -1224,11 +1132,6 @@ static bool rows_ok(const void* ptr, int64_t stride, int32_t H)
 {
     return ptr && ((uintptr_t)ptr & 15) == 0 && stride % 8 == 0 && stride >= (int64_t)H * kHeadD &&
            stride < ((int64_t)1 << 30);
-}
-
-static DiffRows rows_of(const void* ptr, int64_t stride)
-{
-    return DiffRows{static_cast<const char*>(ptr), (uint64_t)stride * 2, 0};
 }
 
 }  // namespace f3s

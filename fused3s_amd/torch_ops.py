@@ -190,6 +190,7 @@ class TorchGraph:
         self._scheduled: Plan | None = None  # diff_attention's plan, where it is not self.plan
         self._reversed: Plan | None = None   # the reversed edges' (prepare_backward)
         self._workspace = {}
+        self._edge_workspaces = {}
 
     def attention(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                   scale: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -249,8 +250,8 @@ class TorchGraph:
         return out
 
     def prepare_backward(self) -> "TorchGraph":
-        """Builds what the gradient of diff_attention reads, a compiled plan of
-        the reversed edges; the first call that needs it does so otherwise.
+        """Builds what the gradients of diff_attention and edge_attention read, a
+        compiled plan of the reversed edges; the first call that needs it does so otherwise.
         Waits for the GPU, so before a capture.  (The leaves of a captured step
         must not belong to an eager step that is still alive, as with torch's
         own operators: capture with detached ones.  A captured call reads this
@@ -284,7 +285,7 @@ class TorchGraph:
         return plan
 
     def _diff_plan(self) -> Plan:
-        """The plan of diff_attention: self.plan, where that follows the
+        """The plan of diff_attention and edge_attention: self.plan, where that follows the
         library's sequence or the windows run on teams; else one made for it by the
         first call (_compiled).  (Waits for the GPU then, so before a capture.)"""
         if self._scheduled is None:
@@ -309,17 +310,23 @@ class TorchGraph:
             size = self._workspace[backward] = need.value
         return torch.empty(size, dtype=torch.uint8, device=self._torch_device) if size else None
 
-    def _check_diff(self, lam, tensors) -> None:
-        """Raises for tensors (by name) that diff_attention does not take."""
+    def _check_exact(self, who: str) -> None:
         if not self.masked:
-            raise ValueError("differential attention is edge-exact: it needs masked=True")
+            raise ValueError(f"{who} is edge-exact: it needs masked=True")
         if _current_device() != self.device:
             raise ValueError(f"the graph is on device {self.device}, which is not the current one")
+
+    def _check_diff(self, lam, tensors) -> None:
+        """Raises for tensors (by name) that diff_attention does not take."""
+        self._check_exact("differential attention")
         device = self._torch_device
         if lam.dtype is not torch.float32 or lam.device != device or lam.shape != (self.heads,):
             raise ValueError(f"lam must be a float32 tensor of {self.heads} weights on the graph's "
                              "device")
-        dtype = None
+        self._check_halves(tensors)
+
+    def _check_halves(self, tensors) -> None:
+        device, dtype = self._torch_device, None
         for name, t, *shapes in tensors:
             if t.dtype not in _DTYPES or t.device != device or (dtype or t.dtype) is not t.dtype:
                 raise ValueError(f"{name} must be a float16 or bfloat16 tensor on the graph's "
@@ -362,17 +369,96 @@ class TorchGraph:
             return _DiffAttention.apply(self, float(scale), lam, qkv)
         return _diff_forward(self, float(scale), lam, *_thirds(qkv, self))
 
+    def _check_edge(self, cap, positions, slopes, tensors):
+        """Raises for what edge_attention does not take (tensors by name); its bias as
+        (cap, dims, positions, slopes)."""
+        self._check_exact("edge attention")
+        self._check_halves(tensors)
+        cap = 0.0 if cap is None else float(cap)
+        if not (cap == 0.0 or 1e-30 < cap < 1e30):
+            raise ValueError(f"cap must be positive (None or 0: none), got {cap}")
+        if (positions is None) != (slopes is None):
+            raise ValueError("positions and slopes come together")
+        if positions is None:
+            return cap, 0, None, None
+        device = self._torch_device
+        if (positions.dtype is not torch.float32 or positions.device != device
+                or positions.dim() not in (1, 2) or positions.shape[0] != self.n
+                or positions.dim() == 2 and not 1 <= positions.shape[1] <= 3):
+            raise ValueError(f"positions must be a float32 tensor of {self.n} nodes' 1 to 3 "
+                             "coordinates on the graph's device")
+        if positions.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("edge attention has no gradient of positions: detach them")
+        if (slopes.dtype is not torch.float32 or slopes.device != device
+                or slopes.shape != (self.heads,)):
+            raise ValueError(f"slopes must be a float32 tensor of {self.heads} weights on the "
+                             "graph's device")
+        return (cap, 1 if positions.dim() == 1 else positions.shape[1], positions.contiguous(),
+                slopes)
+
+    def edge_attention(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float = 1.0,
+                       cap: float | None = None, positions: torch.Tensor | None = None,
+                       slopes: torch.Tensor | None = None) -> torch.Tensor:
+        """Softmax attention over each node's neighbours j, trainable: the weights of v
+        are the softmax of
+            cap * tanh(scale * q.k / cap) - slopes[h] * |positions[i] - positions[j]|
+        (cap None: scale * q.k itself; positions None: no distances).
+        q, k, v: float16 or bfloat16 CUDA tensors [n, H, 64], each row's heads
+        contiguous, rows at any distance of a multiple of 8 values (a slice of a
+        projection's output is taken as it is; other layouts are copied); positions:
+        float32 [n] (times, say) or [n, 1 to 3] (points); slopes: float32 [H].
+        Returns [n, H, 64] in q's type: sums in float32, rounded once; nodes without
+        edges get 0.  Differentiable in q, k, v and slopes (once); tracing, functorch's
+        transforms and forward-mode differentiation are refused.  A graph serves any
+        number of calls at once."""
+        _refuse_unseen("edge_attention", q, k, v, positions, slopes)
+        shape, flat = (self.n, self.heads, HEAD_DIM), (self.n, self.heads * HEAD_DIM)
+        bias = self._check_edge(cap, positions, slopes,
+                                (("q", q, shape, flat), ("k", k, shape, flat), ("v", v, shape, flat)))
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                        or slopes is not None and slopes.requires_grad):
+            self.prepare_backward()
+            return _EdgeAttention.apply(self, float(scale), *bias, q, k, v)
+        return _edge_forward(self, float(scale), *bias, *(_rows(t, self, HEAD_DIM)
+                                                          for t in (q, k, v)))
+
+    def edge_attention_packed(self, qkv: torch.Tensor, scale: float = 1.0,
+                              cap: float | None = None, positions: torch.Tensor | None = None,
+                              slopes: torch.Tensor | None = None) -> torch.Tensor:
+        """edge_attention() on the [n, 3 * H * 64] output of one projection (q, k and v
+        side by side in each row), whose gradient is then one tensor too, written in
+        place of its thirds."""
+        _refuse_unseen("edge_attention_packed", qkv, positions, slopes)
+        bias = self._check_edge(cap, positions, slopes,
+                                (("qkv", qkv, (self.n, 3 * self.heads * HEAD_DIM)),))
+        if torch.is_grad_enabled() and (qkv.requires_grad
+                                        or slopes is not None and slopes.requires_grad):
+            self.prepare_backward()
+            return _EdgeAttention.apply(self, float(scale), *bias, qkv)
+        return _edge_forward(self, float(scale), *bias, *_thirds(qkv, self, HEAD_DIM))
+
+    def _edge_workspace(self, backward: bool) -> torch.Tensor:
+        size = self._edge_workspaces.get(backward)
+        if size is None:
+            need = C.c_int64()
+            check(_lib.hip().f3s_edge_attention_workspace(
+                self._diff_plan().handle, self._reversed.handle if backward else None,
+                C.byref(need)),
+                "f3s_edge_attention_workspace")
+            size = self._edge_workspaces[backward] = need.value
+        return torch.empty(size, dtype=torch.uint8, device=self._torch_device) if size else None
+
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}   # F3S_F16, F3S_BF16
 
 
-def _rows(t: torch.Tensor, graph: TorchGraph) -> torch.Tensor:
+def _rows(t: torch.Tensor, graph: TorchGraph, per_head: int = 2 * HEAD_DIM) -> torch.Tensor:
     """[n, width] with each row contiguous, 16-byte aligned: t itself where its
     layout is that already."""
-    n, width = graph.n, graph.heads * 2 * HEAD_DIM
+    n, width = graph.n, graph.heads * per_head
     if t.is_contiguous() and t.stride(0) == width and t.data_ptr() % 16 == 0:
         return t.view(n, width) if t.dim() == 3 else t
-    if t.dim() == 3 and (t.stride(2) != 1 or t.stride(1) != 2 * HEAD_DIM and graph.heads > 1):
+    if t.dim() == 3 and (t.stride(2) != 1 or t.stride(1) != per_head and graph.heads > 1):
         t = t.contiguous()
     if t.dim() == 3:
         t = t.as_strided((n, width), (t.stride(0), 1))
@@ -382,8 +468,8 @@ def _rows(t: torch.Tensor, graph: TorchGraph) -> torch.Tensor:
     return t
 
 
-def _thirds(qkv: torch.Tensor, graph: TorchGraph):
-    width = graph.heads * 2 * HEAD_DIM
+def _thirds(qkv: torch.Tensor, graph: TorchGraph, per_head: int = 2 * HEAD_DIM):
+    width = graph.heads * per_head
     if qkv.stride(-1) != 1 or qkv.data_ptr() % 16 or (
             graph.n > 1 and (qkv.stride(0) % 8 or qkv.stride(0) < 3 * width)):
         qkv = qkv.clone(memory_format=torch.contiguous_format)
@@ -452,6 +538,70 @@ class _DiffAttention(torch.autograd.Function):
                 ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
                 _raw_stream(graph.device)), "f3s_diff_attention_bwd")
         return None, None, dlam, *grads
+
+
+def _edge_forward(graph: TorchGraph, scale: float, cap, dims, positions, slopes, q, k, v,
+                  lse=None) -> torch.Tensor:
+    n, H = graph.n, graph.heads
+    out = q.new_empty((n, H, HEAD_DIM))
+    if n:
+        plan = graph._diff_plan().handle
+        ws = graph._edge_workspace(False)
+        if dims and not slopes.is_contiguous():
+            slopes = slopes.contiguous()
+        check(_lib.hip().f3s_edge_attention_fwd(
+            plan, q.data_ptr(), _stride(q, n), k.data_ptr(), _stride(k, n), v.data_ptr(),
+            _stride(v, n), out.data_ptr(), H * HEAD_DIM, None if lse is None else lse.data_ptr(),
+            _DTYPES[q.dtype], n, H, scale, cap, positions.data_ptr() if dims else None, dims,
+            slopes.data_ptr() if dims else None, None if ws is None else ws.data_ptr(),
+            0 if ws is None else ws.numel(), _raw_stream(graph.device)), "f3s_edge_attention_fwd")
+    return out
+
+
+class _EdgeAttention(torch.autograd.Function):
+    """edge_attention and its gradient; one packed tensor or three."""
+
+    @staticmethod
+    def forward(ctx, graph, scale, cap, dims, positions, slopes, *tensors):
+        rows = (_thirds(tensors[0], graph, HEAD_DIM) if len(tensors) == 1
+                else [_rows(t, graph, HEAD_DIM) for t in tensors])
+        lse = torch.empty((graph.n, graph.heads), dtype=torch.float32, device=tensors[0].device)
+        if dims:
+            slopes = slopes.contiguous()
+        out = _edge_forward(graph, scale, cap, dims, positions, slopes, *rows, lse=lse)
+        ctx.graph, ctx.scale, ctx.cap, ctx.dims = graph, scale, cap, dims
+        ctx.shapes = [t.shape for t in tensors]
+        ctx.save_for_backward(positions, slopes, lse, *tensors)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        graph, n, H, dims = ctx.graph, ctx.graph.n, ctx.graph.heads, ctx.dims
+        width = H * HEAD_DIM
+        positions, slopes, lse, *tensors = ctx.saved_tensors
+        packed = len(tensors) == 1
+        q, k, v = (_thirds(tensors[0], graph, HEAD_DIM) if packed
+                   else (_rows(t, graph, HEAD_DIM) for t in tensors))
+        grads = [q.new_empty(shape) for shape in ctx.shapes]
+        if packed:
+            dq, dk, dv = (grads[0][:, i * width:(i + 1) * width] for i in range(3))
+        else:
+            dq, dk, dv = (t.view(n, width) for t in grads)
+        dslopes = torch.empty_like(slopes) if dims else None
+        do = _rows(grad, graph, HEAD_DIM)
+        with _on(graph.device):
+            ws = graph._edge_workspace(True)
+            check(_lib.hip().f3s_edge_attention_bwd(
+                graph._diff_plan().handle, graph._reversed.handle, q.data_ptr(), _stride(q, n),
+                k.data_ptr(), _stride(k, n), v.data_ptr(), _stride(v, n), lse.data_ptr(),
+                do.data_ptr(), _stride(do, n), dq.data_ptr(), _stride(dq, n), dk.data_ptr(),
+                _stride(dk, n), dv.data_ptr(), _stride(dv, n),
+                dslopes.data_ptr() if dims else None, _DTYPES[q.dtype], n, H, ctx.scale, ctx.cap,
+                positions.data_ptr() if dims else None, dims, slopes.data_ptr() if dims else None,
+                ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
+                _raw_stream(graph.device)), "f3s_edge_attention_bwd")
+        return None, None, None, None, None, dslopes, *grads
 
 
 # F3S_ACT_NONE ..

@@ -418,6 +418,45 @@ f3s_status f3s_diff_attention_bwd(const f3s_plan* plan, const f3s_plan* reversed
                                   int32_t dtype, int32_t n, int32_t H, float scale, void* workspace,
                                   int64_t workspace_bytes, void* stream);
 
+/* Softmax attention over the edges of a compiled plan with capped scores and a bias
+ * by distance (no reference counterpart), 64 dims per head:
+ *   x = scale Q[i].K[j]
+ *   s = cap tanh(x / cap) - slopes[h] |positions[i] - positions[j]|
+ *   O[i] = sum_j softmax_j(s) V[j]
+ * over the edges (i, j) (masked semantics); rows without edges get 0.  cap 0: s = x
+ * there (else 1e-30 to 1e30); dims 0: no positions.  positions float32 [n][dims], dims 1 to 3, distances
+ * Euclidean in float32; slopes float32 [H].  H is the plan's; a head of a row is 64 contiguous values of `dtype`
+ * (F3S_F16 or F3S_BF16), heads adjacent, rows `*_stride` values apart (a multiple of
+ * 8, at least H * 64), pointers 16-byte aligned.  lse, where not NULL, receives
+ * [n][H] float32 for the gradient.  Sums and softmax statistics are float32, O is
+ * rounded once.  An infinite or NaN value reaches the rows with an edge to its node
+ * only.  A row whose scores are all -inf is 0, as one without edges.
+ * Deterministic.
+ * workspace: f3s_edge_attention_workspace bytes (reversed NULL), 16-byte aligned,
+ * this call's alone until it is done; nothing else is allocated or kept, so calls
+ * may overlap and be captured.  Asynchronous on `stream`. */
+f3s_status f3s_edge_attention_workspace(const f3s_plan* plan, const f3s_plan* reversed,
+                                        int64_t* bytes);
+f3s_status f3s_edge_attention_fwd(const f3s_plan* plan, const uint16_t* Q, int64_t q_stride,
+                                  const uint16_t* K, int64_t k_stride, const uint16_t* V,
+                                  int64_t v_stride, uint16_t* O, int64_t o_stride, float* lse,
+                                  int32_t dtype, int32_t n, int32_t H, float scale, float cap,
+                                  const float* positions, int32_t dims, const float* slopes,
+                                  void* workspace, int64_t workspace_bytes, void* stream);
+/* Its gradient: dQ, dK, dV in `dtype`, dslopes float32 [H] (dims > 0), from dO and
+ * the forward call's lse.  `reversed` is a plan of the reversed edges
+ * (f3s_reverse_csr, converted) of the same n and H, compiled.  No atomics:
+ * deterministic. */
+f3s_status f3s_edge_attention_bwd(const f3s_plan* plan, const f3s_plan* reversed, const uint16_t* Q,
+                                  int64_t q_stride, const uint16_t* K, int64_t k_stride,
+                                  const uint16_t* V, int64_t v_stride, const float* lse,
+                                  const uint16_t* dO, int64_t do_stride, uint16_t* dQ,
+                                  int64_t dq_stride, uint16_t* dK, int64_t dk_stride, uint16_t* dV,
+                                  int64_t dv_stride, float* dslopes, int32_t dtype, int32_t n,
+                                  int32_t H, float scale, float cap, const float* positions,
+                                  int32_t dims, const float* slopes, void* workspace,
+                                  int64_t workspace_bytes, void* stream);
+
 /* Measurement only (no reference counterpart): the device's random-gather
  * ceiling for the fused pass's access pattern.  For each of `count` columns
  * (a multiple of 32) it loads the 128-byte row at byte offset
