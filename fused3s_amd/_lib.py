@@ -81,6 +81,11 @@ HIP_API = {
     "f3s_layer_norm_workspace": (c_i32, [c_i64, c_i64, c_i32, P_i64]),
     "f3s_layer_norm_bwd": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64,
                                    c_i64, c_i32, c_i32, c_vp, c_i64, c_vp]),
+    "f3s_cross_entropy_workspace": (c_i32, [c_i64, c_i64, c_i64, c_i32, P_i64]),
+    "f3s_cross_entropy_fwd": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64,
+                                      c_i64, c_i32, c_i32, c_vp, c_i64, c_vp]),
+    "f3s_cross_entropy_bwd": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp,
+                                      c_vp, c_i64, c_i64, c_i64, c_i32, c_i32, c_vp, c_i64, c_vp]),
     "f3s_reverse_csr": (c_i32, [c_vp, c_vp, c_i32, c_i64, c_vp, c_vp, c_vp]),
     "f3s_diff_attention_workspace": (c_i32, [c_vp, c_vp, P_i64]),
     "f3s_diff_attention_fwd": (c_i32, [c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp,

@@ -26,7 +26,7 @@ CSRC = PKG / "csrc"
 OBJ = PKG / "_build"
 HIP_SOURCES = ["runtime.hip", "convert.hip", "attention.hip", "bsf_util.hip", "naive.hip",
                "probe.hip", "linear.hip", "diff_attention.hip", "gemm.hip",
-               "norm.hip", "edge_attention.hip"]
+               "norm.hip", "edge_attention.hip", "cross_entropy.hip"]
 HOST_SOURCES = ["host/gen.cpp", "host/graph.cpp", "host/graph_file.cpp"]
 ARCH = "gfx950"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

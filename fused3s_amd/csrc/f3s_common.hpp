@@ -45,6 +45,7 @@ hipError_t warm_diff(hipStream_t s);
 hipError_t warm_gemm(hipStream_t s);
 hipError_t warm_norm(hipStream_t s);
 hipError_t warm_edge(hipStream_t s);
+hipError_t warm_loss(hipStream_t s);
 // Looks up the current device's address of f3s_attention_fwd_noalloc's
 // fixed scratch (attention.hip), so its first call does not.
 f3s_status noalloc_setup();

@@ -379,6 +379,7 @@ f3s_status f3s_init(void)
     F3S_HIP(warm_gemm(nullptr));
     F3S_HIP(warm_norm(nullptr));
     F3S_HIP(warm_edge(nullptr));
+    F3S_HIP(warm_loss(nullptr));
     F3S_HIP(hipDeviceSynchronize());
     F3S_TRY(noalloc_setup());
     return F3S_OK;

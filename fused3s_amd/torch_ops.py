@@ -823,6 +823,118 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
     return y if x.dim() == 2 else y.view(x.shape)
 
 
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}   # F3S_LOSS_NONE ..
+
+
+@functools.lru_cache(maxsize=256)
+def _loss_bytes(n, K, V, backward) -> int:
+    need = C.c_int64()
+    check(_lib.hip().f3s_cross_entropy_workspace(n, K, V, backward, C.byref(need)),
+          "f3s_cross_entropy_workspace")
+    return need.value
+
+
+def _loss_workspace(n, K, V, backward, device):
+    size = _loss_bytes(n, K, V, backward)
+    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+
+
+def _loss_forward(x, w, b, target, ignore, reduction, lse=None):
+    (n, K), V = x.shape, w.shape[0]
+    loss = torch.empty(() if reduction else (n,), dtype=torch.float32, device=x.device)
+    ws = _loss_workspace(n, K, V, 0, x.device)
+    check(_lib.hip().f3s_cross_entropy_fwd(
+        x.data_ptr(), _stride(x, n), w.data_ptr(), b.data_ptr() if b is not None else None,
+        target.data_ptr(), ignore, loss.data_ptr(), lse.data_ptr() if lse is not None else None,
+        n, K, V, reduction, _DTYPES[x.dtype], ws.data_ptr() if ws is not None else None,
+        ws.numel() if ws is not None else 0, _raw_stream(x.device.index)), "f3s_cross_entropy_fwd")
+    return loss
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    """linear_cross_entropy()'s matrices and their gradients."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, target, ignore, reduction):
+        lse = torch.empty(x.shape[0] + 1, dtype=torch.float32, device=x.device)
+        ctx.ignore, ctx.reduction = ignore, reduction
+        ctx.save_for_backward(x, w, b, target, lse)
+        return _loss_forward(x, w, b, target, ignore, reduction, lse)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, w, b, target, lse = ctx.saved_tensors
+        (n, K), V = x.shape, w.shape[0]
+        needs = ctx.needs_input_grad
+        empty = lambda wanted, *shape: x.new_empty(shape) if wanted else None
+        dx, dw, db = empty(needs[0], n, K), empty(needs[1], V, K), empty(needs[2], V)
+        if any(needs[:3]):
+            grad = grad.contiguous()
+            with _on(x.device.index):
+                ws = _loss_workspace(n, K, V, 1, x.device)
+                check(_lib.hip().f3s_cross_entropy_bwd(
+                    x.data_ptr(), _stride(x, n), w.data_ptr(),
+                    b.data_ptr() if b is not None else None, target.data_ptr(), ctx.ignore,
+                    lse.data_ptr(), grad.data_ptr(),
+                    *(t.data_ptr() if t is not None else None for t in (dx, dw, db)), n, K, V,
+                    ctx.reduction, _DTYPES[x.dtype], ws.data_ptr() if ws is not None else None,
+                    ws.numel() if ws is not None else 0, _raw_stream(x.device.index)),
+                    "f3s_cross_entropy_bwd")
+        return dx, dw, db, None, None, None
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor,
+                         bias: torch.Tensor | None = None, ignore_index: int = -100,
+                         reduction: str = "mean") -> torch.Tensor:
+    """The cross entropy of the logits x @ weight.T + bias with the classes `target`,
+    without keeping the logits: x [..., K], weight [V, K], bias [V], all float16 or all
+    bfloat16 on one GPU, target [...] int64.  Rows of ignore_index have no loss and no
+    gradient; a target that is no class has NaN as both.  reduction "mean" (over the
+    rows that are not ignored), "sum" or "none"; float32.  Logits are not rounded, sums
+    are float32.  Differentiable (once) in x, weight and bias; for the backward pass the
+    logits are computed again, some classes at a time, and their gradient (up to what
+    multiplies all of it: the mean's divisor, a loss scale) is rounded to the type before
+    the gradients of x and weight are made of it, so these two are rounded twice.
+    Tracing, functorch's transforms and forward-mode differentiation are refused."""
+    _refuse_unseen("linear_cross_entropy", x, weight, target, bias)
+    how = _REDUCTIONS.get(reduction)
+    if how is None:
+        raise ValueError(f"reduction must be one of {list(_REDUCTIONS)}, got {reduction!r}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x [..., K] and weight [V, K] do not fit: {tuple(x.shape)}, "
+                         f"{tuple(weight.shape)}")
+    V, K = weight.shape
+    if V == 0 or K == 0:
+        raise ValueError("weight must not be empty")
+    if bias is not None and bias.shape != (V,):
+        raise ValueError(f"bias must have shape {(V,)}, got {tuple(bias.shape)}")
+    if target.shape != x.shape[:-1]:
+        raise ValueError(f"target must have shape {tuple(x.shape[:-1])}, got {tuple(target.shape)}")
+    dtype, device = x.dtype, x.device
+    if (dtype not in _DTYPES or not x.is_cuda
+            or weight.dtype is not dtype or weight.device != device
+            or bias is not None and (bias.dtype is not dtype or bias.device != device)):
+        raise ValueError("x, weight and bias must be float16 or bfloat16 tensors on a GPU, all of "
+                         "one type and on one device")
+    if target.dtype is not torch.int64 or target.device != device:
+        raise ValueError("target must be an int64 tensor on x's device")
+    if device.index != _current_device():
+        with torch.cuda.device(device):
+            return linear_cross_entropy(x, weight, target, bias, ignore_index, reduction)
+    x2 = _matrix(x if x.dim() == 2 else x.reshape(-1, K))
+    t = target.reshape(-1)
+    t = t if t.is_contiguous() else t.contiguous()
+    w = weight if weight.is_contiguous() else weight.contiguous()
+    b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
+                                    or bias is not None and bias.requires_grad):
+        loss = _LinearCrossEntropy.apply(x2, w, b, t, int(ignore_index), how)
+    else:
+        loss = _loss_forward(x2, w, b, t, int(ignore_index), how)
+    return loss if how else loss.view(target.shape)
+
+
 _LINEAR_FORWARD, _LINEAR = torch.nn.Linear.forward, torch.nn.functional.linear
 
 

@@ -371,6 +371,41 @@ f3s_status f3s_layer_norm_bwd(const void* X, int64_t x_stride, const void* W, co
                               int64_t n, int64_t width, int32_t dtype, int32_t weight_dtype,
                               void* workspace, int64_t workspace_bytes, void* stream);
 
+/* The cross entropy of a linear classifier over V classes without its logits (no
+ * reference counterpart):
+ *   Z = X[n][K] W[V][K]^T + bias[V],  loss_i = log sum_c exp Z_ic - Z_i,target[i]
+ * X, W and bias (NULL: none) in `dtype` (F3S_F16 or F3S_BF16), sums in float32, Z is
+ * not rounded.  Rows of X are x_stride values apart, W is contiguous; no alignment is
+ * needed; rows of a multiple of 16 bytes at 16-byte addresses are the fast ones.
+ * target int64 [n]: rows of ignore_index have no loss and no gradient, a target that
+ * is no class has NaN as both.  loss float32: [n] for F3S_LOSS_NONE, else [1]
+ * (F3S_LOSS_MEAN: over the rows that are not ignored; NaN where all are).  lse, where
+ * not NULL, receives n + 1 float32 for the gradient.  K < 2^22, V < 2^30, n < 2^31.
+ * workspace: f3s_cross_entropy_workspace bytes, 16-byte aligned, this call's alone
+ * until it is done; nothing is allocated, calls may overlap and be captured.
+ * Deterministic.  Asynchronous on `stream`. */
+#define F3S_LOSS_NONE 0
+#define F3S_LOSS_MEAN 1
+#define F3S_LOSS_SUM 2
+f3s_status f3s_cross_entropy_workspace(int64_t n, int64_t K, int64_t V, int32_t backward_pass,
+                                       int64_t* bytes);
+f3s_status f3s_cross_entropy_fwd(const uint16_t* X, int64_t x_stride, const uint16_t* W,
+                                 const uint16_t* bias, const int64_t* target, int64_t ignore_index,
+                                 float* loss, float* lse, int64_t n, int64_t K, int64_t V,
+                                 int32_t reduction, int32_t dtype, void* workspace,
+                                 int64_t workspace_bytes, void* stream);
+/* Its gradient: dX[n][K], dW[V][K], db[V] (contiguous; NULL: not wanted) from dloss,
+ * float32 like loss, and the forward call's lse.  Z is computed again, in pieces of the
+ * classes.  dZ, up to what multiplies all of it, is rounded to `dtype` before dX = dZ W
+ * and dW = dZ^T X are made of it, so these two carry its rounding and their own; db is
+ * summed before that. */
+f3s_status f3s_cross_entropy_bwd(const uint16_t* X, int64_t x_stride, const uint16_t* W,
+                                 const uint16_t* bias, const int64_t* target, int64_t ignore_index,
+                                 const float* lse, const float* dloss, uint16_t* dX, uint16_t* dW,
+                                 uint16_t* db, int64_t n, int64_t K, int64_t V, int32_t reduction,
+                                 int32_t dtype, void* workspace, int64_t workspace_bytes,
+                                 void* stream);
+
 /* The reversed edges of a CSR (no reference counterpart): entry (i, j) becomes
  * (j, i).  d_out_row_ptr holds n + 1 entries, d_out_col_idx nnz.  The order of
  * the entries of a row is not defined (the converter's output does not depend on
