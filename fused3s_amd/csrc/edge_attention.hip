@@ -517,7 +517,7 @@ __device__ void slow_window(const EdgeParams& p, int32_t w, int h, int nitems, F
 // TEAM: a window's four items are its workgroup's waves (small graphs); else a wave
 // takes an item, a window or a segment of one.
 template <typename T, int PASS, bool WIDE, bool TEAM>
-__global__ void __launch_bounds__(kWave * kEdgeWaves) __attribute__((amdgpu_waves_per_eu(4)))
+__global__ void __launch_bounds__(kWave * kEdgeWaves) __attribute__((amdgpu_waves_per_eu(3)))
 edge_kernel(const EdgeParams p)
 {
     typedef typename Half<T>::v8 v8;
