@@ -94,7 +94,7 @@ HIP_API = {
     "f3s_diff_attention_bwd": (c_i32, [c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp,
                                        c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64,
                                        c_vp, c_i32, c_i32, c_i32, c_f32, c_vp, c_i64, c_vp]),
-    "f3s_edge_attention_workspace": (c_i32, [c_vp, c_vp, P_i64]),
+    "f3s_edge_attention_workspace": (c_i32, [c_vp, c_vp, c_i32, P_i64]),
     "f3s_edge_attention_fwd": (c_i32, [c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64,
                                        c_vp, c_i32, c_i32, c_i32, c_f32, c_f32, c_vp, c_i32, c_vp,
                                        c_vp, c_i64, c_vp]),

@@ -27,7 +27,7 @@
 // A value that is infinite or NaN reaches, through the matrix cores, rows of its
 // window that have no edge to it (0 x inf).  So a window whose sums are not finite is
 // done again, edge by edge without them (slow_row): in the same launch where teams
-// share windows, else in one of its own, which finds nothing as a rule.
+// share windows, else in the one that joins segments, which finds none as a rule.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -50,17 +50,19 @@ struct EdgeParams {
     const float* slopes;    // [H] (dims > 0)
     const float* positions; // [n][dims]
     float* lse;             // [n][H], log2; forward: written (NULL: not)
-    float* stats;           // [n][H][2]: lse, D
-    float* slope_parts;     // [H][W]
+    float* stats;           // [n][H][stat_words]: lse, D and the position
+    float* slope_parts;     // [H][slope_windows]
+    float* dslopes;         // [H]
+    int32_t slope_windows;  // of the rows' pass
     const Item* items;
     const int32_t* chunk_base;
     const uint32_t* columns;
     const SplitInfo* splits;
     float* partials;
-    uint32_t* odd;          // [items][H], then [splits][H]: sums that are not finite
+    uint32_t* odd;          // [items][H]: sums that are not finite
     int32_t* slot_item;     // [slots]
     int64_t num_items, num_split;
-    int32_t W, n, H, dims;
+    int32_t W, n, H, dims, stat_words;
     int32_t xcd_contiguous, team;
     // the lists' references: node indices, or node * H * 128 (below kNoRow);
     // node = ((ref >> shift) * magic) >> 31, magic 2^31 or ceil(2^31 / H), which is
@@ -70,6 +72,10 @@ struct EdgeParams {
     float cap;              // 0: none
     float cap_in, cap_log2; // scale / cap; cap log2(e)
 };
+
+// What a node and head have beside their rows, for the columns' pass: one line for lse,
+// D and the position (2, 4 or 8 words), where a position of its own would be another.
+static inline int32_t stat_words(int32_t dims) { return dims == 0 ? 2 : dims <= 2 ? 4 : 8; }
 
 // A wave's sums, tiles of 16 dims, lane (g, r) holding dims 16 t + 4 g + v of row r in
 // tile t (v: the element), and its share of row r's sums of weights.
@@ -170,6 +176,12 @@ struct EdgePlaces {
     uint32_t column;  // what lane r of group g hands the transposing read of tile 0
     uint32_t write;   // piece lane % 8 of row lane / 8
 };
+// (the addresses of all pieces come from these by exclusive or with constants, made
+// where they are used: held in registers, they would be some thirty)
+__device__ __forceinline__ void held(EdgePlaces& p)
+{
+    asm volatile("" : "+v"(p.row), "+v"(p.column), "+v"(p.write));
+}
 __device__ __forceinline__ EdgePlaces edge_places(const _Float16* stage, int lane)
 {
     const int g = lane >> 4, r = lane & 15, i = r >> 2, c = r & 3;
@@ -229,39 +241,68 @@ __device__ __forceinline__ void edge_mix(const EdgePlaces& p, uint32_t stage,
 
 // tanh, to 3e-7 of itself: by its series up to 0.3 (the next term is 6e-8 of it
 // there), else from one exponential, whose 1e-7 are 4e-7 of 0.29.
-__device__ __forceinline__ float edge_tanh(float x)
+constexpr float kNear = 0.3f;
+__device__ __forceinline__ float tanh_near(float x)
 {
-    const float far = __builtin_fmaf(
-        -2.f, __builtin_amdgcn_rcpf(1.f + fast_exp2(2.f * kLog2e * x)), 1.f);
     const float t = x * x;
     float s = __builtin_fmaf(t, 62.f / 2835.f, -17.f / 315.f);
     s = __builtin_fmaf(s, t, 2.f / 15.f);
     s = __builtin_fmaf(s, t, -1.f / 3.f);
-    const float near = __builtin_fmaf(x * t, s, x);
-    return __builtin_fabsf(x) < 0.3f ? near : far;
+    return __builtin_fmaf(x * t, s, x);
+}
+__device__ __forceinline__ float tanh_far(float x)
+{
+    return __builtin_fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + fast_exp2(2.f * kLog2e * x)), 1.f);
 }
 
-// A score in log2 units from the product of its rows, and c = 1 - tanh^2.
-__device__ __forceinline__ float edge_score(const EdgeParams& p, float dot, float& c)
+// Scores in log2 units from the products of their rows, and c = 1 - tanh^2.  (Scores
+// are small beside their cap as a rule: the exponential only where one of the wave's
+// is not.)
+template <int N>
+__device__ __forceinline__ void edge_scores(const EdgeParams& p, float (&s)[N], float (&c)[N])
 {
     if (p.cap == 0.f) {
-        c = 1.f;
-        return dot * p.scale_log2;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            c[j] = 1.f;
+            s[j] *= p.scale_log2;
+        }
+        return;
     }
-    const float t = edge_tanh(dot * p.cap_in);
-    c = __builtin_fmaf(-t, t, 1.f);
-    return t * p.cap_log2;
+    float most = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        s[j] *= p.cap_in;
+        most = __builtin_fmaxf(most, __builtin_fabsf(s[j]));
+    }
+    if (__ballot(!(most < kNear))) {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            s[j] = __builtin_fabsf(s[j]) < kNear ? tanh_near(s[j]) : tanh_far(s[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) s[j] = tanh_near(s[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        c[j] = __builtin_fmaf(-s[j], s[j], 1.f);
+        s[j] *= p.cap_log2;
+    }
 }
 
 struct Position {
     float x, y, z;
 };
-__device__ __forceinline__ float distance(const Position& a, float x, float y, float z, int dims)
+// The square of a distance, and the distance by a power of two of its largest
+// coordinate, so that no square leaves the type.
+__device__ __forceinline__ float squared(const Position& a, float x, float y, float z)
 {
-    float dx = a.x - x;
-    if (dims == 1) return __builtin_fabsf(dx);
-    // (by a power of two of the largest, so that no square leaves the type)
-    float dy = a.y - y, dz = a.z - z;
+    const float dx = a.x - x, dy = a.y - y, dz = a.z - z;
+    return __builtin_fmaf(dz, dz, __builtin_fmaf(dy, dy, dx * dx));
+}
+__device__ __forceinline__ float distance(const Position& a, float x, float y, float z)
+{
+    float dx = a.x - x, dy = a.y - y, dz = a.z - z;
     const int e = __builtin_amdgcn_frexp_expf(
         __builtin_fmaxf(__builtin_fmaxf(__builtin_fabsf(dx), __builtin_fabsf(dy)), __builtin_fabsf(dz)));
     dx = __builtin_amdgcn_ldexpf(dx, -e);
@@ -281,22 +322,38 @@ __device__ __forceinline__ Position position_of(const EdgeParams& p, int64_t nod
     }
     return a;
 }
-// The distances of row r's node to the lane's eight slots.
-__device__ __forceinline__ void distances(const EdgeLds& L, const Position& own, int dims, int lane,
-                                          float (&d)[8])
+// The distances of row r's node to the lane's slots 16 t + 4 g ..
+__device__ __forceinline__ void distances(const EdgeLds& L, const Position& own, int dims, int t,
+                                          int lane, float (&d)[4])
 {
-    const int g = anew(lane) >> 4;
+    const int slot = 16 * t + 4 * (anew(lane) >> 4);
     if (dims == 1) {
-        const f4 a = *reinterpret_cast<const f4*>(&L.pos[4 * g]);
-        const f4 b = *reinterpret_cast<const f4*>(&L.pos[16 + 4 * g]);
+        const f4 a = *reinterpret_cast<const f4*>(&L.pos[slot]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d[j] = __builtin_fabsf(own.x - (j < 4 ? a[j & 3] : b[j & 3]));
+        for (int j = 0; j < 4; ++j) d[j] = __builtin_fabsf(own.x - a[j]);
+        return;
+    }
+    float least = INFINITY, most = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const f4 a = *reinterpret_cast<const f4*>(&L.pos[4 * (slot + j)]);
+        d[j] = squared(own, a[0], a[1], a[2]);
+        least = __builtin_fminf(least, d[j]);
+        most = __builtin_fmaxf(most, d[j]);
+    }
+    if (__ballot(least < 0x1p-100f || !(most < 0x1p126f))) {   // (a loop's 0 among them)
+#pragma unroll 1
+        for (int j = 0; j < 4; ++j) {
+            const f4 a = *reinterpret_cast<const f4*>(&L.pos[4 * (slot + j)]);
+            const float x = distance(own, a[0], a[1], a[2]);
+            d[0] = j == 0 ? x : d[0];
+            d[1] = j == 1 ? x : d[1];
+            d[2] = j == 2 ? x : d[2];
+            d[3] = j == 3 ? x : d[3];
+        }
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const f4 a = *reinterpret_cast<const f4*>(&L.pos[4 * slot_of(g, j)]);
-            d[j] = distance(own, a[0], a[1], a[2], 3);
-        }
+        for (int j = 0; j < 4; ++j) d[j] = __builtin_amdgcn_sqrtf(d[j]);
     }
 }
 
@@ -392,13 +449,13 @@ __device__ __forceinline__ void edge_finish(const EdgeParams& p, EdgeState<PASS>
         const float c = p.scale * i;
         edge_store<T>(p.out1, stage, w, p.n, head_off, lane,
                       [&](int t) { return c * (st.acc[t] * f - d * st.acc[4 + t]); });
-        if (g == 0 && row < p.n) p.stats[((int64_t)row * p.H + h) * 2 + 1] = d;
+        if (g == 0 && row < p.n) p.stats[((int64_t)row * p.H + h) * p.stat_words + 1] = d;
         if (p.dims) {
             // the window's share of dslope: rows 0 to 15 in one fixed order
             float s = row < p.n ? (over_groups(st.yd) - d * over_groups(st.zd)) * i : 0.f;
 #pragma unroll
             for (int off = 8; off >= 1; off >>= 1) s += __shfl_xor(s, off, kWave);
-            if (lane == 0) p.slope_parts[(int64_t)h * p.W + w] = s;
+            if (lane == 0) p.slope_parts[(int64_t)h * p.slope_windows + w] = s;
         }
     } else {
         const float f = p.scale * fast_exp2(st.x);
@@ -439,11 +496,14 @@ __device__ float slow_row(const EdgeParams& p, int32_t w, int h, int r, int nite
                 const int64_t node =
                     (int64_t)(((uint64_t)(ref >> p.ref_shift) * p.ref_magic) >> 31);
                 const float y1 = value(p.x1, node), y2 = value(p.x2, node);
-                float slope_c, dist = 0.f;
-                float s = edge_score(p, wave_sum(a * y1), slope_c);
+                float dist = 0.f, score[1] = {wave_sum(a * y1)}, slopes_c[1];
+                edge_scores(p, score, slopes_c);
+                float s = score[0];
+                const float slope_c = slopes_c[0];
                 if (p.dims) {
                     const Position there = position_of(p, node);
-                    dist = distance(own, there.x, there.y, there.z, p.dims);
+                    dist = p.dims == 1 ? __builtin_fabsf(own.x - there.x)
+                                       : distance(own, there.x, there.y, there.z);
                     s -= slope * dist;
                 }
                 if constexpr (PASS == kForward) {
@@ -462,7 +522,8 @@ __device__ float slow_row(const EdgeParams& p, int32_t w, int h, int r, int nite
                     acc1 += e * g * slope_c * y1;
                     acc2 += e * slope_c * y1;
                 } else {
-                    const float2 st = *reinterpret_cast<const float2*>(p.stats + (node * p.H + h) * 2);
+                    const float2 st =
+                        *reinterpret_cast<const float2*>(p.stats + (node * p.H + h) * p.stat_words);
                     const float e = fast_exp2(s - st.x), g = wave_sum(b * y2);
                     acc1 += e * (g - st.y) * slope_c * y1;
                     acc2 += e * y2;
@@ -480,7 +541,7 @@ __device__ float slow_row(const EdgeParams& p, int32_t w, int h, int r, int nite
     } else if constexpr (PASS == kRows) {
         const float i = l != 0.f ? 1.f / l : 0.f, d = pg * i;
         store(p.out1, p.scale * i * (acc1 - d * acc2));
-        if (lane == 0) p.stats[at * 2 + 1] = d;
+        if (lane == 0) p.stats[at * p.stat_words + 1] = d;
         return (pgd - d * pd) * i;
     } else {
         store(p.out1, p.scale * acc1);
@@ -508,16 +569,40 @@ __device__ void slow_window(const EdgeParams& p, int32_t w, int h, int nitems, F
         if (threadIdx.x == 0 && p.dims) {
             float s = 0.f;
             for (int r = 0; r < 16; ++r) s += lds[r];
-            p.slope_parts[(int64_t)h * p.W + w] = s;
+            p.slope_parts[(int64_t)h * p.slope_windows + w] = s;
         }
         __syncthreads();
+    }
+}
+
+// -sum of a head's windows' shares, by THREADS threads.
+template <int THREADS>
+__device__ __forceinline__ void sum_slopes(const float* __restrict__ src, int32_t W,
+                                           float* __restrict__ out)
+{
+    __shared__ double lds[THREADS / kWave];
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < W; i += 32 * THREADS) {
+        float x[32];   // (in one batch: the loads' latency is all there is)
+#pragma unroll
+        for (int k = 0; k < 32; ++k) x[k] = src[min(i + k * THREADS, (int64_t)W - 1)];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) s += i + k * THREADS < W ? x[k] : 0.f;
+    }
+    s = wave_sum(s);
+    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double t = 0.0;
+        for (int i = 0; i < THREADS / kWave; ++i) t += lds[i];
+        *out = (float)-t;
     }
 }
 
 // TEAM: a window's four items are its workgroup's waves (small graphs); else a wave
 // takes an item, a window or a segment of one.
 template <typename T, int PASS, bool WIDE, bool TEAM>
-__global__ void __launch_bounds__(kWave * kEdgeWaves) __attribute__((amdgpu_waves_per_eu(3)))
+__global__ void __launch_bounds__(kWave * kEdgeWaves) __attribute__((amdgpu_waves_per_eu(PASS == kForward ? 4 : 3)))
 edge_kernel(const EdgeParams p)
 {
     typedef typename Half<T>::v8 v8;
@@ -575,12 +660,16 @@ edge_kernel(const EdgeParams p)
     float lse = 0.f;
     if constexpr (PASS == kRows) {
         lse = p.lse[(int64_t)row * H + h];
-        // (the columns' pass finds it beside D)
-        if (g == 0 && w * 16 + r < n && (!TEAM || wave == 0)) p.stats[((int64_t)row * H + h) * 2] = lse;
+        if (g == 0 && w * 16 + r < n && (!TEAM || wave == 0)) {
+            float* to = p.stats + ((int64_t)row * H + h) * p.stat_words;
+            to[0] = lse;
+            if (p.dims) *reinterpret_cast<f2*>(to + 2) = f2{own.x, own.y};
+            if (p.dims > 2) to[4] = own.z;
+        }
         lse -= kLiftLog2<T>;
     }
 
-    const EdgePlaces at = edge_places(L.x1, lane);
+    EdgePlaces at = edge_places(L.x1, lane);
     const uint32_t masks0 = (uint32_t)(uintptr_t)(LdsPtr)&L.rec[0].rm[0];
     v8 a[4], b[4];
     Position there{0.f, 0.f, 0.f};   // of slot lane % 32
@@ -589,10 +678,11 @@ edge_kernel(const EdgeParams p)
     // A record's words, one per lane: 32 references, 32 masks.  (The lists end in spare
     // records.)
     auto fetch = [&](int32_t c) __attribute__((always_inline)) {
-        return p.columns[(int64_t)c * 64 + lane];
+        return (p.columns + (int64_t)c * 64)[anew(lane)];
     };
     // Into the record of chunk c, and the loads of its slots.
     auto load = [&](int32_t c) __attribute__((always_inline)) {
+        const int lane = anew(threadIdx.x % kWave);
         EdgeRecord& rec = L.rec[(c - cb) & 1];
         const uint32_t ref = __shfl(word, lane & 31, kWave);
         const bool none = ref >= p.no_ref;
@@ -630,9 +720,20 @@ edge_kernel(const EdgeParams p)
             }
         }
         const int64_t i = none ? 0 : node;
-        if (p.dims) there = position_of(p, i);
-        if constexpr (PASS == kColumns)
-            stat = *reinterpret_cast<const f2*>(p.stats + (i * H + h) * 2);
+        if constexpr (PASS == kColumns) {
+            const float* from = p.stats + (i * H + h) * p.stat_words;
+            if (p.dims) {
+                const f4 x = *reinterpret_cast<const f4*>(from);
+                stat = f2{x[0], x[1]};
+                there.x = x[2];
+                there.y = x[3];
+                if (p.dims > 2) there.z = from[4];
+            } else {
+                stat = *reinterpret_cast<const f2*>(from);
+            }
+        } else if (p.dims) {
+            there = position_of(p, i);
+        }
     };
 
     EdgeState<PASS> st;
@@ -645,40 +746,69 @@ edge_kernel(const EdgeParams p)
     }
     for (int32_t c = cb; c < ce; ++c) {
         const uint32_t masks = masks0 + ((c - cb) & 1) * (uint32_t)sizeof(EdgeRecord);
+        held(at);
         edge_write(at, 0, a);
         edge_write(at, kEdgeStage, b);
-        if (p.dims == 1) L.pos[lane & 31] = there.x;
-        else if (p.dims) *reinterpret_cast<f4*>(&L.pos[4 * (lane & 31)]) = f4{there.x, there.y, there.z, 0.f};
-        if constexpr (PASS == kColumns) *reinterpret_cast<f2*>(&L.stats[2 * (lane & 31)]) = stat;
+        const int own_slot = anew(lane) & 31;
+        if (p.dims == 1) L.pos[own_slot] = there.x;
+        else if (p.dims) *reinterpret_cast<f4*>(&L.pos[4 * own_slot]) = f4{there.x, there.y, there.z, 0.f};
+        if constexpr (PASS == kColumns) *reinterpret_cast<f2*>(&L.stats[2 * own_slot]) = stat;
         wave_lds_order();
         if (c + 1 < ce) {
             load(c + 1);
             word = fetch(c + 2);   // (past the item's last: another's, or a spare one)
         }
-        // scores of slots 4 g .. and 16 + 4 g .. of row r, and g = do . v
-        f4 s4[2], g4[2];
+        // Half of the slots at a time (registers): scores of slots 16 t + 4 g .. of row r,
+        // and what the products after them take: w beside acc[4 ..] (forward: acc), u
+        // beside acc[0 .. 3].
+        float w8[8], u8[8];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) s4[t] = edge_products<T>(at, kEdgeHalf * t, o1);
-        if constexpr (PASS != kForward)
+        for (int t = 0; t < 2; ++t) {
+            __builtin_amdgcn_sched_barrier(0);
+            const f4 dots = edge_products<T>(at, kEdgeHalf * t, o1);
+            float s[4] = {dots[0], dots[1], dots[2], dots[3]}, cc[4], dist[4];
+            f4 gs;   // do . v
+            if constexpr (PASS != kForward) gs = edge_products<T>(at, kEdgeStage + kEdgeHalf * t, o2);
+            edge_scores(p, s, cc);
+            if (p.dims) {
+                distances(L, own, p.dims, t, lane, dist);
 #pragma unroll
-            for (int t = 0; t < 2; ++t) g4[t] = edge_products<T>(at, kEdgeStage + kEdgeHalf * t, o2);
-        float s[8], cc[8], dist[8];
+                for (int j = 0; j < 4; ++j) s[j] = __builtin_fmaf(-slope, dist[j], s[j]);
+            }
+            uint32_t on[4];
+            attends_half(masks, t, lane, on);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] = edge_score(p, s4[j >> 2][j & 3], cc[j]);
-        if (p.dims) {
-            distances(L, own, p.dims, lane, dist);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) s[j] = __builtin_fmaf(-slope, dist[j], s[j]);
+            for (int j = 0; j < 4; ++j) {
+                float& w = w8[4 * t + j];
+                [[maybe_unused]] float& u = u8[4 * t + j];
+                if constexpr (PASS == kForward) {
+                    w = where(on[j], s[j], -INFINITY);
+                } else if constexpr (PASS == kRows) {
+                    const float e = where(on[j], fast_exp2(lifted<T>(s[j] - lse, kLiftLog2<T> + 1.f)));
+                    const float eg = where(on[j], e * gs[j]);
+                    st.z += e;
+                    st.y += eg;
+                    if (p.dims) {
+                        const float d = where(on[j], dist[j]);
+                        st.zd = __builtin_fmaf(e, d, st.zd);
+                        st.yd = __builtin_fmaf(eg, d, st.yd);
+                    }
+                    w = where(on[j], e * cc[j]);
+                    u = where(on[j], eg * cc[j]);
+                } else {
+                    const f2 of = *reinterpret_cast<const f2*>(&L.stats[2 * (16 * t + 4 * (anew(lane) >> 4) + j)]);
+                    const float e = where(on[j], fast_exp2(lifted<T>(s[j] - of[0], 0.f)));
+                    u = where(on[j], e * (gs[j] - of[1]) * cc[j]);
+                    w = e * kLift<T>;
+                }
+            }
         }
-        Attends on;
-        attends(masks, lane, on);
+        __builtin_amdgcn_sched_barrier(0);
         if constexpr (PASS == kForward) {
             // the running maximum is moved when a chunk's exceeds it by more than kLazy
+            float top = w8[0];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s[j] = where(on[j], s[j], -INFINITY);
-            float top = s[0];
-#pragma unroll
-            for (int j = 1; j < 8; ++j) top = __builtin_fmaxf(top, s[j]);
+            for (int j = 1; j < 8; ++j) top = __builtin_fmaxf(top, w8[j]);
             top = row_max4(top);
             if (__ballot(top > st.x + kLazy)) {
                 if (top > st.x + kLazy) {
@@ -691,40 +821,15 @@ edge_kernel(const EdgeParams p)
             const float mu = st.x == -INFINITY ? 0.f : st.x;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                s[j] = fast_exp2(s[j] - mu);
-                st.y += s[j];
+                w8[j] = fast_exp2(w8[j] - mu);
+                st.y += w8[j];
             }
-            edge_mix<T>(at, kEdgeStage, s, st.acc);
-        } else if constexpr (PASS == kRows) {
-            float pg[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float e = where(on[j], fast_exp2(lifted<T>(s[j] - lse, kLiftLog2<T> + 1.f)));
-                const float eg = where(on[j], e * g4[j >> 2][j & 3]);
-                st.z += e;
-                st.y += eg;
-                if (p.dims) {
-                    st.zd = __builtin_fmaf(e, where(on[j], dist[j]), st.zd);
-                    st.yd = __builtin_fmaf(eg, where(on[j], dist[j]), st.yd);
-                }
-                s[j] = where(on[j], e * cc[j]);
-                pg[j] = where(on[j], eg * cc[j]);
-            }
-            edge_mix<T>(at, 0, s, st.acc + 4);
-            range_update<T>(st, pg);
-            edge_mix<T>(at, 0, pg, st.acc);
+            edge_mix<T>(at, kEdgeStage, w8, st.acc);
         } else {
-            float ds[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float* of = &L.stats[2 * slot_of(g, j)];
-                const float e = where(on[j], fast_exp2(lifted<T>(s[j] - of[0], 0.f)));
-                ds[j] = where(on[j], e * (g4[j >> 2][j & 3] - of[1]) * cc[j]);
-                s[j] = e * kLift<T>;
-            }
-            edge_mix<T>(at, kEdgeStage, s, st.acc + 4);
-            range_update<T>(st, ds);
-            edge_mix<T>(at, 0, ds, st.acc);
+            edge_mix<T>(at, PASS == kRows ? 0 : kEdgeStage, w8, st.acc + 4);
+            __builtin_amdgcn_sched_barrier(0);
+            range_update<T>(st, u8);
+            edge_mix<T>(at, 0, u8, st.acc);
         }
         wave_lds_order();
     }
@@ -752,7 +857,7 @@ edge_kernel(const EdgeParams p)
     } else {
         const bool any = odd_state(st);
         if (lane == 0) p.odd[item * H + h] = any && slot < 0;
-        if (slot >= 0) {   // a segment: its sums wait for edge_merge_kernel
+        if (slot >= 0) {   // a segment: its sums wait for edge_tail_kernel
             publish(st, p.partials + ((int64_t)slot * H + h) * state_floats<PASS>(), lane);
             if (h == 0 && lane == 0) p.slot_item[slot] = (int32_t)item;
         } else {
@@ -761,70 +866,61 @@ edge_kernel(const EdgeParams p)
     }
 }
 
-// The segments of a split window, in their order.
+// What follows a pass of windows on single waves, one launch of workgroups for each:
+// split windows, their segments joined in order (num_split x H); dslope[h] = -sum of
+// the windows' shares of the rows' pass, in one fixed order (H, columns' pass with
+// positions); the windows whose sums were not finite.
 template <typename T, int PASS>
-__global__ void __launch_bounds__(kWave) edge_merge_kernel(const EdgeParams p)
+__global__ void __launch_bounds__(kWave * kEdgeWaves) edge_tail_kernel(const EdgeParams p)
 {
     __shared__ __align__(16) _Float16 stage[16 * kHeadHalves];
-    const int lane = threadIdx.x;
-    const uint32_t split = blockIdx.x / (uint32_t)p.H, h = blockIdx.x % (uint32_t)p.H;
-    const SplitInfo si = p.splits[split];
-    EdgeState<PASS> st;
-    clear(st);
-    for (int32_t k = 0; k < si.nseg; ++k)
-        absorb(st, p.partials + ((int64_t)(si.first_slot + k) * p.H + h) * state_floats<PASS>(), lane);
-    edge_finish<T, PASS>(p, st, stage, si.w, (int)h, lane);
-    const bool any = odd_state(st);
-    if (lane == 0) p.odd[p.num_items * p.H + blockIdx.x] = any;
-}
-
-// The windows whose sums were not finite.
-template <typename T, int PASS>
-__global__ void __launch_bounds__(kWave * kEdgeWaves) edge_repair_kernel(const EdgeParams p)
-{
     __shared__ float lds[16];
-    const int lane = threadIdx.x % kWave;
-    const uint32_t H = (uint32_t)p.H;
-    const int64_t whole = p.num_items * p.H, units = whole + p.num_split * p.H;
-    for (int64_t base = (int64_t)blockIdx.x * kWave; base < units; base += (int64_t)gridDim.x * kWave) {
+    __shared__ uint32_t odd;
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    const uint32_t H = (uint32_t)p.H, joins = (uint32_t)p.num_split * H;
+    const uint32_t sums = PASS == kColumns && p.dims ? H : 0;
+    if (blockIdx.x < joins) {
+        const uint32_t h = blockIdx.x % H;
+        const SplitInfo si = p.splits[blockIdx.x / H];
+        if (wave == 0) {
+            EdgeState<PASS> st;
+            clear(st);
+            for (int32_t k = 0; k < si.nseg; ++k)
+                absorb(st, p.partials + ((int64_t)(si.first_slot + k) * H + h) * state_floats<PASS>(),
+                       lane);
+            edge_finish<T, PASS>(p, st, stage, si.w, (int)h, lane);
+            const bool any = odd_state(st);
+            if (lane == 0) odd = any;
+        }
+        __syncthreads();
+        if (odd)
+            slow_window<T, PASS>(p, si.w, (int)h, si.nseg,
+                                 [&](int k) { return p.slot_item[si.first_slot + k]; }, lds);
+        return;
+    }
+    if (blockIdx.x < joins + sums) {
+        const uint32_t h = blockIdx.x - joins;
+        sum_slopes<kWave * kEdgeWaves>(p.slope_parts + (int64_t)h * p.slope_windows, p.slope_windows,
+                                       p.dslopes + h);
+        return;
+    }
+    const int64_t units = p.num_items * H, groups = gridDim.x - joins - sums;
+    for (int64_t base = (int64_t)(blockIdx.x - joins - sums) * kWave; base < units;
+         base += groups * kWave) {
         uint64_t flagged = __ballot(base + lane < units && p.odd[min(base + lane, units - 1)] != 0u);
         for (; flagged; flagged &= flagged - 1) {   // (the same for every wave)
             const int64_t at = base + __builtin_ctzll(flagged);
-            if (at < whole) {
-                const int32_t item = (int32_t)(at / H);
-                slow_window<T, PASS>(p, p.items[item].w, (int)(at % H), 1,
-                                     [&](int) { return item; }, lds);
-            } else {
-                const SplitInfo si = p.splits[(at - whole) / H];
-                slow_window<T, PASS>(p, si.w, (int)((at - whole) % H), si.nseg,
-                                     [&](int k) { return p.slot_item[si.first_slot + k]; }, lds);
-            }
+            const int32_t item = (int32_t)(at / H);
+            slow_window<T, PASS>(p, p.items[item].w, (int)(at % H), 1, [&](int) { return item; }, lds);
         }
     }
 }
 
-// dslope[h] = -sum of its windows' shares, in one fixed order.
+// dslopes without a launch to go with (teams, no nodes).
 __global__ void __launch_bounds__(1024)
 edge_slope_kernel(const float* __restrict__ parts, int32_t W, float* __restrict__ dslopes)
 {
-    __shared__ double lds[1024 / kWave];
-    const float* src = parts + (int64_t)blockIdx.x * W;
-    double s = 0.0;
-    for (int32_t i = threadIdx.x; i < W; i += 32 * 1024) {
-        float x[32];   // (in one batch: the loads' latency is all there is)
-#pragma unroll
-        for (int k = 0; k < 32; ++k) x[k] = src[min((int64_t)i + k * 1024, (int64_t)W - 1)];
-#pragma unroll
-        for (int k = 0; k < 32; ++k) s += (int64_t)i + k * 1024 < W ? x[k] : 0.f;
-    }
-    s = wave_sum(s);
-    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        double t = 0.0;
-        for (int i = 0; i < 1024 / kWave; ++i) t += lds[i];
-        dslopes[blockIdx.x] = (float)-t;
-    }
+    sum_slopes<1024>(parts + (int64_t)blockIdx.x * W, W, dslopes + blockIdx.x);
 }
 
 __global__ void warm_edge_kernel() {}
@@ -835,7 +931,7 @@ hipError_t warm_edge(hipStream_t s)
     return hipGetLastError();
 }
 
-constexpr int32_t kEdgeRepairGroups = 1024;
+constexpr int32_t kEdgeScanGroups = 1024;
 
 template <typename T, int PASS, bool WIDE>
 static void launch_edge(const EdgeParams& p, hipStream_t st)
@@ -848,12 +944,10 @@ static void launch_edge(const EdgeParams& p, hipStream_t st)
     }
     const int64_t groups = kXcds * ceil_div(ceil_div(p.num_items, kXcds) * p.H, kEdgeWaves);
     hipLaunchKernelGGL((edge_kernel<T, PASS, WIDE, false>), dim3((unsigned)groups), block, 0, st, p);
-    if (p.num_split > 0)
-        hipLaunchKernelGGL((edge_merge_kernel<T, PASS>), dim3((unsigned)(p.num_split * p.H)),
-                           dim3(kWave), 0, st, p);
-    const int64_t units = (p.num_items + p.num_split) * p.H;
-    hipLaunchKernelGGL((edge_repair_kernel<T, PASS>),
-                       dim3((unsigned)std::min<int64_t>(kEdgeRepairGroups, ceil_div(units, kWave))),
+    const int64_t scans =
+        std::min<int64_t>(kEdgeScanGroups, ceil_div(p.num_items * p.H, kWave));
+    const int64_t sums = PASS == kColumns && p.dims ? p.H : 0;
+    hipLaunchKernelGGL((edge_tail_kernel<T, PASS>), dim3((unsigned)(p.num_split * p.H + sums + scans)),
                        block, 0, st, p);
 }
 
@@ -866,7 +960,7 @@ static EdgeSpace edge_space(const f3s_plan* plan, bool backward)
     EdgeSpace s;   // (teams merge in LDS)
     const f3s_item_set& set = plan->masked;
     if (set.team == 1) {
-        s.items = round_up(sizeof(uint32_t) * (size_t)(set.num_items + set.num_split) * plan->H);
+        s.items = round_up(sizeof(uint32_t) * (size_t)set.num_items * plan->H);
         s.partials = s.items + round_up(sizeof(int32_t) * (size_t)set.num_slots);
         s.bytes = s.partials +
                   round_up(sizeof(float) *
@@ -962,6 +1056,7 @@ static EdgeParams edge_params(int32_t n, float scale, float cap, const float* po
     p.cap_log2 = cap * kLog2e;
     p.positions = positions;
     p.dims = dims;
+    p.stat_words = stat_words(dims);
     p.slopes = slopes;
     return p;
 }
@@ -973,13 +1068,14 @@ using namespace f3s;
 extern "C" {
 
 f3s_status f3s_edge_attention_workspace(const f3s_plan* plan, const f3s_plan* reversed,
-                                        int64_t* bytes)
+                                        int32_t dims, int64_t* bytes)
 {
-    F3S_REQUIRE(plan && bytes, "f3s_edge_attention_workspace: NULL pointer");
+    F3S_REQUIRE(plan && bytes && dims >= 0 && dims <= 3,
+                "f3s_edge_attention_workspace: NULL pointer, or dims not 0 to 3");
     size_t need = edge_space(plan, reversed != nullptr).bytes;
     if (reversed) {
         const size_t cells = (size_t)std::max(plan->compiled_n, 0) * plan->H;
-        need = std::max(need, edge_space(reversed, true).bytes) + round_up(cells * 8) +
+        need = std::max(need, edge_space(reversed, true).bytes) + round_up(cells * 4 * stat_words(dims)) +
                round_up(sizeof(float) * (size_t)plan->W * plan->H);
     }
     *bytes = (int64_t)need;
@@ -1036,7 +1132,7 @@ f3s_status f3s_edge_attention_bwd(const f3s_plan* plan, const f3s_plan* reversed
                 "f3s_edge_attention_bwd: NULL or misaligned pointer, or a row stride that is no "
                 "multiple of 8 or below H * 64");
     int64_t need = 0;
-    F3S_TRY(f3s_edge_attention_workspace(plan, reversed, &need));
+    F3S_TRY(f3s_edge_attention_workspace(plan, reversed, dims, &need));
     F3S_REQUIRE(workspace_bytes >= need && (workspace || need == 0) &&
                     ((uintptr_t)workspace & 15) == 0,
                 "f3s_edge_attention_bwd: workspace too small");
@@ -1047,9 +1143,11 @@ f3s_status f3s_edge_attention_bwd(const f3s_plan* plan, const f3s_plan* reversed
     if (n > 0) {
         char* ws = static_cast<char*>(workspace);
         p.stats = reinterpret_cast<float*>(ws);
-        ws += round_up((size_t)n * H * 8);
+        ws += round_up((size_t)n * H * 4 * p.stat_words);
         p.slope_parts = reinterpret_cast<float*>(ws);
         ws += round_up(sizeof(float) * (size_t)plan->W * H);
+        p.slope_windows = plan->W;
+        p.dslopes = dslopes;
         p.lse = const_cast<float*>(lse);
         EdgeParams rows = p;
         rows.x1 = rows_of(K, k_stride);
@@ -1067,7 +1165,7 @@ f3s_status f3s_edge_attention_bwd(const f3s_plan* plan, const f3s_plan* reversed
         cols.out2 = rows_of(dV, dv_stride);
         F3S_TRY(launch_edge_pass<kColumns>(cols, reversed, dtype, ws, st));
     }
-    if (dims > 0)
+    if (dims > 0 && (n == 0 || reversed->masked.team > 1))
         hipLaunchKernelGGL(edge_slope_kernel, dim3((unsigned)H), dim3(1024), 0, st, p.slope_parts,
                            n > 0 ? plan->W : 0, dslopes);
     F3S_HIP(hipGetLastError());

@@ -59,6 +59,15 @@ __device__ __forceinline__ void attends(uint32_t masks, int lane, Attends& on)
         on[j] = (uint32_t)__builtin_amdgcn_sbfe((int)(j < 4 ? a[j & 3] : b[j & 3]), rbit, 1);
 }
 
+// The same of slots 16 t + 4 g .. alone.
+__device__ __forceinline__ void attends_half(uint32_t masks, int t, int lane, uint32_t (&on)[4])
+{
+    const int l = anew(lane), r = l & 15, rbit = (r & 1) ? 16 + (r >> 1) : (r >> 1);
+    const u4 a = lds_read<u4>(masks + 64 * t + 16 * (l >> 4));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) on[j] = (uint32_t)__builtin_amdgcn_sbfe((int)a[j], rbit, 1);
+}
+
 // Weights of a size of 1 at most, in binary16: with |w| <= 2 they stay below 2^15, and
 // their halves end at 2^-39.  (A node that a row hardly attends, or that only rows of
 // very many edges do, has weights of 2^-17 and less alone: unscaled, 2^-20 was off by

@@ -437,15 +437,15 @@ class TorchGraph:
             return _EdgeAttention.apply(self, float(scale), *bias, qkv)
         return _edge_forward(self, float(scale), *bias, *_thirds(qkv, self, HEAD_DIM))
 
-    def _edge_workspace(self, backward: bool) -> torch.Tensor:
-        size = self._edge_workspaces.get(backward)
+    def _edge_workspace(self, backward: bool, dims: int) -> torch.Tensor:
+        size = self._edge_workspaces.get((backward, dims))
         if size is None:
             need = C.c_int64()
             check(_lib.hip().f3s_edge_attention_workspace(
-                self._diff_plan().handle, self._reversed.handle if backward else None,
+                self._diff_plan().handle, self._reversed.handle if backward else None, dims,
                 C.byref(need)),
                 "f3s_edge_attention_workspace")
-            size = self._edge_workspaces[backward] = need.value
+            size = self._edge_workspaces[backward, dims] = need.value
         return torch.empty(size, dtype=torch.uint8, device=self._torch_device) if size else None
 
 
@@ -546,7 +546,7 @@ def _edge_forward(graph: TorchGraph, scale: float, cap, dims, positions, slopes,
     out = q.new_empty((n, H, HEAD_DIM))
     if n:
         plan = graph._diff_plan().handle
-        ws = graph._edge_workspace(False)
+        ws = graph._edge_workspace(False, dims)
         if dims and not slopes.is_contiguous():
             slopes = slopes.contiguous()
         check(_lib.hip().f3s_edge_attention_fwd(
@@ -591,7 +591,7 @@ class _EdgeAttention(torch.autograd.Function):
         dslopes = torch.empty_like(slopes) if dims else None
         do = _rows(grad, graph, HEAD_DIM)
         with _on(graph.device):
-            ws = graph._edge_workspace(True)
+            ws = graph._edge_workspace(True, dims)
             check(_lib.hip().f3s_edge_attention_bwd(
                 graph._diff_plan().handle, graph._reversed.handle, q.data_ptr(), _stride(q, n),
                 k.data_ptr(), _stride(k, n), v.data_ptr(), _stride(v, n), lse.data_ptr(),

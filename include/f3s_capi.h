@@ -471,7 +471,7 @@ f3s_status f3s_diff_attention_bwd(const f3s_plan* plan, const f3s_plan* reversed
  * this call's alone until it is done; nothing else is allocated or kept, so calls
  * may overlap and be captured.  Asynchronous on `stream`. */
 f3s_status f3s_edge_attention_workspace(const f3s_plan* plan, const f3s_plan* reversed,
-                                        int64_t* bytes);
+                                        int32_t dims, int64_t* bytes);
 f3s_status f3s_edge_attention_fwd(const f3s_plan* plan, const uint16_t* Q, int64_t q_stride,
                                   const uint16_t* K, int64_t k_stride, const uint16_t* V,
                                   int64_t v_stride, uint16_t* O, int64_t o_stride, float* lse,

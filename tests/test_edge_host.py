@@ -16,7 +16,7 @@ from fused3s_amd import _lib
 def test_entry_points_refuse():
     h = _lib.hip()
     need = C.c_int64()
-    assert h.f3s_edge_attention_workspace(None, None, C.byref(need)) == 1
+    assert h.f3s_edge_attention_workspace(None, None, 0, C.byref(need)) == 1
     call = lambda plan=None, n=16, dtype=0, cap=0.0, pos=None, dims=0, slopes=None: \
         h.f3s_edge_attention_fwd(plan, 16, 64, 16, 64, 16, 64, 16, 64, None, dtype, n, 1, 1.0, cap,
                                  pos, dims, slopes, None, 0, None)
