@@ -45,14 +45,18 @@ struct CeParams {
     int32_t reduction;
 };
 
-// A row's blocks joined: 16 rows by 16 parts of the blocks, in a fixed order.
+// A row's blocks joined: ROWS rows by the other threads' parts of the blocks, in a fixed
+// order.  (64 rows of 1,564 blocks, 16 rows a workgroup: 16 us, four: 6; 200,003 rows of
+// two blocks, 16: 15, 256: 5.)
+template <int ROWS>
 __global__ void __launch_bounds__(kLossThreads) loss_join(const CeParams p)
 {
-    __shared__ float2 lds[16][17];
-    __shared__ double sums[16][2];
-    const int in = threadIdx.x % 16, part = threadIdx.x / 16;
-    const int64_t row = (int64_t)blockIdx.x * 16 + in, i = p.first_row + row;
-    const int64_t per = (p.nblocks + 15) / 16, first = part * per, end = min(p.nblocks, first + per);
+    constexpr int kParts = kLossThreads / ROWS;
+    __shared__ float2 lds[kParts][ROWS + 1];
+    const int in = threadIdx.x % ROWS, part = threadIdx.x / ROWS;
+    const int64_t row = (int64_t)blockIdx.x * ROWS + in, i = p.first_row + row;
+    const int64_t per = (p.nblocks + kParts - 1) / kParts, first = part * per,
+                  end = min(p.nblocks, first + per);
     float m = -INFINITY, s = 0.f;
     auto take = [&](float2 b) {
         // (a NaN block's largest may not be NaN, its sum is)
@@ -70,11 +74,14 @@ __global__ void __launch_bounds__(kLossThreads) loss_join(const CeParams p)
             for (int u = 0; u < 8; ++u)
                 if (k + u < end) take(b[u]);
         }
-    lds[part][in] = make_float2(m, s);
-    __syncthreads();
+#pragma unroll
+    for (int step = kParts / 2; step >= 1; step /= 2) {   // part k takes k + step
+        if (part >= step && part < 2 * step) lds[part][in] = make_float2(m, s);
+        __syncthreads();
+        if (part < step) take(lds[part + step][in]);
+    }
+    double loss = 0.0, counts = 0.0;
     if (part == 0) {
-        for (int k = 1; k < 16; ++k) take(lds[k][in]);
-        double loss = 0.0, counts = 0.0;
         if (row < p.rows) {
             const int64_t t = p.target[i];
             const bool none = t == p.ignore;
@@ -87,14 +94,19 @@ __global__ void __launch_bounds__(kLossThreads) loss_join(const CeParams p)
             loss = value;
             counts = none ? 0.0 : 1.0;
         }
-        sums[in][0] = loss;
-        sums[in][1] = counts;
+    }
+    __shared__ double sums[kLossThreads / kWave][2];
+    loss = wave_sum(loss);
+    counts = wave_sum(counts);
+    if (threadIdx.x % kWave == 0) {
+        sums[threadIdx.x / kWave][0] = loss;
+        sums[threadIdx.x / kWave][1] = counts;
     }
     __syncthreads();
     if (threadIdx.x < 2) {
         double t = 0.0;
-        for (int k = 0; k < 16; ++k) t += sums[k][threadIdx.x];
-        p.parts[2 * (p.first_row / 16 + blockIdx.x) + threadIdx.x] = t;
+        for (int k = 0; k < kLossThreads / kWave; ++k) t += sums[k][threadIdx.x];
+        p.parts[2 * (p.first_row / ROWS + blockIdx.x) + threadIdx.x] = t;
     }
 }
 
@@ -252,7 +264,7 @@ static ForwardSpace forward_space(int64_t n, int64_t V)
     s.nblocks = ceil_div(V, 32) + 8;   // (at most: the smallest blocks, and a tile's last ones)
     s.rows = std::max<int64_t>(1024, kBlocksBytes / 8 / s.nblocks / 1024 * 1024);
     s.rows = std::min(s.rows, n);
-    s.picked = up256(sizeof(double) * 2 * (size_t)ceil_div(n, 16));
+    s.picked = up256(sizeof(double) * 2 * (size_t)ceil_div(n, 4));
     s.blocks = s.picked + up256(sizeof(float) * (size_t)s.rows);
     s.bytes = s.blocks + up256(sizeof(float2) * (size_t)s.rows * s.nblocks);
     return s;
@@ -277,7 +289,10 @@ static f3s_status loss_forward(const CeArgs& a, float* loss, float* lse, char* w
     c.lse = lse;
     c.loss = loss;
     c.parts = reinterpret_cast<double*>(ws);
-    c.nparts = ceil_div(a.n, 16);
+    // (rows per workgroup of a join; the rows of a piece are a multiple of 1,024)
+    const int64_t most = ceil_div(a.V, 64);
+    const int join = most <= 16 && a.n >= 4096 ? 256 : a.n <= 2048 ? 4 : 16;
+    c.nparts = ceil_div(a.n, join);
     c.reduction = a.reduction;
     for (int64_t r0 = 0; r0 < a.n; r0 += s.rows) {
         GemmParams p{};
@@ -307,8 +322,10 @@ static f3s_status loss_forward(const CeArgs& a, float* loss, float* lse, char* w
         c.nblocks = blocks_of(tile, p.outs);
         c.rows = p.rows;
         c.first_row = r0;
-        hipLaunchKernelGGL(loss_join, dim3((unsigned)ceil_div(p.rows, 16)), dim3(kLossThreads), 0,
-                           a.st, c);
+        const dim3 grid((unsigned)ceil_div(p.rows, join));
+        if (join == 256) hipLaunchKernelGGL((loss_join<256>), grid, dim3(kLossThreads), 0, a.st, c);
+        else if (join == 4) hipLaunchKernelGGL((loss_join<4>), grid, dim3(kLossThreads), 0, a.st, c);
+        else hipLaunchKernelGGL((loss_join<16>), grid, dim3(kLossThreads), 0, a.st, c);
     }
     if (a.reduction != kNone || lse)
         hipLaunchKernelGGL(loss_total, dim3(1), dim3(1024), 0, a.st, c);

@@ -411,17 +411,19 @@ __global__ void __launch_bounds__(256) norm_wide_sums(const NormParams p)
     out[C + c] = db;
 }
 
-// dw and db from the workgroups' lines, in 64 bits: 16 columns by 16 parts of the
-// lines, the parts added in order.
+// dw and db from the workgroups' lines, in 64 bits: 16 columns by 64 parts of the
+// lines, the parts added in order.  (1,024 lines of 512: 20 us by 16 parts, whose loads
+// were waited for four times, 6 so.)
+constexpr int kJoinParts = 64;
 template <typename W>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(16 * kJoinParts)
 norm_join(const float* __restrict__ parts, int32_t lines, int32_t C, W* __restrict__ dw,
           W* __restrict__ db)
 {
-    __shared__ double lds[16][17];
+    __shared__ double lds[kJoinParts][17];
     const int col = threadIdx.x % 16, part = threadIdx.x / 16;
     const int64_t c = (int64_t)blockIdx.x * 16 + col, width = 2 * (int64_t)C;
-    const int32_t per = (lines + 15) / 16, first = part * per, end = min(lines, first + per);
+    const int32_t per = (lines + kJoinParts - 1) / kJoinParts, first = part * per, end = min(lines, first + per);
     double s = 0.0;
     if (c < width) {
         for (int32_t i = first; i < end; i += 16) {
@@ -437,7 +439,7 @@ norm_join(const float* __restrict__ parts, int32_t lines, int32_t C, W* __restri
     if (part == 0 && c < width) {
         double t = 0.0;
 #pragma unroll
-        for (int v = 0; v < 16; ++v) t += lds[v][col];
+        for (int v = 0; v < kJoinParts; ++v) t += lds[v][col];
         W* out = c < C ? dw : db;
         if (out) out[c < C ? c : c - C] = (W)(float)t;
     }
@@ -544,10 +546,10 @@ static void norm_backward(const NormParams& p, int32_t dtype, void* dw, void* db
     if (!p.parts) return;
     const dim3 join((unsigned)ceil_div(2 * (int64_t)p.C, 16));
     if (p.wide_weights)
-        hipLaunchKernelGGL((norm_join<float>), join, dim3(256), 0, st, p.parts, (int32_t)lines, p.C,
+        hipLaunchKernelGGL((norm_join<float>), join, dim3(16 * kJoinParts), 0, st, p.parts, (int32_t)lines, p.C,
                            static_cast<float*>(dw), static_cast<float*>(db));
     else
-        hipLaunchKernelGGL((norm_join<T>), join, dim3(256), 0, st, p.parts, (int32_t)lines, p.C,
+        hipLaunchKernelGGL((norm_join<T>), join, dim3(16 * kJoinParts), 0, st, p.parts, (int32_t)lines, p.C,
                            static_cast<T*>(dw), static_cast<T*>(db));
 }
 
