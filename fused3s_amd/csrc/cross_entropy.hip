@@ -229,6 +229,359 @@ __global__ void __launch_bounds__(256) loss_zero(T* __restrict__ out, int64_t co
     if (i < count) out[i] = (T)0.f;
 }
 
+// ---- few classes of few inputs: V <= 64, K <= 256, whole pieces ----
+//
+// There x's bytes bound the loss, not its products: W stays in LDS in operand order,
+// rows stream past it, a row's logits never leave the registers, and the backward pass
+// reads x once and writes dx once; dW is summed over a workgroup's rows in registers,
+// and the workgroups' sums in order by a second launch.  (200,003 x 128 -> 47 in
+// binary16, forward and backward pass by tiles: 34 and 103 us in 11 launches; so 13 and
+// 37 in five.)
+constexpr int kFewWaves = 8;
+constexpr int64_t kFewClasses = 64, kFewInputs = 256;
+
+struct FewParams {
+    const char *x, *w, *bias;
+    int64_t ldx;
+    const int64_t* target;
+    int64_t n, ignore;
+    int32_t K, V;
+    int32_t reduction;
+    float* loss;             // forward
+    float* lse;
+    double* parts;           // [workgroups][2]
+    const float* f;          // backward
+    const float* factor;
+    char* dx;                // [n][K] or NULL
+    float* dw;               // [slices][V][K] or NULL
+    float* db;               // [workgroups][V]
+};
+
+// W as the first products' operand: fragment f of class tile i, KF fragments a tile.
+template <typename T, int KF, int NV>
+__device__ __forceinline__ void few_weights(const FewParams& p, typename Half<T>::v8* to)
+{
+    for (int k = threadIdx.x; k < NV * KF * kWave; k += kFewWaves * kWave) {
+        const int l = k % kWave, f = k / kWave % KF, i = k / kWave / KF;
+        const int c = 16 * i + (l & 15), at = 32 * f + 8 * (l >> 4);
+        typename Half<T>::v8 v = {};
+        if (c < p.V && at < p.K)
+            v = *reinterpret_cast<const typename Half<T>::v8*>(
+                reinterpret_cast<const T*>(p.w) + (int64_t)c * p.K + at);
+        to[k] = v;
+    }
+}
+// 16 rows' fragments, dims 32 f + 8 g .. of row r (rows past the last: the last's).
+template <typename T, int KF>
+__device__ __forceinline__ void few_rows_of(const FewParams& p, int64_t first, int lane,
+                                            typename Half<T>::v8 (&x)[KF])
+{
+    const int g = lane >> 4, r = lane & 15;
+    const T* src = reinterpret_cast<const T*>(p.x) + min(first + r, p.n - 1) * p.ldx + 8 * g;
+#pragma unroll
+    for (int f = 0; f < KF; ++f) {
+        x[f] = typename Half<T>::v8{};
+        if (32 * f + 8 * g < p.K)
+            x[f] = *reinterpret_cast<const typename Half<T>::v8*>(src + 32 * f);
+    }
+}
+// Their logits: classes 16 i + 4 g + v of row r.
+template <typename T, int KF, int NV>
+__device__ __forceinline__ void few_logits(const typename Half<T>::v8 (&x)[KF],
+                                           const typename Half<T>::v8* w, const float* bias,
+                                           int lane, f4 (&z)[NV])
+{
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        z[i] = *reinterpret_cast<const f4*>(&bias[16 * i + 4 * (lane >> 4)]);
+#pragma unroll
+        for (int f = 0; f < KF; ++f) z[i] = Half<T>::mfma(w[(i * KF + f) * kWave + lane], x[f], z[i]);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void few_bias(const FewParams& p, float* to)
+{
+    for (int c = threadIdx.x; c < kFewClasses; c += kFewWaves * kWave)
+        to[c] = c >= p.V ? -INFINITY : p.bias ? (float)reinterpret_cast<const T*>(p.bias)[c] : 0.f;
+}
+
+template <typename T, int KF, int NV>
+__global__ void __launch_bounds__(kFewWaves * kWave) few_classes_fwd(const FewParams p)
+{
+    typedef typename Half<T>::v8 v8;
+    __shared__ __align__(16) v8 wl[NV * KF * kWave];
+    __shared__ __align__(16) float bl[kFewClasses];
+    __shared__ double sums[kFewWaves][2];
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    const int g = lane >> 4, r = lane & 15;
+    const int64_t step = (int64_t)gridDim.x * kFewWaves * 16;
+    int64_t first = ((int64_t)blockIdx.x * kFewWaves + wave) * 16;
+    v8 x[KF], next[KF];
+    int64_t t = 0, next_t = 0;
+    auto load = [&](int64_t at) __attribute__((always_inline)) {
+        few_rows_of<T, KF>(p, at, lane, next);
+        next_t = p.target[min(at + r, p.n - 1)];
+    };
+    load(first);
+    few_weights<T, KF, NV>(p, wl);
+    few_bias<T>(p, bl);
+    __syncthreads();
+    double loss = 0.0, counts = 0.0;
+    for (; first < p.n; first += step) {
+#pragma unroll
+        for (int f = 0; f < KF; ++f) x[f] = next[f];
+        t = next_t;
+        if (first + step < p.n) load(first + step);
+        f4 z[NV];
+        few_logits<T, KF, NV>(x, wl, bl, lane, z);
+        float top = -INFINITY, sum = 0.f, picked = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) top = __builtin_fmaxf(top, z[i][v]);
+        top = row_max4(top);
+        const float mu = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                sum += fast_exp2((z[i][v] - mu) * kLog2eF);
+                picked = t == 16 * i + 4 * g + v ? z[i][v] : picked;
+            }
+        sum += __shfl_xor(sum, 16, kWave);
+        sum += __shfl_xor(sum, 32, kWave);
+        // (the target's logit, from the lane that has it)
+        picked = __shfl(picked, (((int)t >> 2) & 3) * 16 + r, kWave);
+        const int64_t row = first + r;
+        if (g == 0 && row < p.n) {
+            const bool none = t == p.ignore;
+            const float l = 0.69314718f * __log2f(sum);
+            const float value = none ? 0.f : t < 0 || t >= p.V ? NAN : (top - picked) + l;
+            if (p.lse) p.lse[row] = top + l;
+            if (p.reduction == kNone) p.loss[row] = value;
+            loss += value;
+            counts += none ? 0.0 : 1.0;
+        }
+    }
+    loss = wave_sum(loss);
+    counts = wave_sum(counts);
+    if (lane == 0) {
+        sums[wave][0] = loss;
+        sums[wave][1] = counts;
+    }
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        double s = 0.0;
+        for (int k = 0; k < kFewWaves; ++k) s += sums[k][threadIdx.x];
+        p.parts[2 * (int64_t)blockIdx.x + threadIdx.x] = s;
+    }
+}
+
+// The operand of a product over rows from a stage of them: 16 columns from 16 t, rows
+// 4 g .. and 16 + 4 g .. of the 32 from `at` on.
+template <typename T>
+__device__ __forceinline__ typename Half<T>::v8 few_columns(const char* at, int stride, int t, int lane)
+{
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef short s8 __attribute__((ext_vector_type(8)));
+    typedef __attribute__((address_space(3))) s4* lds4;
+    const char* from = at + (4 * (lane >> 4) + ((lane & 15) >> 2)) * stride + 32 * t + 8 * (lane & 3);
+    const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)from);
+    const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(from + 16 * stride));
+    return __builtin_bit_cast(typename Half<T>::v8, s8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+}
+
+// 128 rows at a time, 16 a wave: z, dz and dx of a wave's own; then x and dz, through a
+// stage of all 128, for the wave's share of dW's dim tiles (with fewer tiles than waves,
+// of the rows too: a slice each).
+template <typename T, int KF, int NV>
+__global__ void __launch_bounds__(kFewWaves * kWave) few_classes_bwd(const FewParams p)
+{
+    typedef typename Half<T>::v8 v8;
+    typedef typename Half<T>::v4 v4;
+    constexpr int kTiles = 2 * KF, kFrags = (NV + 1) / 2;   // of dims; of classes, 32 each
+    constexpr int kOwn = kTiles >= kFewWaves ? kTiles / kFewWaves : 1;
+    constexpr int kSlices = kTiles >= kFewWaves ? 1 : kFewWaves / kTiles;
+    // (rows that begin 32 bytes apart modulo 256: eight of them read at once)
+    constexpr int kXRow = 64 * KF + 32, kDRow = 32 * NV + (NV > 1 ? 32 : 0);
+    __shared__ __align__(16) v8 wl[NV * KF * kWave];
+    __shared__ __align__(16) v8 wt[kTiles * kFrags * kWave];
+    __shared__ __align__(16) float bl[kFewClasses];
+    __shared__ __align__(16) char xs[kFewWaves * 16 * kXRow];
+    __shared__ __align__(16) char ds[kFewWaves * 16 * kDRow];
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    const int g = lane >> 4, r = lane & 15;
+    const int64_t step = (int64_t)gridDim.x * kFewWaves * 16;
+    int64_t first = (int64_t)blockIdx.x * kFewWaves * 16;   // (of the workgroup)
+    v8 x[KF], next[KF];
+    int64_t next_t = 0;
+    float next_f = 0.f, next_lse = 0.f;
+    auto load = [&](int64_t at) __attribute__((always_inline)) {
+        at += 16 * wave;
+        few_rows_of<T, KF>(p, at, lane, next);
+        const int64_t row = min(at + r, p.n - 1);
+        next_t = p.target[row];
+        next_f = at + r < p.n ? p.f[row] : 0.f;
+        next_lse = p.lse[row];
+    };
+    load(first);
+    few_weights<T, KF, NV>(p, wl);
+    few_bias<T>(p, bl);
+    // W transposed, the classes in the order in which a lane holds a row's dz
+    for (int k = threadIdx.x; k < kTiles * kFrags * kWave; k += kFewWaves * kWave) {
+        const int l = k % kWave, f = k / kWave % kFrags, dim = 16 * (k / kWave / kFrags) + (l & 15);
+        v8 v = {};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int c = 32 * f + slot_of(l >> 4, j);
+            if (c < p.V && dim < p.K) v[j] = reinterpret_cast<const T*>(p.w)[(int64_t)c * p.K + dim];
+        }
+        wt[k] = v;
+    }
+    __syncthreads();
+    const float factor = *p.factor;
+    f4 dw[kOwn][NV], db[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        db[i] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < kOwn; ++u) dw[u][i] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+    char* own_x = xs + wave * 16 * kXRow;
+    char* own_d = ds + wave * 16 * kDRow;
+    for (; first < p.n; first += step) {
+#pragma unroll
+        for (int f = 0; f < KF; ++f) x[f] = next[f];
+        const int64_t t = next_t;
+        const float f = next_f, lse = next_lse;
+        if (first + step < p.n) load(first + step);
+        f4 z[NV];
+        few_logits<T, KF, NV>(x, wl, bl, lane, z);
+        v8 dz[kFrags] = {};
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                float d = fast_exp2((z[i][v] - lse) * kLog2eF);
+                if (t == 16 * i + 4 * g + v) d -= 1.f;
+                d = f == 0.f ? 0.f : d * f;
+                if (NV * 16 > p.V && 16 * i + 4 * g + v >= p.V) d = 0.f;   // (f may be NaN)
+                db[i][v] += d;
+                dz[i / 2][4 * (i & 1) + v] = (T)d;
+            }
+        }
+        if (p.dw) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                *reinterpret_cast<v4*>(own_d + r * kDRow + 2 * (16 * i + 4 * g)) =
+                    (i & 1) ? __builtin_shufflevector(dz[i / 2], dz[i / 2], 4, 5, 6, 7)
+                            : __builtin_shufflevector(dz[i / 2], dz[i / 2], 0, 1, 2, 3);
+#pragma unroll
+            for (int k = 0; k < KF; ++k)   // (rows past the last: with dz of 0, and finite)
+                *reinterpret_cast<v8*>(own_x + r * kXRow + 64 * k + 16 * g) =
+                    first + 16 * wave + r < p.n ? x[k] : v8{};
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < kOwn; ++u) {
+                const int tile = kSlices > 1 ? wave % kTiles : wave + u * kFewWaves;
+                constexpr int kParts = kFewWaves / 2 / kSlices;   // of 32 rows
+#pragma unroll
+                for (int q = 0; q < kParts; ++q) {
+                    const int rows = 32 * ((kSlices > 1 ? wave / kTiles * kParts : 0) + q);
+                    const v8 b = few_columns<T>(xs + rows * kXRow, kXRow, tile, lane);
+#pragma unroll
+                    for (int i = 0; i < NV; ++i)
+                        dw[u][i] = Half<T>::mfma(few_columns<T>(ds + rows * kDRow, kDRow, i, lane), b,
+                                                 dw[u][i]);
+                }
+            }
+            __syncthreads();
+        }
+        if (p.dx) {
+            // dims 16 t + 4 g .. of row r, whole lines through the wave's part of the stage
+#pragma unroll
+            for (int tile = 0; tile < kTiles; ++tile) {
+                f4 d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < kFrags; ++k)
+                    d = Half<T>::mfma(wt[(tile * kFrags + k) * kWave + lane], dz[k], d);
+                *reinterpret_cast<v4*>(own_x + r * kXRow + 2 * (16 * tile + 4 * g)) =
+                    __builtin_convertvector(d * factor, v4);
+            }
+            wave_lds_order();
+            constexpr int kLanes = 4 * KF, kAtOnce = kWave / kLanes;   // per row; rows
+#pragma unroll
+            for (int v = 0; v < 16 / kAtOnce; ++v) {
+                const int rr = v * kAtOnce + lane / kLanes, piece = lane % kLanes;
+                const v8 y = *reinterpret_cast<const v8*>(own_x + rr * kXRow + 16 * piece);
+                const int64_t row = first + 16 * wave + rr;
+                if (row < p.n && 8 * piece < p.K)
+                    *reinterpret_cast<v8*>(reinterpret_cast<T*>(p.dx) + row * p.K + 8 * piece) = y;
+            }
+            wave_lds_order();
+        }
+    }
+    if (p.dw) {
+        const int64_t slice = (int64_t)blockIdx.x * kSlices + (kSlices > 1 ? wave / kTiles : 0);
+#pragma unroll
+        for (int u = 0; u < kOwn; ++u) {
+            const int dim = 16 * (kSlices > 1 ? wave % kTiles : wave + u * kFewWaves) + r;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const int c = 16 * i + 4 * g + v;
+                    if (c < p.V && dim < p.K) p.dw[(slice * p.V + c) * p.K + dim] = dw[u][i][v];
+                }
+        }
+    }
+    if (p.db) {
+        __syncthreads();
+        float* sums = reinterpret_cast<float*>(xs);   // [waves][classes]
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                float s = db[i][v];
+#pragma unroll
+                for (int off = 8; off >= 1; off >>= 1) s += __shfl_xor(s, off, kWave);
+                if (r == 0) sums[wave * kFewClasses + 16 * i + 4 * g + v] = s;
+            }
+        __syncthreads();
+        const int c = threadIdx.x;
+        if (c < p.V) {
+            float s = 0.f;
+            for (int k = 0; k < kFewWaves; ++k) s += sums[k * kFewClasses + c];
+            p.db[(int64_t)blockIdx.x * p.V + c] = s;
+        }
+    }
+}
+
+// dW and db from the slices, times the factor: 16 values by 16 parts of the slices.
+template <typename T>
+__global__ void __launch_bounds__(256)
+few_join(const float* __restrict__ dw, int64_t count, int32_t slices, T* __restrict__ out,
+         const float* __restrict__ db, int64_t classes, int32_t groups, T* __restrict__ out_db,
+         const float* __restrict__ factor)
+{
+    __shared__ float lds[16][17];
+    const int t = threadIdx.x % 16, part = threadIdx.x / 16;
+    const int64_t i = (int64_t)blockIdx.x * 16 + t;
+    const bool is_db = i >= count;
+    const int64_t at = is_db ? i - count : i, stride = is_db ? classes : count;
+    const int32_t many = is_db ? groups : slices, per = (many + 15) / 16;
+    const int32_t first = min(many, part * per), end = min(many, first + per);
+    float s = 0.f;
+    if (i < count + classes) s = split_sum((is_db ? db : dw) + at, stride, first, end);
+    lds[part][t] = s;
+    __syncthreads();
+    if (part || i >= count + classes) return;
+    for (int k = 1; k < 16; ++k) s += lds[k][t];
+    s *= *factor;
+    if (is_db) out_db[at] = (T)s;
+    else out[at] = (T)s;
+}
+
 __global__ void warm_loss_kernel() {}
 
 hipError_t warm_loss(hipStream_t s)
@@ -252,6 +605,54 @@ struct CeArgs {
 static Tiling one_split(int64_t rows, int64_t outs, int64_t depth, bool odd)
 {
     return tiling(rows, outs, depth, depth + 1, odd, false);
+}
+
+static bool takes_few(const CeArgs& a)
+{
+    return a.V <= kFewClasses && a.K <= kFewInputs && a.K % 8 == 0 && a.ldx % 8 == 0 &&
+           (((uintptr_t)a.X | (uintptr_t)a.W) & 15) == 0;
+}
+static int64_t few_groups(int64_t n, bool backward)
+{
+    return std::min<int64_t>(ceil_div(n, kFewWaves * 16), backward ? 256 : 512);
+}
+// Slices of dW: those of a workgroup times the workgroups.
+static int64_t few_slices(int64_t n, int64_t K)
+{
+    return few_groups(n, true) * (K <= 64 ? 2 : 1);
+}
+static FewParams few_params(const CeArgs& a)
+{
+    FewParams p{};
+    p.x = a.X;
+    p.w = a.W;
+    p.bias = a.bias;
+    p.ldx = a.ldx;
+    p.target = a.target;
+    p.n = a.n;
+    p.ignore = a.ignore;
+    p.K = (int32_t)a.K;
+    p.V = (int32_t)a.V;
+    p.reduction = a.reduction;
+    return p;
+}
+template <typename T, bool BACKWARD>
+static void launch_few(const FewParams& p, hipStream_t st)
+{
+    const dim3 grid((unsigned)few_groups(p.n, BACKWARD)), block(kFewWaves * kWave);
+    auto go = [&](auto kf, auto nv) {
+        constexpr int KF = decltype(kf)::value, NV = decltype(nv)::value;
+        if constexpr (BACKWARD) hipLaunchKernelGGL((few_classes_bwd<T, KF, NV>), grid, block, 0, st, p);
+        else hipLaunchKernelGGL((few_classes_fwd<T, KF, NV>), grid, block, 0, st, p);
+    };
+    auto of_k = [&](auto nv) {
+        if (p.K <= 64) go(std::integral_constant<int, 2>{}, nv);
+        else if (p.K <= 128) go(std::integral_constant<int, 4>{}, nv);
+        else go(std::integral_constant<int, 8>{}, nv);
+    };
+    if (p.V <= 16) of_k(std::integral_constant<int, 1>{});
+    else if (p.V <= 32) of_k(std::integral_constant<int, 2>{});
+    else of_k(std::integral_constant<int, 4>{});
 }
 
 // Workspace of a forward pass: the workgroups' sums, z at the targets, the blocks of as
@@ -296,6 +697,18 @@ static f3s_status loss_forward(const CeArgs& a, float* loss, float* lse, char* w
     const int join = most <= 16 && a.n >= 4096 ? 256 : a.n <= 2048 ? 4 : 16;
     c.nparts = ceil_div(a.n, join);
     c.reduction = a.reduction;
+    if (takes_few(a)) {
+        FewParams p = few_params(a);
+        p.loss = loss;
+        p.lse = lse;
+        p.parts = c.parts;
+        c.nparts = few_groups(a.n, false);
+        launch_few<T, false>(p, a.st);
+        if (a.reduction != kNone || lse)
+            hipLaunchKernelGGL(loss_total, dim3(1), dim3(1024), 0, a.st, c);
+        F3S_HIP(hipGetLastError());
+        return F3S_OK;
+    }
     for (int64_t r0 = 0; r0 < a.n; r0 += s.rows) {
         GemmParams p{};
         p.P = a.X + r0 * a.ldx * 2;
@@ -342,6 +755,7 @@ constexpr int64_t kLossShares = 64;   // of the rows' sums of db
 // piece's dz; dx's slices; a piece's splits of dW.
 struct CeSpace {
     size_t factor = 0, largest = 0, sums = 0, shares = 0, db = 0, dz = 0, dx = 0, dw = 0, bytes = 0;
+    size_t few_dw = 0, few_db = 0;   // (few classes)
     int64_t piece = 0, ldz = 0, sum_rows = 0;
     Tiling prob{}, tdx{}, tdw{};
     bool whole_dx = false;   // one piece, one split: dx is written at once
@@ -369,6 +783,11 @@ static CeSpace ce_space(int64_t n, int64_t K, int64_t V)
     s.dw = s.dx + (s.whole_dx ? 0 : up256(sizeof(float) * (size_t)s.tdx.splits * n * K));
     s.bytes = s.dw +
               (s.tdw.splits > 1 ? up256(sizeof(float) * (size_t)s.tdw.splits * s.piece * K) : 0);
+    if (V <= kFewClasses && K <= kFewInputs) {   // (alignment decides later: room for either)
+        s.few_dw = s.sums;
+        s.few_db = s.few_dw + up256(sizeof(float) * (size_t)few_slices(n, K) * V * K);
+        s.bytes = std::max(s.bytes, s.few_db + up256(sizeof(float) * (size_t)few_groups(n, true) * V));
+    }
     return s;
 }
 
@@ -413,6 +832,24 @@ static f3s_status loss_backward(const CeArgs& a, const float* lse, const float* 
     hipLaunchKernelGGL(loss_factors, dim3((unsigned)ceil_div(a.n, kLossThreads)), dim3(kLossThreads),
                        0, a.st, f);
     F3S_HIP(hipGetLastError());
+    if (takes_few(a)) {
+        FewParams p = few_params(a);
+        p.lse = const_cast<float*>(lse);
+        p.f = f.f;
+        p.factor = factor;
+        p.dx = dX;
+        p.dw = dW ? reinterpret_cast<float*>(ws + s.few_dw) : nullptr;
+        p.db = db ? reinterpret_cast<float*>(ws + s.few_db) : nullptr;
+        launch_few<T, true>(p, a.st);
+        const int64_t count = dW ? a.V * a.K : 0, classes = db ? a.V : 0;
+        if (count + classes > 0)
+            hipLaunchKernelGGL((few_join<T>), dim3((unsigned)ceil_div(count + classes, 16)), dim3(256),
+                               0, a.st, p.dw, count, (int32_t)few_slices(a.n, a.K),
+                               reinterpret_cast<T*>(dW), p.db, classes,
+                               (int32_t)few_groups(a.n, true), reinterpret_cast<T*>(db), factor);
+        F3S_HIP(hipGetLastError());
+        return F3S_OK;
+    }
     auto aligned = [](const void* x) { return ((uintptr_t)x & 15) == 0; };
     const bool w_pieces = a.K % 8 == 0 && a.K < (1 << 22) && aligned(a.W);
     const bool x_pieces = a.K % 8 == 0 && a.ldx % 8 == 0 && a.ldx < (1 << 22) && aligned(a.X);

@@ -12,7 +12,10 @@ pytestmark = pytest.mark.gpu
 HALF = [torch.float16, torch.bfloat16]
 SHAPES = [(1, 1, 1), (1, 8, 2), (3, 5, 3), (5, 16, 7), (17, 33, 10), (64, 64, 47), (65, 128, 300),
           (100, 100, 1000), (130, 72, 129), (257, 256, 2049), (2000, 64, 40), (513, 301, 777),
-          (300, 40, 20_000), (1, 512, 5000), (4100, 128, 4099), (20_011, 24, 3)]
+          (300, 40, 20_000), (1, 512, 5000), (4100, 128, 4099), (20_011, 24, 3),
+          # few classes of few inputs, 2 to 8 fragments by 1 to 4 tiles
+          (3000, 256, 64), (1000, 136, 33), (257, 128, 17), (40_000, 40, 64), (130, 200, 16),
+          (127, 64, 32), (129, 8, 64), (5000, 104, 48)]
 
 
 def inputs(n, K, V, dtype, seed, bias=True, ignored=0.2, reduction="mean"):
