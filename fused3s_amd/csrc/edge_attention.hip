@@ -1052,7 +1052,7 @@ static EdgeParams edge_params(int32_t n, float scale, float cap, const float* po
     p.scale = scale;
     p.scale_log2 = scale * kLog2e;
     p.cap = cap;
-    p.cap_in = cap > 0.f ? scale / cap : 0.f;
+    p.cap_in = cap > 0.f ? std::clamp(scale / cap, -FLT_MAX, FLT_MAX) : 0.f;   // (0 x inf)
     p.cap_log2 = cap * kLog2e;
     p.positions = positions;
     p.dims = dims;

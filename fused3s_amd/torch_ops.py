@@ -8,8 +8,10 @@ memory and the stream; the attention is the HIP library's planned pass
 tensors' device pointers, and the layer's projections are its f3s_linear_f16
 (torch.nn.Linear's own product where that kernel is not the better one).  There
 is no CPU fallback, and that pass is forward-only: calling it on tensors that require grad raises.
-Differential attention (two softmax maps per head and their difference) and
-linear(), a projection with bias, activation and residual, have gradients.
+Differential attention (two softmax maps per head and their difference), edge
+attention (one map, scores capped and lowered by distance), linear(), a projection
+with bias, activation and residual, layer_norm() and linear_cross_entropy(), a
+classifier's loss without its logits, have gradients.
 
     graph = TorchGraph(row_ptr, col_idx, heads=4)      # convert + plan + compile once
     o = graph.attention(q, k, v)                       # q/k/v [n, H, 64] fp16 -> fp32
@@ -19,6 +21,11 @@ linear(), a projection with bias, activation and residual, have gradients.
     o = graph.diff_attention(q, k, v, lam)             # q/k/v [n, H, 128] fp16 or bf16, autograd
     y = linear(x, weight, bias, "gelu", residual)      # autograd
     layer = DiffGraphTransformerLayer(in_dim, heads=4, ffn_dim=512).cuda().bfloat16()
+
+    o = graph.edge_attention(q, k, v, 0.125, cap=30.0, positions=t, slopes=s)   # [n, H, 64]
+    y = layer_norm(x, weight, bias)                    # float16, bfloat16 or float32
+    loss = linear_cross_entropy(x, weight, classes)    # mean of the rows' losses
+    layer = EdgeGraphTransformerLayer(in_dim, heads=4, ffn_dim=512, distance=True)
 
 The drop-in launch is also a registered torch operator, on the block-sparse
 form held in torch tensors (no plan, no state between calls):
@@ -954,16 +961,19 @@ def _watched() -> bool:
             or c._functorch.peek_interpreter_stack() is not None or torch.jit.is_tracing())
 
 
+def _has_no_hooks(m: torch.nn.Module) -> bool:
+    hooks = torch.nn.modules.module
+    return not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks
+                or m._backward_pre_hooks or hooks._global_forward_hooks
+                or hooks._global_forward_pre_hooks or hooks._global_backward_hooks
+                or hooks._global_backward_pre_hooks)
+
+
 def _is_plain_linear(m: torch.nn.Module) -> bool:
     """A torch.nn.Linear whose call is its product and nothing else."""
-    hooks = torch.nn.modules.module
     return (type(m) is torch.nn.Linear and "forward" not in m.__dict__
             and torch.nn.Linear.forward is _LINEAR_FORWARD
-            and torch.nn.functional.linear is _LINEAR
-            and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks
-                     or m._backward_pre_hooks or hooks._global_forward_hooks
-                     or hooks._global_forward_pre_hooks or hooks._global_backward_hooks
-                     or hooks._global_backward_pre_hooks))
+            and torch.nn.functional.linear is _LINEAR and _has_no_hooks(m))
 
 
 def _project(m: torch.nn.Module, x: torch.Tensor, watched: bool) -> torch.Tensor:
@@ -1115,6 +1125,73 @@ class DiffGraphTransformerLayer(torch.nn.Module):
                    x if self.residual else None)
         if self.up is not None:
             y = _dense(self.down, _dense(self.up, y, watched, self.activation), watched, None, y)
+        return y
+
+
+_NORM_FORWARD, _NORM = torch.nn.LayerNorm.forward, torch.nn.functional.layer_norm
+
+
+def _norm(m: torch.nn.Module, x: torch.Tensor, watched: bool) -> torch.Tensor:
+    """m(x): layer_norm() where m is a plain LayerNorm of plain tensors of types that it
+    takes and nothing watches the call, else torch's own."""
+    if (not watched and type(m) is torch.nn.LayerNorm and "forward" not in m.__dict__
+            and torch.nn.LayerNorm.forward is _NORM_FORWARD
+            and torch.nn.functional.layer_norm is _NORM and _has_no_hooks(m)
+            and len(m.normalized_shape) == 1 and x.dim() >= 1
+            and x.shape[-1] == m.normalized_shape[0] and type(x) is torch.Tensor and x.is_cuda
+            and x.dtype in _NORM_DTYPES and type(m.weight) in _PLAIN and type(m.bias) in _PLAIN
+            and all(t is None or t.dtype in (x.dtype, torch.float32) and t.device == x.device
+                    for t in (m.weight, m.bias))
+            and (m.weight is None or m.bias is None or m.weight.dtype == m.bias.dtype)):
+        return layer_norm(x, m.weight, m.bias, m.eps)
+    return m(x)
+
+
+class EdgeGraphTransformerLayer(torch.nn.Module):
+    """A pre-norm layer of softmax attention over a graph's edges, optionally with a
+    feed-forward part; trainable.
+
+        h = edge_attention(norm1(x) W_qkv) W_o + x
+        y = activation(norm2(h) W_up) W_down + h      (ffn_dim given)
+
+    cap: scores are capped to cap * tanh(score / cap).  distance: scores are lowered by
+    slopes[h] times the distance of the two nodes' `positions` ([n] or [n, 1 to 3]
+    float32, given to the call), slopes learned, 1/2, 1/4, .. at first.  `heads` heads
+    of 64 dims; the graph has to be made for `heads` heads.  Computes in the module's
+    type (float16 or bfloat16; a float32 module's attention runs in float16)."""
+
+    def __init__(self, in_dim: int, heads: int = 1, bias: bool = True, ffn_dim: int | None = None,
+                 activation: str = "gelu", cap: float | None = None, distance: bool = False,
+                 eps: float = 1e-5):
+        super().__init__()
+        if activation not in _ACTIVATIONS:
+            raise ValueError(f"activation must be one of {list(_ACTIVATIONS)}")
+        self.heads, self.activation, self.cap, self.scale = heads, activation, cap, HEAD_DIM ** -0.5
+        self.norm1 = torch.nn.LayerNorm(in_dim, eps=eps)
+        self.qkv = torch.nn.Linear(in_dim, 3 * heads * HEAD_DIM, bias=bias)
+        self.proj = torch.nn.Linear(heads * HEAD_DIM, in_dim, bias=bias)
+        self.slopes = (torch.nn.Parameter(0.5 ** torch.arange(1, heads + 1).float())
+                       if distance else None)
+        self.norm2 = torch.nn.LayerNorm(in_dim, eps=eps) if ffn_dim else None
+        self.up = torch.nn.Linear(in_dim, ffn_dim, bias=bias) if ffn_dim else None
+        self.down = torch.nn.Linear(ffn_dim, in_dim, bias=bias) if ffn_dim else None
+
+    def forward(self, x: torch.Tensor, graph: TorchGraph,
+                positions: torch.Tensor | None = None) -> torch.Tensor:
+        if graph.heads != self.heads:
+            raise ValueError("graph was planned for a different head count")
+        if (positions is None) != (self.slopes is None):
+            raise ValueError("positions are for a layer made with distance=True")
+        watched = _watched()
+        qkv = _dense(self.qkv, _norm(self.norm1, x, watched), watched)
+        if qkv.dtype not in _DTYPES:
+            qkv = qkv.to(torch.float16)
+        o = graph.edge_attention_packed(qkv, self.scale, self.cap, positions,
+                                        None if self.slopes is None else self.slopes.float())
+        y = _dense(self.proj, o.view(x.shape[0], -1).to(self.proj.weight.dtype), watched, None, x)
+        if self.up is not None:
+            z = _dense(self.up, _norm(self.norm2, y, watched), watched, self.activation)
+            y = _dense(self.down, z, watched, None, y)
         return y
 
 
