@@ -48,7 +48,7 @@ struct CeParams {
 };
 
 // A row's blocks joined: ROWS rows by the other threads' parts of the blocks, in a fixed
-// order.  (64 rows of 1,564 blocks, 16 rows a workgroup: 16 us, four: 6; 200,003 rows of
+// order.  (64 rows of 1,564 blocks, 16 rows a workgroup: 16 us, four: 8; 200,003 rows of
 // two blocks, 16: 15, 256: 5.)
 template <int ROWS>
 __global__ void __launch_bounds__(kLossThreads) loss_join(const CeParams p)
@@ -229,14 +229,377 @@ __global__ void __launch_bounds__(256) loss_zero(T* __restrict__ out, int64_t co
     if (i < count) out[i] = (T)0.f;
 }
 
+// ---- log-sum-exps of few inputs: K <= 256, whole pieces ----
+//
+// There a tile's products are short beside its epilogue, which nothing overlaps.  So a
+// wave keeps 32 rows of x in registers and the classes stream past it, 64 at a time,
+// through LDS, the next ones on their way; several workgroups share a CU.  A lane keeps
+// the largest logit and the sum of its own classes: nothing crosses lanes before the
+// end, and a row leaves one block for each share of the classes (blockIdx.y), not one
+// for each 64.  Bound by the logits' 7 operations each, one exponential among them.
+// (52,802 x 64 -> 10,778 by tiles 411 us a call, 196 so; 200,003 x
+// 128 -> 300 70 and 42; 16,384 x 256 -> 50,021 743 and 447.)
+constexpr int kStreamWaves = 4, kStreamTiles = 2, kStreamRows = 16 * kStreamTiles * kStreamWaves;
+struct StreamParams {
+    const char *x, *w, *bias;
+    int64_t ldx, rows, V;
+    int32_t K;
+    int64_t per;             // chunks of 64 classes in a share
+    const int64_t* target;
+    float2* blocks;          // [shares][rows]
+    float* picked;           // [rows]
+};
+template <typename T, int KS>
+__global__ void __launch_bounds__(kStreamWaves * kWave) stream_lse_kernel(const StreamParams p)
+{
+    typedef typename Half<T>::v8 v8;
+    constexpr int kChunkBytes = 64 * kStep * 2;   // 64 classes by 64 inputs
+    __shared__ __align__(256) char wl[2][KS * kChunkBytes];
+    __shared__ __align__(16) float bl[2][64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int lane = threadIdx.x % kWave;
+    const int g = lane >> 4, r = lane & 15;
+    const int64_t first = (int64_t)blockIdx.x * kStreamRows + wave * 16 * kStreamTiles;
+    const int64_t chunks = (p.V + 63) / 64, begin = blockIdx.y * p.per,
+                  end = min(chunks, begin + p.per);
+    typedef TileAt<false, 64, kStreamWaves> At;
+    float next_bias = 0.f;
+    auto load = [&](int64_t c, int buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+            load_tile(At(p.w, p.K, 64 * c, p.V, kStep * k, p.K), p.K, wl[buf] + k * kChunkBytes, wave,
+                      lane);
+        const int64_t at = 64 * c + threadIdx.x;
+        if (threadIdx.x < 64)
+            next_bias = at >= p.V ? -INFINITY
+                        : p.bias  ? (float)reinterpret_cast<const T*>(p.bias)[at]
+                                  : 0.f;
+    };
+    if (begin < end) load(begin, 0);
+    v8 x[kStreamTiles][2 * KS];
+    int64_t t[kStreamTiles];
+    float m[kStreamTiles], s[kStreamTiles];
+#pragma unroll
+    for (int u = 0; u < kStreamTiles; ++u) {
+        const int64_t row = min(first + 16 * u + r, p.rows - 1);
+        const T* src = reinterpret_cast<const T*>(p.x) + row * p.ldx + 8 * g;
+        t[u] = p.target[row];
+        m[u] = -INFINITY;
+        s[u] = 0.f;
+#pragma unroll
+        for (int f = 0; f < 2 * KS; ++f) {
+            x[u][f] = v8{};
+            if (32 * f + 8 * g < p.K) x[u][f] = *reinterpret_cast<const v8*>(src + 32 * f);
+        }
+    }
+    int buf = 0;
+    for (int64_t c = begin; c < end; ++c, buf ^= 1) {
+        // (loads into LDS are waited for by hand: the barrier does not)
+        __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
+        if (threadIdx.x < 64) bl[buf][threadIdx.x] = next_bias;
+        __syncthreads();
+        if (c + 1 < end) load(c + 1, buf ^ 1);
+        f4 z[4][kStreamTiles];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int u = 0; u < kStreamTiles; ++u)
+                z[i][u] = *reinterpret_cast<const f4*>(&bl[buf][16 * i + 4 * g]);
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int f = 0; f < 2; ++f)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const v8 a = fragment<T, false, 64>(wl[buf] + k * kChunkBytes, i, f, lane);
+#pragma unroll
+                    for (int u = 0; u < kStreamTiles; ++u)
+                        z[i][u] = Half<T>::mfma(a, x[u][2 * k + f], z[i][u]);
+                }
+#pragma unroll
+        for (int u = 0; u < kStreamTiles; ++u) {
+            float top = m[u];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) top = __builtin_fmaxf(top, z[i][u][v]);
+            const float mu = top == -INFINITY ? 0.f : top;
+            float sum = s[u] * fast_exp2((m[u] - mu) * kLog2eF);
+            if (top < -1e38f) {   // (times log2(e) it has none)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) sum += fast_exp2((z[i][u][v] - mu) * kLog2eF);
+            } else {
+                const float mul = mu * kLog2eF;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v)
+                        sum += fast_exp2(__builtin_fmaf(z[i][u][v], kLog2eF, -mul));
+            }
+            s[u] = sum;
+            m[u] = top;
+            const int64_t at = t[u] - 64 * c;
+            if (__ballot(at >= 0 && at < 64)) {
+                float picked = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) picked = at == 16 * i + 4 * g + v ? z[i][u][v] : picked;
+                const int64_t row = first + 16 * u + r;
+                if (at >= 0 && at < 64 && t[u] < p.V && ((at >> 2) & 3) == g && row < p.rows)
+                    p.picked[row] = picked;
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kStreamTiles; ++u) {
+        const float top = row_max4(m[u]);
+        float sum = s[u] * fast_exp2((m[u] - (top == -INFINITY ? 0.f : top)) * kLog2eF);
+        sum += __shfl_xor(sum, 16, kWave);
+        sum += __shfl_xor(sum, 32, kWave);
+        const int64_t row = first + 16 * u + r;
+        if (g == 0 && row < p.rows)
+            p.blocks[(int64_t)blockIdx.y * p.rows + row] = make_float2(top, sum);
+    }
+}
+
+// ---- their gradients: K <= 128, whole pieces ----
+//
+// dz never leaves the registers: two passes of one shape, each with the logits again.
+// A wave keeps 32 rows of its own, the others stream past it, 64 at a time:
+//   dx      its rows are x's, W's stream past: dx += dz W
+//   dW, db  its rows are W's, x's stream past: dW += dz^T x
+// A lane's logits of a row are the operand of the product after them, whose other one is
+// the same rows in LDS, read transposed.  Shares of the streamed rows (blockIdx.y) are
+// added by join_scaled.  One product of five more than by tiles, and none of dz's bytes
+// (52,802 x 64 -> 10,778 trained by tiles 1,324 us, most of it dz in and out; so 744;
+// 200,003 x 128 -> 300 237 and 207.)
+struct GradParams {
+    const char *own, *other;
+    int64_t ld_own, ld_other, owns, others;
+    int32_t K;
+    int64_t per;             // chunks of 64 of the others in a share
+    const char* bias;
+    const int64_t* target;   // of x's rows
+    const float *lse, *f;
+    const float* factor;
+    char* out;               // [owns][K] in the type, times the factor: one share; else
+    float* slices;           // [shares][owns][K]
+    float* sums;             // db: [shares][owns] (NULL: not wanted)
+};
+__device__ __forceinline__ int place_both(int row) { return (row & 6) | ((row >> 3) & 1); }
+template <typename T, int KS, bool CLASSES>
+__global__ void __launch_bounds__(kStreamWaves * kWave) __attribute__((amdgpu_waves_per_eu(2)))
+stream_grad_kernel(const GradParams p)
+{
+    typedef typename Half<T>::v8 v8;
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef short s8 __attribute__((ext_vector_type(8)));
+    typedef __attribute__((address_space(3))) s4* lds4;
+    constexpr int kBytes = 64 * kStep * 2, kDims = 4 * KS;   // 64 rows by 64 inputs; tiles of dims
+    __shared__ __align__(256) char rows[2][KS * kBytes];
+    __shared__ __align__(16) float at1[2][64], at2[2][64];    // bias; lse and f
+    __shared__ __align__(16) int32_t at3[2][64];              // (CLASSES) targets, of the wave's classes
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int lane = threadIdx.x % kWave;
+    const int g = lane >> 4, r = lane & 15;
+    const int64_t block0 = (int64_t)blockIdx.x * kStreamRows, first = block0 + wave * 16 * kStreamTiles;
+    const int64_t chunks = (p.others + 63) / 64, begin = blockIdx.y * p.per,
+                  end = min(chunks, begin + p.per);
+    float next1 = 0.f, next2 = 0.f;
+    int32_t next3 = -1;
+    auto load = [&](int64_t c, int buf) __attribute__((always_inline)) {
+        const __amdgpu_buffer_rsrc_t rs =
+            make_rsrc(p.other + 64 * c * p.ld_other * 2, 0x7fffffffu);
+        const int64_t left = p.others - 64 * c;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {   // 1,024 bytes a wave and load, eight rows
+                const int part = i * kStreamWaves + wave, row = part * 8 + lane / 8;
+                const int piece = (lane % 8) ^ place_both(row);
+                const bool in = row < left && kStep * k + 8 * piece < p.K;
+                const uint32_t at =
+                    in ? (uint32_t)(row * (int32_t)p.ld_other + kStep * k + 8 * piece) * 2 : 0xffffff00u;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    rs, (__attribute__((address_space(3))) void*)(rows[buf] + k * kBytes + part * 1024),
+                    16, (int)at, 0, 0, 0);
+            }
+        const int64_t at = 64 * c + threadIdx.x;
+        if (threadIdx.x < 64) {
+            if constexpr (CLASSES) {
+                const bool in = at < p.others;
+                next1 = in ? p.lse[at] : 0.f;
+                next2 = in ? p.f[at] : 0.f;
+                const int64_t t = in ? p.target[at] - block0 : -1;
+                next3 = t >= 0 && t < kStreamRows ? (int32_t)t : -1;
+            } else {
+                next1 = at >= p.others ? -INFINITY
+                        : p.bias       ? (float)reinterpret_cast<const T*>(p.bias)[at]
+                                       : 0.f;
+            }
+        }
+    };
+    if (begin < end) load(begin, 0);
+    v8 own[kStreamTiles][2 * KS];
+    float own1[kStreamTiles], own2[kStreamTiles], sum[kStreamTiles];   // lse, f; bias
+    int64_t t[kStreamTiles];
+    f4 acc[kStreamTiles][kDims];
+#pragma unroll
+    for (int u = 0; u < kStreamTiles; ++u) {
+        const int64_t row = min(first + 16 * u + r, p.owns - 1);
+        const T* src = reinterpret_cast<const T*>(p.own) + row * p.ld_own + 8 * g;
+#pragma unroll
+        for (int f = 0; f < 2 * KS; ++f) {
+            own[u][f] = v8{};
+            if (32 * f + 8 * g < p.K) own[u][f] = *reinterpret_cast<const v8*>(src + 32 * f);
+        }
+        if constexpr (CLASSES) {
+            own1[u] = p.bias ? (float)reinterpret_cast<const T*>(p.bias)[row] : 0.f;
+        } else {
+            own1[u] = p.lse[row];
+            own2[u] = p.f[row];
+            t[u] = p.target[row];
+        }
+        sum[u] = 0.f;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) acc[u][d] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+    int buf = 0;
+    for (int64_t c = begin; c < end; ++c, buf ^= 1) {
+        // (loads into LDS are waited for by hand: the barrier does not)
+        __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
+        if (threadIdx.x < 64) {
+            at1[buf][threadIdx.x] = next1;
+            if constexpr (CLASSES) {
+                at2[buf][threadIdx.x] = next2;
+                at3[buf][threadIdx.x] = next3;
+            }
+        }
+        __syncthreads();
+        if (c + 1 < end) load(c + 1, buf ^ 1);
+        // logits of the chunk's rows 16 i + 4 g + v and own row r
+        f4 z[4][kStreamTiles];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int u = 0; u < kStreamTiles; ++u)
+                z[i][u] = CLASSES ? f4{own1[u], own1[u], own1[u], own1[u]}
+                                  : *reinterpret_cast<const f4*>(&at1[buf][16 * i + 4 * g]);
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int f = 0; f < 2; ++f)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const v8 a = *reinterpret_cast<const v8*>(
+                        rows[buf] + k * kBytes + (16 * i + r) * 128 +
+                        16 * ((4 * f + g) ^ place_both(r)));
+#pragma unroll
+                    for (int u = 0; u < kStreamTiles; ++u)
+                        z[i][u] = Half<T>::mfma(a, own[u][2 * k + f], z[i][u]);
+                }
+        // dz in their place
+        uint64_t hits = 0;   // (CLASSES) whether a target is among the wave's classes
+        if constexpr (CLASSES) {
+            const int32_t at = at3[buf][lane];
+            hits = __ballot(at >= 0 && at / (16 * kStreamTiles) == wave);
+        }
+#pragma unroll
+        for (int u = 0; u < kStreamTiles; ++u) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f4 lse, f;
+                if constexpr (CLASSES) {
+                    lse = *reinterpret_cast<const f4*>(&at1[buf][16 * i + 4 * g]);
+                    f = *reinterpret_cast<const f4*>(&at2[buf][16 * i + 4 * g]);
+                } else {
+                    lse = f4{own1[u], own1[u], own1[u], own1[u]};
+                    f = f4{own2[u], own2[u], own2[u], own2[u]};
+                }
+#pragma unroll
+                for (int v = 0; v < 4; ++v) z[i][u][v] = fast_exp2((z[i][u][v] - lse[v]) * kLog2eF);
+                if constexpr (CLASSES) {
+                    if (hits) {
+                        const u4 at = *reinterpret_cast<const u4*>(&at3[buf][16 * i + 4 * g]);
+#pragma unroll
+                        for (int v = 0; v < 4; ++v)
+                            z[i][u][v] -= (int)at[v] == (wave * kStreamTiles + u) * 16 + r ? 1.f : 0.f;
+                    }
+                } else {
+                    const int64_t at = t[u] - 64 * c - 16 * i - 4 * g;
+                    if (__ballot(at >= 0 && at < 4)) {
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) z[i][u][v] -= at == v ? 1.f : 0.f;
+                    }
+                }
+                // (0 where f is, whatever z)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) z[i][u][v] = f[v] == 0.f ? 0.f : z[i][u][v] * f[v];
+                if constexpr (CLASSES) sum[u] += (z[i][u][0] + z[i][u][1]) + (z[i][u][2] + z[i][u][3]);
+            }
+        }
+        // times the chunk's rows: their 16 dims from 16 d, rows 32 q + slot_of(g, j)
+        v8 dz[2][kStreamTiles];
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int u = 0; u < kStreamTiles; ++u)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) dz[q][u][j] = (T)z[2 * q + j / 4][u][j % 4];
+#pragma unroll
+        for (int d = 0; d < kDims; ++d)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int row = 32 * q + 4 * g + (r >> 2), at = 2 * (d % 4) + ((r & 3) >> 1);
+                const char* from = rows[buf] + d / 4 * kBytes + row * 128 + 16 * (at ^ place_both(row)) +
+                                   8 * (r & 1);
+                const char* more = rows[buf] + d / 4 * kBytes + (row + 16) * 128 +
+                                   16 * (at ^ place_both(row + 16)) + 8 * (r & 1);
+                const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)from);
+                const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)more);
+                const v8 x = __builtin_bit_cast(v8, s8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+#pragma unroll
+                for (int u = 0; u < kStreamTiles; ++u) acc[u][d] = Half<T>::mfma(x, dz[q][u], acc[u][d]);
+            }
+    }
+    // dims 16 d + 4 g .. of own row r
+    const float factor = p.out ? *p.factor : 1.f;
+#pragma unroll
+    for (int u = 0; u < kStreamTiles; ++u) {
+        const int64_t row = first + 16 * u + r;
+        if (CLASSES && p.sums) {
+            float s = sum[u] + __shfl_xor(sum[u], 16, kWave);
+            s += __shfl_xor(s, 32, kWave);
+            if (g == 0 && row < p.owns) p.sums[blockIdx.y * p.owns + row] = s;
+        }
+        if (row >= p.owns) continue;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) {
+            const int dim = 16 * d + 4 * g;   // (K is a multiple of 8)
+            if (dim >= p.K) continue;
+            if (p.out) {
+                typedef typename Half<T>::v4 v4;
+                struct __attribute__((packed, aligned(2))) Any { v4 v; };
+                reinterpret_cast<Any*>(reinterpret_cast<T*>(p.out) + row * p.K + dim)->v =
+                    __builtin_convertvector(acc[u][d] * factor, v4);
+            } else if (p.slices) {
+                *reinterpret_cast<f4*>(p.slices + (blockIdx.y * p.owns + row) * p.K + dim) = acc[u][d];
+            }
+        }
+    }
+}
+
 // ---- few classes of few inputs: V <= 64, K <= 256, whole pieces ----
 //
 // There x's bytes bound the loss, not its products: W stays in LDS in operand order,
 // rows stream past it, a row's logits never leave the registers, and the backward pass
 // reads x once and writes dx once; dW is summed over a workgroup's rows in registers,
 // and the workgroups' sums in order by a second launch.  (200,003 x 128 -> 47 in
-// binary16, forward and backward pass by tiles: 34 and 103 us in 11 launches; so 13 and
-// 37 in five.)
+// binary16, forward and backward pass by tiles: 33 and 91 us of kernels in 11 launches;
+// so 22 and 42 in five.)
 constexpr int kFewWaves = 8;
 constexpr int64_t kFewClasses = 64, kFewInputs = 256;
 
@@ -673,6 +1036,55 @@ static ForwardSpace forward_space(int64_t n, int64_t V)
     return s;
 }
 
+// (whole pieces, as few classes take; one row's pieces per 64 inputs in a tile)
+static bool takes_stream(const CeArgs& a)
+{
+    return a.K <= kFewInputs && a.K % 8 == 0 && a.ldx % 8 == 0 && a.ldx < (1 << 22) &&
+           (((uintptr_t)a.X | (uintptr_t)a.W) & 15) == 0;
+}
+constexpr int64_t kStreamGroups = 1024;   // four per CU
+template <typename T>
+static void launch_stream(const CeArgs& a, const GemmParams& g, int64_t per, int64_t shares)
+{
+    StreamParams p{};
+    p.x = g.P;
+    p.w = a.W;
+    p.bias = a.bias;
+    p.ldx = a.ldx;
+    p.rows = g.rows;
+    p.V = a.V;
+    p.K = (int32_t)a.K;
+    p.per = per;
+    p.target = g.loss.target;
+    p.blocks = g.loss.blocks;
+    p.picked = g.loss.picked;
+    const dim3 grid((unsigned)ceil_div(p.rows, kStreamRows), (unsigned)shares),
+        block(kStreamWaves * kWave);
+    if (a.K <= 64) hipLaunchKernelGGL((stream_lse_kernel<T, 1>), grid, block, 0, a.st, p);
+    else if (a.K <= 128) hipLaunchKernelGGL((stream_lse_kernel<T, 2>), grid, block, 0, a.st, p);
+    else hipLaunchKernelGGL((stream_lse_kernel<T, 4>), grid, block, 0, a.st, p);
+}
+
+// Gradients so: shares of the streamed rows, as many as fill the chip.
+constexpr int64_t kGradInputs = 128, kGradGroups = 1024;
+static int64_t grad_per(int64_t owns, int64_t others)
+{
+    const int64_t chunks = ceil_div(others, 64), groups = ceil_div(owns, kStreamRows);
+    return ceil_div(chunks, std::min(chunks, std::max<int64_t>(1, kGradGroups / groups)));
+}
+static int64_t grad_shares(int64_t owns, int64_t others)
+{
+    return ceil_div(ceil_div(others, 64), grad_per(owns, others));
+}
+template <typename T, bool CLASSES>
+static void launch_grad(const GradParams& p, hipStream_t st)
+{
+    const dim3 grid((unsigned)ceil_div(p.owns, kStreamRows), (unsigned)grad_shares(p.owns, p.others)),
+        block(kStreamWaves * kWave);
+    if (p.K <= 64) hipLaunchKernelGGL((stream_grad_kernel<T, 1, CLASSES>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((stream_grad_kernel<T, 2, CLASSES>), grid, block, 0, st, p);
+}
+
 static int32_t blocks_of(int32_t tile, int64_t outs)
 {
     return (int32_t)(ceil_div(outs, tile) * (tile == 256 ? 4 : 2));
@@ -692,10 +1104,6 @@ static f3s_status loss_forward(const CeArgs& a, float* loss, float* lse, char* w
     c.lse = lse;
     c.loss = loss;
     c.parts = reinterpret_cast<double*>(ws);
-    // (rows per workgroup of a join; the rows of a piece are a multiple of 1,024)
-    const int64_t most = ceil_div(a.V, 64);
-    const int join = most <= 16 && a.n >= 4096 ? 256 : a.n <= 2048 ? 4 : 16;
-    c.nparts = ceil_div(a.n, join);
     c.reduction = a.reduction;
     if (takes_few(a)) {
         FewParams p = few_params(a);
@@ -709,6 +1117,20 @@ static f3s_status loss_forward(const CeArgs& a, float* loss, float* lse, char* w
         F3S_HIP(hipGetLastError());
         return F3S_OK;
     }
+    const bool stream = takes_stream(a);
+    int64_t per = 0;
+    if (stream) {
+        const int64_t chunks = ceil_div(a.V, 64), groups = ceil_div(std::min(s.rows, a.n), kStreamRows);
+        const int64_t at_once = a.K <= 128 ? kStreamGroups : kStreamGroups / 2;   // (by their LDS)
+        const int64_t shares = std::min(chunks, std::max<int64_t>(1, at_once / groups));
+        per = ceil_div(chunks, shares);
+        c.nblocks = ceil_div(chunks, per);
+    } else {
+        c.nblocks = ceil_div(a.V, 64);   // (or twice as many)
+    }
+    // Rows per workgroup of a join; the rows of a piece are a multiple of 1,024.
+    const int join = c.nblocks <= 16 && a.n >= 4096 ? 256 : a.n <= 2048 ? 4 : 16;
+    c.nparts = ceil_div(a.n, join);
     for (int64_t r0 = 0; r0 < a.n; r0 += s.rows) {
         GemmParams p{};
         p.P = a.X + r0 * a.ldx * 2;
@@ -722,6 +1144,9 @@ static f3s_status loss_forward(const CeArgs& a, float* loss, float* lse, char* w
         p.loss.target = a.target + r0;
         p.loss.blocks = reinterpret_cast<float2*>(ws + s.blocks);
         p.loss.picked = reinterpret_cast<float*>(ws + s.picked);
+        if (stream) {
+            launch_stream<T>(a, p, per, c.nblocks);
+        } else {
         const Tiling t = one_split(p.rows, p.outs, p.depth, a.K % 8 != 0);
         GemmParams q = p;   // (C is not written, and nothing of bias is read in pieces)
         q.bias = nullptr;
@@ -733,8 +1158,9 @@ static f3s_status loss_forward(const CeArgs& a, float* loss, float* lse, char* w
         p.splits = 1;
         if (way == kWhole) launch_tiles<T, false, false, kEpiLse, kWhole>(p, tile, a.st);
         else launch_tiles<T, false, false, kEpiLse, kAny>(p, tile, a.st);
-        F3S_HIP(hipGetLastError());
         c.nblocks = blocks_of(tile, p.outs);
+        }
+        F3S_HIP(hipGetLastError());
         c.rows = p.rows;
         c.first_row = r0;
         const dim3 grid((unsigned)ceil_div(p.rows, join));
@@ -760,6 +1186,20 @@ struct CeSpace {
     Tiling prob{}, tdx{}, tdw{};
     bool whole_dx = false;   // one piece, one split: dx is written at once
 };
+// Where dz stays in registers: db's shares, and the slices of dx, then of dW.
+struct GradSpace {
+    size_t sums = 0, slices = 0, bytes = 0;
+};
+static GradSpace grad_space(int64_t n, int64_t K, int64_t V, size_t begin)
+{
+    const int64_t x = grad_shares(n, V), w = grad_shares(V, n);
+    GradSpace s;
+    s.sums = begin;
+    s.slices = s.sums + up256(sizeof(float) * (size_t)w * V);
+    s.bytes = s.slices + up256(sizeof(float) * (size_t)std::max(x > 1 ? x * n * K : 0,
+                                                                w > 1 ? w * V * K : 0));
+    return s;
+}
 static CeSpace ce_space(int64_t n, int64_t K, int64_t V)
 {
     CeSpace s;
@@ -783,6 +1223,7 @@ static CeSpace ce_space(int64_t n, int64_t K, int64_t V)
     s.dw = s.dx + (s.whole_dx ? 0 : up256(sizeof(float) * (size_t)s.tdx.splits * n * K));
     s.bytes = s.dw +
               (s.tdw.splits > 1 ? up256(sizeof(float) * (size_t)s.tdw.splits * s.piece * K) : 0);
+    if (K <= kGradInputs && K % 8 == 0) s.bytes = std::max(s.bytes, grad_space(n, K, V, s.sums).bytes);
     if (V <= kFewClasses && K <= kFewInputs) {   // (alignment decides later: room for either)
         s.few_dw = s.sums;
         s.few_db = s.few_dw + up256(sizeof(float) * (size_t)few_slices(n, K) * V * K);
@@ -848,6 +1289,43 @@ static f3s_status loss_backward(const CeArgs& a, const float* lse, const float* 
                                reinterpret_cast<T*>(dW), p.db, classes,
                                (int32_t)few_groups(a.n, true), reinterpret_cast<T*>(db), factor);
         F3S_HIP(hipGetLastError());
+        return F3S_OK;
+    }
+    if (a.K <= kGradInputs && takes_stream(a)) {
+        const GradSpace w = grad_space(a.n, a.K, a.V, s.sums);
+        auto pass = [&](auto classes, char* out, size_t slices, char* sums_out) -> f3s_status {
+            constexpr bool kClasses = decltype(classes)::value;
+            GradParams p{};
+            p.own = kClasses ? a.W : a.X;
+            p.other = kClasses ? a.X : a.W;
+            p.ld_own = kClasses ? a.K : a.ldx;
+            p.ld_other = kClasses ? a.ldx : a.K;
+            p.owns = kClasses ? a.V : a.n;
+            p.others = kClasses ? a.n : a.V;
+            p.K = (int32_t)a.K;
+            p.per = grad_per(p.owns, p.others);
+            p.bias = a.bias;
+            p.target = a.target;
+            p.lse = lse;
+            p.f = f.f;
+            p.factor = factor;
+            const int64_t shares = grad_shares(p.owns, p.others), count = p.owns * a.K;
+            if (out && shares == 1) p.out = out;
+            else if (out) p.slices = reinterpret_cast<float*>(ws + slices);
+            p.sums = sums_out ? reinterpret_cast<float*>(ws + w.sums) : nullptr;
+            launch_grad<T, kClasses>(p, a.st);
+            auto join = [&](const float* parts, int64_t values, char* to) {
+                hipLaunchKernelGGL((join_scaled<T>), dim3((unsigned)ceil_div(values, 256)), dim3(256), 0,
+                                   a.st, parts, values, (int32_t)shares, factor,
+                                   reinterpret_cast<T*>(to));
+            };
+            if (p.slices) join(p.slices, count, out);
+            if (p.sums) join(p.sums, p.owns, sums_out);
+            F3S_HIP(hipGetLastError());
+            return F3S_OK;
+        };
+        if (dX) F3S_TRY(pass(std::false_type{}, dX, w.slices, nullptr));
+        if (dW || db) F3S_TRY(pass(std::true_type{}, dW, w.slices, db));
         return F3S_OK;
     }
     auto aligned = [](const void* x) { return ((uintptr_t)x & 15) == 0; };

@@ -58,18 +58,19 @@ struct Place {
     }
 };
 
-template <typename T>
+// (SMALL: C may be below V)
+template <typename T, bool SMALL>
 __device__ __forceinline__ typename Pieces<T>::Raw load_piece(const T* row, int32_t start, int32_t C)
 {
     typedef typename Pieces<T>::Raw Raw;
-    if (C >= Pieces<T>::V) return reinterpret_cast<const AnyPlace<Raw>*>(row + start)->v;
+    if (!SMALL || C >= Pieces<T>::V) return reinterpret_cast<const AnyPlace<Raw>*>(row + start)->v;
     Raw r = {};
 #pragma unroll
     for (int k = 0; k < Pieces<T>::V; ++k)   // (start = C - V < 0: the row's values are the last C)
         if (start + k >= 0) r[k] = row[start + k];
     return r;
 }
-template <typename T>
+template <typename T, bool SMALL>
 __device__ __forceinline__ void store_piece(T* row, int32_t start, int32_t C,
                                             const float (&v)[Pieces<T>::V])
 {
@@ -77,7 +78,7 @@ __device__ __forceinline__ void store_piece(T* row, int32_t start, int32_t C,
     Raw r;
 #pragma unroll
     for (int k = 0; k < Pieces<T>::V; ++k) r[k] = (T)v[k];
-    if (C >= Pieces<T>::V) {
+    if (!SMALL || C >= Pieces<T>::V) {
         reinterpret_cast<AnyPlace<Raw>*>(row + start)->v = r;
         return;
     }
@@ -86,15 +87,32 @@ __device__ __forceinline__ void store_piece(T* row, int32_t start, int32_t C,
         if (start + k >= 0) row[start + k] = r[k];
 }
 // w's or b's values beside a piece.
-template <typename T>
+template <typename T, bool SMALL>
 __device__ __forceinline__ void load_weights(const void* w, int32_t wide, int32_t start, int32_t C,
                                              float other, float (&out)[Pieces<T>::V])
 {
+    constexpr int V = Pieces<T>::V;
+    if (!w) {
 #pragma unroll
-    for (int k = 0; k < Pieces<T>::V; ++k) {
-        const int32_t c = max(start + k, 0);
-        out[k] = !w ? other : wide ? static_cast<const float*>(w)[c]
-                                   : (float)static_cast<const T*>(w)[c];
+        for (int k = 0; k < V; ++k) out[k] = other;
+    } else if (SMALL && C < V) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int32_t c = max(start + k, 0);
+            out[k] = wide ? static_cast<const float*>(w)[c] : (float)static_cast<const T*>(w)[c];
+        }
+    } else if (wide) {
+#pragma unroll
+        for (int q = 0; q < V / 4; ++q) {
+            const f4 a =
+                reinterpret_cast<const AnyPlace<f4>*>(static_cast<const float*>(w) + start + 4 * q)->v;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) out[4 * q + k] = a[k];
+        }
+    } else {
+        const typename Pieces<T>::Raw a = load_piece<T, false>(static_cast<const T*>(w), start, C);
+#pragma unroll
+        for (int k = 0; k < V; ++k) out[k] = (float)a[k];
     }
 }
 
@@ -145,6 +163,16 @@ __device__ __forceinline__ void row_sums_of(float (&x)[N], float (*lds)[N])
     }
 }
 
+// For the compiler new values: what was made of the old ones is not held.
+template <typename R>
+__device__ __forceinline__ void anew_piece(R& a, R& b)
+{
+    u4 x = __builtin_bit_cast(u4, a), y = __builtin_bit_cast(u4, b);
+    asm volatile("" : "+v"(x), "+v"(y));
+    a = __builtin_bit_cast(R, x);
+    b = __builtin_bit_cast(R, y);
+}
+
 constexpr int norm_threads(int lanes) { return lanes > 256 ? lanes : 256; }
 
 template <typename T, int LANES, int NP>
@@ -163,8 +191,8 @@ __global__ void __launch_bounds__(norm_threads(LANES)) norm_fwd_kernel(const Nor
         const Place<V> at(l + j * LANES, C);
         start[j] = at.start;
         skip[j] = at.skip;
-        load_weights<T>(p.w, p.wide_weights, at.start, C, 1.f, w[j]);
-        load_weights<T>(p.b, p.wide_weights, at.start, C, 0.f, b[j]);
+        load_weights<T, LANES == 8>(p.w, p.wide_weights, at.start, C, 1.f, w[j]);
+        load_weights<T, LANES == 8>(p.b, p.wide_weights, at.start, C, 0.f, b[j]);
     }
     const float inv = 1.f / (float)C;
     const int64_t step = (int64_t)gridDim.x * kRows;
@@ -173,7 +201,7 @@ __global__ void __launch_bounds__(norm_threads(LANES)) norm_fwd_kernel(const Nor
     auto load = [&](int64_t r) __attribute__((always_inline)) {
         const T* src = x + min(r, p.n - 1) * p.ldx;
 #pragma unroll
-        for (int j = 0; j < NP; ++j) next[j] = load_piece<T>(src, start[j], C);
+        for (int j = 0; j < NP; ++j) next[j] = load_piece<T, LANES == 8>(src, start[j], C);
     };
     load(row);
     for (int64_t base = (int64_t)blockIdx.x * kRows; base < p.n; base += step, row += step) {
@@ -205,7 +233,7 @@ __global__ void __launch_bounds__(norm_threads(LANES)) norm_fwd_kernel(const Nor
                 if (skip[j] >= V) continue;
 #pragma unroll
                 for (int k = 0; k < V; ++k) v[j][k] = __builtin_fmaf(v[j][k] * r, w[j][k], b[j][k]);
-                store_piece<T>(dst, start[j], C, v[j]);
+                store_piece<T, LANES == 8>(dst, start[j], C, v[j]);
             }
             if (p.stats && l == 0) *reinterpret_cast<float2*>(p.stats + 2 * row) = make_float2(m, r);
         }
@@ -229,7 +257,7 @@ __global__ void __launch_bounds__(norm_threads(LANES)) norm_bwd_kernel(const Nor
         const Place<V> at(l + j * LANES, C);
         start[j] = at.start;
         skip[j] = at.skip;
-        load_weights<T>(p.w, p.wide_weights, at.start, C, 1.f, w[j]);
+        load_weights<T, LANES == 8>(p.w, p.wide_weights, at.start, C, 1.f, w[j]);
 #pragma unroll
         for (int k = 0; k < V; ++k) dw[j][k] = db[j][k] = 0.f;
     }
@@ -244,33 +272,40 @@ __global__ void __launch_bounds__(norm_threads(LANES)) norm_bwd_kernel(const Nor
         const T* sy = dy + r * p.lddy;
         stat = *reinterpret_cast<const float2*>(p.stats + 2 * r);
 #pragma unroll
-        for (int j = 0; j < NP; ++j) nx[j] = load_piece<T>(sx, start[j], C);
+        for (int j = 0; j < NP; ++j) nx[j] = load_piece<T, LANES == 8>(sx, start[j], C);
 #pragma unroll
-        for (int j = 0; j < NP; ++j) ny[j] = load_piece<T>(sy, start[j], C);
+        for (int j = 0; j < NP; ++j) ny[j] = load_piece<T, LANES == 8>(sy, start[j], C);
     };
-    load(row);
+    // (the next row's loads ahead where the registers are there for them)
+    constexpr bool kAhead = LANES < 1024 || NP < 4;
+    if (kAhead) load(row);
     int turn = 0;
     for (int64_t base = (int64_t)blockIdx.x * kRows; base < p.n; base += step, row += step, turn ^= 1) {
+        if (!kAhead) load(row);
         const float m = stat.x, r = stat.y;
         const bool there = row < p.n;
-        float h[NP][V], dh[NP][V], s[2] = {0.f, 0.f};
+        Raw cx[NP], cy[NP];
+        float s[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            cx[j] = nx[j];
+            cy[j] = ny[j];
+        }
+        if (kAhead && base + step < p.n) load(row + step);
 #pragma unroll
         for (int j = 0; j < NP; ++j)
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                const float g = there ? (float)ny[j][k] : 0.f;
-                h[j][k] = ((float)nx[j][k] - m) * r;
+                const float g = there ? (float)cy[j][k] : 0.f, h = ((float)cx[j][k] - m) * r;
                 if (there) {   // (0 x inf of a row that is another's again)
-                    dw[j][k] = __builtin_fmaf(g, h[j][k], dw[j][k]);
+                    dw[j][k] = __builtin_fmaf(g, h, dw[j][k]);
                     db[j][k] += g;
                 }
-                dh[j][k] = g * w[j][k];
                 if (k >= skip[j]) {
-                    s[0] += dh[j][k];
-                    s[1] = __builtin_fmaf(dh[j][k], h[j][k], s[1]);
+                    s[0] = __builtin_fmaf(g, w[j][k], s[0]);
+                    s[1] = __builtin_fmaf(g * w[j][k], h, s[1]);
                 }
             }
-        if (base + step < p.n) load(row + step);
         if (p.y) {
             row_sums_of<LANES, 2>(s, lds[turn]);
             const float s0 = s[0] * inv, s1 = s[1] * inv;
@@ -279,10 +314,14 @@ __global__ void __launch_bounds__(norm_threads(LANES)) norm_bwd_kernel(const Nor
 #pragma unroll
                 for (int j = 0; j < NP; ++j) {
                     if (skip[j] >= V) continue;
+                    // (h and dh again, from the pieces: held, they are 32 registers of a
+                    // workgroup's 128 where rows are widest)
+                    if constexpr (LANES >= 1024) anew_piece(cx[j], cy[j]);
+                    float dx[V];
 #pragma unroll
                     for (int k = 0; k < V; ++k)
-                        dh[j][k] = r * (dh[j][k] - s0 - h[j][k] * s1);
-                    store_piece<T>(dst, start[j], C, dh[j]);
+                        dx[k] = r * ((float)cy[j][k] * w[j][k] - s0 - ((float)cx[j][k] - m) * r * s1);
+                    store_piece<T, LANES == 8>(dst, start[j], C, dx);
                 }
             }
         }
@@ -336,32 +375,52 @@ __device__ __forceinline__ float block_sum(float x, float* lds)
     for (int v = 0; v < kWideThreads / kWave; ++v) s += lds[v];
     return s;
 }
-template <typename T>
-__device__ __forceinline__ float weight_at(const void* w, int32_t wide, int32_t c, float other)
+// f(start, skip) for the thread's pieces of a row.  (C >= V here)
+template <int V, typename F>
+__device__ __forceinline__ void own_pieces(int32_t C, F f)
 {
-    return !w ? other : wide ? static_cast<const float*>(w)[c] : (float)static_cast<const T*>(w)[c];
+    for (int32_t num = threadIdx.x; (int64_t)num * V < C; num += kWideThreads) {
+        const Place<V> at(num, C);
+        f(at.start, at.skip);
+    }
 }
 template <typename T>
 __global__ void __launch_bounds__(kWideThreads) norm_wide_fwd(const NormParams p)
 {
+    constexpr int V = Pieces<T>::V;
+    typedef typename Pieces<T>::Raw Raw;
     __shared__ float lds[kWideThreads / kWave];
     const int32_t C = p.C;
     const float inv = 1.f / (float)C;
     for (int64_t row = blockIdx.x; row < p.n; row += gridDim.x) {
         const T* x = reinterpret_cast<const T*>(p.x) + row * p.ldx;
+        T* y = reinterpret_cast<T*>(p.y) + row * C;
         float s = 0.f;
-        for (int32_t c = threadIdx.x; c < C; c += kWideThreads) s += (float)x[c];
+        own_pieces<V>(C, [&](int32_t start, int32_t skip) {
+            const Raw a = load_piece<T, false>(x, start, C);
+#pragma unroll
+            for (int k = 0; k < V; ++k) s += k >= skip ? (float)a[k] : 0.f;
+        });
         const float m = block_sum(s, lds) * inv;
         s = 0.f;
-        for (int32_t c = threadIdx.x; c < C; c += kWideThreads) {
-            const float d = (float)x[c] - m;
-            s = __builtin_fmaf(d, d, s);
-        }
+        own_pieces<V>(C, [&](int32_t start, int32_t skip) {
+            const Raw a = load_piece<T, false>(x, start, C);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float d = (float)a[k] - m;
+                s = k >= skip ? __builtin_fmaf(d, d, s) : s;
+            }
+        });
         const float r = 1.f / __builtin_sqrtf(__builtin_fmaf(block_sum(s, lds), inv, p.eps));
-        T* y = reinterpret_cast<T*>(p.y) + row * C;
-        for (int32_t c = threadIdx.x; c < C; c += kWideThreads)
-            y[c] = (T)__builtin_fmaf(((float)x[c] - m) * r, weight_at<T>(p.w, p.wide_weights, c, 1.f),
-                                     weight_at<T>(p.b, p.wide_weights, c, 0.f));
+        own_pieces<V>(C, [&](int32_t start, int32_t) {
+            const Raw a = load_piece<T, false>(x, start, C);
+            float w[V], b[V], v[V];
+            load_weights<T, false>(p.w, p.wide_weights, start, C, 1.f, w);
+            load_weights<T, false>(p.b, p.wide_weights, start, C, 0.f, b);
+#pragma unroll
+            for (int k = 0; k < V; ++k) v[k] = __builtin_fmaf(((float)a[k] - m) * r, w[k], b[k]);
+            store_piece<T, false>(y, start, C, v);
+        });
         if (p.stats && threadIdx.x == 0)
             *reinterpret_cast<float2*>(p.stats + 2 * row) = make_float2(m, r);
     }
@@ -369,26 +428,39 @@ __global__ void __launch_bounds__(kWideThreads) norm_wide_fwd(const NormParams p
 template <typename T>
 __global__ void __launch_bounds__(kWideThreads) norm_wide_dx(const NormParams p)
 {
+    constexpr int V = Pieces<T>::V;
+    typedef typename Pieces<T>::Raw Raw;
     __shared__ float lds[kWideThreads / kWave];
     const int32_t C = p.C;
     const float inv = 1.f / (float)C;
     for (int64_t row = blockIdx.x; row < p.n; row += gridDim.x) {
         const T* x = reinterpret_cast<const T*>(p.x) + row * p.ldx;
         const T* dy = reinterpret_cast<const T*>(p.dy) + row * p.lddy;
+        T* dx = reinterpret_cast<T*>(p.y) + row * C;
         const float m = p.stats[2 * row], r = p.stats[2 * row + 1];
         float s0 = 0.f, s1 = 0.f;
-        for (int32_t c = threadIdx.x; c < C; c += kWideThreads) {
-            const float dh = (float)dy[c] * weight_at<T>(p.w, p.wide_weights, c, 1.f);
-            s0 += dh;
-            s1 = __builtin_fmaf(dh, ((float)x[c] - m) * r, s1);
-        }
+        own_pieces<V>(C, [&](int32_t start, int32_t skip) {
+            const Raw a = load_piece<T, false>(x, start, C), d = load_piece<T, false>(dy, start, C);
+            float w[V];
+            load_weights<T, false>(p.w, p.wide_weights, start, C, 1.f, w);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float dh = k >= skip ? (float)d[k] * w[k] : 0.f;
+                s0 += dh;
+                s1 = k >= skip ? __builtin_fmaf(dh, ((float)a[k] - m) * r, s1) : s1;
+            }
+        });
         s0 = block_sum(s0, lds) * inv;
         s1 = block_sum(s1, lds) * inv;
-        T* dx = reinterpret_cast<T*>(p.y) + row * C;
-        for (int32_t c = threadIdx.x; c < C; c += kWideThreads) {
-            const float dh = (float)dy[c] * weight_at<T>(p.w, p.wide_weights, c, 1.f);
-            dx[c] = (T)(r * (dh - s0 - ((float)x[c] - m) * r * s1));
-        }
+        own_pieces<V>(C, [&](int32_t start, int32_t) {
+            const Raw a = load_piece<T, false>(x, start, C), d = load_piece<T, false>(dy, start, C);
+            float w[V], v[V];
+            load_weights<T, false>(p.w, p.wide_weights, start, C, 1.f, w);
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                v[k] = r * ((float)d[k] * w[k] - s0 - ((float)a[k] - m) * r * s1);
+            store_piece<T, false>(dx, start, C, v);
+        });
     }
 }
 // 256 columns of blockIdx.y's share of the rows.
@@ -461,16 +533,21 @@ constexpr int64_t kCus = 256;
 struct NormShape {
     int32_t lanes, pieces;
 };
-static NormShape norm_shape(int64_t C, int32_t dtype)
+static NormShape norm_shape(int64_t C, int32_t dtype, bool backward)
 {
     const int64_t have = ceil_div(C, dtype == F3S_F32 ? 4 : 8);
     for (int32_t lanes : {8, 16, 32, 64})
         if (have <= lanes) return {lanes, 1};
     if (have <= 128) return {64, 2};
+    // (the gradient's registers: 32 values a lane in 512 lanes; 16 in 1,024 spilled, 12,736
+    // wide in bfloat16 486 us a step, 318 so)
+    if (backward && dtype != F3S_F32 && have > 1024 && have <= 2048) return {512, 4};
     for (int32_t lanes : {256, 512, 1024})
         for (int32_t pieces : {1, 2})
             if ((pieces == 2 || lanes == 256) && have <= (int64_t)lanes * pieces)
                 return {lanes, pieces};
+    // (float32: four pieces are as many values as 16-bit types' two)
+    if (dtype == F3S_F32 && have <= 4096) return {1024, 4};
     return {0, 0};
 }
 
@@ -486,7 +563,7 @@ static int64_t wide_lines(int64_t n) { return std::min<int64_t>(n, 64); }
 
 static size_t norm_bytes(int64_t n, int64_t C, int32_t dtype)
 {
-    const NormShape s = norm_shape(C, dtype);
+    const NormShape s = norm_shape(C, dtype, true);
     return sizeof(float) * 2 * (size_t)C * (size_t)(s.lanes ? norm_groups(s, n, true) : wide_lines(n));
 }
 
@@ -506,13 +583,16 @@ static void with_shape(const NormShape& s, F go)
     one(std::integral_constant<int, 256>{}, p1);
     one(std::integral_constant<int, 256>{}, p2);
     one(std::integral_constant<int, 512>{}, p2);
+    if constexpr (sizeof(T) == 2) one(std::integral_constant<int, 512>{}, std::integral_constant<int, 4>{});
     one(std::integral_constant<int, 1024>{}, p2);
+    if constexpr (sizeof(T) == 4)
+        one(std::integral_constant<int, 1024>{}, std::integral_constant<int, 4>{});
 }
 
 template <typename T>
 static void norm_forward(const NormParams& p, int32_t dtype, hipStream_t st)
 {
-    const NormShape s = norm_shape(p.C, dtype);
+    const NormShape s = norm_shape(p.C, dtype, false);
     const dim3 grid((unsigned)norm_groups(s, p.n, false));
     if (!s.lanes) {
         hipLaunchKernelGGL((norm_wide_fwd<T>), grid, dim3(kWideThreads), 0, st, p);
@@ -527,7 +607,7 @@ static void norm_forward(const NormParams& p, int32_t dtype, hipStream_t st)
 template <typename T>
 static void norm_backward(const NormParams& p, int32_t dtype, void* dw, void* db, hipStream_t st)
 {
-    const NormShape s = norm_shape(p.C, dtype);
+    const NormShape s = norm_shape(p.C, dtype, true);
     const dim3 grid((unsigned)norm_groups(s, p.n, true));
     int64_t lines = grid.x;
     if (!s.lanes) {

@@ -15,7 +15,10 @@ SHAPES = [(1, 1, 1), (1, 8, 2), (3, 5, 3), (5, 16, 7), (17, 33, 10), (64, 64, 47
           (300, 40, 20_000), (1, 512, 5000), (4100, 128, 4099), (20_011, 24, 3),
           # few classes of few inputs, 2 to 8 fragments by 1 to 4 tiles
           (3000, 256, 64), (1000, 136, 33), (257, 128, 17), (40_000, 40, 64), (130, 200, 16),
-          (127, 64, 32), (129, 8, 64), (5000, 104, 48)]
+          (127, 64, 32), (129, 8, 64), (5000, 104, 48),
+          # many classes of few inputs: shares of either side, one and two blocks of inputs
+          (1, 64, 65), (127, 8, 128), (129, 64, 129), (3000, 120, 65), (64, 128, 9000),
+          (9000, 128, 70), (333, 256, 1001)]
 
 
 def inputs(n, K, V, dtype, seed, bias=True, ignored=0.2, reduction="mean"):
@@ -66,7 +69,7 @@ def test_step(gpu, n, K, V, dtype, reduction, bias):
                            got["loss"])
 
 
-@pytest.mark.parametrize("K", [40, 41])
+@pytest.mark.parametrize("K", [136, 41, 40])
 @pytest.mark.parametrize("dtype", HALF)
 def test_pieces_of_the_classes(gpu, dtype, K):
     """More of dz than a piece holds, the last piece smaller and ragged."""
