@@ -365,17 +365,18 @@ __global__ void __launch_bounds__(kStreamWaves * kWave) stream_lse_kernel(const 
     }
 }
 
-// ---- their gradients: K <= 128, whole pieces ----
+// ---- their gradients: K <= 256, whole pieces ----
 //
 // dz never leaves the registers: two passes of one shape, each with the logits again.
-// A wave keeps 32 rows of its own, the others stream past it, 64 at a time:
+// A wave keeps 32 rows of its own (16 past 128 inputs, whose sums fill the registers),
+// the others stream past it, 64 at a time:
 //   dx      its rows are x's, W's stream past: dx += dz W
 //   dW, db  its rows are W's, x's stream past: dW += dz^T x
 // A lane's logits of a row are the operand of the product after them, whose other one is
 // the same rows in LDS, read transposed.  Shares of the streamed rows (blockIdx.y) are
-// added by join_scaled.  One product of five more than by tiles, and none of dz's bytes
-// (52,802 x 64 -> 10,778 trained by tiles 1,324 us, most of it dz in and out; so 744;
-// 200,003 x 128 -> 300 237 and 207.)
+// added by join_scaled.  One product of five more than by tiles, and none of dz's bytes.
+// (A training step by tiles and so, us: 52,802 x 64 -> 10,778 1,324 and 690; x 128 1,473
+// and 953; x 256 2,147 and 1,814; 16,384 x 256 -> 50,021 3,277 and 2,457.)
 struct GradParams {
     const char *own, *other;
     int64_t ld_own, ld_other, owns, others;
@@ -390,7 +391,7 @@ struct GradParams {
     float* sums;             // db: [shares][owns] (NULL: not wanted)
 };
 __device__ __forceinline__ int place_both(int row) { return (row & 6) | ((row >> 3) & 1); }
-template <typename T, int KS, bool CLASSES>
+template <typename T, int KS, int TILES, bool CLASSES>
 __global__ void __launch_bounds__(kStreamWaves * kWave) __attribute__((amdgpu_waves_per_eu(2)))
 stream_grad_kernel(const GradParams p)
 {
@@ -398,6 +399,7 @@ stream_grad_kernel(const GradParams p)
     typedef short s4 __attribute__((ext_vector_type(4)));
     typedef short s8 __attribute__((ext_vector_type(8)));
     typedef __attribute__((address_space(3))) s4* lds4;
+    constexpr int kRows = 16 * TILES * kStreamWaves;   // of its own
     constexpr int kBytes = 64 * kStep * 2, kDims = 4 * KS;   // 64 rows by 64 inputs; tiles of dims
     __shared__ __align__(256) char rows[2][KS * kBytes];
     __shared__ __align__(16) float at1[2][64], at2[2][64];    // bias; lse and f
@@ -405,7 +407,7 @@ stream_grad_kernel(const GradParams p)
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int lane = threadIdx.x % kWave;
     const int g = lane >> 4, r = lane & 15;
-    const int64_t block0 = (int64_t)blockIdx.x * kStreamRows, first = block0 + wave * 16 * kStreamTiles;
+    const int64_t block0 = (int64_t)blockIdx.x * kRows, first = block0 + wave * 16 * TILES;
     const int64_t chunks = (p.others + 63) / 64, begin = blockIdx.y * p.per,
                   end = min(chunks, begin + p.per);
     float next1 = 0.f, next2 = 0.f;
@@ -434,7 +436,7 @@ stream_grad_kernel(const GradParams p)
                 next1 = in ? p.lse[at] : 0.f;
                 next2 = in ? p.f[at] : 0.f;
                 const int64_t t = in ? p.target[at] - block0 : -1;
-                next3 = t >= 0 && t < kStreamRows ? (int32_t)t : -1;
+                next3 = t >= 0 && t < kRows ? (int32_t)t : -1;
             } else {
                 next1 = at >= p.others ? -INFINITY
                         : p.bias       ? (float)reinterpret_cast<const T*>(p.bias)[at]
@@ -443,12 +445,12 @@ stream_grad_kernel(const GradParams p)
         }
     };
     if (begin < end) load(begin, 0);
-    v8 own[kStreamTiles][2 * KS];
-    float own1[kStreamTiles], own2[kStreamTiles], sum[kStreamTiles];   // lse, f; bias
-    int64_t t[kStreamTiles];
-    f4 acc[kStreamTiles][kDims];
+    v8 own[TILES][2 * KS];
+    float own1[TILES], own2[TILES], sum[TILES];   // lse, f; bias
+    int64_t t[TILES];
+    f4 acc[TILES][kDims];
 #pragma unroll
-    for (int u = 0; u < kStreamTiles; ++u) {
+    for (int u = 0; u < TILES; ++u) {
         const int64_t row = min(first + 16 * u + r, p.owns - 1);
         const T* src = reinterpret_cast<const T*>(p.own) + row * p.ld_own + 8 * g;
 #pragma unroll
@@ -481,11 +483,11 @@ stream_grad_kernel(const GradParams p)
         __syncthreads();
         if (c + 1 < end) load(c + 1, buf ^ 1);
         // logits of the chunk's rows 16 i + 4 g + v and own row r
-        f4 z[4][kStreamTiles];
+        f4 z[4][TILES];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int u = 0; u < kStreamTiles; ++u)
+            for (int u = 0; u < TILES; ++u)
                 z[i][u] = CLASSES ? f4{own1[u], own1[u], own1[u], own1[u]}
                                   : *reinterpret_cast<const f4*>(&at1[buf][16 * i + 4 * g]);
 #pragma unroll
@@ -498,17 +500,17 @@ stream_grad_kernel(const GradParams p)
                         rows[buf] + k * kBytes + (16 * i + r) * 128 +
                         16 * ((4 * f + g) ^ place_both(r)));
 #pragma unroll
-                    for (int u = 0; u < kStreamTiles; ++u)
+                    for (int u = 0; u < TILES; ++u)
                         z[i][u] = Half<T>::mfma(a, own[u][2 * k + f], z[i][u]);
                 }
         // dz in their place
         uint64_t hits = 0;   // (CLASSES) whether a target is among the wave's classes
         if constexpr (CLASSES) {
             const int32_t at = at3[buf][lane];
-            hits = __ballot(at >= 0 && at / (16 * kStreamTiles) == wave);
+            hits = __ballot(at >= 0 && at / (16 * TILES) == wave);
         }
 #pragma unroll
-        for (int u = 0; u < kStreamTiles; ++u) {
+        for (int u = 0; u < TILES; ++u) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 f4 lse, f;
@@ -526,7 +528,7 @@ stream_grad_kernel(const GradParams p)
                         const u4 at = *reinterpret_cast<const u4*>(&at3[buf][16 * i + 4 * g]);
 #pragma unroll
                         for (int v = 0; v < 4; ++v)
-                            z[i][u][v] -= (int)at[v] == (wave * kStreamTiles + u) * 16 + r ? 1.f : 0.f;
+                            z[i][u][v] -= (int)at[v] == (wave * TILES + u) * 16 + r ? 1.f : 0.f;
                     }
                 } else {
                     const int64_t at = t[u] - 64 * c - 16 * i - 4 * g;
@@ -542,11 +544,11 @@ stream_grad_kernel(const GradParams p)
             }
         }
         // times the chunk's rows: their 16 dims from 16 d, rows 32 q + slot_of(g, j)
-        v8 dz[2][kStreamTiles];
+        v8 dz[2][TILES];
 #pragma unroll
         for (int q = 0; q < 2; ++q)
 #pragma unroll
-            for (int u = 0; u < kStreamTiles; ++u)
+            for (int u = 0; u < TILES; ++u)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) dz[q][u][j] = (T)z[2 * q + j / 4][u][j % 4];
 #pragma unroll
@@ -562,13 +564,13 @@ stream_grad_kernel(const GradParams p)
                 const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)more);
                 const v8 x = __builtin_bit_cast(v8, s8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
 #pragma unroll
-                for (int u = 0; u < kStreamTiles; ++u) acc[u][d] = Half<T>::mfma(x, dz[q][u], acc[u][d]);
+                for (int u = 0; u < TILES; ++u) acc[u][d] = Half<T>::mfma(x, dz[q][u], acc[u][d]);
             }
     }
     // dims 16 d + 4 g .. of own row r
     const float factor = p.out ? *p.factor : 1.f;
 #pragma unroll
-    for (int u = 0; u < kStreamTiles; ++u) {
+    for (int u = 0; u < TILES; ++u) {
         const int64_t row = first + 16 * u + r;
         if (CLASSES && p.sums) {
             float s = sum[u] + __shfl_xor(sum[u], 16, kWave);
@@ -1065,24 +1067,28 @@ static void launch_stream(const CeArgs& a, const GemmParams& g, int64_t per, int
     else hipLaunchKernelGGL((stream_lse_kernel<T, 4>), grid, block, 0, a.st, p);
 }
 
-// Gradients so: shares of the streamed rows, as many as fill the chip.
-constexpr int64_t kGradInputs = 128, kGradGroups = 1024;
-static int64_t grad_per(int64_t owns, int64_t others)
+// Shares of the streamed rows, as many as fill the chip.
+constexpr int64_t kGradInputs = 256, kGradGroups = 1024;
+static int64_t grad_rows(int64_t K) { return K <= 128 ? 128 : 64; }   // of a workgroup's own
+static int64_t grad_per(int64_t owns, int64_t others, int64_t K)
 {
-    const int64_t chunks = ceil_div(others, 64), groups = ceil_div(owns, kStreamRows);
+    const int64_t chunks = ceil_div(others, 64), groups = ceil_div(owns, grad_rows(K));
     return ceil_div(chunks, std::min(chunks, std::max<int64_t>(1, kGradGroups / groups)));
 }
-static int64_t grad_shares(int64_t owns, int64_t others)
+static int64_t grad_shares(int64_t owns, int64_t others, int64_t K)
 {
-    return ceil_div(ceil_div(others, 64), grad_per(owns, others));
+    return ceil_div(ceil_div(others, 64), grad_per(owns, others, K));
 }
 template <typename T, bool CLASSES>
 static void launch_grad(const GradParams& p, hipStream_t st)
 {
-    const dim3 grid((unsigned)ceil_div(p.owns, kStreamRows), (unsigned)grad_shares(p.owns, p.others)),
+    const dim3 grid((unsigned)ceil_div(p.owns, grad_rows(p.K)),
+                    (unsigned)grad_shares(p.owns, p.others, p.K)),
         block(kStreamWaves * kWave);
-    if (p.K <= 64) hipLaunchKernelGGL((stream_grad_kernel<T, 1, CLASSES>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((stream_grad_kernel<T, 2, CLASSES>), grid, block, 0, st, p);
+    if (p.K <= 64) hipLaunchKernelGGL((stream_grad_kernel<T, 1, 2, CLASSES>), grid, block, 0, st, p);
+    else if (p.K <= 128)
+        hipLaunchKernelGGL((stream_grad_kernel<T, 2, 2, CLASSES>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((stream_grad_kernel<T, 4, 1, CLASSES>), grid, block, 0, st, p);
 }
 
 static int32_t blocks_of(int32_t tile, int64_t outs)
@@ -1192,7 +1198,7 @@ struct GradSpace {
 };
 static GradSpace grad_space(int64_t n, int64_t K, int64_t V, size_t begin)
 {
-    const int64_t x = grad_shares(n, V), w = grad_shares(V, n);
+    const int64_t x = grad_shares(n, V, K), w = grad_shares(V, n, K);
     GradSpace s;
     s.sums = begin;
     s.slices = s.sums + up256(sizeof(float) * (size_t)w * V);
@@ -1303,13 +1309,13 @@ static f3s_status loss_backward(const CeArgs& a, const float* lse, const float* 
             p.owns = kClasses ? a.V : a.n;
             p.others = kClasses ? a.n : a.V;
             p.K = (int32_t)a.K;
-            p.per = grad_per(p.owns, p.others);
+            p.per = grad_per(p.owns, p.others, a.K);
             p.bias = a.bias;
             p.target = a.target;
             p.lse = lse;
             p.f = f.f;
             p.factor = factor;
-            const int64_t shares = grad_shares(p.owns, p.others), count = p.owns * a.K;
+            const int64_t shares = grad_shares(p.owns, p.others, a.K), count = p.owns * a.K;
             if (out && shares == 1) p.out = out;
             else if (out) p.slices = reinterpret_cast<float*>(ws + slices);
             p.sums = sums_out ? reinterpret_cast<float*>(ws + w.sums) : nullptr;
