@@ -11,8 +11,10 @@
 //            and z at the target; a second launch joins a row's blocks
 //   backward in pieces of the classes: z again, dz of a piece in its epilogue, in the
 //            type, then its share of dx (float32, added up over the pieces) and its
-//            rows of dW.  A piece's dz is kPieceBytes at most.  So memory goes with n, K and that, not with n V, for one product
-//            of four more than keeping z would take.
+//            rows of dW.  A piece's dz is kPieceBytes at most.  So memory goes with n,
+//            K and that, not with n V, for one product of four more than keeping z
+//            would take.
+// Of few inputs (K <= 256) the logits, and dz, stay in registers: below.
 // dz is rounded to the type, the operand that dx and dW take: these two carry that
 // rounding beside their own; db is summed before it.  What dz is multiplied with
 // throughout (1 / count, a loss scale) comes last, in float32, so that small gradients
@@ -947,6 +949,37 @@ few_join(const float* __restrict__ dw, int64_t count, int32_t slices, T* __restr
     else out[at] = (T)s;
 }
 
+// Rows of K 16-bit values, as rows of Kp with zeros at their ends, eight a thread; and back.
+__global__ void __launch_bounds__(256)
+pad_rows(const uint16_t* __restrict__ from, int64_t ld, uint16_t* __restrict__ to, int64_t rows,
+         int32_t K, int32_t Kp)
+{
+    typedef uint16_t v8 __attribute__((ext_vector_type(8)));
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / (Kp / 8);
+    const int32_t c = (int32_t)(i % (Kp / 8)) * 8;
+    if (row >= rows) return;
+    const uint16_t* src = from + row * ld + c;
+    v8 v = {};
+    if (c + 8 <= K) v = reinterpret_cast<const Unaligned<v8>*>(src)->v;
+    else
+        for (int k = 0; k < K - c; ++k) v[k] = src[k];
+    *reinterpret_cast<v8*>(to + row * Kp + c) = v;
+}
+__global__ void __launch_bounds__(256)
+unpad_rows(const uint16_t* __restrict__ from, uint16_t* __restrict__ to, int64_t rows, int32_t K,
+           int32_t Kp)
+{
+    typedef uint16_t v8 __attribute__((ext_vector_type(8)));
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / (Kp / 8);
+    const int32_t c = (int32_t)(i % (Kp / 8)) * 8;
+    if (row >= rows) return;
+    const v8 v = *reinterpret_cast<const v8*>(from + row * Kp + c);
+    uint16_t* dst = to + row * K + c;
+    if (c + 8 <= K) reinterpret_cast<Unaligned<v8>*>(dst)->v = v;
+    else
+        for (int k = 0; k < K - c; ++k) dst[k] = v[k];
+}
+
 __global__ void warm_loss_kernel() {}
 
 hipError_t warm_loss(hipStream_t s)
@@ -974,8 +1007,7 @@ static Tiling one_split(int64_t rows, int64_t outs, int64_t depth, bool odd)
 
 static bool takes_few(const CeArgs& a)
 {
-    return a.V <= kFewClasses && a.K <= kFewInputs && a.K % 8 == 0 && a.ldx % 8 == 0 &&
-           (((uintptr_t)a.X | (uintptr_t)a.W) & 15) == 0;
+    return a.V <= kFewClasses && a.K <= kFewInputs && a.K % 8 == 0;
 }
 static int64_t few_groups(int64_t n, bool backward)
 {
@@ -1038,12 +1070,7 @@ static ForwardSpace forward_space(int64_t n, int64_t V)
     return s;
 }
 
-// (whole pieces, as few classes take; one row's pieces per 64 inputs in a tile)
-static bool takes_stream(const CeArgs& a)
-{
-    return a.K <= kFewInputs && a.K % 8 == 0 && a.ldx % 8 == 0 && a.ldx < (1 << 22) &&
-           (((uintptr_t)a.X | (uintptr_t)a.W) & 15) == 0;
-}
+static bool takes_stream(const CeArgs& a) { return a.K <= kFewInputs && a.K % 8 == 0; }
 constexpr int64_t kStreamGroups = 1024;   // four per CU
 template <typename T>
 static void launch_stream(const CeArgs& a, const GemmParams& g, int64_t per, int64_t shares)
@@ -1209,7 +1236,20 @@ static GradSpace grad_space(int64_t n, int64_t K, int64_t V, size_t begin)
 static CeSpace ce_space(int64_t n, int64_t K, int64_t V)
 {
     CeSpace s;
+    s.factor = up256(sizeof(float) * (size_t)n);
+    s.largest = s.factor + 256;
+    s.sums = s.largest + up256(sizeof(float) * kLargestGroups);
     const bool odd = K % 8 != 0;
+    if (!odd && V <= kFewClasses && K <= kFewInputs) {
+        s.few_dw = s.sums;
+        s.few_db = s.few_dw + up256(sizeof(float) * (size_t)few_slices(n, K) * V * K);
+        s.bytes = s.few_db + up256(sizeof(float) * (size_t)few_groups(n, true) * V);
+        return s;
+    }
+    if (!odd && K <= kGradInputs) {
+        s.bytes = grad_space(n, K, V, s.sums).bytes;
+        return s;
+    }
     const int64_t fit = std::max<int64_t>(1024, kPieceBytes / 2 / n / 256 * 256);
     const int64_t pieces = ceil_div(V, fit);
     s.piece = pieces == 1 ? V : ceil_div(ceil_div(V, pieces), 256) * 256;
@@ -1219,9 +1259,6 @@ static CeSpace ce_space(int64_t n, int64_t K, int64_t V)
     s.tdw = tiling(s.piece, K, n, kWeightLeast, odd, true);
     s.whole_dx = s.piece >= V && s.tdx.splits == 1;
     s.sum_rows = 2 * ceil_div(n, 64);   // (at most)
-    s.factor = up256(sizeof(float) * (size_t)n);
-    s.largest = s.factor + 256;
-    s.sums = s.largest + up256(sizeof(float) * kLargestGroups);
     s.shares = s.sums + up256(sizeof(float) * (size_t)s.sum_rows * s.ldz);
     s.db = s.shares + up256(sizeof(float) * (size_t)kLossShares * s.ldz);
     s.dz = s.db + up256(sizeof(float) * (size_t)s.ldz);
@@ -1229,13 +1266,62 @@ static CeSpace ce_space(int64_t n, int64_t K, int64_t V)
     s.dw = s.dx + (s.whole_dx ? 0 : up256(sizeof(float) * (size_t)s.tdx.splits * n * K));
     s.bytes = s.dw +
               (s.tdw.splits > 1 ? up256(sizeof(float) * (size_t)s.tdw.splits * s.piece * K) : 0);
-    if (K <= kGradInputs && K % 8 == 0) s.bytes = std::max(s.bytes, grad_space(n, K, V, s.sums).bytes);
-    if (V <= kFewClasses && K <= kFewInputs) {   // (alignment decides later: room for either)
-        s.few_dw = s.sums;
-        s.few_db = s.few_dw + up256(sizeof(float) * (size_t)few_slices(n, K) * V * K);
-        s.bytes = std::max(s.bytes, s.few_db + up256(sizeof(float) * (size_t)few_groups(n, true) * V));
+    return s;
+}
+
+// Rows of K inputs that are no whole pieces are copied to ones that are, padded with
+// zeros, where the products are long beside that.  (bfloat16, as they are and copied, us:
+// 52,802 x 65 -> 10,778 forward 710 and 258, trained 3,051 and 924; x 301 1,059 and 648,
+// 5,768 and 2,945; 1,000 x 301 -> 10,000 46 and 42, trained 186 and 158; 3,000 x 301 ->
+// 1,000 18.6 and 22.2; 64 x 41 -> 50,021 21.5 and 21.9; 1 x 41 -> 70 15 and 21.)
+static bool pads(int64_t n, int64_t K, int64_t V)
+{
+    return K % 8 != 0 && K < (1 << 22) - 8 && n >= 1000 && n * V >= (1 << 23);
+}
+struct PadSpace {
+    size_t x = 0, w = 0, dx = 0, dw = 0, bytes = 0;
+};
+static PadSpace pad_space(int64_t n, int64_t K, int64_t V, bool backward)
+{
+    const int64_t Kp = ceil_div(K, 8) * 8;
+    PadSpace s;
+    s.bytes = backward ? ce_space(n, pads(n, K, V) ? Kp : K, V).bytes : forward_space(n, V).bytes;
+    if (!pads(n, K, V)) return s;
+    const size_t x = up256(2 * (size_t)n * Kp), w = up256(2 * (size_t)V * Kp);
+    s.x = s.bytes;
+    s.w = s.x + x;
+    s.bytes = s.w + w;
+    if (backward) {
+        s.dx = s.bytes;
+        s.dw = s.dx + x;
+        s.bytes = s.dw + w;
     }
     return s;
+}
+static void launch_pad(const char* from, int64_t ld, char* to, int64_t rows, int64_t K, int64_t Kp,
+                       hipStream_t st)
+{
+    hipLaunchKernelGGL(pad_rows, dim3((unsigned)ceil_div(rows * (Kp / 8), 256)), dim3(256), 0, st,
+                       reinterpret_cast<const uint16_t*>(from), ld, reinterpret_cast<uint16_t*>(to),
+                       rows, (int32_t)K, (int32_t)Kp);
+}
+static void launch_unpad(const char* from, char* to, int64_t rows, int64_t K, int64_t Kp,
+                         hipStream_t st)
+{
+    hipLaunchKernelGGL(unpad_rows, dim3((unsigned)ceil_div(rows * (Kp / 8), 256)), dim3(256), 0, st,
+                       reinterpret_cast<const uint16_t*>(from), reinterpret_cast<uint16_t*>(to), rows,
+                       (int32_t)K, (int32_t)Kp);
+}
+// `a` on padded copies in the workspace.
+static CeArgs on_copies(const CeArgs& a, const PadSpace& s, char* ws)
+{
+    CeArgs b = a;
+    b.K = b.ldx = ceil_div(a.K, 8) * 8;
+    b.X = ws + s.x;
+    b.W = ws + s.w;
+    launch_pad(a.X, a.ldx, ws + s.x, a.n, a.K, b.K, a.st);
+    launch_pad(a.W, a.K, ws + s.w, a.V, a.K, b.K, a.st);
+    return b;
 }
 
 // A product of dz and W or x, whose rows are whole pieces beside the padded dz.
@@ -1334,9 +1420,7 @@ static f3s_status loss_backward(const CeArgs& a, const float* lse, const float* 
         if (dW || db) F3S_TRY(pass(std::true_type{}, dW, w.slices, db));
         return F3S_OK;
     }
-    auto aligned = [](const void* x) { return ((uintptr_t)x & 15) == 0; };
-    const bool w_pieces = a.K % 8 == 0 && a.K < (1 << 22) && aligned(a.W);
-    const bool x_pieces = a.K % 8 == 0 && a.ldx % 8 == 0 && a.ldx < (1 << 22) && aligned(a.X);
+    const bool whole = a.K % 8 == 0;   // (the operands' and the results' rows whole pieces)
     for (int64_t v0 = 0; v0 < a.V; v0 += s.piece) {
         const int64_t outs = std::min(s.piece, a.V - v0), ldz = ceil_div(outs, 8) * 8;
         const char* w = a.W + v0 * a.K * 2;
@@ -1357,11 +1441,10 @@ static f3s_status loss_backward(const CeArgs& a, const float* lse, const float* 
         p.loss.lse = lse;
         p.loss.f = f.f;
         p.loss.outs = outs;
-        const bool pieces = w_pieces && x_pieces;
-        const int32_t tile = tile_size(s.prob, pieces ? kWhole : kAny, kEpiProb);
+        const int32_t tile = tile_size(s.prob, whole ? kWhole : kAny, kEpiProb);
         F3S_REQUIRE(ceil_div(p.rows, tile) * ceil_div(p.outs, tile) < ((int64_t)1 << 31),
                     "cross entropy: too many tiles");
-        if (pieces) launch_tiles<T, false, false, kEpiProb, kWhole>(p, tile, a.st);
+        if (whole) launch_tiles<T, false, false, kEpiProb, kWhole>(p, tile, a.st);
         else launch_tiles<T, false, false, kEpiProb, kAny>(p, tile, a.st);
         F3S_HIP(hipGetLastError());
         if (db) {
@@ -1391,15 +1474,15 @@ static f3s_status loss_backward(const CeArgs& a, const float* lse, const float* 
             q.ldq = a.K;
             q.rows = a.n;
             q.outs = a.K;
-            q.depth = w_pieces ? ldz : outs;
+            q.depth = whole ? ldz : outs;
             q.q_end = outs;
             q.add = v0 > 0;
             q.factor = factor;
             q.C = s.whole_dx ? dX : ws + s.dx;
             if (s.whole_dx)
-                F3S_TRY((launch_of_dz<T, false, kEpiScaled>(q, s.tdx, w_pieces && aligned(dX), a.st)));
+                F3S_TRY((launch_of_dz<T, false, kEpiScaled>(q, s.tdx, whole, a.st)));
             else
-                F3S_TRY((launch_of_dz<T, false, kEpiAdd>(q, s.tdx, w_pieces, a.st)));
+                F3S_TRY((launch_of_dz<T, false, kEpiAdd>(q, s.tdx, whole, a.st)));
         }
         if (dW) {
             GemmParams q{};
@@ -1414,10 +1497,10 @@ static f3s_status loss_backward(const CeArgs& a, const float* lse, const float* 
             char* dst = dW + v0 * a.K * 2;
             if (s.tdw.splits == 1) {
                 q.C = dst;
-                F3S_TRY((launch_of_dz<T, true, kEpiScaled>(q, s.tdw, x_pieces && aligned(dst), a.st)));
+                F3S_TRY((launch_of_dz<T, true, kEpiScaled>(q, s.tdw, whole, a.st)));
             } else {
                 q.C = ws + s.dw;
-                F3S_TRY((launch_of_dz<T, true, kEpiPart>(q, s.tdw, x_pieces, a.st)));
+                F3S_TRY((launch_of_dz<T, true, kEpiPart>(q, s.tdw, whole, a.st)));
                 const int64_t count = outs * a.K;
                 hipLaunchKernelGGL((join_scaled<T>), dim3((unsigned)ceil_div(count, 256)), dim3(256),
                                    0, a.st, reinterpret_cast<const float*>(ws + s.dw), count,
@@ -1434,6 +1517,14 @@ static f3s_status loss_backward(const CeArgs& a, const float* lse, const float* 
         F3S_HIP(hipGetLastError());
     }
     return F3S_OK;
+}
+
+// Rows of a multiple of eight inputs: 16-byte addresses, offsets in a tile of 31 bits.
+static bool pieces_ok(const void* X, int64_t x_stride, const void* W, const void* dX, const void* dW,
+                      int64_t K)
+{
+    const uintptr_t all = (uintptr_t)X | (uintptr_t)W | (uintptr_t)dX | (uintptr_t)dW;
+    return K % 8 != 0 || ((all & 15) == 0 && x_stride % 8 == 0 && x_stride < (1 << 22));
 }
 
 static f3s_status check_loss(int64_t n, int64_t K, int64_t V, int32_t reduction, int32_t dtype,
@@ -1462,7 +1553,7 @@ f3s_status f3s_cross_entropy_workspace(int64_t n, int64_t K, int64_t V, int32_t 
 {
     F3S_REQUIRE(bytes, "f3s_cross_entropy_workspace: NULL pointer");
     F3S_TRY(check_loss(n, K, V, F3S_LOSS_NONE, F3S_F16, "f3s_cross_entropy_workspace"));
-    *bytes = (int64_t)(n == 0 ? 0 : backward_pass ? ce_space(n, K, V).bytes : forward_space(n, V).bytes);
+    *bytes = (int64_t)(n == 0 ? 0 : pad_space(n, K, V, backward_pass != 0).bytes);
     return F3S_OK;
 }
 
@@ -1476,8 +1567,11 @@ f3s_status f3s_cross_entropy_fwd(const uint16_t* X, int64_t x_stride, const uint
     F3S_REQUIRE((n == 0 && reduction == kNone) || loss, "f3s_cross_entropy_fwd: NULL pointer");
     F3S_REQUIRE(n == 0 || (X && W && target && x_stride >= K),
                 "f3s_cross_entropy_fwd: NULL pointer, or a row stride below K");
+    F3S_REQUIRE(n == 0 || pieces_ok(X, x_stride, W, nullptr, nullptr, K),
+                "f3s_cross_entropy_fwd: K is a multiple of 8, X's and W's rows are not at 16-byte "
+                "addresses");
     F3S_REQUIRE(n == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 &&
-                           workspace_bytes >= (int64_t)forward_space(n, V).bytes),
+                           workspace_bytes >= (int64_t)pad_space(n, K, V, false).bytes),
                 "f3s_cross_entropy_fwd: workspace too small");
     F3S_TRY(require_device());
     clear_error();
@@ -1493,8 +1587,10 @@ f3s_status f3s_cross_entropy_fwd(const uint16_t* X, int64_t x_stride, const uint
     const CeArgs a{reinterpret_cast<const char*>(X), reinterpret_cast<const char*>(W),
                    reinterpret_cast<const char*>(bias), x_stride, target, ignore_index, n, K, V,
                    reduction, as_stream(stream)};
-    if (dtype == F3S_F16) return loss_forward<_Float16>(a, loss, lse, static_cast<char*>(workspace));
-    return loss_forward<__bf16>(a, loss, lse, static_cast<char*>(workspace));
+    char* ws = static_cast<char*>(workspace);
+    const CeArgs b = pads(n, K, V) ? on_copies(a, pad_space(n, K, V, false), ws) : a;
+    if (dtype == F3S_F16) return loss_forward<_Float16>(b, loss, lse, ws);
+    return loss_forward<__bf16>(b, loss, lse, ws);
 }
 
 f3s_status f3s_cross_entropy_bwd(const uint16_t* X, int64_t x_stride, const uint16_t* W,
@@ -1507,8 +1603,11 @@ f3s_status f3s_cross_entropy_bwd(const uint16_t* X, int64_t x_stride, const uint
     F3S_TRY(check_loss(n, K, V, reduction, dtype, "f3s_cross_entropy_bwd"));
     F3S_REQUIRE(n == 0 || (X && W && target && lse && dloss && x_stride >= K),
                 "f3s_cross_entropy_bwd: NULL pointer, or a row stride below K");
+    F3S_REQUIRE(n == 0 || pieces_ok(X, x_stride, W, dX, dW, K),
+                "f3s_cross_entropy_bwd: K is a multiple of 8, the rows of X, W, dX and dW are not "
+                "at 16-byte addresses");
     F3S_REQUIRE(n == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 &&
-                           workspace_bytes >= (int64_t)ce_space(n, K, V).bytes),
+                           workspace_bytes >= (int64_t)pad_space(n, K, V, true).bytes),
                 "f3s_cross_entropy_bwd: workspace too small");
     F3S_TRY(require_device());
     clear_error();
@@ -1529,11 +1628,24 @@ f3s_status f3s_cross_entropy_bwd(const uint16_t* X, int64_t x_stride, const uint
                    reinterpret_cast<const char*>(bias), x_stride, target, ignore_index, n, K, V,
                    reduction, st};
     char* ws = static_cast<char*>(workspace);
+    char *dx = reinterpret_cast<char*>(dX), *dw = reinterpret_cast<char*>(dW);
+    CeArgs b = a;
+    const PadSpace pad = pad_space(n, K, V, true);
+    if (pads(n, K, V)) {
+        b = on_copies(a, pad, ws);
+        if (dx) dx = ws + pad.dx;
+        if (dw) dw = ws + pad.dw;
+    }
     if (dtype == F3S_F16)
-        return loss_backward<_Float16>(a, lse, dloss, reinterpret_cast<char*>(dX),
-                                       reinterpret_cast<char*>(dW), reinterpret_cast<char*>(db), ws);
-    return loss_backward<__bf16>(a, lse, dloss, reinterpret_cast<char*>(dX),
-                                 reinterpret_cast<char*>(dW), reinterpret_cast<char*>(db), ws);
+        F3S_TRY(loss_backward<_Float16>(b, lse, dloss, dx, dw, reinterpret_cast<char*>(db), ws));
+    else
+        F3S_TRY(loss_backward<__bf16>(b, lse, dloss, dx, dw, reinterpret_cast<char*>(db), ws));
+    if (pads(n, K, V)) {
+        if (dX) launch_unpad(dx, reinterpret_cast<char*>(dX), n, K, b.K, st);
+        if (dW) launch_unpad(dw, reinterpret_cast<char*>(dW), V, K, b.K, st);
+        F3S_HIP(hipGetLastError());
+    }
+    return F3S_OK;
 }
 
 }  // extern "C"

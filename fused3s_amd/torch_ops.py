@@ -933,6 +933,11 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     t = target.reshape(-1)
     t = t if t.is_contiguous() else t.contiguous()
     w = weight if weight.is_contiguous() else weight.contiguous()
+    if K % 8 == 0:   # (rows at 16-byte addresses)
+        if x2.data_ptr() % 16 or x2.shape[0] > 1 and (x2.stride(0) % 8 or x2.stride(0) >= 2**22):
+            x2 = x2.clone(memory_format=torch.contiguous_format)
+        if w.data_ptr() % 16:
+            w = w.clone()
     b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
                                     or bias is not None and bias.requires_grad):

@@ -375,8 +375,10 @@ f3s_status f3s_layer_norm_bwd(const void* X, int64_t x_stride, const void* W, co
  * reference counterpart):
  *   Z = X[n][K] W[V][K]^T + bias[V],  loss_i = log sum_c exp Z_ic - Z_i,target[i]
  * X, W and bias (NULL: none) in `dtype` (F3S_F16 or F3S_BF16), sums in float32, Z is
- * not rounded.  Rows of X are x_stride values apart, W is contiguous; no alignment is
- * needed; rows of a multiple of 16 bytes at 16-byte addresses are the fast ones.
+ * not rounded.  Rows of X are x_stride values apart, W is contiguous.  Where K is a
+ * multiple of 8, X, W (and dX, dW) are 16-byte aligned and x_stride is a multiple of 8
+ * below 2^22; other K need no alignment (and run on padded copies where n and n V are
+ * large).
  * target int64 [n]: rows of ignore_index have no loss and no gradient, a target that
  * is no class has NaN as both.  loss float32: [n] for F3S_LOSS_NONE, else [1]
  * (F3S_LOSS_MEAN: over the rows that are not ignored; NaN where all are).  lse, where

@@ -77,6 +77,26 @@ def test_pieces_of_the_classes(gpu, dtype, K):
     check(step(*x, "mean"), *x, "mean")
 
 
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("n,K,V", [(1024, 1, 8200), (1030, 7, 8191), (140_000, 63, 60),
+                                   (90_001, 5, 130), (1000, 257, 8500), (1025, 301, 9001)])
+def test_padded_rows(gpu, n, K, V, dtype):
+    """Many rows of K inputs that are no multiple of eight, also apart from each other; each
+    gradient alone."""
+    from fused3s_amd.torch_ops import linear_cross_entropy
+    x, w, b, t, dloss = inputs(n, K, V, dtype, n + K)
+    got = step(x, w, b, t, dloss, "mean")
+    check(got, x, w, b, t, dloss, "mean")
+    wide = torch.full((n, K + 3), float("nan"), dtype=dtype, device="cuda")
+    wide[:, 1:K + 1] = x
+    for i, name in ((0, "dx"), (1, "dw")):
+        leaves = [wide[:, 1:K + 1], w.cuda(), b.cuda()]
+        leaves[i] = leaves[i].detach().requires_grad_()
+        loss = linear_cross_entropy(leaves[0], leaves[1], t.cuda(), leaves[2])
+        loss.backward(dloss.cuda())
+        assert torch.equal(leaves[i].grad.cpu(), got[name].cpu()), name
+
+
 def test_pieces_of_the_rows(gpu):
     """More blocks than a forward pass holds at a time."""
     from fused3s_amd.torch_ops import linear_cross_entropy

@@ -24,12 +24,15 @@ def test_entry_points_refuse():
     fwd = lambda x=16, stride=8, w=16, target=16, loss=16, n=4, how=1, dtype=0, ws=16, size=1 << 20: \
         h.f3s_cross_entropy_fwd(x, stride, w, None, target, -100, loss, None, n, 8, 8, how, dtype,
                                 ws, size, None)
-    for bad in (dict(x=None), dict(w=None), dict(target=None), dict(loss=None), dict(stride=7),
+    for bad in (dict(x=8), dict(w=8), dict(stride=12), dict(stride=1 << 22),   # (16-byte rows)
+                dict(x=None), dict(w=None), dict(target=None), dict(loss=None), dict(stride=7),
                 dict(n=-1), dict(how=3), dict(how=-1), dict(dtype=2), dict(ws=None), dict(ws=8),
                 dict(size=8)):
         assert fwd(**bad) == 1, bad
     bwd = lambda lse=16, dloss=16, ws=16, size=1 << 30: h.f3s_cross_entropy_bwd(
         16, 8, 16, None, 16, -100, lse, dloss, 16, 16, None, 4, 8, 8, 1, 0, ws, size, None)
+    assert h.f3s_cross_entropy_bwd(16, 8, 16, None, 16, -100, 16, 16, 16, 24, None, 4, 8, 8, 1, 0,
+                                   16, 1 << 30, None) == 1   # (dW at 8 bytes past a 16)
     assert bwd(lse=None) == 1 and bwd(dloss=None) == 1 and bwd(ws=None) == 1 and bwd(size=8) == 1
     assert b"workspace" in h.f3s_last_error()
 
@@ -45,6 +48,21 @@ def test_workspace_goes_with_a_piece_of_the_classes():
             assert need.value >= last // 2
             last = need.value
         assert last < 2**30, back   # (logits in 16 bits: 33 GB)
+
+
+def test_workspace_of_padded_copies():
+    """Rows of K inputs that are no whole pieces: with many rows and classes, copies of rows
+    that are, beside what those take."""
+    h = _lib.hip()
+    need = C.c_int64()
+    def size(n, K, back):
+        assert h.f3s_cross_entropy_workspace(n, K, 10_000, back, C.byref(need)) == 0
+        return need.value
+    for n, K, Kp, copied in ((999, 41, 41, False), (1000, 41, 48, True), (5000, 257, 264, True),
+                             (5000, 48, 48, False)):
+        for back in (0, 1):
+            copies = (1 + back) * 2 * Kp * (n + 10_000) if copied else 0
+            assert 0 <= size(n, K, back) - size(n, Kp, back) - copies < 1024 or not copied
 
 
 def test_binding_refuses():
