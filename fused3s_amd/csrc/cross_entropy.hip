@@ -212,8 +212,8 @@ __global__ void __launch_bounds__(256)
 join_scaled(const float* __restrict__ parts, int64_t count, int32_t slices,
             const float* __restrict__ factor, T* __restrict__ out)
 {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < count) out[i] = (T)(split_sum(parts + i, count, 0, slices) * *factor);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256)
+        out[i] = (T)(split_sum(parts + i, count, 0, slices) * *factor);
 }
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -239,8 +239,8 @@ __global__ void __launch_bounds__(256) loss_zero(T* __restrict__ out, int64_t co
 // the largest logit and the sum of its own classes: nothing crosses lanes before the
 // end, and a row leaves one block for each share of the classes (blockIdx.y), not one
 // for each 64.  Bound by the logits' 7 operations each, one exponential among them.
-// (52,802 x 64 -> 10,778 by tiles 411 us a call, 196 so; 200,003 x
-// 128 -> 300 70 and 42; 16,384 x 256 -> 50,021 743 and 447.)
+// (By tiles and so, us a call: 52,802 x 64 -> 10,778 411 and 196;
+// 200,003 x 128 -> 300 70 and 42; 16,384 x 256 -> 50,021 743 and 447.)
 constexpr int kStreamWaves = 4, kStreamTiles = 2, kStreamRows = 16 * kStreamTiles * kStreamWaves;
 struct StreamParams {
     const char *x, *w, *bias;
@@ -955,29 +955,35 @@ pad_rows(const uint16_t* __restrict__ from, int64_t ld, uint16_t* __restrict__ t
          int32_t K, int32_t Kp)
 {
     typedef uint16_t v8 __attribute__((ext_vector_type(8)));
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / (Kp / 8);
-    const int32_t c = (int32_t)(i % (Kp / 8)) * 8;
-    if (row >= rows) return;
-    const uint16_t* src = from + row * ld + c;
-    v8 v = {};
-    if (c + 8 <= K) v = reinterpret_cast<const Unaligned<v8>*>(src)->v;
-    else
-        for (int k = 0; k < K - c; ++k) v[k] = src[k];
-    *reinterpret_cast<v8*>(to + row * Kp + c) = v;
+    const int32_t pieces = Kp / 8;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * pieces;
+         i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / pieces;
+        const int32_t c = (int32_t)(i % pieces) * 8;
+        const uint16_t* src = from + row * ld + c;
+        v8 v = {};
+        if (c + 8 <= K) v = reinterpret_cast<const Unaligned<v8>*>(src)->v;
+        else
+            for (int k = 0; k < K - c; ++k) v[k] = src[k];
+        *reinterpret_cast<v8*>(to + row * Kp + c) = v;
+    }
 }
 __global__ void __launch_bounds__(256)
 unpad_rows(const uint16_t* __restrict__ from, uint16_t* __restrict__ to, int64_t rows, int32_t K,
            int32_t Kp)
 {
     typedef uint16_t v8 __attribute__((ext_vector_type(8)));
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / (Kp / 8);
-    const int32_t c = (int32_t)(i % (Kp / 8)) * 8;
-    if (row >= rows) return;
-    const v8 v = *reinterpret_cast<const v8*>(from + row * Kp + c);
-    uint16_t* dst = to + row * K + c;
-    if (c + 8 <= K) reinterpret_cast<Unaligned<v8>*>(dst)->v = v;
-    else
-        for (int k = 0; k < K - c; ++k) dst[k] = v[k];
+    const int32_t pieces = Kp / 8;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * pieces;
+         i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / pieces;
+        const int32_t c = (int32_t)(i % pieces) * 8;
+        const v8 v = *reinterpret_cast<const v8*>(from + row * Kp + c);
+        uint16_t* dst = to + row * K + c;
+        if (c + 8 <= K) reinterpret_cast<Unaligned<v8>*>(dst)->v = v;
+        else
+            for (int k = 0; k < K - c; ++k) dst[k] = v[k];
+    }
 }
 
 __global__ void warm_loss_kernel() {}
@@ -999,6 +1005,12 @@ struct CeArgs {
     int32_t reduction;
     hipStream_t st;
 };
+
+// Workgroups of 256 for so many values, below a grid's limit of threads.
+static unsigned element_groups(int64_t count)
+{
+    return (unsigned)std::min<int64_t>(ceil_div(count, 256), 1 << 20);
+}
 
 static Tiling one_split(int64_t rows, int64_t outs, int64_t depth, bool odd)
 {
@@ -1095,7 +1107,7 @@ static void launch_stream(const CeArgs& a, const GemmParams& g, int64_t per, int
 }
 
 // Shares of the streamed rows, as many as fill the chip.
-constexpr int64_t kGradInputs = 256, kGradGroups = 1024;
+constexpr int64_t kGradGroups = 1024;
 static int64_t grad_rows(int64_t K) { return K <= 128 ? 128 : 64; }   // of a workgroup's own
 static int64_t grad_per(int64_t owns, int64_t others, int64_t K)
 {
@@ -1180,18 +1192,13 @@ static f3s_status loss_forward(const CeArgs& a, float* loss, float* lse, char* w
         if (stream) {
             launch_stream<T>(a, p, per, c.nblocks);
         } else {
-        const Tiling t = one_split(p.rows, p.outs, p.depth, a.K % 8 != 0);
-        GemmParams q = p;   // (C is not written, and nothing of bias is read in pieces)
-        q.bias = nullptr;
-        q.outs = ceil_div(a.V, 8) * 8;
-        const Way way = way_of(q) == kAny ? kAny : kWhole;
-        const int32_t tile = tile_size(t, way, kEpiLse);
-        F3S_REQUIRE(ceil_div(p.rows, tile) * ceil_div(p.outs, tile) < ((int64_t)1 << 31),
-                    "cross entropy: too many tiles");
-        p.splits = 1;
-        if (way == kWhole) launch_tiles<T, false, false, kEpiLse, kWhole>(p, tile, a.st);
-        else launch_tiles<T, false, false, kEpiLse, kAny>(p, tile, a.st);
-        c.nblocks = blocks_of(tile, p.outs);
+            const bool whole = a.K % 8 == 0;
+            const int32_t tile = tile_size(one_split(p.rows, p.outs, p.depth, !whole),
+                                           whole ? kWhole : kAny, kEpiLse);
+            p.splits = 1;
+            if (whole) launch_tiles<T, false, false, kEpiLse, kWhole>(p, tile, a.st);
+            else launch_tiles<T, false, false, kEpiLse, kAny>(p, tile, a.st);
+            c.nblocks = blocks_of(tile, p.outs);
         }
         F3S_HIP(hipGetLastError());
         c.rows = p.rows;
@@ -1246,7 +1253,7 @@ static CeSpace ce_space(int64_t n, int64_t K, int64_t V)
         s.bytes = s.few_db + up256(sizeof(float) * (size_t)few_groups(n, true) * V);
         return s;
     }
-    if (!odd && K <= kGradInputs) {
+    if (!odd && K <= kFewInputs) {
         s.bytes = grad_space(n, K, V, s.sums).bytes;
         return s;
     }
@@ -1301,14 +1308,14 @@ static PadSpace pad_space(int64_t n, int64_t K, int64_t V, bool backward)
 static void launch_pad(const char* from, int64_t ld, char* to, int64_t rows, int64_t K, int64_t Kp,
                        hipStream_t st)
 {
-    hipLaunchKernelGGL(pad_rows, dim3((unsigned)ceil_div(rows * (Kp / 8), 256)), dim3(256), 0, st,
+    hipLaunchKernelGGL(pad_rows, dim3(element_groups(rows * (Kp / 8))), dim3(256), 0, st,
                        reinterpret_cast<const uint16_t*>(from), ld, reinterpret_cast<uint16_t*>(to),
                        rows, (int32_t)K, (int32_t)Kp);
 }
 static void launch_unpad(const char* from, char* to, int64_t rows, int64_t K, int64_t Kp,
                          hipStream_t st)
 {
-    hipLaunchKernelGGL(unpad_rows, dim3((unsigned)ceil_div(rows * (Kp / 8), 256)), dim3(256), 0, st,
+    hipLaunchKernelGGL(unpad_rows, dim3(element_groups(rows * (Kp / 8))), dim3(256), 0, st,
                        reinterpret_cast<const uint16_t*>(from), reinterpret_cast<uint16_t*>(to), rows,
                        (int32_t)K, (int32_t)Kp);
 }
@@ -1383,7 +1390,7 @@ static f3s_status loss_backward(const CeArgs& a, const float* lse, const float* 
         F3S_HIP(hipGetLastError());
         return F3S_OK;
     }
-    if (a.K <= kGradInputs && takes_stream(a)) {
+    if (takes_stream(a)) {
         const GradSpace w = grad_space(a.n, a.K, a.V, s.sums);
         auto pass = [&](auto classes, char* out, size_t slices, char* sums_out) -> f3s_status {
             constexpr bool kClasses = decltype(classes)::value;
@@ -1407,7 +1414,7 @@ static f3s_status loss_backward(const CeArgs& a, const float* lse, const float* 
             p.sums = sums_out ? reinterpret_cast<float*>(ws + w.sums) : nullptr;
             launch_grad<T, kClasses>(p, a.st);
             auto join = [&](const float* parts, int64_t values, char* to) {
-                hipLaunchKernelGGL((join_scaled<T>), dim3((unsigned)ceil_div(values, 256)), dim3(256), 0,
+                hipLaunchKernelGGL((join_scaled<T>), dim3(element_groups(values)), dim3(256), 0,
                                    a.st, parts, values, (int32_t)shares, factor,
                                    reinterpret_cast<T*>(to));
             };
@@ -1502,7 +1509,7 @@ static f3s_status loss_backward(const CeArgs& a, const float* lse, const float* 
                 q.C = ws + s.dw;
                 F3S_TRY((launch_of_dz<T, true, kEpiPart>(q, s.tdw, whole, a.st)));
                 const int64_t count = outs * a.K;
-                hipLaunchKernelGGL((join_scaled<T>), dim3((unsigned)ceil_div(count, 256)), dim3(256),
+                hipLaunchKernelGGL((join_scaled<T>), dim3(element_groups(count)), dim3(256),
                                    0, a.st, reinterpret_cast<const float*>(ws + s.dw), count,
                                    s.tdw.splits, factor, reinterpret_cast<T*>(dst));
                 F3S_HIP(hipGetLastError());
@@ -1511,7 +1518,7 @@ static f3s_status loss_backward(const CeArgs& a, const float* lse, const float* 
     }
     if (dX && !s.whole_dx) {
         const int64_t count = a.n * a.K;
-        hipLaunchKernelGGL((join_scaled<T>), dim3((unsigned)ceil_div(count, 256)), dim3(256), 0, a.st,
+        hipLaunchKernelGGL((join_scaled<T>), dim3(element_groups(count)), dim3(256), 0, a.st,
                            reinterpret_cast<const float*>(ws + s.dx), count, s.tdx.splits, factor,
                            reinterpret_cast<T*>(dX));
         F3S_HIP(hipGetLastError());
@@ -1535,8 +1542,8 @@ static f3s_status check_loss(int64_t n, int64_t K, int64_t V, int32_t reduction,
         set_error(std::string(who) + ": bad size, reduction or dtype");
         return F3S_EINVAL;
     }
-    if (K >= (1 << 22) || V >= ((int64_t)1 << 30) || n >= ((int64_t)1 << 31)) {
-        set_error(std::string(who) + ": K below 2^22, classes below 2^30, n below 2^31");
+    if (K >= (1 << 22) || V >= ((int64_t)1 << 30) || n >= ((int64_t)1 << 30)) {
+        set_error(std::string(who) + ": K below 2^22, classes and n below 2^30");
         return F3S_EUNSUPPORTED;
     }
     return F3S_OK;

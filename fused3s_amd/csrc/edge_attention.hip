@@ -994,7 +994,8 @@ static f3s_status launch_edge_pass(EdgeParams p, const f3s_plan* plan, int32_t d
     p.ref_magic = nodes ? 1u << 31 : (uint32_t)ceil_div((int64_t)1 << 31, p.H);
     p.no_ref = nodes ? kNoIdx : kNoRow;
     if (p.num_items <= 0) return F3S_OK;
-    F3S_REQUIRE((p.num_items + p.num_split) * p.H < ((int64_t)1 << 31) &&
+    F3S_REQUIRE((p.num_items + p.num_split) * p.H < ((int64_t)1 << 24) * 3 &&   // (a grid's threads)
+                    (p.num_split + 1) * p.H < ((int64_t)1 << 23) &&
                     (set.team == 1 || set.team == kTeamSmall),
                 "edge attention: too many work items");
     // Offsets of 32 bits where every streamed tensor ends below kNoRow.

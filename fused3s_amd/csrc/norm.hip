@@ -495,7 +495,8 @@ norm_join(const float* __restrict__ parts, int32_t lines, int32_t C, W* __restri
     __shared__ double lds[kJoinParts][17];
     const int col = threadIdx.x % 16, part = threadIdx.x / 16;
     const int64_t c = (int64_t)blockIdx.x * 16 + col, width = 2 * (int64_t)C;
-    const int32_t per = (lines + kJoinParts - 1) / kJoinParts, first = part * per, end = min(lines, first + per);
+    const int32_t per = (lines + kJoinParts - 1) / kJoinParts, first = part * per,
+                  end = min(lines, first + per);
     double s = 0.0;
     if (c < width) {
         for (int32_t i = first; i < end; i += 16) {
@@ -567,7 +568,7 @@ static size_t norm_bytes(int64_t n, int64_t C, int32_t dtype)
     return sizeof(float) * 2 * (size_t)C * (size_t)(s.lanes ? norm_groups(s, n, true) : wide_lines(n));
 }
 
-template <typename T, typename F>
+template <typename T, bool BACKWARD, typename F>
 static void with_shape(const NormShape& s, F go)
 {
     auto one = [&](auto lanes, auto pieces) {
@@ -583,10 +584,10 @@ static void with_shape(const NormShape& s, F go)
     one(std::integral_constant<int, 256>{}, p1);
     one(std::integral_constant<int, 256>{}, p2);
     one(std::integral_constant<int, 512>{}, p2);
-    if constexpr (sizeof(T) == 2) one(std::integral_constant<int, 512>{}, std::integral_constant<int, 4>{});
-    one(std::integral_constant<int, 1024>{}, p2);
-    if constexpr (sizeof(T) == 4)
-        one(std::integral_constant<int, 1024>{}, std::integral_constant<int, 4>{});
+    std::integral_constant<int, 4> p4;
+    if constexpr (BACKWARD && sizeof(T) == 2) one(std::integral_constant<int, 512>{}, p4);
+    else one(std::integral_constant<int, 1024>{}, p2);
+    if constexpr (sizeof(T) == 4) one(std::integral_constant<int, 1024>{}, p4);
 }
 
 template <typename T>
@@ -598,7 +599,7 @@ static void norm_forward(const NormParams& p, int32_t dtype, hipStream_t st)
         hipLaunchKernelGGL((norm_wide_fwd<T>), grid, dim3(kWideThreads), 0, st, p);
         return;
     }
-    with_shape<T>(s, [&](auto lanes, auto pieces) {
+    with_shape<T, false>(s, [&](auto lanes, auto pieces) {
         constexpr int L = decltype(lanes)::value, N = decltype(pieces)::value;
         hipLaunchKernelGGL((norm_fwd_kernel<T, L, N>), grid, dim3(norm_threads(L)), 0, st, p);
     });
@@ -618,7 +619,7 @@ static void norm_backward(const NormParams& p, int32_t dtype, void* dw, void* db
                                dim3((unsigned)ceil_div(p.C, 256), (unsigned)lines), dim3(256), 0, st,
                                p);
     } else {
-        with_shape<T>(s, [&](auto lanes, auto pieces) {
+        with_shape<T, true>(s, [&](auto lanes, auto pieces) {
             constexpr int L = decltype(lanes)::value, N = decltype(pieces)::value;
             hipLaunchKernelGGL((norm_bwd_kernel<T, L, N>), grid, dim3(norm_threads(L)), 0, st, p);
         });
@@ -626,11 +627,11 @@ static void norm_backward(const NormParams& p, int32_t dtype, void* dw, void* db
     if (!p.parts) return;
     const dim3 join((unsigned)ceil_div(2 * (int64_t)p.C, 16));
     if (p.wide_weights)
-        hipLaunchKernelGGL((norm_join<float>), join, dim3(16 * kJoinParts), 0, st, p.parts, (int32_t)lines, p.C,
-                           static_cast<float*>(dw), static_cast<float*>(db));
+        hipLaunchKernelGGL((norm_join<float>), join, dim3(16 * kJoinParts), 0, st, p.parts,
+                           (int32_t)lines, p.C, static_cast<float*>(dw), static_cast<float*>(db));
     else
-        hipLaunchKernelGGL((norm_join<T>), join, dim3(16 * kJoinParts), 0, st, p.parts, (int32_t)lines, p.C,
-                           static_cast<T*>(dw), static_cast<T*>(db));
+        hipLaunchKernelGGL((norm_join<T>), join, dim3(16 * kJoinParts), 0, st, p.parts,
+                           (int32_t)lines, p.C, static_cast<T*>(dw), static_cast<T*>(db));
 }
 
 template <typename W>

@@ -382,7 +382,7 @@ f3s_status f3s_layer_norm_bwd(const void* X, int64_t x_stride, const void* W, co
  * target int64 [n]: rows of ignore_index have no loss and no gradient, a target that
  * is no class has NaN as both.  loss float32: [n] for F3S_LOSS_NONE, else [1]
  * (F3S_LOSS_MEAN: over the rows that are not ignored; NaN where all are).  lse, where
- * not NULL, receives n + 1 float32 for the gradient.  K < 2^22, V < 2^30, n < 2^31.
+ * not NULL, receives n + 1 float32 for the gradient.  K < 2^22, V and n < 2^30.
  * workspace: f3s_cross_entropy_workspace bytes, 16-byte aligned, this call's alone
  * until it is done; nothing is allocated, calls may overlap and be captured.
  * Deterministic.  Asynchronous on `stream`. */
@@ -461,14 +461,14 @@ f3s_status f3s_diff_attention_bwd(const f3s_plan* plan, const f3s_plan* reversed
  *   s = cap tanh(x / cap) - slopes[h] |positions[i] - positions[j]|
  *   O[i] = sum_j softmax_j(s) V[j]
  * over the edges (i, j) (masked semantics); rows without edges get 0.  cap 0: s = x
- * there (else 1e-30 to 1e30); dims 0: no positions.  positions float32 [n][dims], dims 1 to 3, distances
- * Euclidean in float32; slopes float32 [H].  H is the plan's; a head of a row is 64 contiguous values of `dtype`
- * (F3S_F16 or F3S_BF16), heads adjacent, rows `*_stride` values apart (a multiple of
- * 8, at least H * 64), pointers 16-byte aligned.  lse, where not NULL, receives
- * [n][H] float32 for the gradient.  Sums and softmax statistics are float32, O is
- * rounded once.  An infinite or NaN value reaches the rows with an edge to its node
- * only.  A row whose scores are all -inf is 0, as one without edges.
- * Deterministic.
+ * there (else 1e-30 to 1e30); dims 0: no positions.  positions float32 [n][dims], dims
+ * 1 to 3, distances Euclidean in float32; slopes float32 [H].  H is the plan's; a head
+ * of a row is 64 contiguous values of `dtype` (F3S_F16 or F3S_BF16), heads adjacent,
+ * rows `*_stride` values apart (a multiple of 8, at least H * 64), pointers 16-byte
+ * aligned.  lse, where not NULL, receives [n][H] float32 for the gradient.  Sums and
+ * softmax statistics are float32, O is rounded once.  An infinite or NaN value reaches
+ * the rows with an edge to its node only.  A row whose scores are all -inf is 0, as one
+ * without edges.  Deterministic.
  * workspace: f3s_edge_attention_workspace bytes (reversed NULL), 16-byte aligned,
  * this call's alone until it is done; nothing else is allocated or kept, so calls
  * may overlap and be captured.  Asynchronous on `stream`. */
