@@ -222,6 +222,39 @@ def test_layouts(gpu):
         assert torch.equal(g, want["dw"])
 
 
+@pytest.mark.parametrize("K,V", [(40, 54_000_000), (264, 8_200_001)])
+def test_classes_past_4_gib(gpu, K, V):
+    """Every class but some at both ends and between has a bias of -inf: the loss is theirs."""
+    x, w, _, _, dloss = inputs(5, K, 8, torch.bfloat16, 11)
+    w = torch.randn(V, K, device="cuda", dtype=torch.bfloat16)
+    some = torch.cat([torch.arange(30), V // 2 + torch.arange(30), V - 30 + torch.arange(30)]).cuda()
+    b = torch.full((V,), float("-inf"), device="cuda", dtype=torch.bfloat16)
+    b[some] = torch.linspace(-1, 1, 90, device="cuda").bfloat16()
+    t = torch.tensor([0, 89, 45, 60, 10], device="cuda")
+    got = step(x, w, b, some[t], dloss, "mean")
+    for name in ("dw", "db"):
+        whole, got[name] = got[name], got[name][some]
+        whole[some] = 0
+        assert not whole.any(), name
+        del whole
+    check(got, x, w[some], b[some], t, dloss, "mean")
+
+
+@pytest.mark.parametrize("n,K,V", [(54_000_000, 40, 50), (54_000_000, 40, 100), (8_200_001, 264, 70)])
+def test_rows_past_4_gib(gpu, n, K, V):
+    """Every row but some at both ends and between is ignored: the loss is theirs."""
+    _, w, b, _, dloss = inputs(5, K, V, torch.bfloat16, 12, reduction="sum")
+    x = torch.randn(n, K, device="cuda", dtype=torch.bfloat16)
+    some = torch.cat([torch.arange(30), n // 2 + torch.arange(30), n - 30 + torch.arange(30)]).cuda()
+    t = torch.full((n,), -100, device="cuda")
+    t[some] = torch.randint(V, (90,), device="cuda")
+    got = step(x, w, b, t, dloss, "sum")
+    whole, got["dx"] = got["dx"], got["dx"][some]
+    whole[some] = 0
+    assert not whole.any()
+    check(got, x[some], w, b, t[some], dloss, "sum")
+
+
 def test_streams_and_capture(gpu):
     """Two calls at once, and a captured step replayed with new inputs, each replay against
     the eager result."""

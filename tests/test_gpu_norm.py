@@ -130,6 +130,20 @@ def test_odd_values_stay_in_their_row(gpu):
         assert got["dw"].isnan().all() and torch.equal(got["db"], clean["db"])
 
 
+@pytest.mark.parametrize("n,C", [(17_000_001, 128), (40_000, 56_000)])
+def test_past_32_bit_offsets(gpu, n, C):
+    """Rows at both ends and between; the others' dy is 0."""
+    _, w, b, dy = inputs(90, C, torch.bfloat16, torch.bfloat16, 13)
+    x = torch.randn(n, C, device="cuda", dtype=torch.bfloat16)
+    some = torch.cat([torch.arange(30), n // 2 + torch.arange(30), n - 30 + torch.arange(30)]).cuda()
+    whole = torch.zeros(n, C, device="cuda", dtype=torch.bfloat16)
+    whole[some] = dy
+    got = step(x, w, b, whole)
+    for name in ("y", "dx"):
+        got[name] = got[name][some]
+    check(got, x[some], w, b, dy)
+
+
 def test_other_stream_and_capture(gpu):
     """On a stream of its own, and captured and replayed with new inputs, each replay
     against the eager result."""
