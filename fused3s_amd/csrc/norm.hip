@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(256) norm_wide_sums(const NormParams p)
 
 // dw and db from the workgroups' lines, in 64 bits: 16 columns by 64 parts of the
 // lines, the parts added in order.  (1,024 lines of 512: 20 us by 16 parts, whose loads
-// were waited for four times, 6 so.)
+// were waited for four times, 7 so.)
 constexpr int kJoinParts = 64;
 template <typename W>
 __global__ void __launch_bounds__(16 * kJoinParts)
@@ -541,7 +541,7 @@ static NormShape norm_shape(int64_t C, int32_t dtype, bool backward)
         if (have <= lanes) return {lanes, 1};
     if (have <= 128) return {64, 2};
     // (the gradient's registers: 32 values a lane in 512 lanes; 16 in 1,024 spilled, 12,736
-    // wide in bfloat16 486 us a step, 318 so)
+    // wide in bfloat16 486 us a step, 298 so)
     if (backward && dtype != F3S_F32 && have > 1024 && have <= 2048) return {512, 4};
     for (int32_t lanes : {256, 512, 1024})
         for (int32_t pieces : {1, 2})
