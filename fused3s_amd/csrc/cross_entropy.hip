@@ -239,8 +239,8 @@ __global__ void __launch_bounds__(256) loss_zero(T* __restrict__ out, int64_t co
 // the largest logit and the sum of its own classes: nothing crosses lanes before the
 // end, and a row leaves one block for each share of the classes (blockIdx.y), not one
 // for each 64.  Bound by the logits' 7 operations each, one exponential among them.
-// (By tiles and so, us a call: 52,802 x 64 -> 10,778 411 and 196;
-// 200,003 x 128 -> 300 70 and 42; 16,384 x 256 -> 50,021 743 and 447.)
+// (By tiles and so, us a call: 52,802 x 64 -> 10,778 411 and 150;
+// 200,003 x 128 -> 300 70 and 41; 16,384 x 256 -> 50,021 743 and 430.)
 constexpr int kStreamWaves = 4, kStreamTiles = 2, kStreamRows = 16 * kStreamTiles * kStreamWaves;
 struct StreamParams {
     const char *x, *w, *bias;
@@ -377,8 +377,8 @@ __global__ void __launch_bounds__(kStreamWaves * kWave) stream_lse_kernel(const 
 // A lane's logits of a row are the operand of the product after them, whose other one is
 // the same rows in LDS, read transposed.  Shares of the streamed rows (blockIdx.y) are
 // added by join_scaled.  One product of five more than by tiles, and none of dz's bytes.
-// (A training step by tiles and so, us: 52,802 x 64 -> 10,778 1,324 and 690; x 128 1,473
-// and 953; x 256 2,147 and 1,814; 16,384 x 256 -> 50,021 3,277 and 2,457.)
+// (A training step by tiles and so, us: 52,802 x 64 -> 10,778 1,324 and 672; x 128 1,473
+// and 879; x 256 2,147 and 1,669; 16,384 x 256 -> 50,021 3,277 and 2,303.)
 struct GradParams {
     const char *own, *other;
     int64_t ld_own, ld_other, owns, others;
@@ -1064,26 +1064,60 @@ static void launch_few(const FewParams& p, hipStream_t st)
     else of_k(std::integral_constant<int, 4>{});
 }
 
-// Workspace of a forward pass: the workgroups' sums, z at the targets, the blocks of as
-// many rows at a time as kBlocksBytes hold.
+// Chunks of 64 streamed rows in a share, for `groups` workgroups of which `slots` run at
+// once: the least rounds of shares, whose starts and ends are some two chunks, and whose
+// results `cost` chunks where there are several.  (By this and with one round's groups
+// at most, us: 52,802 x 64 -> 10,778 143 and 172 forward, 672 and 687 trained; 272,567 x
+// 128 -> 23,790 1,906 and 2,413, 8,849 and 10,017; 70,000 x 64 -> 5,000 93 and 134, 422
+// and 482.)
+static int64_t share_of(int64_t groups, int64_t chunks, int64_t slots, double cost)
+{
+    int64_t best = chunks;
+    double least = INFINITY;
+    auto look = [&](int64_t shares) {
+        const int64_t per = ceil_div(chunks, std::min(chunks, std::max<int64_t>(1, shares)));
+        shares = ceil_div(chunks, per);
+        const double t = (double)ceil_div(groups * shares, slots) * (double)(per + 2) +
+                         (shares > 1 ? cost * (double)shares : 0.0);
+        if (t < least) {
+            least = t;
+            best = per;
+        }
+    };
+    for (int64_t k = 1; k <= 8; ++k) look(k);
+    for (int64_t k = 1; k <= 4; ++k) look(k * slots / groups);
+    return best;
+}
+
+static bool streams(int64_t K) { return K <= kFewInputs && K % 8 == 0; }
+// (by their LDS; four, two per CU)
+static int64_t stream_slots(int64_t K) { return K <= 128 ? 1024 : 512; }
+
+// Workspace of a forward pass: the workgroups' sums, z at the targets, the blocks: one a
+// share of the classes, or of as many rows at a time as kBlocksBytes hold.
 struct ForwardSpace {
     size_t picked = 0, blocks = 0, bytes = 0;
-    int64_t rows = 0, nblocks = 0;
+    int64_t rows = 0, nblocks = 0, per = 0;
 };
-static ForwardSpace forward_space(int64_t n, int64_t V)
+static ForwardSpace forward_space(int64_t n, int64_t K, int64_t V)
 {
     ForwardSpace s;
-    s.nblocks = ceil_div(V, 32) + 8;   // (at most: the smallest blocks, and a tile's last ones)
-    s.rows = std::max<int64_t>(1024, kBlocksBytes / 8 / s.nblocks / 1024 * 1024);
-    s.rows = std::min(s.rows, n);
+    if (streams(K)) {
+        const int64_t chunks = ceil_div(V, 64);
+        s.per = share_of(ceil_div(n, kStreamRows), chunks, stream_slots(K), 0.0);
+        s.nblocks = ceil_div(chunks, s.per);
+        s.rows = n;
+    } else {
+        s.nblocks = ceil_div(V, 32) + 8;   // (at most: the smallest blocks, and a tile's last ones)
+        s.rows = std::max<int64_t>(1024, kBlocksBytes / 8 / s.nblocks / 1024 * 1024);
+        s.rows = std::min(s.rows, n);
+    }
     s.picked = up256(sizeof(double) * 2 * (size_t)ceil_div(n, 4));
     s.blocks = s.picked + up256(sizeof(float) * (size_t)s.rows);
     s.bytes = s.blocks + up256(sizeof(float2) * (size_t)s.rows * s.nblocks);
     return s;
 }
 
-static bool takes_stream(const CeArgs& a) { return a.K <= kFewInputs && a.K % 8 == 0; }
-constexpr int64_t kStreamGroups = 1024;   // four per CU
 template <typename T>
 static void launch_stream(const CeArgs& a, const GemmParams& g, int64_t per, int64_t shares)
 {
@@ -1106,13 +1140,14 @@ static void launch_stream(const CeArgs& a, const GemmParams& g, int64_t per, int
     else hipLaunchKernelGGL((stream_lse_kernel<T, 4>), grid, block, 0, a.st, p);
 }
 
-// Shares of the streamed rows, as many as fill the chip.
-constexpr int64_t kGradGroups = 1024;
+// Shares of the streamed rows.  A chunk takes some 2.2 us, an output's slice 8 bytes at
+// 4 TB/s, written and read.
+constexpr int64_t kGradSlots = 512;   // two per CU
 static int64_t grad_rows(int64_t K) { return K <= 128 ? 128 : 64; }   // of a workgroup's own
 static int64_t grad_per(int64_t owns, int64_t others, int64_t K)
 {
-    const int64_t chunks = ceil_div(others, 64), groups = ceil_div(owns, grad_rows(K));
-    return ceil_div(chunks, std::min(chunks, std::max<int64_t>(1, kGradGroups / groups)));
+    return share_of(ceil_div(owns, grad_rows(K)), ceil_div(others, 64), kGradSlots,
+                    (double)owns * (double)K * (8 / 4e6 / 2.2));
 }
 static int64_t grad_shares(int64_t owns, int64_t others, int64_t K)
 {
@@ -1138,7 +1173,7 @@ static int32_t blocks_of(int32_t tile, int64_t outs)
 template <typename T>
 static f3s_status loss_forward(const CeArgs& a, float* loss, float* lse, char* ws)
 {
-    const ForwardSpace s = forward_space(a.n, a.V);
+    const ForwardSpace s = forward_space(a.n, a.K, a.V);
     CeParams c{};
     c.target = a.target;
     c.n = a.n;
@@ -1162,17 +1197,8 @@ static f3s_status loss_forward(const CeArgs& a, float* loss, float* lse, char* w
         F3S_HIP(hipGetLastError());
         return F3S_OK;
     }
-    const bool stream = takes_stream(a);
-    int64_t per = 0;
-    if (stream) {
-        const int64_t chunks = ceil_div(a.V, 64), groups = ceil_div(std::min(s.rows, a.n), kStreamRows);
-        const int64_t at_once = a.K <= 128 ? kStreamGroups : kStreamGroups / 2;   // (by their LDS)
-        const int64_t shares = std::min(chunks, std::max<int64_t>(1, at_once / groups));
-        per = ceil_div(chunks, shares);
-        c.nblocks = ceil_div(chunks, per);
-    } else {
-        c.nblocks = ceil_div(a.V, 64);   // (or twice as many)
-    }
+    const bool stream = streams(a.K);
+    c.nblocks = stream ? s.nblocks : ceil_div(a.V, 64);   // (or twice as many)
     // Rows per workgroup of a join; the rows of a piece are a multiple of 1,024.
     const int join = c.nblocks <= 16 && a.n >= 4096 ? 256 : a.n <= 2048 ? 4 : 16;
     c.nparts = ceil_div(a.n, join);
@@ -1190,7 +1216,7 @@ static f3s_status loss_forward(const CeArgs& a, float* loss, float* lse, char* w
         p.loss.blocks = reinterpret_cast<float2*>(ws + s.blocks);
         p.loss.picked = reinterpret_cast<float*>(ws + s.picked);
         if (stream) {
-            launch_stream<T>(a, p, per, c.nblocks);
+            launch_stream<T>(a, p, s.per, c.nblocks);
         } else {
             const bool whole = a.K % 8 == 0;
             const int32_t tile = tile_size(one_split(p.rows, p.outs, p.depth, !whole),
@@ -1292,8 +1318,10 @@ static PadSpace pad_space(int64_t n, int64_t K, int64_t V, bool backward)
 {
     const int64_t Kp = ceil_div(K, 8) * 8;
     PadSpace s;
-    s.bytes = backward ? ce_space(n, pads(n, K, V) ? Kp : K, V).bytes : forward_space(n, V).bytes;
-    if (!pads(n, K, V)) return s;
+    const bool copies = pads(n, K, V);
+    s.bytes = backward ? ce_space(n, copies ? Kp : K, V).bytes
+                       : forward_space(n, copies ? Kp : K, V).bytes;
+    if (!copies) return s;
     const size_t x = up256(2 * (size_t)n * Kp), w = up256(2 * (size_t)V * Kp);
     s.x = s.bytes;
     s.w = s.x + x;
@@ -1390,7 +1418,7 @@ static f3s_status loss_backward(const CeArgs& a, const float* lse, const float* 
         F3S_HIP(hipGetLastError());
         return F3S_OK;
     }
-    if (takes_stream(a)) {
+    if (streams(a.K)) {
         const GradSpace w = grad_space(a.n, a.K, a.V, s.sums);
         auto pass = [&](auto classes, char* out, size_t slices, char* sums_out) -> f3s_status {
             constexpr bool kClasses = decltype(classes)::value;

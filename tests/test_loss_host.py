@@ -38,16 +38,16 @@ def test_entry_points_refuse():
 
 
 def test_workspace_goes_with_a_piece_of_the_classes():
-    """Not with n V: the backward pass's for a million classes is a piece's."""
+    """Not with n V: the backward pass's for a million classes is a piece's.  (Fewer
+    classes may need more: what few inputs leave goes with the shares of the classes.)"""
     h = _lib.hip()
     need = C.c_int64()
-    for back in (0, 1):
-        last = 0
-        for V in (2, 47, 1000, 50_021, 1_000_000):
-            assert h.f3s_cross_entropy_workspace(16_384, 64, V, back, C.byref(need)) == 0
-            assert need.value >= last // 2
-            last = need.value
-        assert last < 2**30, back   # (logits in 16 bits: 33 GB)
+    for K in (64, 264):
+        for back in (0, 1):
+            for V in (2, 47, 1000, 50_021, 1_000_000):
+                assert h.f3s_cross_entropy_workspace(16_384, K, V, back, C.byref(need)) == 0
+                # (logits in 16 bits of a million: 33 GB)
+                assert 0 < need.value < 2**30, (K, V, back)
 
 
 def test_workspace_of_padded_copies():
