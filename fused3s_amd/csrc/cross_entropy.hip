@@ -16,7 +16,8 @@
 //            would take.
 // Of few inputs (K <= 256) the logits, and dz, stay in registers: below.
 // dz is rounded to the type, the operand that dx and dW take: these two carry that
-// rounding beside their own; db is summed before it.  What dz is multiplied with
+// rounding beside their own; db is summed before it.  (Of few classes, where bytes bound
+// the passes and not products, it goes on as the sum of two 16-bit values.)  What dz is multiplied with
 // throughout (1 / count, a loss scale) comes last, in float32, so that small gradients
 // do not vanish: dz itself is of size 1 at most, in binary16 times 2^14, as a class
 // of probability 1e-9 still has its 11 bits then.
@@ -760,7 +761,9 @@ __device__ __forceinline__ typename Half<T>::v8 few_columns(const char* at, int 
 
 // 128 rows at a time, 16 a wave: z, dz and dx of a wave's own; then x and dz, through a
 // stage of all 128, for the wave's share of dW's dim tiles (with fewer tiles than waves,
-// of the rows too: a slice each).
+// of the rows too: a slice each).  dz is the sum of two 16-bit values (split8): rounded
+// once, it added as much to the error of dx and dW as their own rounding.  (200,003 x
+// 128 -> 47 trained, kernels: 62 us rounded, 67 so; x 256 -> 47 112 and 120.)
 template <typename T, int KF, int NV>
 __global__ void __launch_bounds__(kFewWaves * kWave) few_classes_bwd(const FewParams p)
 {
@@ -771,11 +774,13 @@ __global__ void __launch_bounds__(kFewWaves * kWave) few_classes_bwd(const FewPa
     constexpr int kSlices = kTiles >= kFewWaves ? 1 : kFewWaves / kTiles;
     // (rows that begin 32 bytes apart modulo 256: eight of them read at once)
     constexpr int kXRow = 64 * KF + 32, kDRow = 32 * NV + (NV > 1 ? 32 : 0);
+    // dz's halves lie in LDS side by side, or (256 inputs, 64 classes: 160 KB) in turn
+    constexpr int kDBytes = kFewWaves * 16 * kDRow, kInTurn = KF == 8 && NV == 4 ? 2 : 1;
     __shared__ __align__(16) v8 wl[NV * KF * kWave];
     __shared__ __align__(16) v8 wt[kTiles * kFrags * kWave];
     __shared__ __align__(16) float bl[kFewClasses];
     __shared__ __align__(16) char xs[kFewWaves * 16 * kXRow];
-    __shared__ __align__(16) char ds[kFewWaves * 16 * kDRow];
+    __shared__ __align__(16) char ds[2 / kInTurn * kDBytes];
     const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
     const int g = lane >> 4, r = lane & 15;
     const int64_t step = (int64_t)gridDim.x * kFewWaves * 16;
@@ -821,10 +826,12 @@ __global__ void __launch_bounds__(kFewWaves * kWave) few_classes_bwd(const FewPa
         for (int f = 0; f < KF; ++f) x[f] = next[f];
         const int64_t t = next_t;
         const float f = next_f, lse = next_lse;
-        if (first + step < p.n) load(first + step);
+        if (kInTurn == 1 && first + step < p.n) load(first + step);
         f4 z[NV];
         few_logits<T, KF, NV>(x, wl, bl, lane, z);
-        v8 dz[kFrags] = {};
+        // as the sum of two 16-bit values
+        v8 dz[2][kFrags];
+        float whole[kFrags][8] = {};
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
 #pragma unroll
@@ -834,19 +841,30 @@ __global__ void __launch_bounds__(kFewWaves * kWave) few_classes_bwd(const FewPa
                 d = f == 0.f ? 0.f : d * f;
                 if (NV * 16 > p.V && 16 * i + 4 * g + v >= p.V) d = 0.f;   // (f may be NaN)
                 db[i][v] += d;
-                dz[i / 2][4 * (i & 1) + v] = (T)d;
+                whole[i / 2][4 * (i & 1) + v] = d;
             }
         }
-        if (p.dw) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
-                *reinterpret_cast<v4*>(own_d + r * kDRow + 2 * (16 * i + 4 * g)) =
-                    (i & 1) ? __builtin_shufflevector(dz[i / 2], dz[i / 2], 4, 5, 6, 7)
-                            : __builtin_shufflevector(dz[i / 2], dz[i / 2], 0, 1, 2, 3);
+        for (int k = 0; k < kFrags; ++k) split8<T>(whole[k], dz[0][k], dz[1][k]);
+        if (p.dw) {
 #pragma unroll
             for (int k = 0; k < KF; ++k)   // (rows past the last: with dz of 0, and finite)
                 *reinterpret_cast<v8*>(own_x + r * kXRow + 64 * k + 16 * g) =
                     first + 16 * wave + r < p.n ? x[k] : v8{};
+        }
+        // (registers: behind the logits, where x is done with)
+        if (kInTurn > 1 && first + step < p.n) load(first + step);
+#pragma unroll
+        for (int turn = 0; turn < (p.dw ? kInTurn : 0); ++turn) {
+#pragma unroll
+            for (int half = 0; half < 2 / kInTurn; ++half)
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const v8 of = dz[kInTurn > 1 ? turn : half][i / 2];
+                    *reinterpret_cast<v4*>(own_d + half * kDBytes + r * kDRow + 2 * (16 * i + 4 * g)) =
+                        (i & 1) ? __builtin_shufflevector(of, of, 4, 5, 6, 7)
+                                : __builtin_shufflevector(of, of, 0, 1, 2, 3);
+                }
             __syncthreads();
 #pragma unroll
             for (int u = 0; u < kOwn; ++u) {
@@ -857,9 +875,12 @@ __global__ void __launch_bounds__(kFewWaves * kWave) few_classes_bwd(const FewPa
                     const int rows = 32 * ((kSlices > 1 ? wave / kTiles * kParts : 0) + q);
                     const v8 b = few_columns<T>(xs + rows * kXRow, kXRow, tile, lane);
 #pragma unroll
-                    for (int i = 0; i < NV; ++i)
-                        dw[u][i] = Half<T>::mfma(few_columns<T>(ds + rows * kDRow, kDRow, i, lane), b,
-                                                 dw[u][i]);
+                    for (int half = 0; half < 2 / kInTurn; ++half)
+#pragma unroll
+                        for (int i = 0; i < NV; ++i)
+                            dw[u][i] = Half<T>::mfma(
+                                few_columns<T>(ds + half * kDBytes + rows * kDRow, kDRow, i, lane), b,
+                                dw[u][i]);
                 }
             }
             __syncthreads();
@@ -870,8 +891,11 @@ __global__ void __launch_bounds__(kFewWaves * kWave) few_classes_bwd(const FewPa
             for (int tile = 0; tile < kTiles; ++tile) {
                 f4 d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int k = 0; k < kFrags; ++k)
-                    d = Half<T>::mfma(wt[(tile * kFrags + k) * kWave + lane], dz[k], d);
+                for (int k = 0; k < kFrags; ++k) {
+                    const v8 w = wt[(tile * kFrags + k) * kWave + lane];
+                    d = Half<T>::mfma(w, dz[0][k], d);
+                    d = Half<T>::mfma(w, dz[1][k], d);
+                }
                 *reinterpret_cast<v4*>(own_x + r * kXRow + 2 * (16 * tile + 4 * g)) =
                     __builtin_convertvector(d * factor, v4);
             }

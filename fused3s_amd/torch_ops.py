@@ -902,7 +902,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     are float32.  Differentiable (once) in x, weight and bias; for the backward pass the
     logits are computed again, some classes at a time, and their gradient (up to what
     multiplies all of it: the mean's divisor, a loss scale) is rounded to the type before
-    the gradients of x and weight are made of it, so these two are rounded twice.
+    the gradients of x and weight are made of it, so these two are rounded twice (once
+    where V is 64 and K 256 at most, K a multiple of 8).
     Tracing, functorch's transforms and forward-mode differentiation are refused."""
     _refuse_unseen("linear_cross_entropy", x, weight, target, bias)
     how = _REDUCTIONS.get(reduction)
