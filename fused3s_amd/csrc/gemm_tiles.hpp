@@ -585,25 +585,11 @@ gemm_kernel(const GemmParams p)
                         top = __builtin_fmaxf(top, acc[i][j][v]);
                     }
                 top = row_max4(top);
-                // (a block of classes that a bias of the type's lowest value takes out:
-                // times log2(e) it has none)
-                if (__ballot(top < -1e38f)) {
-                    const float mu = top == -INFINITY ? 0.f : top;
+                const float mu = top == -INFINITY ? 0.f : top;
 #pragma unroll
-                    for (int i = 0; i < kNo; ++i)
+                for (int i = 0; i < kNo; ++i)
 #pragma unroll
-                        for (int v = 0; v < 4; ++v)   // (every row its own way)
-                            sum += fast_exp2(top < -1e38f
-                                                 ? (acc[i][j][v] - mu) * kLog2eF
-                                                 : __builtin_fmaf(acc[i][j][v], kLog2eF, -mu * kLog2eF));
-                } else {
-                    const float mu = top * kLog2eF;
-#pragma unroll
-                    for (int i = 0; i < kNo; ++i)
-#pragma unroll
-                        for (int v = 0; v < 4; ++v)
-                            sum += fast_exp2(__builtin_fmaf(acc[i][j][v], kLog2eF, -mu));
-                }
+                    for (int v = 0; v < 4; ++v) sum += fast_exp2((acc[i][j][v] - mu) * kLog2eF);
                 sum += __shfl_xor(sum, 16, kWave);
                 sum += __shfl_xor(sum, 32, kWave);
                 if (g == 0 && row < p.rows) blocks[row] = make_float2(top, sum);
@@ -661,18 +647,11 @@ gemm_kernel(const GemmParams p)
                 } else if constexpr (EPI == kEpiProb) {
                     const RowInfo of = info[S::rows * wr + 16 * j + rr];
                     if (row < p.rows && out < p.outs) {
-                        // (8 operations a value, one exponential among them, as many as the
+                        // (9 operations a value, one exponential among them, as many as the
                         // products of 64 steps take; 14 of them: 97 us for 16,384 x 512 ->
                         // 4,096, where nothing overlaps them)
                         float d[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                        if (of.lse < -1e38f) {   // (times log2(e) it has none)
-                            each(d, [&](float z) { return fast_exp2((z - of.lse) * kLog2eF); });
-                        } else {
-                            const float lse = of.lse * kLog2eF;
-                            each(d, [&](float z) {
-                                return fast_exp2(__builtin_fmaf(z, kLog2eF, -lse));
-                            });
-                        }
+                        each(d, [&](float z) { return fast_exp2((z - of.lse) * kLog2eF); });
                         const int t = of.t - (int)out;
                         if (t >= 0 && t < 8 && of.t >= 0) {
 #pragma unroll
