@@ -13,9 +13,9 @@
 // Three passes of one shape: a wave takes a window of 16 rows of one head and streams
 // the rows at the other ends of its edges past it, 32 a chunk, two 128-byte rows each:
 //   forward  k, v past q:       m, l and the sums of p v
-//   rows     k, v past q, do:   the sums of p g c k, p c k, p g and p:
-//            dq = scale (sum p g c k - D sum p c k) needs no second sweep for D, and
-//            nothing of o is kept from the forward pass but a log-sum-exp
+//   rows     k, v past q, do:   the sums of p g' c k, p c k, p g' and p, g' = g - the mean
+//            of the row's first g: dq = scale (sum p g' c k - D' sum p c k) needs no second
+//            sweep for D, and nothing of o is kept from the forward pass but a log-sum-exp
 //   columns  q, do past k, v, on the plan of the reversed edges: dk, dv; no atomics
 // What bounds them is the random 256 bytes per edge and head.
 //
@@ -80,14 +80,14 @@ static inline int32_t stat_words(int32_t dims) { return dims == 0 ? 2 : dims <= 
 // A wave's sums, tiles of 16 dims, lane (g, r) holding dims 16 t + 4 g + v of row r in
 // tile t (v: the element), and its share of row r's sums of weights.
 //   forward: tiles 0-3 sum p v, scaled by 2^-x, x the running maximum; y: l
-//   rows:    0-3 sum p g c k, scaled by 2^-x; 4-7 sum p c k; y: sum p g, z: sum p,
-//            yd, zd: the same times the distance
+//   rows:    0-3 sum p g' c k, scaled by 2^-x; 4-7 sum p c k; y: sum p g', z: sum p,
+//            yd, zd: the same times the distance; ref: g - g', mass: recentre()
 //   columns: 0-3 sum ds q, scaled by 2^-x; 4-7 dv
 template <int PASS>
 struct EdgeState {
     static constexpr int tiles = PASS == kForward ? 4 : 8;
     f4 acc[tiles];
-    float x, y, z, yd, zd;
+    float x, y, z, yd, zd, ref, mass;
 };
 // floats of a published state
 template <int PASS>
@@ -100,6 +100,7 @@ __device__ __forceinline__ void clear(EdgeState<PASS>& s)
     for (int t = 0; t < s.tiles; ++t) s.acc[t] = f4{0.f, 0.f, 0.f, 0.f};
     s.x = -INFINITY;
     s.y = s.z = s.yd = s.zd = 0.f;
+    s.ref = s.mass = 0.f;
 }
 
 template <int PASS>
@@ -116,6 +117,10 @@ __device__ __forceinline__ void publish(const EdgeState<PASS>& s, float* dst, in
     for (int t = 0; t < s.tiles; ++t) *reinterpret_cast<f4*>(&dst[(t * kWave + lane) * 4]) = s.acc[t];
     *reinterpret_cast<f4*>(&dst[(s.tiles * kWave + lane) * 4]) = f4{s.x, s.y, s.z, s.yd};
     dst[(s.tiles + 1) * kWave * 4 + lane] = s.zd;
+    if constexpr (PASS == kRows) {
+        dst[((s.tiles + 1) * 4 + 1) * kWave + lane] = s.ref;
+        dst[((s.tiles + 1) * 4 + 2) * kWave + lane] = s.mass;
+    }
 }
 
 // Takes a published state into s.
@@ -128,14 +133,30 @@ __device__ __forceinline__ void absorb(EdgeState<PASS>& s, const float* src, int
 #pragma unroll
     for (int t = 0; t < s.tiles; ++t)
         a[t] = *reinterpret_cast<const f4*>(&src[(t * kWave + lane) * 4]);
+    const float ref = PASS == kRows ? src[((s.tiles + 1) * 4 + 1) * kWave + lane] : 0.f;
+    const float mass = PASS == kRows ? src[((s.tiles + 1) * 4 + 2) * kWave + lane] : 0.f;
     __builtin_amdgcn_sched_barrier(0);
-    const float top = __builtin_fmaxf(s.x, w[0]);
+    float top = __builtin_fmaxf(s.x, w[0]);
+    // (rows) the lighter one's sums move to the heavier one's reference
+    const bool moves = mass > s.mass;   // (s does)
+    const float apart = moves ? s.ref - ref : ref - s.ref;
+    if (PASS == kRows && apart != 0.f)   // (a scale in which it is of a size)
+        top = __builtin_fmaxf(top, (float)(__builtin_amdgcn_frexp_expf(apart) - 24));
     const float mine = top == -INFINITY ? 0.f : fast_exp2(s.x - top);
     const float theirs = top == -INFINITY ? 0.f : fast_exp2(w[0] - top);
     rescale(s, mine);
     if constexpr (PASS == kForward) {
         s.y = s.y * mine + w[1] * theirs;
     } else {
+        if constexpr (PASS == kRows) {
+            s.y = __builtin_fmaf(apart, moves ? s.z : w[2], s.y);
+            s.yd = __builtin_fmaf(apart, moves ? s.zd : zd, s.yd);
+            const float by = apart != 0.f ? apart * fast_exp2(-top) : 0.f;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) s.acc[t] += by * (moves ? s.acc[4 + t] : a[4 + t]);
+            s.ref = moves ? ref : s.ref;
+            s.mass = __builtin_fmaxf(mass, s.mass);
+        }
         s.y += w[1];
         s.z += w[2];
         s.yd += w[3];
@@ -383,6 +404,48 @@ __device__ __forceinline__ void range_update(EdgeState<PASS>& st, float (&w)[8])
     }
 }
 
+// Sum over the four lanes that hold a row.
+__device__ __forceinline__ float row_sum4(float x)
+{
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    const float y = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// What the rows' pass takes from g: the mean of those so far, so that weights are rounded
+// after what is common to them has been taken out.  (Values of mean 64 left an error of
+// 1.6e-3 in bfloat16's dq, beside its own rounding's 1.65e-3, where sums of p g c k were
+// rounded first.)  u, w: a chunk's p g' c and p c, in the sums' y and z already.  The mean
+// is taken anew, and all sums moved to it, where the weights so far have become four times
+// those of the last one: a far-off g of a small weight then does not stay what all others
+// are taken from.
+template <typename T, int PASS>
+__device__ __forceinline__ void recentre(EdgeState<PASS>& st, float (&u)[8], const float (&w)[8])
+{
+    const float mass = row_sum4(st.z);
+    if (!__ballot(mass > 4.f * st.mass)) return;
+    const float away = row_sum4(st.y) / mass;
+    if (!(mass > 4.f * st.mass && __builtin_fabsf(away) <= FLT_MAX)) return;
+    if (st.mass > 0.f && away != 0.f) {
+        float by = away;
+        if constexpr (Half<T>::kRange) {   // (a scale in which it is of a size)
+            const float x = __builtin_fmaxf(st.x, (float)(__builtin_amdgcn_frexp_expf(away) - 24));
+            rescale(st, fast_exp2(st.x - x));
+            st.x = x;
+            by *= fast_exp2(-x);
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) st.acc[t] -= by * st.acc[4 + t];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u[j] = __builtin_fmaf(-away, w[j], u[j]);
+    st.y = __builtin_fmaf(-away, st.z, st.y);
+    st.yd = __builtin_fmaf(-away, st.zd, st.yd);
+    st.ref += away;
+    st.mass = mass;
+}
+
 // Rows of 64 values leave whole, through a stage of 16 rows: val(t) is the lane's part
 // of tile t, dims 16 t + 4 g .. + 3.
 template <typename T, typename F>
@@ -444,12 +507,13 @@ __device__ __forceinline__ void edge_finish(const EdgeParams& p, EdgeState<PASS>
         // The weights' own sum (1, but for the rounding of the log-sum-exp) divides.
         const float l = over_groups(st.z);
         const float i = l != 0.f ? 1.f / l : 0.f;
-        const float d = over_groups(st.y) * i;
+        const float d = over_groups(st.y) * i;   // (from the reference)
         const float f = fast_exp2(st.x);   // (0: unset)
         const float c = p.scale * i;
         edge_store<T>(p.out1, stage, w, p.n, head_off, lane,
                       [&](int t) { return c * (st.acc[t] * f - d * st.acc[4 + t]); });
-        if (g == 0 && row < p.n) p.stats[((int64_t)row * p.H + h) * p.stat_words + 1] = d;
+        if (g == 0 && row < p.n)
+            p.stats[((int64_t)row * p.H + h) * p.stat_words + 1] = l != 0.f ? d + st.ref : 0.f;
         if (p.dims) {
             // the window's share of dslope: rows 0 to 15 in one fixed order
             float s = row < p.n ? (over_groups(st.yd) - d * over_groups(st.zd)) * i : 0.f;
@@ -785,7 +849,7 @@ edge_kernel(const EdgeParams p)
                     w = where(on[j], s[j], -INFINITY);
                 } else if constexpr (PASS == kRows) {
                     const float e = where(on[j], fast_exp2(lifted<T>(s[j] - lse, kLiftLog2<T> + 1.f)));
-                    const float eg = where(on[j], e * gs[j]);
+                    const float eg = where(on[j], e * (gs[j] - st.ref));
                     st.z += e;
                     st.y += eg;
                     if (p.dims) {
@@ -826,6 +890,7 @@ edge_kernel(const EdgeParams p)
             }
             edge_mix<T>(at, kEdgeStage, w8, st.acc);
         } else {
+            if constexpr (PASS == kRows) recentre<T>(st, u8, w8);
             edge_mix<T>(at, PASS == kRows ? 0 : kEdgeStage, w8, st.acc + 4);
             __builtin_amdgcn_sched_barrier(0);
             range_update<T>(st, u8);
