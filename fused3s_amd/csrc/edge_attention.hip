@@ -332,6 +332,15 @@ __device__ __forceinline__ float distance(const Position& a, float x, float y, f
     return __builtin_amdgcn_ldexpf(
         __builtin_amdgcn_sqrtf(__builtin_fmaf(dz, dz, __builtin_fmaf(dy, dy, dx * dx))), e);
 }
+// Infinite coordinates: of a window's rows as +inf, at the edges' other ends as -inf, so
+// that the distance of two nodes of which either is infinitely far is infinite, not NaN.
+__device__ __forceinline__ Position facing(Position a, float infinity)
+{
+    a.x = __builtin_fabsf(a.x) == INFINITY ? infinity : a.x;
+    a.y = __builtin_fabsf(a.y) == INFINITY ? infinity : a.y;
+    a.z = __builtin_fabsf(a.z) == INFINITY ? infinity : a.z;
+    return a;
+}
 __device__ __forceinline__ Position position_of(const EdgeParams& p, int64_t node)
 {
     Position a{0.f, 0.f, 0.f};
@@ -544,7 +553,7 @@ __device__ float slow_row(const EdgeParams& p, int32_t w, int h, int r, int nite
         return (float)reinterpret_cast<const T*>(x.ptr + node * x.stride)[h * kD + lane];
     };
     const float a = value(p.own1, row), b = PASS == kForward ? 0.f : value(p.own2, row);
-    const Position own = position_of(p, row);
+    const Position own = facing(position_of(p, row), INFINITY);
     const float slope = p.dims ? p.slopes[h] * kLog2e : 0.f;
     const float lse = PASS == kRows ? p.lse[at] : 0.f;
     float m = -INFINITY, l = 0.f, pg = 0.f, pd = 0.f, pgd = 0.f;   // (uniform)
@@ -565,7 +574,7 @@ __device__ float slow_row(const EdgeParams& p, int32_t w, int h, int r, int nite
                 float s = score[0];
                 const float slope_c = slopes_c[0];
                 if (p.dims) {
-                    const Position there = position_of(p, node);
+                    const Position there = facing(position_of(p, node), -INFINITY);
                     dist = p.dims == 1 ? __builtin_fabsf(own.x - there.x)
                                        : distance(own, there.x, there.y, there.z);
                     s -= slope * dist;
@@ -579,6 +588,7 @@ __device__ float slow_row(const EdgeParams& p, int32_t w, int h, int r, int nite
                     m = top;
                 } else if constexpr (PASS == kRows) {
                     const float e = fast_exp2(s - lse), g = wave_sum(b * y2);
+                    if (e == 0.f) dist = 0.f;   // (an infinite one)
                     l += e;
                     pg += e * g;
                     pd += e * dist;
@@ -719,7 +729,7 @@ edge_kernel(const EdgeParams p)
 #pragma unroll
         for (int f = 0; f < 2; ++f) o2[f] = *reinterpret_cast<const v8*>(src + 64 * f);
     }
-    const Position own = position_of(p, row);
+    const Position own = facing(position_of(p, row), INFINITY);
     const float slope = p.dims ? scalar_load(p.slopes + h) * kLog2e : 0.f;
     float lse = 0.f;
     if constexpr (PASS == kRows) {
@@ -814,8 +824,11 @@ edge_kernel(const EdgeParams p)
         edge_write(at, 0, a);
         edge_write(at, kEdgeStage, b);
         const int own_slot = anew(lane) & 31;
-        if (p.dims == 1) L.pos[own_slot] = there.x;
-        else if (p.dims) *reinterpret_cast<f4*>(&L.pos[4 * own_slot]) = f4{there.x, there.y, there.z, 0.f};
+        if (p.dims) {
+            const Position to = facing(there, -INFINITY);
+            if (p.dims == 1) L.pos[own_slot] = to.x;
+            else *reinterpret_cast<f4*>(&L.pos[4 * own_slot]) = f4{to.x, to.y, to.z, 0.f};
+        }
         if constexpr (PASS == kColumns) *reinterpret_cast<f2*>(&L.stats[2 * own_slot]) = stat;
         wave_lds_order();
         if (c + 1 < ce) {
@@ -853,7 +866,7 @@ edge_kernel(const EdgeParams p)
                     st.z += e;
                     st.y += eg;
                     if (p.dims) {
-                        const float d = where(on[j], dist[j]);
+                        const float d = e != 0.f ? dist[j] : 0.f;   // (an infinite one's e is 0)
                         st.zd = __builtin_fmaf(e, d, st.zd);
                         st.yd = __builtin_fmaf(eg, d, st.yd);
                     }

@@ -413,7 +413,8 @@ class TorchGraph:
         q, k, v: float16 or bfloat16 CUDA tensors [n, H, 64], each row's heads
         contiguous, rows at any distance of a multiple of 8 values (a slice of a
         projection's output is taken as it is; other layouts are copied); positions:
-        float32 [n] (times, say) or [n, 1 to 3] (points); slopes: float32 [H].
+        float32 [n] (times, say) or [n, 1 to 3] (points); slopes: float32 [H].  Where
+        slopes are positive, a node with an infinite coordinate is taken out of the graph.
         Returns [n, H, 64] in q's type: sums in float32, rounded once; nodes without
         edges get 0.  Differentiable in q, k, v and slopes (once); tracing, functorch's
         transforms and forward-mode differentiation are refused.  A graph serves any
