@@ -11,9 +11,10 @@
 //            and z at the target; a second launch joins a row's blocks
 //   backward in pieces of the classes: z again, dz of a piece in its epilogue, in the
 //            type, then its share of dx (float32, added up over the pieces) and its
-//            rows of dW.  A piece's dz is kPieceBytes at most.  So memory goes with n,
-//            K and that, not with n V, for one product of four more than keeping z
-//            would take.
+//            rows of dW.  A piece's dz is kPieceBytes at most: past kPieceRows rows they
+//            are taken a block at a time, and dW is added up over the blocks (float32).
+//            So memory goes with V K and a block's K, not with n V, for one product of
+//            four more than keeping z would take.
 // Of few inputs (K <= 256) the logits, and dz, stay in registers: below.
 // dz is rounded to the type, the operand that dx and dW take: these two carry that
 // rounding beside their own; db is summed before it.  (Of few classes, where bytes bound
@@ -32,6 +33,7 @@ namespace f3s {
 // 1,024 MB: 8.9, 8.9, 8.5, 9.1: fewer launches and additions of dx against what the
 // Infinity Cache holds.)
 constexpr int64_t kPieceBytes = 512 << 20;    // of dz
+constexpr int64_t kPieceRows = kPieceBytes / 2 / 1024;   // so that a piece has 1,024 classes
 constexpr int64_t kBlocksBytes = 256 << 20;   // of a forward pass's blocks
 constexpr int kLossThreads = 256;
 
@@ -215,6 +217,19 @@ join_scaled(const float* __restrict__ parts, int64_t count, int32_t slices,
 {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256)
         out[i] = (T)(split_sum(parts + i, count, 0, slices) * *factor);
+}
+// Slices of one of several blocks' product added onto those of the blocks before; after
+// the last block, times the factor.
+template <typename T>
+__global__ void __launch_bounds__(256)
+join_blocks(const float* __restrict__ parts, int64_t count, int32_t slices, float* __restrict__ sums,
+            bool first, bool last, const float* __restrict__ factor, T* __restrict__ out)
+{
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+        const float s = (first ? 0.f : sums[i]) + split_sum(parts + i, count, 0, slices);
+        if (last) out[i] = (T)(s * *factor);
+        else sums[i] = s;
+    }
 }
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -1262,10 +1277,12 @@ constexpr int64_t kLargestGroups = 128;
 constexpr int64_t kLossShares = 64;   // of the rows' sums of db
 
 // Workspace of a backward pass: f, the factor, the largest gradients; db's sums; a
-// piece's dz; dx's slices; a piece's splits of dW.
+// piece's dz; dx's slices; a piece's splits of dW; dW and db of the blocks of rows so far.
 struct CeSpace {
     size_t factor = 0, largest = 0, sums = 0, shares = 0, db = 0, dz = 0, dx = 0, dw = 0, bytes = 0;
     size_t few_dw = 0, few_db = 0;   // (few classes)
+    size_t all_dw = 0, all_db = 0;   // (several blocks)
+    int64_t rows = 0;                // of a block
     int64_t piece = 0, ldz = 0, sum_rows = 0;
     Tiling prob{}, tdx{}, tdw{};
     bool whole_dx = false;   // one piece, one split: dx is written at once
@@ -1301,22 +1318,26 @@ static CeSpace ce_space(int64_t n, int64_t K, int64_t V)
         s.bytes = grad_space(n, K, V, s.sums).bytes;
         return s;
     }
-    const int64_t fit = std::max<int64_t>(1024, kPieceBytes / 2 / n / 256 * 256);
-    const int64_t pieces = ceil_div(V, fit);
+    const int64_t blocks = ceil_div(n, kPieceRows);
+    s.rows = blocks == 1 ? n : ceil_div(ceil_div(n, blocks), 256) * 256;
+    const int64_t fit = kPieceBytes / 2 / s.rows / 256 * 256, pieces = ceil_div(V, fit);
     s.piece = pieces == 1 ? V : ceil_div(ceil_div(V, pieces), 256) * 256;
     s.ldz = ceil_div(s.piece, 8) * 8;
-    s.prob = one_split(n, s.ldz, K, odd);
-    s.tdx = tiling(n, K, s.piece, kForwardLeast, odd, false);
-    s.tdw = tiling(s.piece, K, n, kWeightLeast, odd, true);
+    s.prob = one_split(s.rows, s.ldz, K, odd);
+    s.tdx = tiling(s.rows, K, s.piece, kForwardLeast, odd, false);
+    s.tdw = tiling(s.piece, K, s.rows, kWeightLeast, odd, true);
     s.whole_dx = s.piece >= V && s.tdx.splits == 1;
-    s.sum_rows = 2 * ceil_div(n, 64);   // (at most)
+    s.sum_rows = 2 * ceil_div(s.rows, 64);   // (at most)
     s.shares = s.sums + up256(sizeof(float) * (size_t)s.sum_rows * s.ldz);
     s.db = s.shares + up256(sizeof(float) * (size_t)kLossShares * s.ldz);
     s.dz = s.db + up256(sizeof(float) * (size_t)s.ldz);
-    s.dx = s.dz + up256(2 * (size_t)n * s.ldz);
-    s.dw = s.dx + (s.whole_dx ? 0 : up256(sizeof(float) * (size_t)s.tdx.splits * n * K));
-    s.bytes = s.dw +
-              (s.tdw.splits > 1 ? up256(sizeof(float) * (size_t)s.tdw.splits * s.piece * K) : 0);
+    s.dx = s.dz + up256(2 * (size_t)s.rows * s.ldz);
+    s.dw = s.dx + (s.whole_dx ? 0 : up256(sizeof(float) * (size_t)s.tdx.splits * s.rows * K));
+    s.all_dw = s.dw + (s.tdw.splits > 1 || blocks > 1
+                           ? up256(sizeof(float) * (size_t)s.tdw.splits * s.piece * K)
+                           : 0);
+    s.all_db = s.all_dw + (blocks > 1 ? up256(sizeof(float) * (size_t)V * K) : 0);
+    s.bytes = s.all_db + (blocks > 1 ? up256(sizeof(float) * (size_t)V) : 0);
     return s;
 }
 
@@ -1474,25 +1495,35 @@ static f3s_status loss_backward(const CeArgs& a, const float* lse, const float* 
         return F3S_OK;
     }
     const bool whole = a.K % 8 == 0;   // (the operands' and the results' rows whole pieces)
-    for (int64_t v0 = 0; v0 < a.V; v0 += s.piece) {
+    const bool blocks = s.rows < a.n;
+    // A piece of the classes, v0 .., over the rows r0 ..
+    auto piece = [&](int64_t r0, int64_t rows, int64_t v0) -> f3s_status {
+        const bool first = r0 == 0, last = r0 + rows == a.n;
         const int64_t outs = std::min(s.piece, a.V - v0), ldz = ceil_div(outs, 8) * 8;
-        const char* w = a.W + v0 * a.K * 2;
+        const char *x = a.X + r0 * a.ldx * 2, *w = a.W + v0 * a.K * 2;
+        // (several blocks) slices of dW or db onto those of the blocks before
+        auto onto = [&](const float* parts, int64_t count, int32_t slices, size_t sums, int64_t at,
+                        char* out) {
+            hipLaunchKernelGGL((join_blocks<T>), dim3(element_groups(count)), dim3(256), 0, a.st, parts,
+                               count, slices, reinterpret_cast<float*>(ws + sums) + at, first, last,
+                               factor, reinterpret_cast<T*>(out) + at);
+        };
         GemmParams p{};
-        p.P = a.X;
+        p.P = x;
         p.ldp = a.ldx;
         p.Q = w;
         p.ldq = a.K;
-        p.rows = a.n;
+        p.rows = rows;
         p.outs = ldz;
         p.depth = a.K;
         p.bias = a.bias ? a.bias + v0 * 2 : nullptr;
         p.C = ws + s.dz;
         p.sums = db ? reinterpret_cast<float*>(ws + s.sums) : nullptr;
         p.splits = 1;
-        p.loss.target = a.target;
+        p.loss.target = a.target + r0;
         p.loss.first = v0;
-        p.loss.lse = lse;
-        p.loss.f = f.f;
+        p.loss.lse = lse + r0;
+        p.loss.f = f.f + r0;
         p.loss.outs = outs;
         const int32_t tile = tile_size(s.prob, whole ? kWhole : kAny, kEpiProb);
         F3S_REQUIRE(ceil_div(p.rows, tile) * ceil_div(p.outs, tile) < ((int64_t)1 << 31),
@@ -1502,21 +1533,24 @@ static f3s_status loss_backward(const CeArgs& a, const float* lse, const float* 
         F3S_HIP(hipGetLastError());
         if (db) {
             const float* sums = p.sums;
-            int64_t rows = 2 * ceil_div(a.n, tile);
+            int64_t many = 2 * ceil_div(rows, tile);
             const unsigned nx = (unsigned)ceil_div(ldz, 64);
-            if (rows > 512) {   // shares of them first
+            if (many > 512) {   // shares of them first
                 float* shares = reinterpret_cast<float*>(ws + s.shares);
-                const int64_t ny = std::min<int64_t>(kLossShares, ceil_div(rows, 64));
+                const int64_t ny = std::min<int64_t>(kLossShares, ceil_div(many, 64));
                 hipLaunchKernelGGL((column_sums<float>), dim3(nx, (unsigned)ny), dim3(256), 0, a.st,
-                                   sums, rows, ldz, shares);
+                                   sums, many, ldz, shares);
                 sums = shares;
-                rows = ny;
+                many = ny;
             }
-            float* whole = reinterpret_cast<float*>(ws + s.db);
-            hipLaunchKernelGGL((column_sums<float>), dim3(nx, 1), dim3(256), 0, a.st, sums, rows, ldz,
-                               whole);
-            hipLaunchKernelGGL((cast_scaled<T>), dim3((unsigned)ceil_div(outs, 256)), dim3(256), 0,
-                               a.st, whole, outs, factor, reinterpret_cast<T*>(db) + v0);
+            float* all = reinterpret_cast<float*>(ws + s.db);
+            hipLaunchKernelGGL((column_sums<float>), dim3(nx, 1), dim3(256), 0, a.st, sums, many, ldz,
+                               all);
+            if (blocks)
+                onto(all, outs, 1, s.all_db, v0, db);
+            else
+                hipLaunchKernelGGL((cast_scaled<T>), dim3((unsigned)ceil_div(outs, 256)), dim3(256), 0,
+                                   a.st, all, outs, factor, reinterpret_cast<T*>(db) + v0);
             F3S_HIP(hipGetLastError());
         }
         if (dX) {
@@ -1525,13 +1559,13 @@ static f3s_status loss_backward(const CeArgs& a, const float* lse, const float* 
             q.ldp = ldz;
             q.Q = w;
             q.ldq = a.K;
-            q.rows = a.n;
+            q.rows = rows;
             q.outs = a.K;
             q.depth = whole ? ldz : outs;
             q.q_end = outs;
             q.add = v0 > 0;
             q.factor = factor;
-            q.C = s.whole_dx ? dX : ws + s.dx;
+            q.C = s.whole_dx ? dX + r0 * a.K * 2 : ws + s.dx;
             if (s.whole_dx)
                 F3S_TRY((launch_of_dz<T, false, kEpiScaled>(q, s.tdx, whole, a.st)));
             else
@@ -1541,33 +1575,42 @@ static f3s_status loss_backward(const CeArgs& a, const float* lse, const float* 
             GemmParams q{};
             q.P = ws + s.dz;
             q.ldp = ldz;
-            q.Q = a.X;
+            q.Q = x;
             q.ldq = a.ldx;
             q.rows = outs;
             q.outs = a.K;
-            q.depth = q.q_end = a.n;
+            q.depth = q.q_end = rows;
             q.factor = factor;
             char* dst = dW + v0 * a.K * 2;
-            if (s.tdw.splits == 1) {
+            if (s.tdw.splits == 1 && !blocks) {
                 q.C = dst;
                 F3S_TRY((launch_of_dz<T, true, kEpiScaled>(q, s.tdw, whole, a.st)));
             } else {
                 q.C = ws + s.dw;
                 F3S_TRY((launch_of_dz<T, true, kEpiPart>(q, s.tdw, whole, a.st)));
                 const int64_t count = outs * a.K;
-                hipLaunchKernelGGL((join_scaled<T>), dim3(element_groups(count)), dim3(256),
-                                   0, a.st, reinterpret_cast<const float*>(ws + s.dw), count,
-                                   s.tdw.splits, factor, reinterpret_cast<T*>(dst));
+                const float* parts = reinterpret_cast<const float*>(ws + s.dw);
+                if (blocks)
+                    onto(parts, count, s.tdw.splits, s.all_dw, v0 * a.K, dW);
+                else
+                    hipLaunchKernelGGL((join_scaled<T>), dim3(element_groups(count)), dim3(256), 0,
+                                       a.st, parts, count, s.tdw.splits, factor,
+                                       reinterpret_cast<T*>(dst));
                 F3S_HIP(hipGetLastError());
             }
         }
-    }
-    if (dX && !s.whole_dx) {
-        const int64_t count = a.n * a.K;
-        hipLaunchKernelGGL((join_scaled<T>), dim3(element_groups(count)), dim3(256), 0, a.st,
-                           reinterpret_cast<const float*>(ws + s.dx), count, s.tdx.splits, factor,
-                           reinterpret_cast<T*>(dX));
-        F3S_HIP(hipGetLastError());
+        return F3S_OK;
+    };
+    for (int64_t r0 = 0; r0 < a.n; r0 += s.rows) {
+        const int64_t rows = std::min(s.rows, a.n - r0);
+        for (int64_t v0 = 0; v0 < a.V; v0 += s.piece) F3S_TRY(piece(r0, rows, v0));
+        if (dX && !s.whole_dx) {
+            const int64_t count = rows * a.K;
+            hipLaunchKernelGGL((join_scaled<T>), dim3(element_groups(count)), dim3(256), 0, a.st,
+                               reinterpret_cast<const float*>(ws + s.dx), count, s.tdx.splits, factor,
+                               reinterpret_cast<T*>(dX) + r0 * a.K);
+            F3S_HIP(hipGetLastError());
+        }
     }
     return F3S_OK;
 }

@@ -58,3 +58,21 @@ def test_pieces_of_the_rows(gpu, n, K, V):
         at = slice(r0, r0 + n // 7)
         Reference(x[at], w, b, t[at], "none").check("loss", loss[at])
     assert abs(float(loss.double().sum()) - float(total)) <= 2.0 ** -23 * float(total)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("n,K,V", [(300_000, 264, 1500), (300_001, 301, 3001), (262_145, 320, 70)])
+def test_blocks_of_the_rows(gpu, n, K, V, dtype):
+    """More rows than the logits' gradient is taken of at a time, one piece of the classes
+    and several; each gradient alone."""
+    from fused3s_amd.torch_ops import linear_cross_entropy
+    x, w, b, t, dloss = inputs(n, K, V, dtype, 6, ignored=0.5)
+    got = step(x, w, b, t, dloss, "mean")
+    check(got, x, w, b, t, dloss, "mean")
+    same(got, step(x, w, b, t, dloss, "mean"))
+    for i, name in ((0, "dx"), (1, "dw"), (2, "db")):
+        leaves = [x, w, b]
+        leaves[i] = leaves[i].detach().requires_grad_()
+        g, = torch.autograd.grad(linear_cross_entropy(leaves[0], leaves[1], t, leaves[2]), [leaves[i]],
+                                 dloss)
+        assert torch.equal(g, got[name]), name
