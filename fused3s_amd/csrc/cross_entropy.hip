@@ -1099,16 +1099,17 @@ static void launch_few(const FewParams& p, hipStream_t st)
 
 // Chunks of 64 streamed rows in a share, for `groups` workgroups of which `slots` run at
 // once: the least rounds of shares, whose starts and ends are some two chunks, and whose
-// results `cost` chunks where there are several.  (By this and with one round's groups
-// at most, us: 52,802 x 64 -> 10,778 143 and 172 forward, 672 and 687 trained; 272,567 x
-// 128 -> 23,790 1,906 and 2,413, 8,849 and 10,017; 70,000 x 64 -> 5,000 93 and 134, 422
-// and 482.)
-static int64_t share_of(int64_t groups, int64_t chunks, int64_t slots, double cost)
+// results `cost` chunks where there are several; `most` shares at most.  (By this and with
+// one round's groups at most, us: 52,802 x 64 -> 10,778 143 and 172 forward, 672 and 687
+// trained; 272,567 x 128 -> 23,790 1,906 and 2,413, 8,849 and 10,017; 70,000 x 64 -> 5,000
+// 93 and 134, 422 and 482.)
+static int64_t share_of(int64_t groups, int64_t chunks, int64_t slots, double cost, int64_t most)
 {
+    most = std::max<int64_t>(1, std::min(most, chunks));
     int64_t best = chunks;
     double least = INFINITY;
     auto look = [&](int64_t shares) {
-        const int64_t per = ceil_div(chunks, std::min(chunks, std::max<int64_t>(1, shares)));
+        const int64_t per = ceil_div(chunks, std::min(most, std::max<int64_t>(1, shares)));
         shares = ceil_div(chunks, per);
         const double t = (double)ceil_div(groups * shares, slots) * (double)(per + 2) +
                          (shares > 1 ? cost * (double)shares : 0.0);
@@ -1137,7 +1138,7 @@ static ForwardSpace forward_space(int64_t n, int64_t K, int64_t V)
     ForwardSpace s;
     if (streams(K)) {
         const int64_t chunks = ceil_div(V, 64);
-        s.per = share_of(ceil_div(n, kStreamRows), chunks, stream_slots(K), 0.0);
+        s.per = share_of(ceil_div(n, kStreamRows), chunks, stream_slots(K), 0.0, chunks);
         s.nblocks = ceil_div(chunks, s.per);
         s.rows = n;
     } else {
@@ -1174,13 +1175,14 @@ static void launch_stream(const CeArgs& a, const GemmParams& g, int64_t per, int
 }
 
 // Shares of the streamed rows.  A chunk takes some 2.2 us, an output's slice 8 bytes at
-// 4 TB/s, written and read.
+// 4 TB/s, written and read.  The slices, float32, are kSliceBytes at most.
+constexpr int64_t kSliceBytes = 512 << 20;
 constexpr int64_t kGradSlots = 512;   // two per CU
 static int64_t grad_rows(int64_t K) { return K <= 128 ? 128 : 64; }   // of a workgroup's own
 static int64_t grad_per(int64_t owns, int64_t others, int64_t K)
 {
     return share_of(ceil_div(owns, grad_rows(K)), ceil_div(others, 64), kGradSlots,
-                    (double)owns * (double)K * (8 / 4e6 / 2.2));
+                    (double)owns * (double)K * (8 / 4e6 / 2.2), kSliceBytes / (owns * K * 4));
 }
 static int64_t grad_shares(int64_t owns, int64_t others, int64_t K)
 {

@@ -30,3 +30,14 @@ def test_more_than_256_inputs(n, V):
     for K, Kp in ((257, 264), (301, 304)):
         copies = 4 * (n + V) * Kp
         assert workspace(n, K, V, 1) <= workspace(n, Kp, V, 1) + copies + 512 * MIB
+
+
+@pytest.mark.parametrize("n", [1, 64, 1000, 16_384, 200_003, 500_000, 1_000_000, 8_200_001, 54_000_000])
+@pytest.mark.parametrize("V", [2, 64, 65, 1000, 10_000, 100_003, 1_000_000, 54_000_000])
+def test_up_to_256_inputs(n, V):
+    """512 MB of the gradients' slices; db's, of up to 4,096 shares of the rows of few
+    classes and few of many."""
+    for K in (8, 64, 128, 136, 256):
+        assert workspace(n, K, V, 1) <= 512 * MIB + 8 * n + 64 * MIB + 4 * 16 * V, (n, K, V)
+        # (forward: 8 bytes a row and share of the classes)
+        assert workspace(n, K, V, 0) <= 80 * n + 64 * MIB, (n, K, V)
