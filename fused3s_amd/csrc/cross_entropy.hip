@@ -243,8 +243,8 @@ cast_scaled(const float* __restrict__ in, int64_t count, const float* __restrict
 template <typename T>
 __global__ void __launch_bounds__(256) loss_zero(T* __restrict__ out, int64_t count)
 {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < count) out[i] = (T)0.f;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256)
+        out[i] = (T)0.f;
 }
 
 // ---- log-sum-exps of few inputs: K <= 256, whole pieces ----
@@ -1713,8 +1713,8 @@ f3s_status f3s_cross_entropy_bwd(const uint16_t* X, int64_t x_stride, const uint
     if (n == 0) {
         auto zero = [&](uint16_t* out, int64_t count) {
             if (out)
-                hipLaunchKernelGGL((loss_zero<_Float16>), dim3((unsigned)ceil_div(count, 256)),
-                                   dim3(256), 0, st, reinterpret_cast<_Float16*>(out), count);
+                hipLaunchKernelGGL((loss_zero<_Float16>), dim3(element_groups(count)), dim3(256), 0, st,
+                                   reinterpret_cast<_Float16*>(out), count);
         };
         zero(dW, V * K);
         zero(db, V);
