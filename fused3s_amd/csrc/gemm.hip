@@ -348,8 +348,8 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 fill_zero(T* __restrict__ out, int64_t count)
 {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < count) out[i] = (T)0.f;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256)
+        out[i] = (T)0.f;
 }
 
 __global__ void warm_gemm_kernel() {}
@@ -749,7 +749,9 @@ f3s_status f3s_linear_bwd(const uint16_t* X, int64_t x_stride, const uint16_t* W
     if (n == 0) {
         auto zero = [&](uint16_t* out, int64_t count) {
             if (out)
-                hipLaunchKernelGGL((fill_zero<_Float16>), dim3((unsigned)ceil_div(count, 256)),
+                // (below a grid's limit of threads)
+                hipLaunchKernelGGL((fill_zero<_Float16>),
+                                   dim3((unsigned)std::min<int64_t>(ceil_div(count, 256), 1 << 20)),
                                    dim3(256), 0, st, reinterpret_cast<_Float16*>(out), count);
         };
         zero(dW, M * K);
