@@ -192,9 +192,9 @@ __global__ void __launch_bounds__(kLossThreads) loss_factors(const FactorParams 
     if (p.largest) {
         float m = 0.f;
         for (int k = 0; k < p.many; ++k) m = __builtin_fmaxf(m, p.largest[k]);
-        // (kept where its inverse is one too)
+        // (kept where it over 2^14 and that's inverse are ones too)
         const int e = m > 0.f ? __builtin_amdgcn_frexp_expf(m) : 0;
-        unit = __builtin_amdgcn_ldexpf(1.f, e < -120 ? -120 : e > 120 ? 120 : e);
+        unit = __builtin_amdgcn_ldexpf(1.f, e < -110 ? -110 : e > 120 ? 120 : e);
     }
     const int64_t i = (int64_t)blockIdx.x * kLossThreads + threadIdx.x;
     if (i < p.n) {
