@@ -77,9 +77,16 @@ struct EdgeParams {
 // D and the position (2, 4 or 8 words), where a position of its own would be another.
 static inline int32_t stat_words(int32_t dims) { return dims == 0 ? 2 : dims <= 2 ? 4 : 8; }
 
+// The forward pass's weights are 2^kLazy at most: in binary16 raised to 2^14, so that the
+// small ones of a row of many edges keep their bits.  (3,000 equal weights of 2^-18 beside
+// one of 1, unraised: their sum was off by 2^-9 of itself.)
+template <typename T>
+constexpr float kSoftLog2 = Half<T>::kRange ? 14.f - kLazy : 0.f;
+
 // A wave's sums, tiles of 16 dims, lane (g, r) holding dims 16 t + 4 g + v of row r in
 // tile t (v: the element), and its share of row r's sums of weights.
-//   forward: tiles 0-3 sum p v, scaled by 2^-x, x the running maximum; y: l
+//   forward: tiles 0-3 sum p v, scaled by 2^-x, x the running maximum (binary16: by
+//            kSoftLog2 more); y: l, as they
 //   rows:    0-3 sum p g' c k, scaled by 2^-x; 4-7 sum p c k; y: sum p g', z: sum p,
 //            yd, zd: the same times the distance; ref: g - g', mass: recentre()
 //   columns: 0-3 sum ds q, scaled by 2^-x; 4-7 dv
@@ -511,7 +518,7 @@ __device__ __forceinline__ void edge_finish(const EdgeParams& p, EdgeState<PASS>
             return l != 0.f ? st.acc[t] * f : f4{0.f, 0.f, 0.f, 0.f};
         });
         if (p.lse && g == 0 && row < p.n)
-            p.lse[(int64_t)row * p.H + h] = l != 0.f ? st.x + __log2f(l) : 0.f;
+            p.lse[(int64_t)row * p.H + h] = l != 0.f ? st.x + (__log2f(l) - kSoftLog2<T>) : 0.f;
     } else if constexpr (PASS == kRows) {
         // The weights' own sum (1, but for the rounding of the log-sum-exp) divides.
         const float l = over_groups(st.z);
@@ -895,7 +902,7 @@ edge_kernel(const EdgeParams p)
                     st.x = top;
                 }
             }
-            const float mu = st.x == -INFINITY ? 0.f : st.x;
+            const float mu = (st.x == -INFINITY ? 0.f : st.x) - kSoftLog2<T>;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 w8[j] = fast_exp2(w8[j] - mu);
