@@ -21,7 +21,11 @@
 // the passes and not products, it goes on as the sum of two 16-bit values.)  What dz is multiplied with
 // throughout (1 / count, a loss scale) comes last, in float32, so that small gradients
 // do not vanish: dz itself is of size 1 at most, in binary16 times 2^14, as a class
-// of probability 1e-9 still has its 11 bits then.
+// of probability 4e-9 still has its 11 bits then.  (As two 16-bit values it would take a
+// product more for each of dx and dW: with few inputs 52,802 x 64 -> 10,778 trained 675 ->
+// 821 us, 16,384 x 256 -> 50,021 2,264 -> 2,679; where dz goes through memory twice its
+// bytes too.  Rounded, these gradients are at most 1.41 times as far off as by their own
+// rounding alone.)
 // What bounds it is the matrix cores, with many classes; with few, x.
 #include <cmath>
 

@@ -180,7 +180,7 @@ __device__ __forceinline__ void absorb(EdgeState<PASS>& s, const float* src, int
 // pieces, which the transposing reads take, then lie in distinct banks without padding.
 // One record of the lists (offsets into x1 and x2, or node indices; row masks) per
 // chunk, two in turn, and what the chunk's slots have beside their rows.
-// 9,984 bytes: 16 waves fit a CU's 160 KB.
+// 9,728 bytes: 16 waves fit a CU's 160 KB.
 __device__ __forceinline__ int edge_swizzle(int row) { return (row & 6) | ((row >> 3) & 1); }
 struct EdgeRecord {
     uint32_t at1[kChunk], at2[kChunk], rm[kChunk];

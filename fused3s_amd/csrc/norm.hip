@@ -547,7 +547,8 @@ static NormShape norm_shape(int64_t C, int32_t dtype, bool backward)
         for (int32_t pieces : {1, 2})
             if ((pieces == 2 || lanes == 256) && have <= (int64_t)lanes * pieces)
                 return {lanes, pieces};
-    // (float32: four pieces are as many values as 16-bit types' two)
+    // (float32: four pieces are as many values as 16-bit types' two; of the gradient's
+    // registers 11 spill)
     if (dtype == F3S_F32 && have <= 4096) return {1024, 4};
     return {0, 0};
 }

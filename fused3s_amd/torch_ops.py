@@ -899,7 +899,9 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     without keeping the logits: x [..., K], weight [V, K], bias [V], all float16 or all
     bfloat16 on one GPU, target [...] int64.  Rows of ignore_index have no loss and no
     gradient; a target that is no class has NaN as both.  reduction "mean" (over the
-    rows that are not ignored), "sum" or "none"; float32.  Logits are not rounded, sums
+    rows that are not ignored), "sum" or "none"; float32.  (An ignored row's x is
+    multiplied by 0 in weight's gradient: infinite or NaN values of it are NaN there, as
+    in torch.)  Logits are not rounded, sums
     are float32.  Differentiable (once) in x, weight and bias; for the backward pass the
     logits are computed again, some classes at a time, and their gradient (up to what
     multiplies all of it: the mean's divisor, a loss scale) is rounded to the type before
