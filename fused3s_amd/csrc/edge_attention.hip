@@ -117,6 +117,13 @@ __device__ __forceinline__ void rescale(EdgeState<PASS>& s, float factor)
     for (int t = 0; t < 4; ++t) s.acc[t] *= factor;
 }
 
+// (rows) The least scale of sums that what moves a reference by x is added to: there it is
+// 2^24, or less where 2 to the scale has no inverse.
+__device__ __forceinline__ float scale_of(float x)
+{
+    return __builtin_fmaxf((float)(__builtin_amdgcn_frexp_expf(x) - 24), -100.f);
+}
+
 template <int PASS>
 __device__ __forceinline__ void publish(const EdgeState<PASS>& s, float* dst, int lane)
 {
@@ -147,8 +154,7 @@ __device__ __forceinline__ void absorb(EdgeState<PASS>& s, const float* src, int
     // (rows) the lighter one's sums move to the heavier one's reference
     const bool moves = mass > s.mass;   // (s does)
     const float apart = moves ? s.ref - ref : ref - s.ref;
-    if (PASS == kRows && apart != 0.f)   // (a scale in which it is of a size)
-        top = __builtin_fmaxf(top, (float)(__builtin_amdgcn_frexp_expf(apart) - 24));
+    if (PASS == kRows && apart != 0.f) top = __builtin_fmaxf(top, scale_of(apart));
     const float mine = top == -INFINITY ? 0.f : fast_exp2(s.x - top);
     const float theirs = top == -INFINITY ? 0.f : fast_exp2(w[0] - top);
     rescale(s, mine);
@@ -445,8 +451,8 @@ __device__ __forceinline__ void recentre(EdgeState<PASS>& st, float (&u)[8], con
     if (!(mass > 4.f * st.mass && __builtin_fabsf(away) <= FLT_MAX)) return;
     if (st.mass > 0.f && away != 0.f) {
         float by = away;
-        if constexpr (Half<T>::kRange) {   // (a scale in which it is of a size)
-            const float x = __builtin_fmaxf(st.x, (float)(__builtin_amdgcn_frexp_expf(away) - 24));
+        if constexpr (Half<T>::kRange) {
+            const float x = __builtin_fmaxf(st.x, scale_of(away));
             rescale(st, fast_exp2(st.x - x));
             st.x = x;
             by *= fast_exp2(-x);

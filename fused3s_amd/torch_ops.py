@@ -901,8 +901,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     gradient; a target that is no class has NaN as both.  reduction "mean" (over the
     rows that are not ignored), "sum" or "none"; float32.  (An ignored row's x is
     multiplied by 0 in weight's gradient: infinite or NaN values of it are NaN there, as
-    in torch.)  Logits are not rounded, sums
-    are float32.  Differentiable (once) in x, weight and bias; for the backward pass the
+    in torch.)  Logits are not rounded, sums are float32.  Differentiable (once) in x, weight and bias; for the backward pass the
     logits are computed again, some classes at a time, and their gradient (up to what
     multiplies all of it: the mean's divisor, a loss scale) is rounded to the type before
     the gradients of x and weight are made of it, so these two are rounded twice (once

@@ -2,6 +2,7 @@
 a row has nearly the same do.v, and dq is made of the differences."""
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
@@ -65,3 +66,32 @@ def test_values_of_a_large_mean(gpu, n, H, hubs, dtype, mean, cap, dims):
         # (a row's sums are of some 2^13 edges at most, added in chains of 2^9 and less)
         err = (got["dslopes"].double() - want).abs()
         assert bool((err <= (((e + 2.0 ** -15) * size + rest) * dist).sum((1, 2)) + 2.0 ** -24 * want.abs()).all())
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("n", [120, 17_000])
+def test_a_weight_near_the_least(gpu, n, dtype):
+    """Rows whose do.v are all the same but for that of one edge, whose weight is 2^-80 to
+    2^-140: dq is finite and what that edge leaves of it, within the columns' bound."""
+    from _edge_reference import Reference
+    from fused3s_amd.torch_ops import TorchGraph
+    rows, width = 48, 100   # (rows of `width` edges; the others have a loop each)
+    rp = np.concatenate([np.arange(rows + 1) * width,
+                         rows * width + np.arange(1, n - rows + 1)]).astype(np.int32)
+    ci = np.concatenate([np.tile(np.arange(width), rows), np.arange(rows, n)]).astype(np.int32)
+    x = {name: torch.zeros(n, 1, 64, device="cuda") for name in ("q", "k", "v", "do")}
+    for name, value in (("v", 1.0), ("do", 1.0)):
+        x[name][:] = value
+    low = 60                               # the one edge's other end, in a later chunk
+    x["v"][low] = 3.0
+    x["q"][:rows, 0, 0] = torch.linspace(55, 97, rows, device="cuda").floor()
+    x["k"][low, 0, 0] = -1.0
+    x["k"][:width, 0, 1] = 1.0
+    x = {name: t.to(dtype) for name, t in x.items()}
+    got = step(TorchGraph(rp, ci, heads=1), x, scale=1.0)
+    few = slice(0, 100)                    # (all edges of these rows are among these nodes)
+    small = {name: t[few] for name, t in x.items()}
+    rp = np.concatenate([rp[:rows + 1], rp[rows] + np.arange(1, 100 - rows + 1)]).astype(np.int32)
+    ref = Reference(*(small[name] for name in ("q", "k", "v", "do")), rp, ci[:rp[-1]], 1.0)
+    for name in ("o", "dq", "dk", "dv"):
+        ref.check(name, got[name][few])
