@@ -399,8 +399,10 @@ f3s_status f3s_cross_entropy_fwd(const uint16_t* X, int64_t x_stride, const uint
 /* Its gradient: dX[n][K], dW[V][K], db[V] (contiguous; NULL: not wanted) from dloss,
  * float32 like loss, and the forward call's lse.  Z is computed again, in pieces of the
  * classes.  dZ, up to what multiplies all of it, is rounded to `dtype` before dX = dZ W
- * and dW = dZ^T X are made of it, so these two carry its rounding and their own; db is
- * summed before that. */
+ * and dW = dZ^T X are made of it, so these two carry its rounding and their own (of up to
+ * 64 classes and 256 inputs their own only); db is summed before that.  The workspace's
+ * logits' gradient takes 512 MB at most (K > 256; beside it dX of up to 262,144 rows, past
+ * that many dW, and their splits in float32), slices of dX and dW as much (K <= 256). */
 f3s_status f3s_cross_entropy_bwd(const uint16_t* X, int64_t x_stride, const uint16_t* W,
                                  const uint16_t* bias, const int64_t* target, int64_t ignore_index,
                                  const float* lse, const float* dloss, uint16_t* dX, uint16_t* dW,
@@ -462,7 +464,8 @@ f3s_status f3s_diff_attention_bwd(const f3s_plan* plan, const f3s_plan* reversed
  *   O[i] = sum_j softmax_j(s) V[j]
  * over the edges (i, j) (masked semantics); rows without edges get 0.  cap 0: s = x
  * there (else 1e-30 to 1e30); dims 0: no positions.  positions float32 [n][dims], dims
- * 1 to 3, distances Euclidean in float32; slopes float32 [H].  H is the plan's; a head
+ * 1 to 3, distances Euclidean in float32 (infinite where a coordinate of either node is:
+ * with positive slopes such a node is taken out); slopes float32 [H].  H is the plan's; a head
  * of a row is 64 contiguous values of `dtype` (F3S_F16 or F3S_BF16), heads adjacent,
  * rows `*_stride` values apart (a multiple of 8, at least H * 64), pointers 16-byte
  * aligned.  lse, where not NULL, receives [n][H] float32 for the gradient.  Sums and
