@@ -617,7 +617,7 @@ stream_grad_kernel(const GradParams p)
 // reads x once and writes dx once; dW is summed over a workgroup's rows in registers,
 // and the workgroups' sums in order by a second launch.  (200,003 x 128 -> 47 in
 // binary16, forward and backward pass by tiles: 33 and 91 us of kernels in 11 launches;
-// so 22 and 42 in five.)
+// so 22 and 45 in five.)
 constexpr int kFewWaves = 8;
 constexpr int64_t kFewClasses = 64, kFewInputs = 256;
 
@@ -1104,9 +1104,9 @@ static void launch_few(const FewParams& p, hipStream_t st)
 // Chunks of 64 streamed rows in a share, for `groups` workgroups of which `slots` run at
 // once: the least rounds of shares, whose starts and ends are some two chunks, and whose
 // results `cost` chunks where there are several; `most` shares at most.  (By this and with
-// one round's groups at most, us: 52,802 x 64 -> 10,778 143 and 172 forward, 672 and 687
-// trained; 272,567 x 128 -> 23,790 1,906 and 2,413, 8,849 and 10,017; 70,000 x 64 -> 5,000
-// 93 and 134, 422 and 482.)
+// one round's groups at most, us: 52,802 x 64 -> 10,778 672 and 687 trained; 272,567 x 128
+// -> 23,790 1,906 and 2,413 forward, 8,849 and 10,017 trained; 70,000 x 64 -> 5,000 422 and
+// 482 trained.)
 static int64_t share_of(int64_t groups, int64_t chunks, int64_t slots, double cost, int64_t most)
 {
     most = std::max<int64_t>(1, std::min(most, chunks));
